@@ -23,7 +23,8 @@ extern "C" {
 
 /* element types */
 enum { MMX_F32 = 0, MMX_BF16 = 1, MMX_I8 = 2, MMX_I32 = 3, MMX_I4 = 4 /* packed weights only */,
-       MMX_U8 = 5 /* unsigned bytes: mmx_repack_b, mmx_gemm_u8, mmx_matvec_u8 only */ };
+       MMX_U8 = 5 /* unsigned bytes: mmx_repack_b, mmx_gemm_u8, mmx_matvec_u8 only */,
+       MMX_F8 = 6 /* 8-bit floating point, e4m3 (largest value 448): mmx_repack_b and the entry points named fp8 or moe, mmx_block_norm */ };
 
 /* error codes */
 enum {
@@ -92,7 +93,8 @@ int mmx_init(int device);
  *     lane = n%32 + 32*((k%KS)/(KS/2)),  byte offset in the lane = (k%(KS/2))*sizeof(T),
  * zero padded in K up to a multiple of 128 bytes per column and in N up to a multiple of 32.
  * dtype MMX_U8 (unsigned weights, for mmx_gemm_u8): the int8 layout holding u - 128, i.e. every byte with its sign
- * bit inverted (the padding stays zero). */
+ * bit inverted (the padding stays zero).  dtype MMX_F8 (for mmx_gemm_fp8, mmx_mlp_fp8, mmx_moe_experts): the int8 layout of the
+ * bytes as they are. */
 size_t mmx_packed_b_bytes(int dtype, int K, int N);
 int mmx_repack_b(int dtype, const void* B, int64_t ldb_bytes, int K, int N, int transpose, void* packed,
                  void* stream);
@@ -252,6 +254,94 @@ int mmx_mlp(const void* x, int64_t ldx_bytes, const void* w_gate_up, const void*
 int mmx_mlp_splitk(const void* x, int64_t ldx_bytes, const void* w_gate_up, const void* w_down, void* h,
                    int64_t ldh_bytes, void* y, int64_t ldy_bytes, int M, int K, int N, int down_k_splits,
                    void* workspace, size_t workspace_bytes, void* stream);
+
+/* ==== the feed-forward block in 8-bit floating point (no counterpart in the reference) ==========================
+ * Numbers of MMX_F8 (e4m3: 4 bits of exponent, 3 of mantissa, NaN, no infinities) come with fp32 scales, one for each block of
+ * 128.  Activations [M, K]: scales[k / 128][m], rows of scales ld_scales (>= M) elements apart.  Weights [N, K]:
+ * scales[n / 128][k / 128], contiguous; any values.  In a gate/up pair gate's rows of scales come first, then up's.
+ * Rows of quantised activations are 16-byte aligned and lie a multiple of 16 bytes apart; they hold ceil(K / 128) * 128 bytes, and
+ * the bytes from K on must be zero (every entry point here that writes such rows writes them so).
+ * With M (or T) = 0 these calls do nothing. */
+
+/* x [M, K] (MMX_BF16 or MMX_F32) -> q, scales: scales[kb][m] is the least power of two, 2^-126 at least, with which the block's
+ * largest magnitude is at most 448; q = x / scale to nearest even.  (x / scale is exact, so the result does not depend on how it is computed.)  A block that
+ * holds an infinity or a NaN gets the scale NaN. */
+int mmx_quantize_rows_fp8(int x_dtype, const void* x, int64_t ldx_bytes, int M, int K, void* q, int64_t ldq_bytes, float* scales,
+                          int64_t ld_scales, void* stream);
+
+/* bf16 weights, [K, N] or with transpose [N, K], to packed e4m3 (mmx_packed_b_bytes(MMX_F8, K, N) bytes) and their scales, chosen per
+ * block of 128 x 128 in the same way.  pair: 0; or 1 / 2: the gate / up half of a pair of N columns each (N % 32 == 0), where
+ * packed and scales are those of the whole pair, mmx_packed_b_bytes(MMX_F8, K, 2 N) bytes and 2 * ceil(N / 128) rows. */
+int mmx_quantize_pack_fp8(const void* W, int64_t ldw_bytes, int K, int N, int transpose, int pair, void* packed, float* scales,
+                          void* stream);
+/* mmx_repack_gate_up for e4m3 weights (both [N, K]) that come with scales of their own: put gate's rows of scales before up's. */
+int mmx_repack_gate_up_fp8(const void* w_gate, const void* w_up, int64_t ldw_bytes, int K, int N, void* packed, void* stream);
+
+/* C = PP( A . B ), A [M, K] e4m3 with scales, or MMX_BF16 / MMX_F32, quantised as by mmx_quantize_rows_fp8 on the way (a_scales = NULL);
+ * B packed e4m3 with scales.  Each block's sum is multiplied by both scales and added in fp32.  Within a block the matrix cores align the
+ * products of eight neighbouring k to the largest of them and cut off what lies more than 13 bits below its leading one: a result is good to some
+ * 1.5e-5 of its typical size, for C in fp32 too.  ep: any of BIAS, GELU, or SILU_GATE alone
+ * (then B is a gate/up pair, N counts both, and C has N / 2 columns; silu is computed to some 2^-20 here); C fp32 or bf16.
+ * scratch: 256-byte aligned device memory, mmx_gemm_fp8_scratch_bytes() bytes (0: none needed), free to reuse once the call's work
+ * on `stream` has finished.  C must not overlap A. */
+size_t mmx_gemm_fp8_scratch_bytes(int a_dtype, int M, int K, int N);
+int mmx_gemm_fp8(int a_dtype, const void* A, int64_t lda_bytes, const float* a_scales, int64_t ld_a_scales, const void* Bpacked,
+                 const float* b_scales, int M, int K, int N, const mmx_epilogue* ep, void* scratch, size_t scratch_bytes, void* stream);
+
+/* mmx_mlp over e4m3 weights: y [M, K] = down( silu(x . gate) * (x . up) ), both products as mmx_gemm_fp8; the fp32 result of the first is quantised
+ * without being rounded to bf16 in between.  x as A above; w_gate_up of [K, 2 N], w_down of [N, K], N % 32 == 0; y MMX_BF16 or MMX_F32. */
+size_t mmx_mlp_fp8_scratch_bytes(int x_dtype, int M, int K, int N);
+int mmx_mlp_fp8(int x_dtype, const void* x, int64_t ldx_bytes, const float* x_scales, int64_t ld_x_scales, const void* w_gate_up,
+                const float* gate_up_scales, const void* w_down, const float* down_scales, int y_dtype, void* y, int64_t ldy_bytes, int M,
+                int K, int N, void* scratch, size_t scratch_bytes, void* stream);
+
+/* ---- a mixture-of-experts layer for a few tokens -------------------------------------------------------------
+ * Routing of T tokens x [T, H] bf16 over E experts, router [E, H] bf16: logits l = x . router^T, p = softmax(l) or, with MMX_MOE_SIGMOID, 1 / (1 + e^-l);
+ * ids[t][0..top_k) = the experts of the largest p + bias (bias [E] or NULL), in descending order, the lowest index of equal ones (a NaN counts as the least);
+ * weights[t][j] = scale * p, with MMX_MOE_RENORMALIZE divided by the sum of the chosen p.  1 <= top_k <= min(E, 16), E <= 1024.
+ * logits: scratch of T * E doubles. */
+enum { MMX_MOE_SIGMOID = 1, MMX_MOE_RENORMALIZE = 2 };
+int mmx_moe_route(const void* x, int64_t ldx_bytes, const void* router, int64_t ldr_bytes, int T, int H, int E, int top_k, int flags,
+                  float scale, const float* bias, double* logits, int32_t* ids, float* weights, void* stream);
+
+/* y[t] = sum over j of weights[t][j] * down_e( silu(gate_e . x[t]) * (up_e . x[t]) ), e = ids[t][j]; an id outside [0, E) stands for no
+ * expert, one that a token names twice counts with both weights.  w_dtype MMX_BF16 (scales NULL) or MMX_F8; the weights of the experts lie one behind the
+ * other: w_gate_up E times a pair of [H, 2 I] (mmx_repack_gate_up / _fp8, mmx_quantize_pack_fp8), w_down E times [I, H]
+ * (mmx_repack_b of the torch layout [H, I] with transpose = 1), scales likewise.  I % 32 == 0.  x stays bf16, sums are
+ * fp32, the intermediate enters the second product with 16 bits of mantissa.  Every chosen expert's weights are read once per 32 tokens:
+ * for many tokens gather them by expert and use mmx_gemm.  h: scratch of T * top_k * 2 * I bf16, 16-byte aligned.  y MMX_BF16 or MMX_F32. */
+int mmx_moe_experts(int w_dtype, const void* x, int64_t ldx_bytes, const int32_t* ids, const float* weights, int T, int H, int I, int E,
+                    int top_k, const void* w_gate_up, const float* gate_up_scales, const void* w_down, const float* down_scales, void* h,
+                    int y_dtype, void* y, int64_t ldy_bytes, void* stream);
+
+/* ---- the norms behind and in front of a block, its gate and the residual stream, in one pass ------------------
+ *     u = f                                                     or, with post,  f / sqrt(mean(f^2) + eps) * (weight_offset + post_weight)
+ *     r = residual + scale * gate * u
+ *     z = r (as it is in fp32)                                  or, with pre,   r / sqrt(mean(r^2) + eps) * (weight_offset + pre_weight)
+ * f, gate and the weights are bf16, rows of f [M, H]; residual and r are both residual_dtype, MMX_BF16 or MMX_F32; z is MMX_BF16, or MMX_F8 with scales as
+ * mmx_quantize_rows_fp8 gives them (of z in fp32).  NULL: residual (zero), gate (one), post_weight / pre_weight (the norm without weights), r or z (not
+ * wanted; one of them is).  ld_gate_bytes = 0: one row of gate for all.  r may be residual itself; apart from that outputs overlap nothing.
+ * H <= 32768. */
+typedef struct mmx_block_norm_args {
+    const void* f;
+    int64_t ldf_bytes;
+    const void* residual;
+    int64_t ld_residual_bytes;
+    const void* post_weight;
+    const void* gate;
+    int64_t ld_gate_bytes;
+    const void* pre_weight;
+    void* r;
+    int64_t ldr_bytes;
+    void* z;
+    int64_t ldz_bytes;
+    float* z_scales;
+    int64_t ld_z_scales; /* elements */
+    int32_t residual_dtype, z_dtype;
+    int32_t post, pre;
+    float scale, eps, weight_offset;
+} mmx_block_norm_args;
+int mmx_block_norm(const mmx_block_norm_args* args, int M, int H, void* stream);
 
 /* ---- introspection / tuning (no reference counterpart) --------------------------------------- */
 /* Force the MFMA tile shape ("256x256", "256x192", "128x256", "128x192", "128x128", "128x64", "64x128" (aligned

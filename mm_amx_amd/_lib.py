@@ -9,7 +9,7 @@ import warnings
 
 import torch
 
-F32, BF16, I8, I32, I4, U8 = 0, 1, 2, 3, 4, 5
+F32, BF16, I8, I32, I4, U8, F8 = 0, 1, 2, 3, 4, 5, 6
 PP_NONE, PP_DEQUANT, PP_BIAS, PP_GELU, PP_QUANT, PP_SILU_GATE = 0, 1, 2, 4, 8, 16
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -21,7 +21,9 @@ EXPORTS = ["mmx_last_error", "mmx_init", "mmx_packed_b_bytes", "mmx_repack_b", "
            "mmx_quantize_pack_int4", "mmx_dequant_packed", "mmx_gemm", "mmx_gemm_splitk",
            "mmx_gemm_splitk_static", "mmx_gemm_workspace_bytes", "mmx_gemm_unpacked_workspace_bytes", "mmx_gemm_unpacked",
            "mmx_gemm_u8_scratch_bytes", "mmx_gemm_u8", "mmx_matvec_u8", "mmx_matvec", "mmx_mlp", "mmx_mlp_splitk", "mmx_set_tile",
-           "mmx_set_option", "mmx_last_kernel"]
+           "mmx_set_option", "mmx_last_kernel",
+           "mmx_quantize_rows_fp8", "mmx_quantize_pack_fp8", "mmx_repack_gate_up_fp8", "mmx_gemm_fp8_scratch_bytes", "mmx_gemm_fp8",
+           "mmx_mlp_fp8_scratch_bytes", "mmx_mlp_fp8", "mmx_moe_route", "mmx_moe_experts", "mmx_block_norm"]
 # measurement aids (include/mm_amx_amd_bench.h)
 BENCH_EXPORTS = ["mmx_time_gemm", "mmx_probe_mfma", "mmx_probe_read"]
 
@@ -38,6 +40,13 @@ class _Epilogue(C.Structure):
     _fields_ = [("steps", C.c_uint32), ("out_dtype", C.c_int32), ("C", C.c_void_p), ("ldc_bytes", C.c_int64),
                 ("bias", C.c_void_p), ("deq_scale", C.c_float), ("deq_scale_per_oc", C.c_void_p),
                 ("q_scale", C.c_float), ("q_scale_per_oc", C.c_void_p)]
+
+
+class _BlockNorm(C.Structure):
+    _fields_ = [("f", C.c_void_p), ("ldf_bytes", C.c_int64), ("residual", C.c_void_p), ("ld_residual_bytes", C.c_int64), ("post_weight", C.c_void_p),
+                ("gate", C.c_void_p), ("ld_gate_bytes", C.c_int64), ("pre_weight", C.c_void_p), ("r", C.c_void_p), ("ldr_bytes", C.c_int64),
+                ("z", C.c_void_p), ("ldz_bytes", C.c_int64), ("z_scales", C.c_void_p), ("ld_z_scales", C.c_int64), ("residual_dtype", C.c_int32),
+                ("z_dtype", C.c_int32), ("post", C.c_int32), ("pre", C.c_int32), ("scale", C.c_float), ("eps", C.c_float), ("weight_offset", C.c_float)]
 
 
 _lib = None
@@ -123,6 +132,17 @@ def lib():
         l.mmx_probe_mfma.argtypes = [C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.POINTER(C.c_float),
                                      C.POINTER(C.c_float)]
         l.mmx_probe_read.argtypes = [C.c_void_p, C.c_size_t, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p]
+        p, i, n, z, f = C.c_void_p, C.c_int, C.c_int64, C.c_size_t, C.c_float  # the entry points of ffn.py
+        l.mmx_quantize_rows_fp8.argtypes = [i, p, n, i, i, p, n, p, n, p]
+        l.mmx_quantize_pack_fp8.argtypes = [p, n, i, i, i, i, p, p, p]
+        l.mmx_repack_gate_up_fp8.argtypes = [p, p, n, i, i, p, p]
+        l.mmx_gemm_fp8_scratch_bytes.restype = l.mmx_mlp_fp8_scratch_bytes.restype = z
+        l.mmx_gemm_fp8_scratch_bytes.argtypes = l.mmx_mlp_fp8_scratch_bytes.argtypes = [i, i, i, i]
+        l.mmx_gemm_fp8.argtypes = [i, p, n, p, n, p, p, i, i, i, C.POINTER(_Epilogue), p, z, p]
+        l.mmx_mlp_fp8.argtypes = [i, p, n, p, n, p, p, p, p, i, p, n, i, i, i, p, z, p]
+        l.mmx_moe_route.argtypes = [p, n, p, n, i, i, i, i, i, f, p, p, p, p, p]
+        l.mmx_moe_experts.argtypes = [i, p, n, p, p, i, i, i, i, i, p, p, p, p, p, i, p, n, p]
+        l.mmx_block_norm.argtypes = [C.POINTER(_BlockNorm), i, i, p]
         global _native
         _native = _host_module(l)
         _lib = l
@@ -167,7 +187,7 @@ def _dev(t, what):
     return t
 
 
-_DT = {torch.float32: F32, torch.bfloat16: BF16, torch.int8: I8, torch.int32: I32, torch.uint8: U8}
+_DT = {torch.float32: F32, torch.bfloat16: BF16, torch.int8: I8, torch.int32: I32, torch.uint8: U8, torch.float8_e4m3fn: F8}
 
 
 def dtype_code(t):
@@ -230,16 +250,16 @@ def packed_b_bytes(dtype, K, N):
 
 
 def repack_b(B, transpose=False):
-    """B [K,N] (or [N,K] with transpose) bf16/int8/uint8 on the GPU -> packed weights (uint8 tensor).  uint8 weights
-    (for gemm_u8) are stored as u - 128 in the int8 layout."""
+    """B [K,N] (or [N,K] with transpose) bf16/int8/uint8/e4m3 on the GPU -> packed weights (uint8 tensor).  uint8 weights
+    (for gemm_u8) are stored as u - 128 in the int8 layout, e4m3 weights (for gemm_fp8) as they are."""
     if _native is not None and _initialised:  # as in gemm()
         made = _made(_native.repack, B, transpose)
         if made is not None:
             return made
     _dev(B, "B")
     dt = dtype_code(B)
-    if dt not in (BF16, I8, U8):
-        raise MmxError("B must be bf16, int8 or uint8")
+    if dt not in (BF16, I8, U8, F8):
+        raise MmxError("B must be bf16, int8, uint8 or e4m3")
     K, N = (B.shape[1], B.shape[0]) if transpose else B.shape
     out = torch.empty(packed_b_bytes(dt, K, N), dtype=torch.uint8, device=B.device)
     _check(lib().mmx_repack_b(dt, B.data_ptr(), _row_stride_bytes(B), K, N, int(transpose), out.data_ptr(), _stream()))
@@ -404,7 +424,7 @@ def _packed_bytes_host(dtype, K, N):
         return 0
     if dtype == I4:
         return ((N + 31) // 32) * ((K + 255) // 256 * 4) * 1024
-    es = 2 if dtype == BF16 else 1 if dtype in (I8, U8) else 0
+    es = 2 if dtype == BF16 else 1 if dtype in (I8, U8, F8) else 0
     return ((N + 31) // 32) * 32 * ((K * es + 127) // 128 * 128)
 
 

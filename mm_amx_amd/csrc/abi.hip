@@ -121,6 +121,8 @@ int wave_count() { return g_waves; }
 int decode_pair() { return g_decode_pair; }
 
 static int elesz_of(int dtype) { return dtype == MMX_BF16 ? 2 : (dtype == MMX_I8 || dtype == MMX_U8) ? 1 : 0; }
+// of packed weights
+static int packed_elesz(int dtype) { return dtype == MMX_F8 ? 1 : elesz_of(dtype); }
 
 static int out_size(int dtype) {
     switch (dtype) {
@@ -131,7 +133,7 @@ static int out_size(int dtype) {
     }
 }
 
-static int make_epilogue(const mmx_epilogue* in, int a_dtype, int b_dtype, int M, int n0, int n1, Epilogue* out) {
+int make_epilogue(const mmx_epilogue* in, int a_dtype, int b_dtype, int M, int n0, int n1, Epilogue* out) {
     if (!in) return set_error(MMX_E_INVALID, "epilogue descriptor is NULL");
     if (!in->C) return set_error(MMX_E_INVALID, "epilogue: output pointer C is NULL");
     const int sz = out_size(in->out_dtype);
@@ -313,15 +315,15 @@ size_t mmx_packed_b_bytes(int dtype, int K, int N) {
         if (K <= 0 || N <= 0) return 0;
         return (size_t)((N + 31) / 32) * ((size_t)(K + 255) / 256 * 4) * 1024;
     }
-    const int es = elesz_of(dtype);
+    const int es = packed_elesz(dtype);
     if (!es || K <= 0 || N <= 0) return 0;
     const size_t kpad_bytes = ((size_t)K * es + 127) / 128 * 128;
     return (size_t)((N + 31) / 32) * 32 * kpad_bytes;
 }
 
 int mmx_repack_b(int dtype, const void* B, int64_t ldb_bytes, int K, int N, int transpose, void* packed, void* stream) {
-    const int es = elesz_of(dtype);
-    if (!es) return set_error(MMX_E_INVALID, "mmx_repack_b: dtype %d is neither bf16 nor (u)int8", dtype);
+    const int es = packed_elesz(dtype);
+    if (!es) return set_error(MMX_E_INVALID, "mmx_repack_b: dtype %d is neither bf16, (u)int8 nor e4m3", dtype);
     if (!B || !packed) return set_error(MMX_E_INVALID, "mmx_repack_b: NULL pointer");
     if (K <= 0 || N <= 0) return set_error(MMX_E_INVALID, "mmx_repack_b: K and N must be positive");
     const int64_t min_ld = (int64_t)(transpose ? K : N) * es;

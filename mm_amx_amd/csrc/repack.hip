@@ -248,6 +248,9 @@ int launch_repack(int elesz, const void* B, int64_t ldb, int K, int N, int trans
 int launch_repack_gate_up(const void* wg, const void* wu, int64_t ldw, int K, int N, void* out, hipStream_t st) {
     return launch_repack_rows<2, true>(wg, wu, ldw, K, N, 2 * N / 32, out, st, 0);
 }
+int launch_repack_gate_up_bytes(const void* wg, const void* wu, int64_t ldw, int K, int N, void* out, hipStream_t st) {
+    return launch_repack_rows<1, true>(wg, wu, ldw, K, N, 2 * N / 32, out, st, 0);
+}
 
 // Rows of any alignment and length (16 bytes and more) to rows of `pitch` bytes, a multiple of 128, zero behind their end.
 __global__ __launch_bounds__(256) void align_rows_kernel(const char* __restrict__ A, int64_t lda, int pieces, int row_bytes, char* __restrict__ out, int per_row) {

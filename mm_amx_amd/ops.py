@@ -11,6 +11,7 @@ import enum
 import torch
 
 from . import _lib as L
+from . import ffn
 
 
 class Steps(enum.IntFlag):
@@ -205,20 +206,112 @@ class LinearNxN:
         return other
 
 
+class LinearFp8:
+    """LinearNxN over weights in 8-bit floating point, e4m3 with a scale for each block of 128 x 128:
+    ``set_weight(w[N,K])`` takes bf16 weights, which are quantised, or e4m3 weights with their ``scales`` [N/128, K/128] (rounded up);
+    ``forward(x[M,K], y[M,N])`` quantises x per row and 128 of K (or takes it quantised: Fp8Rows) and writes into the caller's y, bf16 or
+    fp32.  N and K are any.  With a ``bias`` (fp32 [N]) it is added before y is rounded."""
+
+    def __init__(self):
+        self.name = ""
+        self.m_N = self.m_K = 0
+        self._packed = self._scales = None
+
+    def set_weight(self, weight, scales=None):
+        packed, scales = ffn.pack_fp8(weight, scales)
+        self.m_N, self.m_K = weight.shape
+        self._packed, self._scales = packed, scales
+
+    def forward(self, x, y, bias=None):
+        if self._packed is None:
+            raise L.MmxError("forward: set_weight has not been called")
+        if len(x.shape) != 2 or x.shape[1] != self.m_K:
+            raise L.MmxError(f"forward: x must be [M, {self.m_K}]")
+        ffn.gemm_fp8(x, self._packed, self._scales, self.m_N, L.Epilogue(y, L.PP_NONE if bias is None else L.PP_BIAS, bias=bias))
+
+    def __deepcopy__(self, memo):
+        other = LinearFp8()
+        other.name, other.m_N, other.m_K = self.name, self.m_N, self.m_K
+        other._packed, other._scales = copy.deepcopy(self._packed), copy.deepcopy(self._scales)
+        return other
+
+
+class MoE:
+    """A mixture-of-experts layer for a few tokens.  ``setup(router[E,H], w_gate[E,I,H], w_up[E,I,H], w_down[E,H,I])`` packs the experts'
+    weights: bf16; with ``compress="fp8"`` bf16 weights quantised to e4m3 with a scale for each block of 128 x 128; or e4m3 weights with
+    their ``scales`` (gate's and up's [E, I/128, H/128], down's [E, H/128, I/128], rounded up).  ``run(x[T,H]) -> y[T,H]`` chooses ``top_k`` experts for each
+    token (see moe_route; ``bias`` [E] moves the choice, not the weights) and adds up what they make of it.  I is a multiple of 32.  Every
+    chosen expert's weights are read once per 32 tokens, so the layer is meant for tens of tokens; it takes any number."""
+
+    def __init__(self, top_k, scoring="softmax", renormalize=True, scale=1.0):
+        if scoring not in ("softmax", "sigmoid"):
+            raise L.MmxError("MoE: scoring is 'softmax' or 'sigmoid'")
+        self.top_k, self.scoring, self.renormalize, self.scale = top_k, scoring, renormalize, scale
+        self.E = self.H = self.I = 0
+        self.router = self.bias = self.gate_up = self.down = None
+
+    def setup(self, router, w_gate, w_up, w_down, scales=None, bias=None, compress=None):
+        if any(not isinstance(w, torch.Tensor) or w.dim() != 3 for w in (w_gate, w_up, w_down)):
+            raise L.MmxError("setup: w_gate, w_up and w_down must be 3-D tensors, an expert each along the first")
+        E, I, H = w_gate.shape
+        if tuple(w_up.shape) != (E, I, H) or tuple(w_down.shape) != (E, H, I) or tuple(router.shape) != (E, H):
+            raise L.MmxError("setup: w_up must be shaped as w_gate [E, I, H], w_down [E, H, I], router [E, H]")
+        if I % 32 or 0 in (E, I, H):
+            raise L.MmxError(f"setup: experts of {I} columns (a positive multiple of 32 is needed)")
+        if compress not in (None, "fp8") or (compress and scales is not None):
+            raise L.MmxError("setup: compress is 'fp8', for weights that come without scales")
+        f8 = scales is not None or compress == "fp8"
+        code, blocks = (L.F8 if f8 else L.BF16), lambda n: -(-n // 128)
+        new = lambda *shape, **kw: torch.empty(shape, device=w_gate.device, **kw)  # noqa: E731
+        gate_up = new(E, L._packed_bytes_host(code, H, 2 * I), dtype=torch.uint8)
+        down = new(E, L._packed_bytes_host(code, I, H), dtype=torch.uint8)
+        if f8:
+            s_gate_up, s_down = new(E, 2 * blocks(I), blocks(H)), new(E, blocks(H), blocks(I))
+            for e in range(E):
+                s = None if scales is None else [t[e] for t in scales]
+                ffn.pack_gate_up_fp8(w_gate[e], w_up[e], None if s is None else s[:2], out=(gate_up[e], s_gate_up[e]))
+                ffn.pack_fp8(w_down[e], None if s is None else s[2], out=(down[e], s_down[e]))
+            self.gate_up, self.down = (gate_up.view(-1), s_gate_up), (down.view(-1), s_down)
+        else:
+            for e in range(E):
+                gate_up[e].copy_(L.repack_gate_up(w_gate[e], w_up[e]))
+                down[e].copy_(L.repack_b(w_down[e], transpose=True))
+            self.gate_up, self.down = gate_up.view(-1), down.view(-1)
+        self.E, self.H, self.I, self.router, self.bias = E, H, I, router, bias
+
+    def run(self, x, y=None):
+        if self.gate_up is None:
+            raise L.MmxError("run: setup has not been called")
+        if x.dim() != 2 or x.shape[1] != self.H:
+            raise L.MmxError(f"run: x must be [T, {self.H}]")
+        ids, weights = ffn.moe_route(x, self.router, self.top_k, self.scoring, self.renormalize, self.scale, self.bias)
+        return ffn.moe_experts(x, ids, weights, self.gate_up, self.down, self.E, self.I, y=y)
+
+
 class MLP:
     """AMX_MLP::MLP (tests/amx-mlp.cpp:740-784): ``setup(w_gate[N,K], w_up[N,K], w_down[K,N])``
     (torch nn.Linear.weight layouts), then ``run(x[M,K]) -> y[M,K]`` computing
-    bf16(silu(x·Wg^T) * (x·Wu^T)) fused in the gate/up epilogue, then the down projection."""
+    bf16(silu(x·Wg^T) * (x·Wu^T)) fused in the gate/up epilogue, then the down projection.
+
+    With ``compress="fp8"`` the bf16 weights are quantised to e4m3, with ``scales`` (gate's, up's and down's, a block of 128 x 128 each) they are e4m3 already;
+    run then quantises x and the intermediate per row and 128 columns, or takes x as Fp8Rows."""
 
     def __init__(self):
         self.m_N = self.m_K = 0
         self.gate_up = self.down = None
         self.actUp = None
 
-    def setup(self, w_gate, w_up, w_down):
+    def setup(self, w_gate, w_up, w_down, scales=None, compress=None):
         N, K = w_gate.shape
         if tuple(w_down.shape) != (K, N):
             raise L.MmxError("setup: w_down must be [K, N]")
+        if compress not in (None, "fp8") or (compress and scales is not None):
+            raise L.MmxError("setup: compress is 'fp8', for weights that come without scales")
+        if scales is not None or compress:
+            gate_up = ffn.pack_gate_up_fp8(w_gate, w_up, None if scales is None else scales[:2])
+            self.down = ffn.pack_fp8(w_down, None if scales is None else scales[2])
+            self.gate_up, self.m_N, self.m_K = gate_up, N, K
+            return
         self.m_N, self.m_K = N, K
         self.gate_up = L.repack_gate_up(w_gate, w_up)
         self.down = L.repack_b(w_down, transpose=True)
@@ -226,8 +319,10 @@ class MLP:
     def run(self, x, y=None):
         if self.gate_up is None:
             raise L.MmxError("run: setup has not been called")
-        if x.dim() != 2 or x.shape[1] != self.m_K:
+        if len(x.shape) != 2 or x.shape[1] != self.m_K:
             raise L.MmxError(f"run: x must be [M, {self.m_K}]")
+        if isinstance(self.gate_up, tuple):
+            return ffn.mlp_fp8(x, self.gate_up, self.down, self.m_N, y=y)
         M = x.shape[0]
         if self.actUp is None or self.actUp.shape[0] < M:  # setM (tests/amx-mlp.cpp:771-776)
             self.actUp = torch.empty((M, self.m_N), dtype=torch.bfloat16, device=x.device)

@@ -170,12 +170,22 @@ __global__ __launch_bounds__(512) void fp8_rows_kernel(const Fp8Gemm g) {
     }
 }
 
-// ---- many rows: tiles through LDS --------------------------------------------------------------------------------------
-// A workgroup computes BM rows x BN columns, its NW wavefronts a grid of WGM x (NW / WGM).  Stages of 128 k (one block: A rows of
-// 128 bytes, B whole fragments, and the stage's scales) go from memory straight into a ring of R LDS slots.  A wavefront walks
-// its rows 16 at a time against all its columns' fragments, which it holds in registers.  The one barrier per stage stands
-// in front of the last 16 rows: all of this stage has been read into registers then, so its slot is free for the loads of
-// stage kb + R, and the next stage has landed, so its first fragments are fetched beside the last rows' products.
+// ---- many rows: tiles ----------------------------------------------------------------------------------------------------
+// A workgroup computes BM rows x BN columns, its NW wavefronts a grid of WGM x (NW / WGM).  A stage is 128 k, one block.  A's rows of 128 bytes
+// and the stage's scales go from memory straight into a ring of R LDS slots.  A wavefront walks its rows 16 at a time against all its
+// columns' fragments, which it holds in registers.  The one barrier per stage stands in front of the last 16 rows: all of this
+// stage has been read into registers then, so its slot is free for the loads of stage kb + R (issued during the next stage), and the next stage has landed, so its
+// first fragments are fetched beside the last rows' products.
+// What bounds it: at 4096 x 8192 x 4096 the matrix cores are busy for 56 % of a stage's cycles, and the chip's power holds the clock at 2.0 GHz; a loop of nothing but these
+// products and multiply-adds runs at 3.2 PFLOP/s on random values, 4.3 on zeros.
+// Where the chunks of a row of A lie in LDS: chunk ^ turn(row), 0 ... 7.  An LDS cycle serves 16 lanes of a ds_read_b128, 256 bytes, and takes them as
+// lanes 0-3, 12-15, 20-23, 24-27 (and 4-11, 16-19, 28-31, and the same of the other half): eight rows' chunk c and the other eight's c ^ 2.  Two rows lie in
+// 256 bytes, so row / 2 has to be spread over the eight positions, the first eight's and the second's without a common one: {0, 1, 6, 7} go to {0, 1, 2, 3},
+// which c ^ 2 maps to itself.  (With row / 2 as it is, every read took twice its cycles.)
+__device__ __forceinline__ int turn(int row) {
+    const int x = row >> 1 & 7;
+    return ((x >> 2 ^ x >> 1) & 1) << 2 | (x >> 2) << 1 | (x & 1);
+}
 template <int BM, int BN, int NW, int WGM, int R>
 struct Fp8Tile {
     static constexpr int WGN = NW / WGM, WM = BM / WGM, WN = BN / WGN;
@@ -183,17 +193,20 @@ struct Fp8Tile {
     static constexpr int A_B = BM * 128, B_B = BN * 128, SA_B = BM * 4, SB_B = 256;
     static constexpr int STAGE = A_B + B_B + SA_B + SB_B;
     static constexpr int BYTES = R * STAGE;
-    static constexpr int LOADS = (BM + BN) / 8 / NW;  // of 1 KiB per wavefront and stage
-    static_assert((BM + BN) / 8 % NW == 0 && BM % 64 == 0, "every wavefront issues the same number of loads");
+    static constexpr int PIECES = (A_B + B_B) / 1024, LOADS = PIECES / NW;  // loads of 1 KiB: of a stage, of a wavefront
+    static constexpr int A_LOADS = BM / 8 / NW;  // of them of A, the first ones
+    static_assert(PIECES % NW == 0 && BM / 8 % NW == 0 && BM % 64 == 0, "every wavefront issues the same number of loads");
     // wavefront w < BM / 64 brings 64 rows' scales, the others B's (again): one load each
     static_assert(BM / 64 < NW, "a wavefront is left for B's scales");
 };
 
 template <int BM, int BN, int NW, int WGM, int R>
-__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4, NW / 4))) void fp8_tile_kernel(const Fp8Gemm g, int tiles_m, int total,
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void fp8_tile_kernel(const Fp8Gemm g, int tiles_m, int total,
                                                                                                           int per_xcd) {
     using T = Fp8Tile<BM, BN, NW, WGM, R>;
     constexpr int MI = T::MI, NJ = T::NJ, STAGE = T::STAGE, LOADS = T::LOADS;
+    using lds_u32x4 = __attribute__((address_space(3))) const u32x4;
+    using lds_float = __attribute__((address_space(3))) const float;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     // neighbouring workgroups go to different XCDs: each XCD gets a run of tiles, rows fastest, which share their columns' weights
     const int L = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
@@ -204,60 +217,84 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
     const int wm = wave / T::WGN, wn = wave % T::WGN;
     const int c = lane & 15, quad = lane >> 4;
     const int nkb = g.nkb;
+    const bool younger = wave >= NW / 2;
 
     // ---- loads: this wavefront's pieces of 1 KiB of a stage, as offsets from the stage's place in A and B
     const char* const a_base = g.A + (int64_t)m0 * g.lda;
     const char* const b_base = g.Bp + (int64_t)panel0 * g.panel_stride;
     const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem);
+    auto panel_off = [&](int p) __attribute__((always_inline)) {  // of the tile's panel p; a tile may reach past the last panel: that one again, never stored
+        const int panel = panel0 + p < g.npanels ? panel0 + p : g.npanels - 1;
+        return (uint32_t)(panel - panel0) * (uint32_t)g.panel_stride;
+    };
     uint32_t off[LOADS];
 #pragma unroll
     for (int i = 0; i < LOADS; i++) {
         const int piece = i * NW + wave;
-        if (piece < BM / 8) {
-            // 8 rows x 128 bytes: the 16-byte chunk c of row r lies at position c ^ (r & 7), so that the 16 rows which an MFMA
-            // operand is read from fall into different banks
+        if (i < T::A_LOADS) {
+            // 8 rows x 128 bytes, the 16-byte chunk c of row r at position c ^ turn(r)
             const int row = piece * 8 + (lane >> 3);
             int m = m0 + row;
             m = m < g.M ? m : g.M - 1;
-            off[i] = (uint32_t)(m - m0) * (uint32_t)g.lda + (uint32_t)(((lane & 7) ^ (row & 7)) * 16);
+            off[i] = (uint32_t)(m - m0) * (uint32_t)g.lda + (uint32_t)(((lane & 7) ^ turn(row)) * 16);
         } else {
             const int frag = piece - BM / 8;
-            int panel = panel0 + (frag >> 2);
-            panel = panel < g.npanels ? panel : g.npanels - 1;
-            off[i] = (uint32_t)(panel - panel0) * (uint32_t)g.panel_stride + (uint32_t)((frag & 3) * 1024 + lane * 16);
+            off[i] = panel_off(frag >> 2) + (uint32_t)((frag & 3) * 1024 + lane * 16);
         }
     }
+    // The 16 columns that the wavefront's tile j is of, in halves of panels.  A gate/up pair has its gate columns in tiles 0 ... NJ / 2 - 1 and the same of up's
+    // behind them.
+    const bool pair = g.pair_up != 0;
+    auto half_of = [&](int j) __attribute__((always_inline)) {
+        if (!pair) return wn * NJ + j;
+        const int col = wn * (NJ / 2) + (j < NJ / 2 ? j : j - NJ / 2);
+        return (col >> 1) * 4 + (col & 1) + (j < NJ / 2 ? 0 : 2);
+    };
+    uint32_t b_off[NJ], sb_off[NJ];  // B's bytes of tile j in a stage, less the lane's place; and its scale
+#pragma unroll
+    for (int j = 0; j < NJ; j++) {
+        const int half = half_of(j);
+        b_off[j] = __builtin_amdgcn_readfirstlane((uint32_t)(half >> 1) * 4096u + (uint32_t)(half & 1) * 256u);
+        sb_off[j] = __builtin_amdgcn_readfirstlane((uint32_t)(half >> 1) * 4u);
+    }
+    const uint32_t b_lane = (uint32_t)(quad * 1024 + c * 16);
     // the scales: 64 rows of A's, or one for each of the tile's panels
-    const char* s_src;
+    const char* s_base;
+    uint32_t s_off, s_dst;
     int64_t s_step;
-    uint32_t s_dst;
     if (wave < BM / 64) {
-        int m = m0 + wave * 64 + lane;
-        m = m < g.M ? m : g.M - 1;
-        s_src = reinterpret_cast<const char*>(g.sA + m);
+        const int m = wave * 64 + lane;
+        s_base = reinterpret_cast<const char*>(g.sA + m0);
+        s_off = (uint32_t)(m0 + m < g.M ? m : g.M - 1 - m0) * 4u;
         s_step = g.ld_sA * 4;
         s_dst = T::A_B + T::B_B + wave * 256;
     } else {
         int panel = panel0 + lane % (BN / 32);
         panel = panel < g.npanels ? panel : g.npanels - 1;
-        s_src = reinterpret_cast<const char*>(g.sB + (int64_t)scale_row(g, panel) * nkb);
+        const int row0 = __builtin_amdgcn_readfirstlane(scale_row(g, panel0));  // (the first panel's: gate's, where it is a pair)
+        s_base = reinterpret_cast<const char*>(g.sB + (int64_t)row0 * nkb);
+        s_off = (uint32_t)(scale_row(g, panel) - row0) * (uint32_t)nkb * 4u;
         s_step = 4;
         s_dst = T::A_B + T::B_B + T::SA_B;
     }
-    auto load_stage = [&](int kb, int slot) __attribute__((always_inline)) {
-        const uint32_t at = lds0 + slot * STAGE;
-        const char* const a = a_base + (int64_t)kb * 128;
-        const char* const b = b_base + (int64_t)kb * 4096;
-        unrolled<0, LOADS>([&](auto ic) __attribute__((always_inline)) {
-            constexpr int i = decltype(ic)::value;
+    // Number ic of this wavefront's loads of stage kb, the last of which is the scales.  lanes: all (-1), or none (0) past the last stage - such a load brings
+    // nothing and counts like any other, so the counts that are waited for are the same throughout.
+    auto load = [&](auto ic, int kb, int slot, int lanes) __attribute__((always_inline)) {
+        constexpr int i = decltype(ic)::value;
+        const uint32_t st = lds0 + slot * STAGE;
+        lanes = __builtin_amdgcn_readfirstlane(lanes);
+        if constexpr (i < LOADS) {
             const int piece = i * NW + wave;
-            const char* const src = piece < BM / 8 ? a : b;
-            const uint32_t to = at + piece * 1024, from = off[i];
-            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(to), "v"(from), "s"(src) : "memory");
-        });
-        const char* const s = s_src + kb * s_step;
-        const uint32_t to = at + s_dst;
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(to), "v"(s) : "memory");
+            const char* const src = i < T::A_LOADS ? a_base + (int64_t)kb * 128 : b_base + (int64_t)kb * 4096;
+            const uint32_t to = st + piece * 1024, from = off[i];
+            asm volatile("s_mov_b32 m0, %0\n\ts_mov_b32 exec_lo, %3\n\ts_mov_b32 exec_hi, %3\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b64 exec, -1"
+                         : : "s"(to), "v"(from), "s"(src), "s"(lanes) : "memory");
+        } else {
+            const char* const src = s_base + kb * s_step;
+            const uint32_t to = st + s_dst, from = s_off;
+            asm volatile("s_mov_b32 m0, %0\n\ts_mov_b32 exec_lo, %3\n\ts_mov_b32 exec_hi, %3\n\tglobal_load_lds_dword %1, %2\n\ts_mov_b64 exec, -1"
+                         : : "s"(to), "v"(from), "s"(src), "s"(lanes) : "memory");
+        }
     };
 
     f32x4 acc[MI][NJ];
@@ -265,86 +302,147 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4,
     for (int i = 0; i < MI; i++)
 #pragma unroll
         for (int j = 0; j < NJ; j++) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    i32x8 fa[2], fb[NJ];
-    float sa[MI], sb[(NJ + 1) / 2];
+    u32x4 fa[3][2], fb[NJ][2];  // the operands of 16 rows, now and next, and of all columns: two 16-byte halves each
+    float sa[3], sb[NJ];
 
-    const int a_row = (wm * T::WM + c) * 128, a_x0 = ((2 * quad) ^ (c & 7)) * 16, a_x1 = ((2 * quad + 1) ^ (c & 7)) * 16;
-    auto read_a = [&](const char* st, int i) __attribute__((always_inline)) {
-        const char* const p = st + a_row + i * 2048;
-        return join(*reinterpret_cast<const u32x4*>(p + a_x0), *reinterpret_cast<const u32x4*>(p + a_x1));
+    // where this lane reads in a stage: the two halves of A's operands, A's scales, and B and its scales (what is behind a tile's place are constants)
+    uint32_t at_a[2], at_sa, at_b;
+    auto places = [&](int slot) __attribute__((always_inline)) {
+        const uint32_t st = lds0 + slot * STAGE, a = st + (wm * T::WM + c) * 128;
+        at_a[0] = a + ((2 * quad) ^ turn(c)) * 16;
+        at_a[1] = a + ((2 * quad + 1) ^ turn(c)) * 16;
+        at_sa = st + T::A_B + T::B_B + (wm * T::WM + c) * 4;
+        at_b = st + T::A_B + b_lane;
+        asm volatile("" : "+v"(at_a[0]), "+v"(at_a[1]), "+v"(at_sa));
     };
-    auto read_b = [&](const char* st, int j) __attribute__((always_inline)) {
-        const int tile = wn * NJ + j;  // of 16 columns
-        const char* const p = st + T::A_B + (tile >> 1) * 4096 + quad * 1024 + ((tile & 1) * 16 + c) * 16;
-        return join(*reinterpret_cast<const u32x4*>(p), *reinterpret_cast<const u32x4*>(p + 512));
-    };
-    auto read_scales = [&](const char* st) __attribute__((always_inline)) {
-        const float* const pa = reinterpret_cast<const float*>(st + T::A_B + T::B_B) + wm * T::WM + c;
-#pragma unroll
-        for (int i = 0; i < MI; i++) sa[i] = pa[i * 16];
-        const float* const pb = reinterpret_cast<const float*>(st + T::A_B + T::B_B + T::SA_B) + ((wn * NJ) >> 1);
-#pragma unroll
-        for (int j = 0; j < (NJ + 1) / 2; j++) sb[j] = pb[j];
+    auto read_a = [&](int i, int half) __attribute__((always_inline)) { return *reinterpret_cast<lds_u32x4*>(at_a[half] + i * 2048); };
+    auto read_b = [&](int j, int half) __attribute__((always_inline)) { return *reinterpret_cast<lds_u32x4*>(at_b + b_off[j] + half * 512); };
+    auto read_sa = [&](int i) __attribute__((always_inline)) { return *reinterpret_cast<lds_float*>(at_sa + i * 64); };
+    auto read_sb = [&](int slot, int j) __attribute__((always_inline)) {
+        return *reinterpret_cast<lds_float*>(lds0 + slot * STAGE + T::A_B + T::B_B + T::SA_B + sb_off[j]);
     };
 
-    unrolled<0, R>([&](auto rc) __attribute__((always_inline)) {
+    unrolled<0, R - 1>([&](auto rc) __attribute__((always_inline)) {
         constexpr int r = decltype(rc)::value;
-        if (r < nkb) load_stage(r, r);
+        unrolled<0, LOADS + 1>([&](auto ic) __attribute__((always_inline)) { load(ic, r, r, __builtin_amdgcn_readfirstlane((r - nkb) >> 31)); });
+    });
+    asm volatile("s_waitcnt vmcnt(%0)" : : "n"((R - 2) * (LOADS + 1)) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    places(0);
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+#pragma unroll
+        for (int j = 0; j < NJ; j++) fb[j][h] = read_b(j, h);
+        fa[0][h] = read_a(0, h);
+        fa[1][h] = read_a(1, h);
+    }
+    sa[0] = read_sa(0);
+    sa[1] = read_sa(1);
+#pragma unroll
+    for (int j = 0; j < NJ; j++) sb[j] = read_sb(0, j);
+    __builtin_amdgcn_sched_barrier(0);
+
+    // One slot per MFMA, in this order and no other (the compiler would gather the multiply-adds behind the last of them): the MFMA; the multiply-adds of
+    // the one LAG slots before, whose result is there by now; an LDS read for the rows or the stage to come; a load.
+    // The loads are spread over the slots in front of the barrier: issued behind one another they hold up the wavefronts, the products and all, until the address unit has taken them.
+    constexpr int LAG = 2, SLOTS = MI * NJ, SPAN = MI > 2 ? (MI - 2) * NJ : MI > 1 ? NJ : 1;
+    f32x4 p[LAG + 1];
+    float s[LAG + 1];
+    int slot = 0;
+    auto stage = [&](auto turn_c, int kb) __attribute__((always_inline)) {
+        constexpr int F = decltype(turn_c)::value * MI % 3;  // the first rows' operands: the three sets go round
+        const int next = slot + 1 < R ? slot + 1 : 0;
+        const int more = __builtin_amdgcn_readfirstlane((kb + R - 1 - nkb) >> 31), free_slot = slot > 0 ? slot - 1 : R - 1;
+        float sb_next[NJ];
+        unrolled<0, SLOTS + LAG>([&](auto tc) __attribute__((always_inline)) {
+            constexpr int t = decltype(tc)::value, i = t / NJ, j = t % NJ;
+            if constexpr (t == SLOTS - NJ) {
+                // in front of the last rows: everything of this stage is in registers (their operands arrive now), and the next one has landed
+                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"((R - 2) * (LOADS + 1)) : "memory");
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                places(next);
+            }
+            if constexpr (NW > 4 && t < SLOTS && j == 0) {
+                // Of a SIMD's two wavefronts the older one is served first: it was at the barrier 670 of a stage's 3300 cycles before the other,
+                // which then had the SIMD to itself and could not fill it.  The younger one is served first for the first half.
+                // (256 x 192, 4096 x 8192 x 4096: 186 -> 183 us; 256 x 256: 130 -> 125.)
+                if constexpr (i == 0 || i == MI / 2) {
+                    if (younger) __builtin_amdgcn_s_setprio(i == 0 ? 1 : 0);
+                }
+            }
+            if constexpr (t < SLOTS) {
+                p[t % (LAG + 1)] = mfma_e4m3(join(fb[j][0], fb[j][1]), join(fa[(F + i) % 3][0], fa[(F + i) % 3][1]));
+                s[t % (LAG + 1)] = sa[(F + i) % 3] * sb[j];
+            }
+            if constexpr (t >= LAG) {
+                constexpr int d = t - LAG;
+                f32x4& a = acc[d / NJ][d % NJ];
+#pragma unroll
+                for (int e = 0; e < 4; e++) a[e] = __builtin_fmaf(p[d % (LAG + 1)][e], s[d % (LAG + 1)], a[e]);
+                asm volatile("" : "+v"(a));
+            }
+            if constexpr (t < SLOTS) {
+                unrolled<0, LOADS + 1>([&](auto ic) __attribute__((always_inline)) {
+                    if constexpr (decltype(ic)::value * SPAN / (LOADS + 1) == t) load(ic, kb + R - 1, free_slot, more);
+                });
+                if constexpr (i < MI - 2) {
+                    constexpr int n = (F + i + 2) % 3;
+                    if constexpr (j == 0) sa[n] = read_sa(i + 2);
+                    if constexpr (NJ == 1) {
+                        fa[n][0] = read_a(i + 2, 0);
+                        fa[n][1] = read_a(i + 2, 1);
+                    } else if constexpr (j < 2) {
+                        fa[n][j] = read_a(i + 2, j);
+                    }
+                } else if constexpr (i == MI - 1) {
+                    // (past the last stage these read what an earlier one left there: never used)
+                    constexpr int n0 = (F + MI) % 3, n1 = (F + MI + 1) % 3;
+                    if constexpr (j == 0) {
+                        fa[n0][0] = read_a(0, 0);
+                        fa[n0][1] = read_a(0, 1);
+                        sa[n0] = read_sa(0);
+#pragma unroll
+                        for (int n = 0; n < NJ; n++) sb_next[n] = read_sb(next, n);
+                    }
+                    fb[j][0] = read_b(j, 0);
+                    fb[j][1] = read_b(j, 1);
+                    if constexpr (j == NJ - 1) {
+                        fa[n1][0] = read_a(1, 0);
+                        fa[n1][1] = read_a(1, 1);
+                        sa[n1] = read_sa(1);
+                    }
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        });
+#pragma unroll
+        for (int n = 0; n < NJ; n++) sb[n] = sb_next[n];
+        slot = next;
+    };
+    // stages in turn until the sets of registers are where they were
+    constexpr int TURN = MI % 3 ? 3 : 1;
+    int kb = 0;
+    for (; kb + TURN <= nkb; kb += TURN) unrolled<0, TURN>([&](auto pc) __attribute__((always_inline)) { stage(pc, kb + decltype(pc)::value); });
+    unrolled<0, TURN - 1>([&](auto pc) __attribute__((always_inline)) {
+        if (kb + decltype(pc)::value < nkb) stage(pc, kb + decltype(pc)::value);
     });
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    {
-#pragma unroll
-        for (int j = 0; j < NJ; j++) fb[j] = read_b(smem, j);
-        fa[0] = read_a(smem, 0);
-        read_scales(smem);
-    }
-    int slot = 0;
-    for (int kb = 0; kb < nkb; kb++) {
-        const char* const st = smem + slot * STAGE;
-        const int next = slot + 1 < R ? slot + 1 : 0;
-        const char* const st_next = smem + next * STAGE;
-        unrolled<0, MI>([&](auto ic) __attribute__((always_inline)) {
-            constexpr int i = decltype(ic)::value;
-            constexpr bool LAST = i == MI - 1;
-            if constexpr (!LAST) {
-                fa[(i + 1) & 1] = read_a(st, i + 1);
-            } else {
-                asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-                __syncthreads();
-                if (kb + R < nkb) load_stage(kb + R, slot);
-            }
-            unrolled<0, NJ>([&](auto jc) __attribute__((always_inline)) {
-                constexpr int j = decltype(jc)::value;
-                const f32x4 p = mfma_e4m3(fb[j], fa[i & 1]);
-                const float s = sa[i] * sb[j >> 1];
-#pragma unroll
-                for (int e = 0; e < 4; e++) acc[i][j][e] = __builtin_fmaf(p[e], s, acc[i][j][e]);
-            });
-        });
-        // (past the last stage these read what an earlier one left there: never used)
-#pragma unroll
-        for (int j = 0; j < NJ; j++) fb[j] = read_b(st_next, j);
-        fa[0] = read_a(st_next, 0);
-        read_scales(st_next);
-        slot = next;
-    }
 
     // ---- post-op: a lane holds columns n + 0..3 of row m of each 16 x 16 tile
 #pragma unroll
     for (int i = 0; i < MI; i++) {
         const int m = m0 + wm * T::WM + i * 16 + c;
         if (m >= g.M) continue;
-        if (g.pair_up) {
-            if constexpr (NJ % 4 == 0) {
+        if (pair) {
+            if constexpr (NJ % 2 == 0) {
 #pragma unroll
-                for (int j = 0; j < NJ; j++) {
-                    if (j & 2) continue;  // panels alternate: two gate tiles, two up tiles
-                    const int pair = ((panel0 * 2 + wn * NJ + j) >> 2);
+                for (int j = 0; j < NJ / 2; j++) {
                     float r[4];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) r[e] = silu32(acc[i][j][e]) * acc[i][j + 2][e];
-                    const int n = pair * 32 + (j & 1) * 16 + quad * 4;
+                    for (int e = 0; e < 4; e++) r[e] = silu32(acc[i][j][e]) * acc[i][j + NJ / 2][e];
+                    const int n = panel0 * 16 + (wn * (NJ / 2) + j) * 16 + quad * 4;
                     if (n < g.N / 2) store4(g.ep, m, n, g.N / 2, r);
                 }
             }
@@ -383,12 +481,45 @@ static int launch_rows(const Fp8Gemm& g, hipStream_t st, const char* name) {
     return check_hip(hipGetLastError(), "fp8_rows_kernel launch");
 }
 
+// Which tile: the least of rounds * (fixed + blocks of k * stage), a round being as many tiles as fit on the chip, with the constants below fitted to
+// 4096 x 8192 x 4096, 1024 x 11008 x 4096, 2048 x 4096 x 11008, 512 x 4096 x 4096 and 256 x 4096 x 11008 (us; "fixed" holds the first loads and the post-op).
+// us at 2048 x 4096 x 11008 / 1024 x 11008 x 4096 / 512 x 4096 x 4096 / 391 x 1000 x 3001:
+//     256x192   114 / 102 / 44 / 18.6        128x128   144 / 63 / 23 / 10.1
+//      64x128   145 /  65 / 17 /  7.4         64x64    203 / 85 / 18 /  7.4
+struct TileCost {
+    int bm, bn, per_cu;
+    float fixed_us, stage_us;
+};
+static constexpr TileCost TILES[4] = {{256, 192, 1, 9.0f, 1.34f}, {128, 128, 1, 5.2f, 0.67f}, {64, 128, 2, 5.5f, 0.66f}, {64, 64, 2, 2.9f, 0.46f}};
+
+static int choose_tile(const Fp8Gemm& g) {
+    int best = 0;
+    double least = 0;
+    for (int i = 0; i < 4; i++) {
+        const TileCost& t = TILES[i];
+        const int64_t tiles = (int64_t)((g.M + t.bm - 1) / t.bm) * ((g.npanels * 32 + t.bn - 1) / t.bn), at_once = (int64_t)num_cus() * t.per_cu;
+        // (a round that is not full leaves each of its tiles more of the chip)
+        const double full = (double)(tiles / at_once), rest = (double)(tiles % at_once) / at_once;
+        const double us = (full + (rest > 0 ? 0.55 + 0.45 * rest : 0)) * (t.fixed_us + g.nkb * t.stage_us);
+        if (i == 0 || us < least) {
+            best = i;
+            least = us;
+        }
+    }
+    return best;
+}
+
 int launch_gemm_fp8(const Fp8Gemm& g, hipStream_t st) {
     const bool pair = g.pair_up != 0;
     if (g.M <= 16) return pair ? launch_rows<1, 2, true>(g, st, "fp8_rows_16_pair") : launch_rows<1, 1, false>(g, st, "fp8_rows_16");
     if (g.M <= 32) return pair ? launch_rows<2, 2, true>(g, st, "fp8_rows_32_pair") : launch_rows<2, 2, false>(g, st, "fp8_rows_32");
-    if (g.M <= 128) return pair ? launch_rows<4, 2, true>(g, st, "fp8_rows_64_pair") : launch_rows<4, 2, false>(g, st, "fp8_rows_64");
-    return launch_tile<256, 256, 8, 2, 2>(g, st, "fp8_256x256");
+    switch (choose_tile(g)) {
+    case 0:  // (a wavefront of a pair needs as many gate columns as up's: 64 x 96 of the tile instead of 128 x 48)
+        return pair ? launch_tile<256, 192, 8, 4, 2>(g, st, "fp8_256x192_pair") : launch_tile<256, 192, 8, 2, 2>(g, st, "fp8_256x192");
+    case 1: return launch_tile<128, 128, 8, 2, 4>(g, st, "fp8_128x128");
+    case 2: return launch_tile<64, 128, 4, 1, 3>(g, st, "fp8_64x128");
+    default: return launch_tile<64, 64, 4, 2, 4>(g, st, "fp8_64x64");
+    }
 }
 
 }  // namespace mmx

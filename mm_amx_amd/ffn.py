@@ -54,7 +54,9 @@ class Fp8Rows:
 
     @classmethod
     def empty(cls, M, K, device):
-        return cls(torch.empty((M, _blocks(K) * BLOCK), dtype=_E4M3, device=device), torch.empty((_blocks(K), M), device=device), K)
+        # rows a multiple of 2 KiB apart meet in few channels of the L2: they get 128 bytes more between them
+        n = _blocks(K) * BLOCK
+        return cls(torch.empty((M, n + 128 if n % 2048 == 0 else n), dtype=_E4M3, device=device)[:, :n], torch.empty((_blocks(K), M), device=device), K)
 
     @classmethod
     def of(cls, q, scales):

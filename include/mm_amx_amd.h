@@ -309,10 +309,12 @@ int mmx_moe_route(const void* x, int64_t ldx_bytes, const void* router, int64_t 
  * other: w_gate_up E times a pair of [H, 2 I] (mmx_repack_gate_up / _fp8, mmx_quantize_pack_fp8), w_down E times [I, H]
  * (mmx_repack_b of the torch layout [H, I] with transpose = 1), scales likewise.  I % 32 == 0.  x stays bf16, sums are
  * fp32, the intermediate enters the second product with 16 bits of mantissa.  Every chosen expert's weights are read once per 32 tokens:
- * for many tokens gather them by expert and use mmx_gemm.  h: scratch of T * top_k * 2 * I bf16, 16-byte aligned.  y MMX_BF16 or MMX_F32. */
+ * for many tokens gather them by expert and use mmx_gemm.  scratch: 256-byte aligned device memory,
+ * mmx_moe_experts_scratch_bytes() bytes, free to reuse once the call's work on `stream` has finished.  y MMX_BF16 or MMX_F32. */
+size_t mmx_moe_experts_scratch_bytes(int T, int H, int I, int top_k);
 int mmx_moe_experts(int w_dtype, const void* x, int64_t ldx_bytes, const int32_t* ids, const float* weights, int T, int H, int I, int E,
-                    int top_k, const void* w_gate_up, const float* gate_up_scales, const void* w_down, const float* down_scales, void* h,
-                    int y_dtype, void* y, int64_t ldy_bytes, void* stream);
+                    int top_k, const void* w_gate_up, const float* gate_up_scales, const void* w_down, const float* down_scales,
+                    int y_dtype, void* y, int64_t ldy_bytes, void* scratch, size_t scratch_bytes, void* stream);
 
 /* ---- the norms behind and in front of a block, its gate and the residual stream, in one pass ------------------
  *     u = f                                                     or, with post,  f / sqrt(mean(f^2) + eps) * (weight_offset + post_weight)

@@ -23,7 +23,7 @@ EXPORTS = ["mmx_last_error", "mmx_init", "mmx_packed_b_bytes", "mmx_repack_b", "
            "mmx_gemm_u8_scratch_bytes", "mmx_gemm_u8", "mmx_matvec_u8", "mmx_matvec", "mmx_mlp", "mmx_mlp_splitk", "mmx_set_tile",
            "mmx_set_option", "mmx_last_kernel",
            "mmx_quantize_rows_fp8", "mmx_quantize_pack_fp8", "mmx_repack_gate_up_fp8", "mmx_gemm_fp8_scratch_bytes", "mmx_gemm_fp8",
-           "mmx_mlp_fp8_scratch_bytes", "mmx_mlp_fp8", "mmx_moe_route", "mmx_moe_experts", "mmx_block_norm"]
+           "mmx_mlp_fp8_scratch_bytes", "mmx_mlp_fp8", "mmx_moe_route", "mmx_moe_experts_scratch_bytes", "mmx_moe_experts", "mmx_block_norm"]
 # measurement aids (include/mm_amx_amd_bench.h)
 BENCH_EXPORTS = ["mmx_time_gemm", "mmx_probe_mfma", "mmx_probe_read"]
 
@@ -141,7 +141,9 @@ def lib():
         l.mmx_gemm_fp8.argtypes = [i, p, n, p, n, p, p, i, i, i, C.POINTER(_Epilogue), p, z, p]
         l.mmx_mlp_fp8.argtypes = [i, p, n, p, n, p, p, p, p, i, p, n, i, i, i, p, z, p]
         l.mmx_moe_route.argtypes = [p, n, p, n, i, i, i, i, i, f, p, p, p, p, p]
-        l.mmx_moe_experts.argtypes = [i, p, n, p, p, i, i, i, i, i, p, p, p, p, p, i, p, n, p]
+        l.mmx_moe_experts_scratch_bytes.restype = z
+        l.mmx_moe_experts_scratch_bytes.argtypes = [i, i, i, i]
+        l.mmx_moe_experts.argtypes = [i, p, n, p, p, i, i, i, i, i, p, p, p, p, i, p, n, p, z, p]
         l.mmx_block_norm.argtypes = [C.POINTER(_BlockNorm), i, i, p]
         global _native
         _native = _host_module(l)

@@ -47,6 +47,15 @@ __device__ __forceinline__ uint32_t to_fp8x4(float a, float b, float c, float d)
 // border between two of e4m3 should fall on its own side.  (The bf16 MLP's sigmoid has a reciprocal of 14 bits.)
 __device__ __forceinline__ float silu32(float x) { return x * __builtin_amdgcn_rcpf(1.0f + __expf(-x)); }
 
+// eight bf16 in 32 bits
+__device__ __forceinline__ void widen8(u32x4 w, float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        v[2 * e] = u2f(w[e] << 16);
+        v[2 * e + 1] = u2f(w[e] & 0xffff0000u);
+    }
+}
+
 // 8 or 16 values of a row in 32 bits, from element `at` on; what lies past the row's len elements is zero and not touched
 template <int N>
 __device__ __forceinline__ void load_row_f32(const uint16_t* row, int at, int len, float (&v)[N]) {

@@ -16,6 +16,7 @@ int launch_moe_route(const void* x, int64_t ldx, const void* Wr, int64_t ldr, in
 int launch_moe_experts(bool f8, const void* x, int64_t ldx_bytes, const int* ids, const float* weights, int T, int H, int I, int E, int k,
                        const void* w_gate_up, const float* s_gate_up, const void* w_down, const float* s_down, void* h, void* y, int64_t ldy, int y_f32,
                        hipStream_t st);
+size_t moe_scratch_bytes(int T, int H, int I, int k);
 int launch_block_norm(const NormArgs& g, bool residual_f32, hipStream_t st);
 
 static bool misaligned(const void* p, int to) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(to - 1)) != 0; }
@@ -231,9 +232,13 @@ int mmx_moe_route(const void* x, int64_t ldx_bytes, const void* router, int64_t 
                             weights, static_cast<hipStream_t>(stream));
 }
 
+size_t mmx_moe_experts_scratch_bytes(int T, int H, int I, int top_k) {
+    return T <= 0 || H <= 0 || I <= 0 || top_k <= 0 ? 0 : moe_scratch_bytes(T, H, I, top_k);
+}
+
 int mmx_moe_experts(int w_dtype, const void* x, int64_t ldx_bytes, const int32_t* ids, const float* weights, int T, int H, int I, int E, int top_k,
-                    const void* w_gate_up, const float* gate_up_scales, const void* w_down, const float* down_scales, void* h, int y_dtype, void* y,
-                    int64_t ldy_bytes, void* stream) {
+                    const void* w_gate_up, const float* gate_up_scales, const void* w_down, const float* down_scales, int y_dtype, void* y,
+                    int64_t ldy_bytes, void* scratch, size_t scratch_bytes, void* stream) {
     const char* const who = "mmx_moe_experts";
     int rc = check_sizes(who, T, H, I);
     if (rc) return rc;
@@ -243,14 +248,15 @@ int mmx_moe_experts(int w_dtype, const void* x, int64_t ldx_bytes, const int32_t
     if (y_dtype != MMX_F32 && y_dtype != MMX_BF16) return set_error(MMX_E_INVALID, "%s: output dtype %d (bf16 and fp32 exist)", who, y_dtype);
     if (T == 0) return MMX_OK;
     if ((rc = check_rows(who, "x", x, ldx_bytes, T, H, 2)) || (rc = check_rows(who, "y", y, ldy_bytes, T, H, y_dtype == MMX_F32 ? 4 : 2))) return rc;
-    if (!ids || !weights || !h || !w_gate_up || !w_down) return set_error(MMX_E_INVALID, "%s: NULL pointer", who);
-    if (misaligned(ids, 4) || misaligned(weights, 4) || misaligned(h, 16) || misaligned(w_gate_up, 16) || misaligned(w_down, 16))
-        return set_error(MMX_E_INVALID, "%s: ids and weights are not aligned to their element size, or h or packed weights not to 16 bytes", who);
+    if (!ids || !weights || !w_gate_up || !w_down) return set_error(MMX_E_INVALID, "%s: NULL pointer", who);
+    if (misaligned(ids, 4) || misaligned(weights, 4) || misaligned(w_gate_up, 16) || misaligned(w_down, 16))
+        return set_error(MMX_E_INVALID, "%s: ids and weights are not aligned to their element size, or packed weights not to 16 bytes", who);
+    if ((rc = check_scratch(who, scratch, scratch_bytes, moe_scratch_bytes(T, H, I, top_k)))) return rc;
     const bool f8 = w_dtype == MMX_F8;
     if (f8 ? !gate_up_scales || !down_scales : gate_up_scales || down_scales)
         return set_error(MMX_E_INVALID, "%s: e4m3 weights come with scales, bf16 weights without", who);
     if (misaligned(gate_up_scales, 4) || misaligned(down_scales, 4)) return set_error(MMX_E_INVALID, "%s: scales are not aligned to their element size", who);
-    return launch_moe_experts(f8, x, ldx_bytes, ids, weights, T, H, I, E, top_k, w_gate_up, gate_up_scales, w_down, down_scales, h, y, ldy_bytes,
+    return launch_moe_experts(f8, x, ldx_bytes, ids, weights, T, H, I, E, top_k, w_gate_up, gate_up_scales, w_down, down_scales, scratch, y, ldy_bytes,
                               y_dtype == MMX_F32, static_cast<hipStream_t>(stream));
 }
 

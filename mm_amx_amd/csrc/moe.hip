@@ -14,116 +14,122 @@ constexpr int MOE_GROUP = 32;   // tokens that one pass over an expert's weights
 constexpr int MOE_TOP_K = 16;   // experts of a token at most
 constexpr int MOE_EXPERTS = 1024;
 constexpr int MOE_SLOTS = MOE_GROUP * MOE_TOP_K;
+constexpr int MOE_SPLITS = 4;
+
+int num_cus();
 
 // ---- routing ----------------------------------------------------------------------------------------------------------
-// A wavefront takes one expert and up to 8 tokens.  Which expert is chosen hangs on the order of near-equal logits, so they are
+// A wavefront takes one expert and TB tokens.  Which expert is chosen hangs on the order of near-equal logits, so they are
 // summed more exactly than 32 bits: products of bf16 are exact in 32 bits, eight of them are added there, the rest in 64.
+// What bounds it is latency: few tokens per wavefront, so that there are many, and all loads of a step before its products (8 tokens x 128 experts x 4096 with all
+// eight tokens in a wavefront, each load behind a test: 37 us).
 template <int TB>
 __global__ __launch_bounds__(256) void moe_logits_kernel(const uint16_t* __restrict__ x, int64_t ldx, const uint16_t* __restrict__ Wr, int64_t ldr, int T,
                                                          int H, int E, double* __restrict__ logits) {
     const int lane = threadIdx.x & 63, e = blockIdx.x * 4 + (threadIdx.x >> 6), t0 = blockIdx.y * TB;
     if (e >= E) return;
+    const uint16_t* const w_row = Wr + e * ldr;
+    const uint16_t* x_row[TB];
     double sum[TB];
 #pragma unroll
-    for (int t = 0; t < TB; t++) sum[t] = 0.0;
-    for (int h = lane * 8; h < H; h += 512) {
-        float w[8];
-        load_row_f32(Wr + e * ldr, h, H, w);
+    for (int t = 0; t < TB; t++) {
+        x_row[t] = x + (int64_t)(t0 + t < T ? t0 + t : T - 1) * ldx;
+        sum[t] = 0.0;
+    }
+    auto add = [&](const float (&w)[8], const float (&v)[8], double& to) __attribute__((always_inline)) {
+        float s = v[0] * w[0];
+#pragma unroll
+        for (int i = 1; i < 8; i++) s = __builtin_fmaf(v[i], w[i], s);
+        to += (double)s;
+    };
+    constexpr int U = TB == 1 ? 4 : 2;
+    int h = lane * 8;
+    for (; h - lane * 8 + U * 512 <= H; h += U * 512) {  // (uniform: whole steps)
+        u32x4 wv[U], xv[U][TB];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            __builtin_memcpy(&wv[u], __builtin_assume_aligned(w_row + h + u * 512, 2), 16);
+#pragma unroll
+            for (int t = 0; t < TB; t++) __builtin_memcpy(&xv[u][t], __builtin_assume_aligned(x_row[t] + h + u * 512, 2), 16);
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            float w[8], v[8];
+            widen8(wv[u], w);
+#pragma unroll
+            for (int t = 0; t < TB; t++) {
+                widen8(xv[u][t], v);
+                add(w, v, sum[t]);
+            }
+        }
+    }
+    for (; h < H; h += 512) {
+        float w[8], v[8];
+        load_row_f32(w_row, h, H, w);
 #pragma unroll
         for (int t = 0; t < TB; t++) {
-            if (t0 + t >= T) break;
-            float v[8];
-            load_row_f32(x + (t0 + t) * ldx, h, H, v);
-            float s = v[0] * w[0];
-#pragma unroll
-            for (int i = 1; i < 8; i++) s = __builtin_fmaf(v[i], w[i], s);
-            sum[t] += (double)s;
+            load_row_f32(x_row[t], h, H, v);
+            add(w, v, sum[t]);
         }
     }
 #pragma unroll
     for (int t = 0; t < TB; t++) {
-        if (t0 + t >= T) break;
 #pragma unroll
         for (int d = 32; d >= 1; d >>= 1) sum[t] += __shfl_xor(sum[t], d);
-        if (lane == 0) logits[(int64_t)(t0 + t) * E + e] = sum[t];
+        if (lane == 0 && t0 + t < T) logits[(int64_t)(t0 + t) * E + e] = sum[t];
     }
 }
 
-// A wavefront per token.  A NaN counts as less than any number, so that there are always k different experts.
-template <int PER>  // experts per lane
-__global__ __launch_bounds__(64) void moe_topk_kernel(const double* __restrict__ logits, int E, int k, int sigmoid, int renormalize, float scale,
-                                                      const float* __restrict__ bias, int* __restrict__ ids, float* __restrict__ weights) {
-    const int lane = threadIdx.x;
+// A workgroup per token, a thread per expert: its place among all of them is the number of those in front of it, counted against every key in LDS (chosen one after
+// another by a maximum over the wavefront, 8 of 64 took 7.5 us).  A NaN counts as less than any number, so that there are always k different experts.
+__global__ void moe_topk_kernel(const double* __restrict__ logits, int E, int k, int sigmoid, int renormalize, float scale, const float* __restrict__ bias,
+                                int* __restrict__ ids, float* __restrict__ weights) {
+    __shared__ double keys[MOE_EXPERTS];
+    __shared__ double tops[MOE_EXPERTS / 64];
+    __shared__ float totals[MOE_EXPERTS / 64], chosen[MOE_TOP_K];
+    const int e = threadIdx.x, lane = e & 63, wave = e >> 6, waves = blockDim.x >> 6;
     const int64_t t = blockIdx.x;
-    double l[PER], key[PER];
-    double top = -__builtin_inf();
+    const double l = e < E ? logits[t * E + e] : -__builtin_inf();
+    double top = l;
+    float total = 1.0f, u;
+    if (sigmoid) {
+        u = 1.0f / (1.0f + expf(-(float)l));
+    } else {  // softmax's terms against the largest logit
 #pragma unroll
-    for (int i = 0; i < PER; i++) {
-        const int e = i * 64 + lane;
-        l[i] = e < E ? logits[t * E + e] : 0.0;
-        if (e < E) top = __builtin_fmax(top, l[i]);
+        for (int d = 32; d >= 1; d >>= 1) top = __builtin_fmax(top, __shfl_xor(top, d));
+        if (lane == 0) tops[wave] = top;
+        __syncthreads();
+        for (int w = 0; w < waves; w++) top = __builtin_fmax(top, tops[w]);
+        u = e < E ? expf((float)(l - top)) : 0.0f;
+        total = u;
+#pragma unroll
+        for (int d = 32; d >= 1; d >>= 1) total += __shfl_xor(total, d);
+        if (lane == 0) totals[wave] = total;
+        __syncthreads();
+        total = totals[0];
+        for (int w = 1; w < waves; w++) total += totals[w];
     }
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) top = __builtin_fmax(top, __shfl_xor(top, d));
-    // p = u / total: softmax's terms against the largest logit, or the sigmoid itself
-    float total = 0.0f;
-#pragma unroll
-    for (int i = 0; i < PER; i++) {
-        const int e = i * 64 + lane;
-        double p = l[i];  // (without a bias the logits have the order of the p, and no two of them meet in rounding)
-        if (e < E && bias) p = (sigmoid ? 1.0 / (1.0 + exp(-l[i])) : exp(l[i] - top));
-        key[i] = p;
-        if (e < E && !sigmoid) total += expf((float)(l[i] - top));
+    // (without a bias the logits have the order of the p, and no two of them meet in rounding)
+    double key = l;
+    if (bias && e < E) key = (sigmoid ? 1.0 / (1.0 + exp(-l)) : exp(l - top) / (double)total) + (double)bias[e];
+    if (!(key == key)) key = -__builtin_inf();
+    keys[e] = key;
+    if (e < k) chosen[e] = 0.0f;
+    __syncthreads();
+    int before = 0;
+#pragma unroll 8
+    for (int o = 0; o < E; o++) {
+        const double other = keys[o];
+        before += other > key || (other == key && o < e);
     }
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) total += __shfl_xor(total, d);
-    if (bias) {
-#pragma unroll
-        for (int i = 0; i < PER; i++) {
-            const int e = i * 64 + lane;
-            if (e < E) key[i] = (sigmoid ? key[i] : key[i] / (double)total) + (double)bias[e];
-        }
-    }
-    uint32_t open = 0;  // this lane's experts that can be chosen still
-#pragma unroll
-    for (int i = 0; i < PER; i++) {
-        if (i * 64 + lane < E) open |= 1u << i;
-        if (!(key[i] == key[i])) key[i] = -__builtin_inf();
-    }
-    int my_id = 0;
-    float my_u = 0.0f, chosen = 0.0f;
-    for (int j = 0; j < k; j++) {
-        double best = 0.0;
-        int at = -1;
-        double l_best = 0.0;
-#pragma unroll
-        for (int i = 0; i < PER; i++)
-            if ((open >> i & 1) && (at < 0 || key[i] > best)) {
-                best = key[i];
-                l_best = l[i];
-                at = i * 64 + lane;
-            }
-#pragma unroll
-        for (int d = 32; d >= 1; d >>= 1) {
-            const double o = __shfl_xor(best, d), ol = __shfl_xor(l_best, d);
-            const int oa = __shfl_xor(at, d);
-            if (oa >= 0 && (at < 0 || o > best || (o == best && oa < at))) {
-                best = o;
-                l_best = ol;
-                at = oa;
-            }
-        }
-        if ((at & 63) == lane) open &= ~(1u << (at >> 6));
-        const float u = sigmoid ? (float)(1.0 / (1.0 + exp(-l_best))) : expf((float)(l_best - top));
-        chosen += u;
-        if (j == lane) {
-            my_id = at;
-            my_u = u;
-        }
-    }
-    if (lane < k) {
-        ids[t * k + lane] = my_id;
-        weights[t * k + lane] = scale * my_u / (renormalize ? chosen : sigmoid ? 1.0f : total);
+    const bool mine = e < E && before < k;
+    if (mine) chosen[before] = u;
+    __syncthreads();
+    if (mine) {
+        float sum = 0.0f;
+        for (int j = 0; j < k; j++) sum += chosen[j];
+        ids[t * k + before] = e;
+        weights[t * k + before] = scale * u / (renormalize ? sum : total);
     }
 }
 
@@ -131,16 +137,14 @@ int launch_moe_route(const void* x, int64_t ldx, const void* Wr, int64_t ldr, in
                      const float* bias, double* logits, int* ids, float* weights, hipStream_t st) {
     const auto xp = static_cast<const uint16_t*>(x), wp = static_cast<const uint16_t*>(Wr);
     const unsigned gx = (unsigned)((E + 3) / 4);
-    if (T == 1) hipLaunchKernelGGL(moe_logits_kernel<1>, dim3(gx), dim3(256), 0, st, xp, ldx / 2, wp, ldr / 2, T, H, E, logits);
-    else hipLaunchKernelGGL(moe_logits_kernel<8>, dim3(gx, (unsigned)((T + 7) / 8)), dim3(256), 0, st, xp, ldx / 2, wp, ldr / 2, T, H, E, logits);
-    int rc = check_hip(hipGetLastError(), "moe_logits_kernel launch");
+    const int tb = (int64_t)T * E <= 2048 ? 1 : 4;  // (wavefronts for all CUs first, then less of the router read again)
+    const unsigned gy = (unsigned)((T + tb - 1) / tb);
+    if (gy > 65535) return set_error(MMX_E_INVALID, "mmx_moe_route: too many tokens for one launch");
+    if (tb == 1) hipLaunchKernelGGL(moe_logits_kernel<1>, dim3(gx, gy), dim3(256), 0, st, xp, ldx / 2, wp, ldr / 2, T, H, E, logits);
+    else hipLaunchKernelGGL(moe_logits_kernel<4>, dim3(gx, gy), dim3(256), 0, st, xp, ldx / 2, wp, ldr / 2, T, H, E, logits);
+    const int rc = check_hip(hipGetLastError(), "moe_logits_kernel launch");
     if (rc) return rc;
-#define MMX_TOPK(PER) hipLaunchKernelGGL(moe_topk_kernel<PER>, dim3((unsigned)T), dim3(64), 0, st, logits, E, k, sigmoid, renormalize, scale, bias, ids, weights)
-    if (E <= 64) MMX_TOPK(1);
-    else if (E <= 128) MMX_TOPK(2);
-    else if (E <= 256) MMX_TOPK(4);
-    else MMX_TOPK(16);
-#undef MMX_TOPK
+    hipLaunchKernelGGL(moe_topk_kernel, dim3((unsigned)T), dim3((unsigned)((E + 63) / 64 * 64)), 0, st, logits, E, k, sigmoid, renormalize, scale, bias, ids, weights);
     return check_hip(hipGetLastError(), "moe_topk_kernel launch");
 }
 
@@ -159,6 +163,8 @@ struct MoeArgs {
     char* y;
     int64_t ldy;
     int y_f32;
+    float* parts;         // [splits][T][H] sums of a part of the experts each, or NULL: straight to y
+    int splits;
 };
 
 // The experts that the tokens [t0, t0 + n / k) chose, in ascending order.  flags: LDS, E bytes.
@@ -228,49 +234,74 @@ __device__ __forceinline__ bf16x8 load8(const uint16_t* row, int at, int len) {
     return __builtin_bit_cast(bf16x8, w);
 }
 
-// Gate and up: a workgroup takes one chosen expert and 16 columns of each, its eight wavefronts units of k in turn.
+// STEPS operands of a unit of k of a token's row; zero from len on
 template <typename W>
+__device__ __forceinline__ void load_steps(const uint16_t* row, int k0, int quad, int len, bool whole, bf16x8 (&x)[W::STEPS]) {
+    if (whole) {  // (uniform)
+#pragma unroll
+        for (int s = 0; s < W::STEPS; s++) __builtin_memcpy(&x[s], __builtin_assume_aligned(row + k0 + W::k_of(s, quad), 2), 16);
+    } else {
+#pragma unroll
+        for (int s = 0; s < W::STEPS; s++) x[s] = load8(row, k0 + W::k_of(s, quad), len);
+    }
+}
+
+// Gate and up: a workgroup takes one chosen expert and 16 columns of each, its eight wavefronts units of k in turn, U of them at a time so that many loads are
+// in flight.
+template <typename W, int MT>
 __global__ __launch_bounds__(512) void moe_up_kernel(const MoeArgs g, int col_units) {
-    constexpr int NW = 8;
+    constexpr int NW = 8, U = W::F8 || MT > 1 ? 2 : 4;  // (more, and fewer wavefronts fit: e4m3, 8 tokens, 128 experts of 4096 x 1536, 120 us with 4 wavefronts on a SIMD, 177 with 3)
     __shared__ uint8_t flags[MOE_EXPERTS];
     __shared__ uint16_t list[MOE_SLOTS];
     __shared__ int found[2];  // the expert, and how many slots chose it
-    __shared__ __attribute__((aligned(16))) f32x4 red[NW][4][64];
+    __shared__ __attribute__((aligned(16))) f32x4 red[NW][2 * MT][64];
     const int t0 = blockIdx.y * MOE_GROUP, tokens = g.T - t0 < MOE_GROUP ? g.T - t0 : MOE_GROUP;
     const int first = t0 * g.k, n = tokens * g.k;
     const int a = blockIdx.x / col_units, u = blockIdx.x - a * col_units;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    mark_experts(g, first, n, flags);
-    if (wave == 0) {
-        int left = a, expert = -1;
-        for (int e0 = 0; e0 < g.E && expert < 0; e0 += 64) {
-            const uint64_t has = __builtin_amdgcn_ballot_w64(e0 + lane < g.E && flags[e0 + lane]);
-            const int here = __builtin_popcountll(has);
-            if (left < here) {
-                uint64_t rest = has;
-                for (int i = 0; i < left; i++) rest &= rest - 1;
-                expert = e0 + __builtin_ctzll(rest);
+    int expert, count;
+    if (tokens == 1) {  // its slots are the chosen experts themselves
+        expert = a < n ? g.ids[first + a] : -1;
+        if ((unsigned)expert >= (unsigned)g.E || !first_of_token(g.ids + first, a, g.k)) expert = -1;
+        count = 1;
+        if (threadIdx.x == 0) list[0] = (uint16_t)a;
+    } else {
+        mark_experts(g, first, n, flags);
+        if (wave == 0) {
+            int left = a, is = -1;
+            for (int e0 = 0; e0 < g.E && is < 0; e0 += 64) {
+                const uint64_t has = __builtin_amdgcn_ballot_w64(e0 + lane < g.E && flags[e0 + lane]);
+                const int here = __builtin_popcountll(has);
+                if (left < here) {
+                    uint64_t rest = has;
+                    for (int i = 0; i < left; i++) rest &= rest - 1;
+                    is = e0 + __builtin_ctzll(rest);
+                }
+                left -= here;
             }
-            left -= here;
-        }
-        int count = 0;
-        if (expert >= 0) {
-            for (int i0 = 0; i0 < n; i0 += 64) {
-                const int i = i0 + lane;
-                const bool mine = i < n && g.ids[first + i] == expert && first_of_token(g.ids + first, i, g.k);
-                const uint64_t all = __builtin_amdgcn_ballot_w64(mine);
-                if (mine) list[count + __builtin_popcountll(all & ((1ull << lane) - 1))] = (uint16_t)i;
-                count += __builtin_popcountll(all);
+            int slots = 0;
+            if (is >= 0) {
+                for (int i0 = 0; i0 < n; i0 += 64) {
+                    const int i = i0 + lane;
+                    const bool mine = i < n && g.ids[first + i] == is && first_of_token(g.ids + first, i, g.k);
+                    const uint64_t all = __builtin_amdgcn_ballot_w64(mine);
+                    if (mine) list[slots + __builtin_popcountll(all & ((1ull << lane) - 1))] = (uint16_t)i;
+                    slots += __builtin_popcountll(all);
+                }
             }
-        }
-        if (lane == 0) {
-            found[0] = expert;
-            found[1] = count;
+            if (lane == 0) {
+                found[0] = is;
+                found[1] = slots;
+            }
         }
     }
     __syncthreads();
-    const int expert = found[0], count = found[1];
+    if (tokens > 1) {
+        expert = found[0];
+        count = found[1];
+    }
     if (expert < 0) return;  // (fewer experts were chosen than there are workgroups for)
+    expert = __builtin_amdgcn_readfirstlane(expert);
 
     const int c = lane & 15, quad = lane >> 4, half = u & 1;
     const int kunits = (g.H + W::KU - 1) / W::KU;
@@ -281,67 +312,75 @@ __global__ __launch_bounds__(512) void moe_up_kernel(const MoeArgs g, int col_un
         w_at[j] = g.W + expert * g.expert_bytes + (int64_t)((u >> 1) * 2 + j) * g.panel_stride;
         s_at[j] = W::F8 ? g.scales + ((int64_t)expert * g.scale_rows + j * (g.scale_rows >> 1) + (u >> 3)) * kunits : nullptr;
     }
-    for (int i0 = 0; i0 < count; i0 += 32) {
-        const uint16_t* x_at[2];
+    for (int i0 = 0; i0 < count; i0 += 16 * MT) {
+        const uint16_t* x_at[MT];
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
+        for (int i = 0; i < MT; i++) {
             const int s = i0 + i * 16 + c;
             x_at[i] = g.x + (int64_t)(t0 + list[s < count ? s : count - 1] / g.k) * g.ldx;
         }
-        auto pass = [&](auto mt_c) __attribute__((always_inline)) {
-            constexpr int MT = decltype(mt_c)::value;
+        {
             f32x4 acc[MT][2];
 #pragma unroll
             for (int i = 0; i < MT; i++) acc[i][0] = acc[i][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            for (int ku = wave; ku < kunits; ku += NW) {
-                u32x4 w[2][W::LOADS];
+            auto units = [&](auto u_c, int ku0) __attribute__((always_inline)) {
+                constexpr int N = decltype(u_c)::value;
+                u32x4 w[N][2][W::LOADS];
+                float sc[N][2];
 #pragma unroll
-                for (int j = 0; j < 2; j++)
+                for (int v = 0; v < N; v++)
 #pragma unroll
-                    for (int l = 0; l < W::LOADS; l++)
-                        w[j][l] = *reinterpret_cast<const u32x4*>(w_at[j] + (int64_t)ku * 4096 + W::offset(l, quad, half * 16 + c));
-                bf16x8 x[MT][W::STEPS];
+                    for (int j = 0; j < 2; j++) {
 #pragma unroll
-                for (int i = 0; i < MT; i++)
-#pragma unroll
-                    for (int s = 0; s < W::STEPS; s++) x[i][s] = load8(x_at[i], ku * W::KU + W::k_of(s, quad), g.H);
-#pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    f32x4 p[MT];
-#pragma unroll
-                    for (int i = 0; i < MT; i++) p[i] = W::F8 ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : acc[i][j];
-#pragma unroll
-                    for (int s = 0; s < W::STEPS; s++) {
-                        const bf16x8 b = W::operand(w[j], s);
-#pragma unroll
-                        for (int i = 0; i < MT; i++) p[i] = mfma_bf16(b, x[i][s], p[i]);
+                        for (int l = 0; l < W::LOADS; l++)
+                            w[v][j][l] = *reinterpret_cast<const u32x4*>(w_at[j] + (int64_t)(ku0 + v * NW) * 4096 + W::offset(l, quad, half * 16 + c));
+                        sc[v][j] = W::F8 ? s_at[j][ku0 + v * NW] : 1.0f;
                     }
-                    if constexpr (W::F8) {
-                        const float sc = s_at[j][ku];
 #pragma unroll
-                        for (int i = 0; i < MT; i++)
+                for (int v = 0; v < N; v++) {
+                    const int k0 = (ku0 + v * NW) * W::KU;
+                    bf16x8 x[MT][W::STEPS];
 #pragma unroll
-                            for (int e = 0; e < 4; e++) acc[i][j][e] = __builtin_fmaf(p[i][e], sc, acc[i][j][e]);
-                    } else {
+                    for (int i = 0; i < MT; i++) load_steps<W>(x_at[i], k0, quad, g.H, k0 + W::KU <= g.H, x[i]);
 #pragma unroll
-                        for (int i = 0; i < MT; i++) acc[i][j] = p[i];
+                    for (int j = 0; j < 2; j++) {
+                        f32x4 p[MT];
+#pragma unroll
+                        for (int i = 0; i < MT; i++) p[i] = W::F8 ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : acc[i][j];
+#pragma unroll
+                        for (int s = 0; s < W::STEPS; s++) {
+                            const bf16x8 b = W::operand(w[v][j], s);
+#pragma unroll
+                            for (int i = 0; i < MT; i++) p[i] = mfma_bf16(b, x[i][s], p[i]);
+                        }
+#pragma unroll
+                        for (int i = 0; i < MT; i++) {
+                            if constexpr (W::F8) {
+#pragma unroll
+                                for (int e = 0; e < 4; e++) acc[i][j][e] = __builtin_fmaf(p[i][e], sc[v][j], acc[i][j][e]);
+                            } else {
+                                acc[i][j] = p[i];
+                            }
+                        }
                     }
                 }
-            }
+            };
+            int ku = wave;
+            for (; ku + (U - 1) * NW < kunits; ku += U * NW) units(std::integral_constant<int, U>{}, ku);
+            for (; ku < kunits; ku += NW) units(std::integral_constant<int, 1>{}, ku);
 #pragma unroll
             for (int i = 0; i < MT; i++) {
                 red[wave][2 * i][lane] = acc[i][0];
                 red[wave][2 * i + 1][lane] = acc[i][1];
             }
-        };
-        if (count - i0 > 16) pass(std::integral_constant<int, 2>{});
-        else pass(std::integral_constant<int, 1>{});
+        }
         __syncthreads();
         // 64 lanes per 16 tokens: tile i, lane l holds columns 4 (l / 16) + 0..3 of its token l % 16
-        if (threadIdx.x < 128) {
+        if (threadIdx.x < 64 * MT) {
             const int i = threadIdx.x >> 6, s = i0 + i * 16 + c;
             if (s < count) {
                 float gate[4] = {0, 0, 0, 0}, up[4] = {0, 0, 0, 0};
+#pragma unroll
                 for (int w = 0; w < NW; w++) {
                     const f32x4 a0 = red[w][2 * i][lane], a1 = red[w][2 * i + 1][lane];
 #pragma unroll
@@ -370,106 +409,189 @@ __global__ __launch_bounds__(512) void moe_up_kernel(const MoeArgs g, int col_un
     }
 }
 
-// Down: a workgroup takes 16 columns of the result for the group's tokens and walks all their experts, (expert, unit of k) in
-// turn per wavefront.  The MFMA's second side is the tokens themselves: one that did not choose the expert has zeros there, so all
-// experts' products add up in the same registers.  h enters as the sum of two bf16: rounded to one, its error would be as large
-// as that of the result's own rounding.
-template <typename W>
-__global__ __launch_bounds__(512) void moe_down_kernel(const MoeArgs g) {
-    constexpr int NW = 8, MT = 2;
-    __shared__ uint8_t flags[MOE_EXPERTS];
-    __shared__ uint16_t rank[MOE_EXPERTS];            // position of an expert among the chosen ones
-    __shared__ uint16_t expert_of[MOE_SLOTS];
-    __shared__ int16_t slot_of[MOE_SLOTS * MOE_GROUP];  // [chosen expert][token]: the token's slot, -1 for none
+// Down: a workgroup takes 16 columns of the result for the group's tokens.  A wavefront takes a part of an expert's k at a time, multiplies it with the rows of h of the slots that
+// chose the expert, and adds what comes out to its own copy of the tokens' 16 columns in LDS; at the end the copies are added in the order of the wavefronts, so the result
+// does not depend on who was first.  (With the second side of the MFMA the tokens themselves, those that did not choose the expert as rows of zeros, all experts add up in the
+// same registers, but the zeros have to be loaded: 32 tokens, 2 of 16 experts, 1000 x 1376, 39 us.)
+// h enters as the sum of two bf16: rounded to one, its error would be as large as that of the result's own rounding.  Sixteen wavefronts, each with the weights of U units on their way:
+// a narrow layer has columns for a part of the CUs only.
+template <typename W, int MT>  // MT: 16 tokens each
+__global__ __launch_bounds__(1024) void moe_down_kernel(const MoeArgs g) {
+    constexpr int NW = 16, TOKENS = 16 * MT, SLOTS = TOKENS * MOE_TOP_K, U = W::F8 ? 2 : 4;
+    constexpr uint16_t NONE = 0xffff;
+    __shared__ uint16_t named[SLOTS], expert_at[SLOTS];  // a slot's expert as it is named, and NONE for a slot that does not count
+    __shared__ uint16_t sorted[SLOTS], start[SLOTS + 1]; // the slots by expert, and where each expert's begin
+    __shared__ uint8_t begins[SLOTS];
     __shared__ int chosen;
-    __shared__ __attribute__((aligned(16))) f32x4 red[NW][MT][64];
+    __shared__ __attribute__((aligned(16))) float part[NW][TOKENS][16];
     const int t0 = blockIdx.y * MOE_GROUP, tokens = g.T - t0 < MOE_GROUP ? g.T - t0 : MOE_GROUP;
     const int first = t0 * g.k, n = tokens * g.k;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    mark_experts(g, first, n, flags);
-    if (wave == 0) {
-        int before = 0;
-        for (int e0 = 0; e0 < g.E; e0 += 64) {
-            const bool is = e0 + lane < g.E && flags[e0 + lane];
-            const uint64_t has = __builtin_amdgcn_ballot_w64(is);
-            if (is) {
-                const int at = before + __builtin_popcountll(has & ((1ull << lane) - 1));
-                rank[e0 + lane] = (uint16_t)at;
-                expert_of[at] = (uint16_t)(e0 + lane);
+    for (int i = threadIdx.x; i < n; i += NW * 64) {
+        const int e = g.ids[first + i];
+        named[i] = (unsigned)e < (unsigned)g.E ? (uint16_t)e : NONE;  // (-1 or anything else out of range: no expert)
+        begins[i] = 0;
+    }
+    for (int i = lane; i < TOKENS * 16; i += 64) (&part[wave][0][0])[i] = 0.0f;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += NW * 64) {
+        uint16_t e = named[i];
+        for (int o = i - i % g.k; o < i; o++)
+            if (named[o] == e) e = NONE;  // (its token has named it before: that slot has both weights)
+        expert_at[i] = e;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += NW * 64) {
+        const uint16_t e = expert_at[i];
+        if (e != NONE) {
+            int before = 0, same = 0;
+#pragma unroll 4
+            for (int o = 0; o < n; o++) {
+                const uint16_t other = expert_at[o];
+                before += other < e;
+                same += other == e && o < i;
             }
-            before += __builtin_popcountll(has);
+            sorted[before + same] = (uint16_t)i;
+            if (same == 0) begins[before] = 1;
         }
-        if (lane == 0) chosen = before;
+    }
+    __syncthreads();
+    if (wave == 0) {
+        int count = 0, valid = 0;
+        for (int i0 = 0; i0 < n; i0 += 64) {
+            const bool is = i0 + lane < n && begins[i0 + lane];
+            const uint64_t has = __builtin_amdgcn_ballot_w64(is);
+            if (is) start[count + __builtin_popcountll(has & ((1ull << lane) - 1))] = (uint16_t)(i0 + lane);
+            count += __builtin_popcountll(has);
+            valid += __builtin_popcountll(__builtin_amdgcn_ballot_w64(i0 + lane < n && expert_at[i0 + lane] != NONE));
+        }
+        if (lane == 0) {
+            start[count] = (uint16_t)valid;
+            chosen = count;
+        }
     }
     __syncthreads();
     const int experts = chosen;
-    for (int i = threadIdx.x; i < experts * MOE_GROUP; i += NW * 64) slot_of[i] = -1;
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += NW * 64) {
-        const int e = g.ids[first + i];
-        if ((unsigned)e < (unsigned)g.E && first_of_token(g.ids + first, i, g.k)) slot_of[rank[e] * MOE_GROUP + i / g.k] = (int16_t)i;
-    }
-    __syncthreads();
 
     const int c = lane & 15, quad = lane >> 4, u = blockIdx.x, half = u & 1;
     const int kunits = (g.I + W::KU - 1) / W::KU;
-    f32x4 acc[MT];
+    // parts of an expert's k: as many as give every wavefront four or more, of U units or more
+    int parts = experts > 0 ? (4 * NW * g.splits + experts - 1) / experts : 1;
+    if (parts > (kunits + U - 1) / U) parts = (kunits + U - 1) / U;
+    for (int item = blockIdx.z * NW + wave; item < experts * parts; item += NW * g.splits) {
+        const int a = item / parts, piece = item - a * parts;
+        const int begin = __builtin_amdgcn_readfirstlane((int)start[a]), end = __builtin_amdgcn_readfirstlane((int)start[a + 1]);
+        const int expert = __builtin_amdgcn_readfirstlane((int)expert_at[sorted[begin]]);
+        const char* const w_at = g.W + expert * g.expert_bytes + (int64_t)(u >> 1) * g.panel_stride;
+        const float* const s_at = W::F8 ? g.scales + ((int64_t)expert * g.scale_rows + (u >> 3)) * kunits : nullptr;
+        const int ku_end = (piece + 1) * kunits / parts;
+        for (int b = begin; b < end; b += 16) {
+            const bool live = b + c < end;
+            const int slot = sorted[live ? b + c : begin];
+            const uint16_t* const h = g.h + (int64_t)(first + slot) * 2 * g.I;
+            f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+            auto units = [&](auto u_c, int ku0) __attribute__((always_inline)) {
+                constexpr int N = decltype(u_c)::value;
+                u32x4 w[N][W::LOADS];
+                float sc[N];
+                bf16x8 hi[N][W::STEPS], lo[N][W::STEPS];
 #pragma unroll
-    for (int i = 0; i < MT; i++) acc[i] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int it = wave; it < experts * kunits; it += NW) {
-        const int a = it / kunits, ku = it - a * kunits, expert = expert_of[a];
-        const char* const w_at = g.W + expert * g.expert_bytes + (int64_t)(u >> 1) * g.panel_stride + (int64_t)ku * 4096;
-        u32x4 w[W::LOADS];
+                for (int v = 0; v < N; v++) {
 #pragma unroll
-        for (int l = 0; l < W::LOADS; l++) w[l] = *reinterpret_cast<const u32x4*>(w_at + W::offset(l, quad, half * 16 + c));
-        const float sc = W::F8 ? g.scales[((int64_t)expert * g.scale_rows + (u >> 3)) * kunits + ku] : 1.0f;
-#pragma unroll
-        for (int i = 0; i < MT; i++) {
-            if (i * 16 >= tokens) break;
-            const int slot = slot_of[a * MOE_GROUP + i * 16 + c];
-            const uint16_t* const h = g.h + (int64_t)(first + (slot < 0 ? 0 : slot)) * 2 * g.I;
-            f32x4 p = W::F8 ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : acc[i];
-#pragma unroll
-            for (int s = 0; s < W::STEPS; s++) {
-                const int at = ku * W::KU + W::k_of(s, quad);
-                bf16x8 hi = {0, 0, 0, 0, 0, 0, 0, 0}, lo = hi;
-                if (slot >= 0 && at < g.I) {  // (I is a multiple of 32: eight values are there or not)
-                    hi = load8(h, at, g.I);
-                    lo = load8(h + g.I, at, g.I);
+                    for (int l = 0; l < W::LOADS; l++)
+                        w[v][l] = *reinterpret_cast<const u32x4*>(w_at + (int64_t)(ku0 + v) * 4096 + W::offset(l, quad, half * 16 + c));
+                    sc[v] = W::F8 ? s_at[ku0 + v] : 1.0f;
                 }
-                const bf16x8 b = W::operand(w, s);
-                p = mfma_bf16(b, hi, p);
-                p = mfma_bf16(b, lo, p);
-            }
-            if constexpr (W::F8) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) acc[i][e] = __builtin_fmaf(p[e], sc, acc[i][e]);
-            } else {
-                acc[i] = p;
+                for (int v = 0; v < N; v++)
+#pragma unroll
+                    for (int s = 0; s < W::STEPS; s++) {
+                        const int at = (ku0 + v) * W::KU + W::k_of(s, quad);
+                        hi[v][s] = lo[v][s] = bf16x8{0, 0, 0, 0, 0, 0, 0, 0};
+                        if (live && at < g.I) {  // (I is a multiple of 32: eight values are there or not)
+                            hi[v][s] = *reinterpret_cast<const bf16x8*>(h + at);
+                            lo[v][s] = *reinterpret_cast<const bf16x8*>(h + g.I + at);
+                        }
+                    }
+#pragma unroll
+                for (int v = 0; v < N; v++) {
+                    f32x4 p = W::F8 ? f32x4{0.0f, 0.0f, 0.0f, 0.0f} : acc;
+#pragma unroll
+                    for (int s = 0; s < W::STEPS; s++) {
+                        const bf16x8 o = W::operand(w[v], s);
+                        p = mfma_bf16(o, hi[v][s], p);
+                        p = mfma_bf16(o, lo[v][s], p);
+                    }
+                    if constexpr (W::F8) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) acc[e] = __builtin_fmaf(p[e], sc[v], acc[e]);
+                    } else {
+                        acc = p;
+                    }
+                }
+            };
+            int ku = piece * kunits / parts;
+            for (; ku + U <= ku_end; ku += U) units(std::integral_constant<int, U>{}, ku);
+            for (; ku < ku_end; ku++) units(std::integral_constant<int, 1>{}, ku);
+            if (live) {
+                f32x4* const to = reinterpret_cast<f32x4*>(&part[wave][slot / g.k][quad * 4]);
+                f32x4 sum = *to;
+#pragma unroll
+                for (int e = 0; e < 4; e++) sum[e] += acc[e];
+                *to = sum;
             }
         }
     }
-#pragma unroll
-    for (int i = 0; i < MT; i++) red[wave][i][lane] = acc[i];
     __syncthreads();
-    if (threadIdx.x < 128) {
-        const int t = (threadIdx.x >> 6) * 16 + c, n0 = u * 16 + quad * 4;
+    if (threadIdx.x < TOKENS * 4) {
+        const int t = threadIdx.x >> 2, n0 = u * 16 + (threadIdx.x & 3) * 4;
         if (t < tokens) {
             float r[4] = {0, 0, 0, 0};
+#pragma unroll
             for (int w = 0; w < NW; w++) {
-                const f32x4 v = red[w][threadIdx.x >> 6][lane];
+                const f32x4 v = *reinterpret_cast<const f32x4*>(&part[w][t][(threadIdx.x & 3) * 4]);
 #pragma unroll
                 for (int e = 0; e < 4; e++) r[e] += v[e];
             }
             char* const row = g.y + (int64_t)(t0 + t) * g.ldy;
+            float* const to = g.parts ? g.parts + ((int64_t)blockIdx.z * g.T + t0 + t) * g.H : reinterpret_cast<float*>(row);
 #pragma unroll
             for (int e = 0; e < 4; e++) {
                 if (n0 + e >= g.H) break;
-                if (g.y_f32) reinterpret_cast<float*>(row)[n0 + e] = r[e];
+                if (g.parts || g.y_f32) to[n0 + e] = r[e];
                 else reinterpret_cast<uint16_t*>(row)[n0 + e] = to_bf16(r[e]);
             }
         }
     }
+}
+
+// y = the splits' sums, in their order
+__global__ __launch_bounds__(256) void moe_add_kernel(const MoeArgs g) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, all = (int64_t)g.T * g.H;
+    if (i >= all) return;
+    float v[MOE_SPLITS];
+#pragma unroll
+    for (int z = 0; z < MOE_SPLITS; z++) v[z] = z < g.splits ? g.parts[z * all + i] : 0.0f;
+    float sum = v[0];
+#pragma unroll
+    for (int z = 1; z < MOE_SPLITS; z++) sum += v[z];
+    const int64_t t = i / g.H;
+    char* const row = g.y + t * g.ldy;
+    if (g.y_f32) reinterpret_cast<float*>(row)[i - t * g.H] = sum;
+    else reinterpret_cast<uint16_t*>(row)[i - t * g.H] = to_bf16(sum);
+}
+
+// Into how many workgroups the down products of 16 columns are split: a narrow layer's columns are a workgroup each for a part of the CUs only.  The sums then go through memory
+// and one more launch, which has to be worth it (32 tokens, 2 of 16 experts, 1000 x 1376: 30.5 us whole,
+// 16.7 + 2.5 in four; of 2048 columns, 128 workgroups, the whole kernel takes 11 us for 33 MB).
+static int moe_splits(int T, int H) {
+    const int64_t tiles = (int64_t)((H + 15) / 16) * ((T + MOE_GROUP - 1) / MOE_GROUP), cus = num_cus();
+    return tiles * 3 > cus ? 1 : tiles * MOE_SPLITS <= cus ? MOE_SPLITS : 2;
+}
+static size_t moe_h_bytes(int T, int I, int k) { return ((size_t)T * k * 2 * I * 2 + 255) & ~(size_t)255; }
+size_t moe_scratch_bytes(int T, int H, int I, int k) {
+    const int splits = moe_splits(T, H);
+    return moe_h_bytes(T, I, k) + (splits > 1 ? (size_t)splits * T * H * 4 : 0);
 }
 
 int launch_moe_experts(bool f8, const void* x, int64_t ldx_bytes, const int* ids, const float* weights, int T, int H, int I, int E, int k,
@@ -495,7 +617,8 @@ int launch_moe_experts(bool f8, const void* x, int64_t ldx_bytes, const int* ids
     g.expert_bytes = g.panel_stride * (I / 32 * 2);
     g.scales = s_gate_up;
     g.scale_rows = 2 * ((I + 127) / 128);
-    hipLaunchKernelGGL((f8 ? moe_up_kernel<W_fp8> : moe_up_kernel<W_bf16>), dim3((unsigned)grid, groups), dim3(512), 0, st, g, units);
+    const auto up = T <= 16 ? (f8 ? moe_up_kernel<W_fp8, 1> : moe_up_kernel<W_bf16, 1>) : f8 ? moe_up_kernel<W_fp8, 2> : moe_up_kernel<W_bf16, 2>;
+    hipLaunchKernelGGL(up, dim3((unsigned)grid, groups), dim3(512), 0, st, g, units);
     int rc = check_hip(hipGetLastError(), "moe_up_kernel launch");
     if (rc) return rc;
     g.W = static_cast<const char*>(w_down);
@@ -503,8 +626,14 @@ int launch_moe_experts(bool f8, const void* x, int64_t ldx_bytes, const int* ids
     g.expert_bytes = g.panel_stride * ((H + 31) / 32);
     g.scales = s_down;
     g.scale_rows = (H + 127) / 128;
-    hipLaunchKernelGGL((f8 ? moe_down_kernel<W_fp8> : moe_down_kernel<W_bf16>), dim3((unsigned)((H + 15) / 16), groups), dim3(512), 0, st, g);
-    return check_hip(hipGetLastError(), "moe_down_kernel launch");
+    g.splits = moe_splits(T, H);
+    g.parts = g.splits > 1 ? reinterpret_cast<float*>(static_cast<char*>(h) + moe_h_bytes(T, I, k)) : nullptr;
+    const auto down = T <= 16 ? (f8 ? moe_down_kernel<W_fp8, 1> : moe_down_kernel<W_bf16, 1>) : f8 ? moe_down_kernel<W_fp8, 2> : moe_down_kernel<W_bf16, 2>;
+    hipLaunchKernelGGL(down, dim3((unsigned)((H + 15) / 16), groups, (unsigned)g.splits), dim3(1024), 0, st, g);
+    rc = check_hip(hipGetLastError(), "moe_down_kernel launch");
+    if (rc || g.splits == 1) return rc;
+    hipLaunchKernelGGL(moe_add_kernel, dim3((unsigned)(((int64_t)T * H + 255) / 256)), dim3(256), 0, st, g);
+    return check_hip(hipGetLastError(), "moe_add_kernel launch");
 }
 
 }  // namespace mmx

@@ -301,9 +301,10 @@ def moe_experts(x, ids, weights, gate_up, down, E, I, y=None):
     if T == 0:
         return y
     k = ids.shape[1]
-    h = torch.empty(T * k * 2 * I, dtype=torch.bfloat16, device=x.device)
-    L._check(L.lib().mmx_moe_experts(L.F8 if f8 else L.BF16, x.data_ptr(), _rows(x), ids.data_ptr(), weights.data_ptr(), T, H, I, E, k, *parts, h.data_ptr(),
-                                     L.dtype_code(y), y.data_ptr(), _rows(y), L._stream()))
+    need = L.lib().mmx_moe_experts_scratch_bytes(T, H, I, k)
+    scratch = _scratch(need, x.device)
+    L._check(L.lib().mmx_moe_experts(L.F8 if f8 else L.BF16, x.data_ptr(), _rows(x), ids.data_ptr(), weights.data_ptr(), T, H, I, E, k, *parts,
+                                     L.dtype_code(y), y.data_ptr(), _rows(y), scratch.data_ptr(), need, L._stream()))
     return y
 
 

@@ -76,9 +76,11 @@ def test_experts(lib):
                       (dict(H=0), "positive"), (dict(T=-1), "negative")):
         refused(route(**bad), word)
     assert route(T=0) == 0
-    ex = lambda **k: lib.mmx_moe_experts(*{**dict(dt=1, x=P, ldx=256, ids=P, w=P, T=4, H=128, I=64, E=8, k=2, gu=P, gs=None, d=P, ds=None, h=P, yt=1, y=P, ldy=256, st=None), **k}.values())  # noqa: E731
+    need = lib.mmx_moe_experts_scratch_bytes(4, 128, 64, 2)
+    assert need >= 4 * 2 * 2 * 64 * 2 and lib.mmx_moe_experts_scratch_bytes(0, 128, 64, 2) == 0
+    ex = lambda **k: lib.mmx_moe_experts(*{**dict(dt=1, x=P, ldx=256, ids=P, w=P, T=4, H=128, I=64, E=8, k=2, gu=P, gs=None, d=P, ds=None, yt=1, y=P, ldy=256, scratch=P, n=need, st=None), **k}.values())  # noqa: E731
     for bad, word in ((dict(dt=2), "dtype"), (dict(I=40), "32"), (dict(I=0), "positive"), (dict(E=0), "experts"), (dict(k=17), "top_k"), (dict(yt=2), "dtype"), (dict(x=None), "NULL"),
-                      (dict(ldy=254), "apart"), (dict(ids=None), "NULL"), (dict(h=P + 8), "16 bytes"), (dict(gu=P + 8), "16 bytes"), (dict(dt=6), "scales"), (dict(gs=P, ds=P), "scales"),
+                      (dict(ldy=254), "apart"), (dict(ids=None), "NULL"), (dict(n=need - 1), "scratch"), (dict(scratch=P + 128), "256-byte"), (dict(gu=P + 8), "16 bytes"), (dict(dt=6), "scales"), (dict(gs=P, ds=P), "scales"),
                       (dict(dt=6, gs=P, ds=P + 2), "aligned")):
         refused(ex(**bad), word)
     assert ex(T=0) == 0

@@ -113,7 +113,7 @@ def test_route_with_nan_stays_in_range():
 
 # ---- experts -----------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("T,H,I,E,k", [(1, 64, 32, 1, 1), (1, 1000, 96, 8, 3), (3, 129, 32, 5, 2), (8, 512, 160, 16, 4), (16, 256, 64, 3, 2), (17, 300, 288, 4, 4), (32, 130, 96, 2, 1),
-                                      (33, 264, 128, 8, 2), (70, 100, 64, 6, 3), (5, 33, 416, 40, 16)])
+                                      (33, 264, 128, 8, 2), (70, 100, 64, 6, 3), (5, 33, 416, 40, 16), (2, 2064, 64, 4, 2), (20, 1200, 96, 5, 2)])
 @pytest.mark.parametrize("f8", [False, True])
 def test_experts(T, H, I, E, k, f8):
     moe, full = layer(E, H, I, f8, min(k, E))

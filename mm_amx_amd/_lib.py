@@ -73,7 +73,8 @@ def _host_module(l):
     _host_call.bind(*(C.cast(f, C.c_void_p).value for f in (
         l.mmx_gemm_splitk, l.mmx_gemm_workspace_bytes, l.mmx_gemm_unpacked, l.mmx_gemm_unpacked_workspace_bytes, l.mmx_matvec,
         l.mmx_packed_b_bytes, l.mmx_repack_b, l.mmx_quantize_weights_scratch, l.mmx_quantize_weights_scaled, l.mmx_quantize_pack_int4,
-        l.mmx_quantize_pack_scaled)))
+        l.mmx_quantize_pack_scaled, l.mmx_quantize_rows_fp8, l.mmx_gemm_fp8_scratch_bytes, l.mmx_gemm_fp8, l.mmx_mlp_fp8_scratch_bytes, l.mmx_mlp_fp8,
+        l.mmx_moe_route, l.mmx_moe_experts_scratch_bytes, l.mmx_moe_experts, l.mmx_block_norm)))
     return _host_call
 
 
@@ -236,12 +237,12 @@ def _column_operand(v, name):
         raise MmxError(f"{name} must be a contiguous fp32 tensor on the GPU")
 
 
-def _made(native, *args):
-    """What a native packing or quantising call on the current GPU has made; None: not a regular call, nothing was done."""
+def _made(native, *args, at_end=()):
+    """What a native call on the current GPU has made (0 for one that makes nothing); None: not a regular call, nothing was done."""
     device = _current_device()
     if device not in _initialised:
         return None
-    made = native(*args, device, _raw_stream(device))
+    made = native(*args, device, _raw_stream(device), *at_end)
     if type(made) is int:
         _check(made)
     return made

@@ -3,7 +3,7 @@
 //
 // What bounds a small product is the host: the same checks as Python statements, the descriptor as a ctypes structure, the query
 // of the workspace and the call through ctypes took 9.7 us for 256 x 256 x 256, under 4 us of which are on the device; 4.7 now.
-// (One decode row over 512 x 512 int4 weights 9.2 -> 4.2, a 64 x 512 x 512 layer with a bias 10.2 -> 5.2.)  The functions below
+// (A norm of one row 16.7 -> BN, a linear layer in e4m3 LIN, one decode row over 512 x 512 int4 weights 9.2 -> 4.2, a 64 x 512 x 512 layer with a bias 10.2 -> 5.2.)  The functions below
 // take the calls that are regular in every respect - tensors of exactly torch's own type on one GPU, the current one, everything
 // large enough - and leave all others to the Python form (they return None, and have done nothing), which accepts them or says
 // what is wrong.  They keep nothing from one call for the next.
@@ -390,11 +390,273 @@ PyObject* quantize_pack_int4(PyObject*, PyObject* const* a, Py_ssize_t count) {
     }
 }
 
-// bind(addresses of the eleven entry points, in the order below)
+// ---- the feed-forward block in 8-bit floating point ----------------------------------------------------------------------
+decltype(&mmx_quantize_rows_fp8) call_quantize_rows = nullptr;
+decltype(&mmx_gemm_fp8_scratch_bytes) call_gemm_fp8_need = nullptr;
+decltype(&mmx_gemm_fp8) call_gemm_fp8 = nullptr;
+decltype(&mmx_mlp_fp8_scratch_bytes) call_mlp_fp8_need = nullptr;
+decltype(&mmx_mlp_fp8) call_mlp_fp8 = nullptr;
+decltype(&mmx_moe_route) call_moe_route = nullptr;
+decltype(&mmx_moe_experts_scratch_bytes) call_moe_need = nullptr;
+decltype(&mmx_moe_experts) call_moe_experts = nullptr;
+decltype(&mmx_block_norm) call_block_norm = nullptr;
+
+int64_t blocks(int64_t n) { return (n + 127) / 128; }
+
+int float_code(const at::Tensor& t) {  // bf16 or fp32
+    const int c = code_of(t.scalar_type());
+    if (c != MMX_BF16 && c != MMX_F32) throw Leave();
+    return c;
+}
+
+const float* floats(PyObject* o, int device, at::IntArrayRef sizes) {
+    const at::Tensor& t = tensor_on(o, device);
+    if (t.scalar_type() != at::kFloat || !t.is_contiguous() || t.sizes() != sizes) throw Leave();
+    return static_cast<const float*>(t.mutable_data_ptr());
+}
+
+const void* packed_bytes(PyObject* o, int device, int64_t need) {
+    const at::Tensor& t = tensor_on(o, device);
+    void* const p = t.mutable_data_ptr();
+    if (t.scalar_type() != at::kByte || t.dim() != 1 || !t.is_contiguous() || t.numel() < need || (reinterpret_cast<uintptr_t>(p) & 15)) throw Leave();
+    return p;
+}
+int64_t packed_e4m3(int64_t K, int64_t N) { return (N + 31) / 32 * 32 * blocks(K) * 128; }
+
+// Activations: (bf16 or fp32 rows, None, K), or the padded rows, the scales and K of quantised ones
+struct Activations {
+    const at::Tensor* t;
+    int dtype, M, K;
+    const void* data;
+    int64_t ld, ld_scales;
+    const float* scales;
+};
+Activations activations(PyObject* const* a, int device) {
+    const Matrix x = matrix(a[0], device);
+    Activations r = {x.t, 0, x.rows, 0, x.data, x.ld, 0, nullptr};
+    if (!whole_number(a[2], 1, 1 << 30, r.K)) throw Leave();
+    if (a[1] == Py_None) {
+        r.dtype = float_code(*x.t);
+        if (x.cols != r.K) throw Leave();
+        return r;
+    }
+    r.dtype = MMX_F8;
+    const at::Tensor& s = tensor_on(a[1], device);
+    if (x.t->scalar_type() != at::kFloat8_e4m3fn || x.cols != blocks(r.K) * 128 || s.scalar_type() != at::kFloat || s.dim() != 2 || s.size(0) != blocks(r.K) ||
+        s.size(1) != r.M || (s.stride(1) != 1 && r.M != 1)) throw Leave();
+    r.scales = static_cast<const float*>(s.mutable_data_ptr());
+    r.ld_scales = s.size(0) <= 1 ? r.M : s.stride(0);
+    return r;
+}
+
+// a result [M, N] in bf16 or fp32: the caller's, or made here in bf16
+at::Tensor result(PyObject* o, int device, int64_t M, int64_t N, const at::Tensor& like) {
+    if (o == Py_None) return make({M, N}, at::kBFloat16, like);
+    const at::Tensor& y = tensor_on(o, device);
+    if (y.dim() != 2 || y.size(0) != M || y.size(1) != N) throw Leave();
+    float_code(y);
+    return y;
+}
+
+// quantize_fp8(x, device, stream) -> (padded rows, scales)
+PyObject* quantize_fp8(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    if (count != 3 || !call_quantize_rows) Py_RETURN_NONE;
+    try {
+        int device, rc = 0;
+        if (!whole_number(a[1], 0, 1 << 20, device)) throw Leave();
+        const Matrix x = matrix(a[0], device);
+        const int dt = float_code(*x.t);
+        void* const stream = stream_of(a[2]);
+        at::Tensor q, s;
+        if (!unlocked([&] {
+                const int64_t n = blocks(x.cols) * 128;
+                q = make({x.rows, n % 2048 ? n : n + 128}, at::kFloat8_e4m3fn, *x.t).narrow(1, 0, n);
+                s = make({blocks(x.cols), x.rows}, at::kFloat, *x.t);
+                rc = call_quantize_rows(dt, x.data, x.ld, x.rows, x.cols, q.mutable_data_ptr(), q.stride(0), static_cast<float*>(s.mutable_data_ptr()), x.rows, stream);
+            })) throw Leave();
+        return rc ? PyLong_FromLong(rc) : Py_BuildValue("(NN)", THPVariable_Wrap(q), THPVariable_Wrap(s));
+    } catch (...) {
+        Py_RETURN_NONE;
+    }
+}
+
+// gemm_fp8(x, x_scales, K, packed, scales, N, device, stream, C, steps, bias, deq, deq_per_oc, q, q_per_oc)
+PyObject* gemm_fp8(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    if (count != 15 || !call_gemm_fp8) Py_RETURN_NONE;
+    int rc = 0;
+    try {
+        int N, device;
+        if (!whole_number(a[6], 0, 1 << 20, device) || !whole_number(a[5], 1, 1 << 30, N)) throw Leave();
+        const Activations x = activations(a, device);
+        const mmx_epilogue e = epilogue_of(a + 8, device, x.M, N);
+        const bool pair = e.steps & MMX_PP_SILU_GATE;
+        const at::Tensor& C = tensor_on(a[8], device);
+        if (C.size(0) != x.M || C.size(1) != (pair ? N / 2 : N) || (a[10] != Py_None && tensor_on(a[10], device).numel() != N)) throw Leave();
+        const void* const w = packed_bytes(a[3], device, packed_e4m3(x.K, N));
+        const float* const s = floats(a[4], device, {pair ? 2 * blocks(N / 2) : blocks(N), blocks(x.K)});
+        void* const stream = stream_of(a[7]);
+        if (!unlocked([&] {
+                const size_t need = call_gemm_fp8_need(x.dtype, x.M, x.K, N);
+                at::Tensor scratch;
+                if (need) scratch = make({(int64_t)need}, at::kByte, *x.t);
+                rc = call_gemm_fp8(x.dtype, x.data, x.ld, x.scales, x.ld_scales, w, s, x.M, x.K, N, &e, need ? scratch.mutable_data_ptr() : nullptr, need, stream);
+            })) throw Leave();
+    } catch (...) {
+        Py_RETURN_NONE;
+    }
+    return PyLong_FromLong(rc);
+}
+
+// mlp_fp8(x, x_scales, K, gate_up, gate_up_scales, down, down_scales, N, y, device, stream) -> y
+PyObject* mlp_fp8(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    if (count != 11 || !call_mlp_fp8) Py_RETURN_NONE;
+    try {
+        int N, device, rc = 0;
+        if (!whole_number(a[9], 0, 1 << 20, device) || !whole_number(a[7], 1, 1 << 29, N) || N % 32) throw Leave();
+        const Activations x = activations(a, device);
+        const void* const gu = packed_bytes(a[3], device, packed_e4m3(x.K, 2 * (int64_t)N));
+        const float* const gus = floats(a[4], device, {2 * blocks(N), blocks(x.K)});
+        const void* const d = packed_bytes(a[5], device, packed_e4m3(N, x.K));
+        const float* const ds = floats(a[6], device, {blocks(x.K), blocks(N)});
+        void* const stream = stream_of(a[10]);
+        at::Tensor y;
+        if (!unlocked([&] {
+                y = result(a[8], device, x.M, x.K, *x.t);
+                const size_t need = call_mlp_fp8_need(x.dtype, x.M, x.K, N);
+                const at::Tensor scratch = make({(int64_t)need}, at::kByte, *x.t);
+                rc = call_mlp_fp8(x.dtype, x.data, x.ld, x.scales, x.ld_scales, gu, gus, d, ds, code_of(y.scalar_type()), y.mutable_data_ptr(), row_stride_bytes(y), x.M, x.K, N,
+                                  scratch.mutable_data_ptr(), need, stream);
+            })) throw Leave();
+        return rc ? PyLong_FromLong(rc) : THPVariable_Wrap(y);
+    } catch (...) {
+        Py_RETURN_NONE;
+    }
+}
+
+// moe(x, router, bias, top_k, flags, scale, gate_up, gate_up_scales, down, down_scales, I, y, device, stream) -> y: routing and experts
+PyObject* moe(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    if (count != 14 || !call_moe_route || !call_moe_experts) Py_RETURN_NONE;
+    try {
+        int k, flags, I, device, rc = 0;
+        if (!whole_number(a[12], 0, 1 << 20, device) || !whole_number(a[3], 1, 16, k) || !whole_number(a[4], 0, 3, flags) || !PyFloat_CheckExact(a[5]) ||
+            !whole_number(a[10], 32, 1 << 29, I) || I % 32) throw Leave();
+        const Matrix x = matrix(a[0], device), router = matrix(a[1], device);
+        const int T = x.rows, H = x.cols, E = router.rows;
+        if (x.t->scalar_type() != at::kBFloat16 || router.t->scalar_type() != at::kBFloat16 || router.cols != H || E > 1024 || k > E) throw Leave();
+        const float scale = (float)PyFloat_AS_DOUBLE(a[5]);
+        const float* const bias = a[2] == Py_None ? nullptr : floats(a[2], device, {E});
+        const bool f8 = a[7] != Py_None;
+        const auto bytes = [&](int64_t K, int64_t N) { return f8 ? packed_e4m3(K, N) : (N + 31) / 32 * 32 * ((K * 2 + 127) / 128 * 128); };
+        const void* const gu = packed_bytes(a[6], device, E * bytes(H, 2 * (int64_t)I));
+        const void* const d = packed_bytes(a[8], device, E * bytes(I, H));
+        const float* const gus = f8 ? floats(a[7], device, {E, 2 * blocks(I), blocks(H)}) : nullptr;
+        const float* const ds = f8 ? floats(a[9], device, {E, blocks(H), blocks(I)}) : nullptr;
+        if (!f8 && a[9] != Py_None) throw Leave();
+        void* const stream = stream_of(a[13]);
+        at::Tensor y;
+        if (!unlocked([&] {
+                y = result(a[11], device, T, H, *x.t);
+                const auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
+                const size_t logits = up((size_t)T * E * 8), ids = up((size_t)T * k * 4), need = call_moe_need(T, H, I, k);
+                const at::Tensor memory = make({(int64_t)(logits + 2 * ids + need)}, at::kByte, *x.t);
+                char* const at = static_cast<char*>(memory.mutable_data_ptr());
+                int32_t* const chosen = reinterpret_cast<int32_t*>(at + logits);
+                float* const weights = reinterpret_cast<float*>(at + logits + ids);
+                rc = call_moe_route(x.data, x.ld, router.data, router.ld, T, H, E, k, flags, scale, bias, reinterpret_cast<double*>(at), chosen, weights, stream);
+                if (!rc)
+                    rc = call_moe_experts(f8 ? MMX_F8 : MMX_BF16, x.data, x.ld, chosen, weights, T, H, I, E, k, gu, gus, d, ds, code_of(y.scalar_type()), y.mutable_data_ptr(),
+                                          row_stride_bytes(y), at + logits + 2 * ids, need, stream);
+            })) throw Leave();
+        return rc ? PyLong_FromLong(rc) : THPVariable_Wrap(y);
+    } catch (...) {
+        Py_RETURN_NONE;
+    }
+}
+
+// block_norm(f, residual, post, post_weight, gate, scale, pre, pre_weight, eps, offset, quantize, r, device, stream) -> (r, z) or (r, padded rows of z, scales)
+PyObject* block_norm(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    if (count != 14 || !call_block_norm) Py_RETURN_NONE;
+    try {
+        int device, rc = 0;
+        if (!whole_number(a[12], 0, 1 << 20, device) || !PyBool_Check(a[2]) || !PyBool_Check(a[6]) || !PyBool_Check(a[10]) || !PyFloat_CheckExact(a[5]) ||
+            !PyFloat_CheckExact(a[8]) || !PyFloat_CheckExact(a[9])) throw Leave();
+        const Matrix f = matrix(a[0], device);
+        const int64_t M = f.rows, H = f.cols;
+        if (f.t->scalar_type() != at::kBFloat16) throw Leave();
+        mmx_block_norm_args n = {};
+        n.f = f.data;
+        n.ldf_bytes = f.ld;
+        n.residual_dtype = MMX_BF16;
+        const auto same = [&](PyObject* o) {
+            const Matrix m = matrix(o, device);
+            if (m.rows != M || m.cols != H) throw Leave();
+            return m;
+        };
+        if (a[1] != Py_None) {
+            const Matrix m = same(a[1]);
+            n.residual_dtype = float_code(*m.t);
+            n.residual = m.data;
+            n.ld_residual_bytes = m.ld;
+        }
+        const auto vector = [&](PyObject* o) -> const void* {
+            if (o == Py_None) return nullptr;
+            const at::Tensor& t = tensor_on(o, device);
+            if (t.scalar_type() != at::kBFloat16 || t.dim() != 1 || t.numel() != H || !t.is_contiguous()) throw Leave();
+            return t.mutable_data_ptr();
+        };
+        n.post = a[2] == Py_True;
+        n.post_weight = vector(a[3]);
+        n.pre = a[6] == Py_True;
+        n.pre_weight = vector(a[7]);
+        if ((n.post_weight && !n.post) || (n.pre_weight && !n.pre)) throw Leave();
+        if (a[4] != Py_None && tensor_on(a[4], device).dim() == 2) {
+            const Matrix m = same(a[4]);
+            if (m.t->scalar_type() != at::kBFloat16) throw Leave();
+            n.gate = m.data;
+            n.ld_gate_bytes = M == 1 ? 0 : m.ld;
+        } else {
+            n.gate = vector(a[4]);
+        }
+        n.scale = (float)PyFloat_AS_DOUBLE(a[5]);
+        n.eps = (float)PyFloat_AS_DOUBLE(a[8]);
+        n.weight_offset = (float)PyFloat_AS_DOUBLE(a[9]);
+        const bool quantize = a[10] == Py_True;
+        const at::ScalarType stream_type = n.residual_dtype == MMX_F32 ? at::kFloat : at::kBFloat16;
+        if (a[11] != Py_None && same(a[11]).t->scalar_type() != stream_type) throw Leave();
+        void* const stream = stream_of(a[13]);
+        at::Tensor r, z, s;
+        if (!unlocked([&] {
+                r = a[11] == Py_None ? make({M, H}, stream_type, *f.t) : THPVariable_Unpack(a[11]);
+                n.r = r.mutable_data_ptr();
+                n.ldr_bytes = row_stride_bytes(r);
+                if (quantize) {
+                    const int64_t p = blocks(H) * 128;
+                    z = make({M, p % 2048 ? p : p + 128}, at::kFloat8_e4m3fn, *f.t).narrow(1, 0, p);
+                    s = make({blocks(H), M}, at::kFloat, *f.t);
+                    n.z_scales = static_cast<float*>(s.mutable_data_ptr());
+                    n.ld_z_scales = M;
+                    n.z_dtype = MMX_F8;
+                    n.ldz_bytes = z.stride(0);
+                } else {
+                    z = make({M, H}, at::kBFloat16, *f.t);
+                    n.z_dtype = MMX_BF16;
+                    n.ldz_bytes = 2 * H;
+                }
+                n.z = z.mutable_data_ptr();
+                rc = call_block_norm(&n, (int)M, (int)H, stream);
+            })) throw Leave();
+        if (rc) return PyLong_FromLong(rc);
+        return quantize ? Py_BuildValue("(NNN)", THPVariable_Wrap(r), THPVariable_Wrap(z), THPVariable_Wrap(s)) : Py_BuildValue("(NN)", THPVariable_Wrap(r), THPVariable_Wrap(z));
+    } catch (...) {
+        Py_RETURN_NONE;
+    }
+}
+
+// bind(addresses of the twenty entry points, in the order below)
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t count) {
-    constexpr int ENTRIES = 11;
+    constexpr int ENTRIES = 20;
     if (count != ENTRIES) {
-        PyErr_SetString(PyExc_TypeError, "bind takes eleven addresses");
+        PyErr_SetString(PyExc_TypeError, "bind takes twenty addresses");
         return nullptr;
     }
     void* at[ENTRIES];
@@ -413,12 +675,22 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t count) {
     set(call_quantize_scaled);
     set(call_quantize_int4);
     set(call_quantize_pack_scaled);
+    set(call_quantize_rows);
+    set(call_gemm_fp8_need);
+    set(call_gemm_fp8);
+    set(call_mlp_fp8_need);
+    set(call_mlp_fp8);
+    set(call_moe_route);
+    set(call_moe_need);
+    set(call_moe_experts);
+    set(call_block_norm);
     Py_RETURN_NONE;
 }
 
 #define METHOD(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {METHOD(gemm), METHOD(gemm_unpacked), METHOD(gemm_packing), METHOD(matvec), METHOD(repack), METHOD(quantize), METHOD(quantize_scaled),
-                         METHOD(quantize_pack_int4), METHOD(quantize_pack_scaled), METHOD(bind), {nullptr, nullptr, 0, nullptr}};
+                         METHOD(quantize_pack_int4), METHOD(quantize_pack_scaled), METHOD(quantize_fp8),
+                         METHOD(gemm_fp8), METHOD(mlp_fp8), METHOD(moe), METHOD(block_norm), METHOD(bind), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host_call", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -104,6 +104,10 @@ class Fp8Rows:
 def quantize_fp8(x):
     """x [M, K] bf16 or fp32 -> Fp8Rows: a scale for each row and 128 of k, the least power of two with which the block's largest magnitude is
     at most 448."""
+    if L._native is not None and L._initialised:  # (regular calls; None: not one, nothing was done)
+        made = L._made(L._native.quantize_fp8, x)
+        if made is not None:
+            return Fp8Rows(made[0], made[1], x.shape[1])
     _gpu(x, "x", (torch.bfloat16, torch.float32), 2)
     M, K = x.shape
     if K == 0:
@@ -184,6 +188,10 @@ def _activations(x, what):
     return L.dtype_code(x), x.shape[0], x.shape[1], x.data_ptr(), _rows(x), None, 0
 
 
+def _native_activations(x):
+    return (x.padded, x.scales, x.K) if type(x) is Fp8Rows else (x, None, x.shape[1])
+
+
 def _packed(p, s, what, K, N, rows):
     _gpu(p, what, (torch.uint8,), 1)
     _gpu(s, f"{what}'s scales", (torch.float32,), 2)
@@ -207,6 +215,10 @@ def gemm_fp8(A, Bpacked, b_scales, N, ep):
     ep: PP_BIAS, PP_GELU or both, or PP_SILU_GATE alone, into bf16 or fp32."""
     if not isinstance(ep, L.Epilogue):
         raise MmxError("ep must be an Epilogue")
+    if L._native is not None and L._initialised and len(getattr(A, "shape", ())) == 2:
+        rc = L._made(L._native.gemm_fp8, *_native_activations(A), Bpacked, b_scales, N, at_end=(ep.C, ep.steps, ep.bias, ep.deq, ep.deq_oc, ep.q, ep.q_oc))
+        if rc is not None:
+            return
     if not isinstance(N, int) or N <= 0:
         raise MmxError(f"N = {N} must be a positive int")
     dt, M, K, a, lda, s, ld_s = _activations(A, "A")
@@ -230,6 +242,10 @@ def gemm_fp8(A, Bpacked, b_scales, N, ep):
 def mlp_fp8(x, gate_up, down, N, y=None):
     """y = (silu(x . gate) * (x . up)) . down over e4m3 weights: x [M, K] as in gemm_fp8; gate_up, down: (packed, scales) pairs of pack_gate_up_fp8 and of
     pack_fp8 of the [K, N] down_proj weight.  y [M, K] bf16 or fp32 (default: a new bf16 tensor)."""
+    if L._native is not None and L._initialised and len(getattr(x, "shape", ())) == 2:
+        made = L._made(L._native.mlp_fp8, *_native_activations(x), *gate_up, *down, N, y)
+        if made is not None:
+            return made
     if not isinstance(N, int) or N <= 0 or N % 32:
         raise MmxError("N must be a positive multiple of 32")
     dt, M, K, a, lda, s, ld_s = _activations(x, "x")
@@ -269,6 +285,17 @@ def moe_route(x, router, top_k, scoring="softmax", renormalize=True, scale=1.0, 
         L._check(L.lib().mmx_moe_route(x.data_ptr(), _rows(x), router.data_ptr(), _rows(router), T, H, E, top_k, _SCORING[scoring] | (_RENORMALIZE if renormalize else 0),
                                        scale, _ptr(bias), logits.data_ptr(), ids.data_ptr(), weights.data_ptr(), L._stream()))
     return ids, weights
+
+
+def moe(x, router, top_k, gate_up, down, I, scoring="softmax", renormalize=True, scale=1.0, bias=None, y=None):
+    """moe_route and moe_experts of its choices: a whole layer."""
+    if L._native is not None and L._initialised and scoring in _SCORING:
+        made = L._made(L._native.moe, x, router, bias, top_k, _SCORING[scoring] | (_RENORMALIZE if renormalize else 0), scale,
+                       *(gate_up if type(gate_up) is tuple else (gate_up, None)), *(down if type(down) is tuple else (down, None)), I, y)
+        if made is not None:
+            return made
+    ids, weights = moe_route(x, router, top_k, scoring, renormalize, scale, bias)
+    return moe_experts(x, ids, weights, gate_up, down, router.shape[0], I, y=y)
 
 
 def moe_experts(x, ids, weights, gate_up, down, E, I, y=None):
@@ -318,6 +345,10 @@ def block_norm(f, residual=None, *, post=False, post_weight=None, gate=None, sca
 
     -> (r, z).  residual [M, H] bf16 or fp32, r like it (bf16 without one); gate bf16 [H], or [M, H] for a gate per row; weights bf16 [H] or None.
     z is bf16, or with quantize Fp8Rows.  r, z: where to put them (r may be residual itself)."""
+    if L._native is not None and L._initialised and z is None:
+        made = L._made(L._native.block_norm, f, residual, post, post_weight, gate, scale, pre, pre_weight, eps, weight_offset, quantize, r)
+        if made is not None:
+            return (made[0], Fp8Rows(made[1], made[2], f.shape[1])) if quantize else made
     _gpu(f, "f", (torch.bfloat16,), 2)
     M, H = f.shape
     if H == 0:

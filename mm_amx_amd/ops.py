@@ -246,7 +246,7 @@ class MoE:
     def __init__(self, top_k, scoring="softmax", renormalize=True, scale=1.0):
         if scoring not in ("softmax", "sigmoid"):
             raise L.MmxError("MoE: scoring is 'softmax' or 'sigmoid'")
-        self.top_k, self.scoring, self.renormalize, self.scale = top_k, scoring, renormalize, scale
+        self.top_k, self.scoring, self.renormalize, self.scale = top_k, scoring, renormalize, float(scale)
         self.E = self.H = self.I = 0
         self.router = self.bias = self.gate_up = self.down = None
 
@@ -284,8 +284,7 @@ class MoE:
             raise L.MmxError("run: setup has not been called")
         if x.dim() != 2 or x.shape[1] != self.H:
             raise L.MmxError(f"run: x must be [T, {self.H}]")
-        ids, weights = ffn.moe_route(x, self.router, self.top_k, self.scoring, self.renormalize, self.scale, self.bias)
-        return ffn.moe_experts(x, ids, weights, self.gate_up, self.down, self.E, self.I, y=y)
+        return ffn.moe(x, self.router, self.top_k, self.gate_up, self.down, self.I, self.scoring, self.renormalize, self.scale, self.bias, y)
 
 
 class MLP:

@@ -102,7 +102,7 @@ __device__ __forceinline__ u32x4 to_fp8x16(const float (&v)[16], float inv) {
 }
 
 // What the products in 8-bit floating point are made of.  A: rows of e4m3, lda bytes apart, 16-byte aligned, zero from K up to the
-// next multiple of 128; sA[kb * ld_sA + m].  B: packed as mmx_repack_b packs bytes; sB[row of B's scales][kb].
+// next multiple of 128; sA[kb * ld_sA + m].  Or, where fp8_takes_bf16(M, K), rows of K bf16 that lie anywhere, and sA = NULL.  B: packed as mmx_repack_b packs bytes; sB[row of B's scales][kb].
 struct Fp8Gemm {
     const char* A;
     int64_t lda;
@@ -112,7 +112,7 @@ struct Fp8Gemm {
     int64_t panel_stride;  // bytes of a 32-column panel
     const float* sB;
     int M, N;     // N: packed columns (both of a gate/up pair)
-    int nkb;      // blocks of 128 k
+    int K, nkb;   // nkb: blocks of 128 k
     int npanels;
     int pair_up;  // gate/up pair: rows of gate's scales before up's; 0: plain columns
     Epilogue ep;
@@ -141,5 +141,7 @@ struct NormArgs {
     int M, H;
     int post, pre, z_f8;
 };
+
+bool fp8_takes_bf16(int M, int K);
 
 }  // namespace mmx

@@ -66,23 +66,25 @@ static int check_sizes(const char* who, int M, int K, int N) {
 }
 
 // quantised rows in scratch: the bytes, then the scales
-static size_t rows_bytes(int M, int K) { return round256((size_t)M * padded_k(K)) + round256((size_t)blocks_of(K) * M * 4); }
+// (rows a multiple of 2 KiB apart meet in few channels of the L2)
+static int64_t pitch_of(int K) { return padded_k(K) % 2048 ? padded_k(K) : padded_k(K) + 128; }
+static size_t rows_bytes(int M, int K) { return round256((size_t)M * pitch_of(K)) + round256((size_t)blocks_of(K) * M * 4); }
 struct Rows {
     const char* q;
     int64_t ld;
     const float* scales;
     int64_t ld_scales;
 };
-// A as quantised rows: as given, or made in scratch
+// A as quantised rows: as given, or made in scratch; or as bf16 rows that the product quantises itself
 static int quantised(int dtype, const void* A, int64_t lda, const float* scales, int64_t ld_scales, int M, int K, char* scratch, Rows* out,
                      hipStream_t st) {
-    if (dtype == MMX_F8) {
+    if (dtype == MMX_F8 || (dtype == MMX_BF16 && fp8_takes_bf16(M, K))) {
         *out = {static_cast<const char*>(A), lda, scales, ld_scales};
         return MMX_OK;
     }
-    float* const s = reinterpret_cast<float*>(scratch + round256((size_t)M * padded_k(K)));
-    *out = {scratch, padded_k(K), s, M};
-    return launch_quantize_rows_fp8(dtype == MMX_F32, A, lda, M, K, scratch, padded_k(K), s, M, st);
+    float* const s = reinterpret_cast<float*>(scratch + round256((size_t)M * pitch_of(K)));
+    *out = {scratch, pitch_of(K), s, M};
+    return launch_quantize_rows_fp8(dtype == MMX_F32, A, lda, M, K, scratch, pitch_of(K), s, M, st);
 }
 
 static Fp8Gemm product(const Rows& a, const void* Bp, const float* b_scales, int M, int K, int N, bool pair, const Epilogue& ep) {
@@ -92,6 +94,7 @@ static Fp8Gemm product(const Rows& a, const void* Bp, const float* b_scales, int
     g.sA = a.scales;
     g.ld_sA = a.ld_scales;
     g.Bp = static_cast<const char*>(Bp);
+    g.K = K;
     g.nkb = blocks_of(K);
     g.panel_stride = (int64_t)g.nkb * 4096;
     g.sB = b_scales;
@@ -150,7 +153,7 @@ int mmx_repack_gate_up_fp8(const void* w_gate, const void* w_up, int64_t ldw_byt
 }
 
 size_t mmx_gemm_fp8_scratch_bytes(int a_dtype, int M, int K, int N) {
-    if (M <= 0 || K <= 0 || N <= 0 || (a_dtype != MMX_BF16 && a_dtype != MMX_F32)) return 0;
+    if (M <= 0 || K <= 0 || N <= 0 || (a_dtype != MMX_BF16 && a_dtype != MMX_F32) || (a_dtype == MMX_BF16 && fp8_takes_bf16(M, K))) return 0;
     return rows_bytes(M, K);
 }
 

@@ -59,14 +59,18 @@ __device__ __forceinline__ f32x4 mfma_e4m3(i32x8 a, i32x8 b) {
 // A workgroup computes 16 NT columns of 16 MT rows; its eight wavefronts take blocks of k in turn, straight from memory into
 // registers, and add their sums in LDS in the order of the wavefronts.
 // PAIR: the first column tile is gate's, the second up's, 16 columns of the result.
-template <int MT, int NT, bool PAIR>
+// QUANTIZE: A is bf16 rows, which every workgroup quantises into LDS while its first weights are on their way (one row of 4096 x 11008: 8.5 us on quantised rows, which take a launch of
+// 2.5 us more, and 9.3 so; quantised in every wavefront's registers, whose number leaves two wavefronts on a SIMD, 16.5).
+template <int MT, int NT, bool PAIR, bool QUANTIZE>
 __global__ __launch_bounds__(512) void fp8_rows_kernel(const Fp8Gemm g) {
     static_assert(!PAIR || NT == 2, "a gate and an up tile");
     constexpr int NW = 8;
     __shared__ __attribute__((aligned(16))) f32x4 red[NW][MT * NT][64];
+    extern __shared__ __attribute__((aligned(16))) char rows[];  // QUANTIZE: M rows of row_pitch(K) bytes, then their scales [M][nkb]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 15, quad = lane >> 4;
     const int m0 = blockIdx.y * (16 * MT);
+    const int pitch = g.nkb * 128 + 16;  // (16 bytes more: neighbouring rows in other banks)
 
     const char* w_at[NT];
     const float* s_at[NT];
@@ -86,51 +90,89 @@ __global__ __launch_bounds__(512) void fp8_rows_kernel(const Fp8Gemm g) {
     for (int i = 0; i < MT; i++) {
         int m = m0 + i * 16 + c;
         m = m < g.M ? m : g.M - 1;
-        x_at[i] = g.A + (int64_t)m * g.lda + quad * 32;
-        sx_at[i] = g.sA + m;
+        x_at[i] = (QUANTIZE ? rows + m * pitch : g.A + (int64_t)m * g.lda) + quad * 32;
+        sx_at[i] = QUANTIZE ? reinterpret_cast<const float*>(rows + g.M * pitch) + m * g.nkb : g.sA + m;
     }
+    const int64_t sx_step = QUANTIZE ? 1 : g.ld_sA;
     f32x4 acc[MT][NT];
 #pragma unroll
     for (int i = 0; i < MT; i++)
 #pragma unroll
         for (int j = 0; j < NT; j++) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 
-    auto blocks = [&](auto u_c, int kb) __attribute__((always_inline)) {  // U blocks of k: kb, kb + NW, ...
-        constexpr int U = decltype(u_c)::value;
-        i32x8 w[U][NT], x[U][MT];
-        float sw[U][NT], sx[U][MT];
+    // U blocks of k: kb, kb + NW, ...
+    constexpr int U = MT * NT <= 2 ? 4 : 2;
+    auto load = [&](auto n_c, int kb, u32x4 (&w)[U][NT][2], float (&sw)[U][NT]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int k = kb + u * NW;
+        for (int u = 0; u < decltype(n_c)::value; u++)
 #pragma unroll
             for (int j = 0; j < NT; j++) {
-                const u32x4* p = reinterpret_cast<const u32x4*>(w_at[j] + (int64_t)k * 4096);
-                w[u][j] = join(p[0], p[32]);
-                sw[u][j] = s_at[j][k];
+                const u32x4* p = reinterpret_cast<const u32x4*>(w_at[j] + (int64_t)(kb + u * NW) * 4096);
+                w[u][j][0] = p[0];
+                w[u][j][1] = p[32];
+                sw[u][j] = s_at[j][kb + u * NW];
             }
+    };
+    auto multiply = [&](auto n_c, int kb, const u32x4 (&w)[U][NT][2], const float (&sw)[U][NT]) __attribute__((always_inline)) {
+        constexpr int N = decltype(n_c)::value;
+        u32x4 x[N][MT][2];
+        float sx[N][MT];
+#pragma unroll
+        for (int u = 0; u < N; u++)
 #pragma unroll
             for (int i = 0; i < MT; i++) {
-                const u32x4* p = reinterpret_cast<const u32x4*>(x_at[i] + (int64_t)k * 128);
-                x[u][i] = join(p[0], p[1]);
-                sx[u][i] = sx_at[i][k * g.ld_sA];
+                const u32x4* p = reinterpret_cast<const u32x4*>(x_at[i] + (int64_t)(kb + u * NW) * 128);
+                x[u][i][0] = p[0];
+                x[u][i][1] = p[1];
+                sx[u][i] = sx_at[i][(kb + u * NW) * sx_step];
             }
-        }
 #pragma unroll
-        for (int u = 0; u < U; u++)
+        for (int u = 0; u < N; u++)
 #pragma unroll
             for (int i = 0; i < MT; i++)
 #pragma unroll
                 for (int j = 0; j < NT; j++) {
-                    const f32x4 p = mfma_e4m3(w[u][j], x[u][i]);
+                    const f32x4 p = mfma_e4m3(join(w[u][j][0], w[u][j][1]), join(x[u][i][0], x[u][i][1]));
                     const float s = sx[u][i] * sw[u][j];
 #pragma unroll
                     for (int e = 0; e < 4; e++) acc[i][j][e] = __builtin_fmaf(p[e], s, acc[i][j][e]);
                 }
     };
-    constexpr int U = MT * NT <= 2 ? 4 : 2;
+    typedef std::integral_constant<int, U> all_c;
+    typedef std::integral_constant<int, 1> one_c;
+    u32x4 w[U][NT][2];
+    float sw[U][NT];
     int kb = wave;
-    for (; kb + (U - 1) * NW < g.nkb; kb += U * NW) blocks(std::integral_constant<int, U>{}, kb);
-    for (; kb < g.nkb; kb += NW) blocks(std::integral_constant<int, 1>{}, kb);
+    if constexpr (QUANTIZE) {
+        const bool ahead = kb + (U - 1) * NW < g.nkb;
+        if (ahead) load(all_c(), kb, w, sw);
+        for (int b = threadIdx.x >> 3; b < g.M * g.nkb; b += NW * 8) {  // (whole groups of eight lanes)
+            const int m = b / g.nkb, k = b - m * g.nkb, part = threadIdx.x & 7;
+            float v[16];
+            load_row_f32(reinterpret_cast<const uint16_t*>(g.A + m * g.lda), k * BLOCK + part * 16, g.K, v);
+            uint32_t top = 0;
+#pragma unroll
+            for (int e = 0; e < 16; e++) top = umax(top, abs_bits(v[e]));
+#pragma unroll
+            for (int d = 1; d < 8; d *= 2) top = umax(top, (uint32_t)__shfl_xor((int)top, d));
+            const float s = fp8_scale_of(top);
+            *reinterpret_cast<u32x4*>(rows + m * pitch + k * BLOCK + part * 16) = to_fp8x16(v, fp8_inverse(s));
+            if (part == 0) reinterpret_cast<float*>(rows + g.M * pitch)[b] = s;
+        }
+        __syncthreads();
+        if (ahead) {
+            multiply(all_c(), kb, w, sw);
+            kb += U * NW;
+        }
+    }
+    for (; kb + (U - 1) * NW < g.nkb; kb += U * NW) {
+        load(all_c(), kb, w, sw);
+        multiply(all_c(), kb, w, sw);
+    }
+    for (; kb < g.nkb; kb += NW) {
+        load(one_c(), kb, w, sw);
+        multiply(one_c(), kb, w, sw);
+    }
 
 #pragma unroll
     for (int i = 0; i < MT; i++)
@@ -473,11 +515,16 @@ static int launch_tile(const Fp8Gemm& g, hipStream_t st, const char* name) {
     return check_hip(hipGetLastError(), "fp8_tile_kernel launch");
 }
 
-template <int MT, int NT, bool PAIR>
+static size_t quantized_in_lds(int M, int K) {
+    const size_t nkb = ((size_t)K + BLOCK - 1) / BLOCK;
+    return (size_t)M * (nkb * 128 + 16) + (size_t)M * nkb * 4;
+}
+template <int MT, int NT, bool PAIR, bool QUANTIZE = false>
 static int launch_rows(const Fp8Gemm& g, hipStream_t st, const char* name) {
     note_kernel(name);
     const unsigned cols = PAIR ? (unsigned)g.npanels : (unsigned)((g.N + 16 * NT - 1) / (16 * NT));
-    hipLaunchKernelGGL((fp8_rows_kernel<MT, NT, PAIR>), dim3(cols, (unsigned)((g.M + 16 * MT - 1) / (16 * MT))), dim3(512), 0, st, g);
+    hipLaunchKernelGGL((fp8_rows_kernel<MT, NT, PAIR, QUANTIZE>), dim3(cols, (unsigned)((g.M + 16 * MT - 1) / (16 * MT))), dim3(512),
+                       QUANTIZE ? quantized_in_lds(g.M, g.K) : 0, st, g);
     return check_hip(hipGetLastError(), "fp8_rows_kernel launch");
 }
 
@@ -509,9 +556,17 @@ static int choose_tile(const Fp8Gemm& g) {
     return best;
 }
 
+// Whether the kernel for few rows quantises bf16 rows on the way
+// (us, with a launch of its own / on the way: 1 x 4096 x 11008 11.0 / 9.3, 1 x 11008 x 4096 11.4 / 10.5, 4 x 4096 x 11008 11.3 / 11.2, 8 x 2048 x 2048 4.8 / 4.3,
+// 8 x 4096 x 11008 11.5 / 14.6, 2 x 11008 x 4096 11.5 / 11.4)
+bool fp8_takes_bf16(int M, int K) { return M <= 8 && (int64_t)M * K <= 16384; }
+
 int launch_gemm_fp8(const Fp8Gemm& g, hipStream_t st) {
     const bool pair = g.pair_up != 0;
+    if (!g.sA) return pair ? launch_rows<1, 2, true, true>(g, st, "fp8_rows_16_pair_bf16") : launch_rows<1, 1, false, true>(g, st, "fp8_rows_16_bf16");
     if (g.M <= 16) return pair ? launch_rows<1, 2, true>(g, st, "fp8_rows_16_pair") : launch_rows<1, 1, false>(g, st, "fp8_rows_16");
+    // (16 columns a workgroup where 32 would leave half of the CUs without one: 24 x 8192 x 1024 10.5 -> 9.7 us, 20 x 2048 x 2048 4.3 -> 3.9; 32 x 4096 x 11008 13.2 -> 15.9)
+    if (g.M <= 32 && !pair && 2 * g.npanels <= num_cus()) return launch_rows<2, 1, false>(g, st, "fp8_rows_32");
     if (g.M <= 32) return pair ? launch_rows<2, 2, true>(g, st, "fp8_rows_32_pair") : launch_rows<2, 2, false>(g, st, "fp8_rows_32");
     switch (choose_tile(g)) {
     case 0:  // (a wavefront of a pair needs as many gate columns as up's: 64 x 96 of the tile instead of 128 x 48)

@@ -3,7 +3,7 @@
 //
 // What bounds a small product is the host: the same checks as Python statements, the descriptor as a ctypes structure, the query
 // of the workspace and the call through ctypes took 9.7 us for 256 x 256 x 256, under 4 us of which are on the device; 4.7 now.
-// (A norm of one row 16.7 -> BN, a linear layer in e4m3 LIN, one decode row over 512 x 512 int4 weights 9.2 -> 4.2, a 64 x 512 x 512 layer with a bias 10.2 -> 5.2.)  The functions below
+// (A norm of one row 16.7 -> 5.9, a linear layer in e4m3 of one token 15.8 -> 10.3; one decode row over 512 x 512 int4 weights 9.2 -> 4.2, a 64 x 512 x 512 layer with a bias 10.2 -> 5.2.)  The functions below
 // take the calls that are regular in every respect - tensors of exactly torch's own type on one GPU, the current one, everything
 // large enough - and leave all others to the Python form (they return None, and have done nothing), which accepts them or says
 // what is wrong.  They keep nothing from one call for the next.
@@ -449,9 +449,9 @@ Activations activations(PyObject* const* a, int device) {
     return r;
 }
 
-// a result [M, N] in bf16 or fp32: the caller's, or made here in bf16
-at::Tensor result(PyObject* o, int device, int64_t M, int64_t N, const at::Tensor& like) {
-    if (o == Py_None) return make({M, N}, at::kBFloat16, like);
+// the caller's result [M, N] in bf16 or fp32, if there is one (else it is made in bf16)
+at::Tensor result(PyObject* o, int device, int64_t M, int64_t N) {
+    if (o == Py_None) return at::Tensor();
     const at::Tensor& y = tensor_on(o, device);
     if (y.dim() != 2 || y.size(0) != M || y.size(1) != N) throw Leave();
     float_code(y);
@@ -519,9 +519,9 @@ PyObject* mlp_fp8(PyObject*, PyObject* const* a, Py_ssize_t count) {
         const void* const d = packed_bytes(a[5], device, packed_e4m3(N, x.K));
         const float* const ds = floats(a[6], device, {blocks(x.K), blocks(N)});
         void* const stream = stream_of(a[10]);
-        at::Tensor y;
+        at::Tensor y = result(a[8], device, x.M, x.K);
         if (!unlocked([&] {
-                y = result(a[8], device, x.M, x.K, *x.t);
+                if (!y.defined()) y = make({x.M, x.K}, at::kBFloat16, *x.t);
                 const size_t need = call_mlp_fp8_need(x.dtype, x.M, x.K, N);
                 const at::Tensor scratch = make({(int64_t)need}, at::kByte, *x.t);
                 rc = call_mlp_fp8(x.dtype, x.data, x.ld, x.scales, x.ld_scales, gu, gus, d, ds, code_of(y.scalar_type()), y.mutable_data_ptr(), row_stride_bytes(y), x.M, x.K, N,
@@ -553,9 +553,9 @@ PyObject* moe(PyObject*, PyObject* const* a, Py_ssize_t count) {
         const float* const ds = f8 ? floats(a[9], device, {E, blocks(H), blocks(I)}) : nullptr;
         if (!f8 && a[9] != Py_None) throw Leave();
         void* const stream = stream_of(a[13]);
-        at::Tensor y;
+        at::Tensor y = result(a[11], device, T, H);
         if (!unlocked([&] {
-                y = result(a[11], device, T, H, *x.t);
+                if (!y.defined()) y = make({T, H}, at::kBFloat16, *x.t);
                 const auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
                 const size_t logits = up((size_t)T * E * 8), ids = up((size_t)T * k * 4), need = call_moe_need(T, H, I, k);
                 const at::Tensor memory = make({(int64_t)(logits + 2 * ids + need)}, at::kByte, *x.t);
@@ -574,6 +574,7 @@ PyObject* moe(PyObject*, PyObject* const* a, Py_ssize_t count) {
 }
 
 // block_norm(f, residual, post, post_weight, gate, scale, pre, pre_weight, eps, offset, quantize, r, device, stream) -> (r, z) or (r, padded rows of z, scales)
+//   r: where to put it, None: made here, False: not wanted
 PyObject* block_norm(PyObject*, PyObject* const* a, Py_ssize_t count) {
     if (count != 14 || !call_block_norm) Py_RETURN_NONE;
     try {
@@ -622,13 +623,17 @@ PyObject* block_norm(PyObject*, PyObject* const* a, Py_ssize_t count) {
         n.weight_offset = (float)PyFloat_AS_DOUBLE(a[9]);
         const bool quantize = a[10] == Py_True;
         const at::ScalarType stream_type = n.residual_dtype == MMX_F32 ? at::kFloat : at::kBFloat16;
-        if (a[11] != Py_None && same(a[11]).t->scalar_type() != stream_type) throw Leave();
+        const bool keep = a[11] != Py_False;
+        if (keep && a[11] != Py_None && same(a[11]).t->scalar_type() != stream_type) throw Leave();
         void* const stream = stream_of(a[13]);
         at::Tensor r, z, s;
+        if (keep && a[11] != Py_None) r = THPVariable_Unpack(a[11]);
         if (!unlocked([&] {
-                r = a[11] == Py_None ? make({M, H}, stream_type, *f.t) : THPVariable_Unpack(a[11]);
-                n.r = r.mutable_data_ptr();
-                n.ldr_bytes = row_stride_bytes(r);
+                if (keep) {
+                    if (!r.defined()) r = make({M, H}, stream_type, *f.t);
+                    n.r = r.mutable_data_ptr();
+                    n.ldr_bytes = row_stride_bytes(r);
+                }
                 if (quantize) {
                     const int64_t p = blocks(H) * 128;
                     z = make({M, p % 2048 ? p : p + 128}, at::kFloat8_e4m3fn, *f.t).narrow(1, 0, p);
@@ -646,7 +651,8 @@ PyObject* block_norm(PyObject*, PyObject* const* a, Py_ssize_t count) {
                 rc = call_block_norm(&n, (int)M, (int)H, stream);
             })) throw Leave();
         if (rc) return PyLong_FromLong(rc);
-        return quantize ? Py_BuildValue("(NNN)", THPVariable_Wrap(r), THPVariable_Wrap(z), THPVariable_Wrap(s)) : Py_BuildValue("(NN)", THPVariable_Wrap(r), THPVariable_Wrap(z));
+        PyObject* const kept = keep ? THPVariable_Wrap(r) : (Py_INCREF(Py_None), Py_None);
+        return quantize ? Py_BuildValue("(NNN)", kept, THPVariable_Wrap(z), THPVariable_Wrap(s)) : Py_BuildValue("(NN)", kept, THPVariable_Wrap(z));
     } catch (...) {
         Py_RETURN_NONE;
     }

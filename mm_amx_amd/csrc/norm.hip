@@ -42,19 +42,80 @@ __device__ __forceinline__ void store8(T* row, int at, int len, const float (&v)
     }
 }
 
+// Eight values of a row as they are in memory, so that they can be on their way long before they are needed; zero past the row's len.
+template <typename T>
+struct Raw8 {
+    u32x4 w[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T* row, int at, int len) {
+        constexpr int PER = 16 / (int)sizeof(T);
+#pragma unroll
+        for (int q = 0; q < (int)sizeof(T) / 2; q++) {
+            const int from = at + q * PER;
+            if (from + PER <= len) {
+                __builtin_memcpy(&w[q], __builtin_assume_aligned(row + from, sizeof(T)), 16);  // (the hardware takes any address)
+            } else {
+                w[q] = u32x4{0u, 0u, 0u, 0u};
+                if (from < len) {
+#pragma unroll
+                    for (int e = 0; e < PER; e++)
+                        if (from + e < len) {
+                            if constexpr (sizeof(T) == 2) w[q][e >> 1] |= (uint32_t)row[from + e] << (16 * (e & 1));
+                            else w[q][e] = f2u(row[from + e]);
+                        }
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        if constexpr (sizeof(T) == 2) {
+            widen8(w[0], v);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = u2f(w[e >> 2][e & 3]);
+        }
+    }
+};
+
 // TPR threads per row, each NC chunks of 8 neighbouring values: chunk threadIdx + TPR * i.  A block of 128 is 16 neighbouring threads.
+// Everything is asked for before the first sum: behind it, and the barrier in it, each of them would be one more trip to memory (one row of 4096 4.7 -> 3.9 us, 8192 rows 51 -> 44, 6.0 TB/s).
 template <typename TR, int TPR, int NC>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void block_norm_kernel(const NormArgs g) {
     constexpr int ROWS = TPR >= 256 ? 1 : 256 / TPR;
+    constexpr bool AHEAD = NC <= 2;  // (registers)
     __shared__ float part[TPR / 64 > 1 ? TPR / 64 : 1];
     const int tid = threadIdx.x % TPR;
     const int m = blockIdx.x * ROWS + threadIdx.x / TPR;
     if (m >= g.M) return;  // (a row's threads are a workgroup or whole wavefronts)
     const float inv_h = 1.0f / (float)g.H;
     float v[NC][8];
-    const uint16_t* const f = g.f + m * g.ld_f;
+    Raw8<uint16_t> post_w[NC], gate[NC], pre_w[NC];
+    Raw8<TR> old[NC];
+    auto at_of = [&](int i) __attribute__((always_inline)) { return (tid + TPR * i) * 8; };
+    auto load_old = [&]() __attribute__((always_inline)) {
+        if (g.residual) {
 #pragma unroll
-    for (int i = 0; i < NC; i++) load_row_f32(f, (tid + TPR * i) * 8, g.H, v[i]);
+            for (int i = 0; i < NC; i++) old[i].load(static_cast<const TR*>(g.residual) + m * g.ld_residual, at_of(i), g.H);
+        }
+    };
+    auto load_weights = [&](const uint16_t* row, Raw8<uint16_t> (&w)[NC]) __attribute__((always_inline)) {
+        if (row) {
+#pragma unroll
+            for (int i = 0; i < NC; i++) w[i].load(row, at_of(i), g.H);
+        }
+    };
+    {
+        Raw8<uint16_t> f[NC];
+#pragma unroll
+        for (int i = 0; i < NC; i++) f[i].load(g.f + m * g.ld_f, at_of(i), g.H);
+        load_old();
+        if constexpr (AHEAD) {
+            load_weights(g.post_weight, post_w);
+            load_weights(g.gate ? g.gate + m * g.ld_gate : nullptr, gate);
+            load_weights(g.pre_weight, pre_w);
+        }
+#pragma unroll
+        for (int i = 0; i < NC; i++) f[i].get(v[i]);
+    }
     if (g.post) {
         float sq = 0.0f;
 #pragma unroll
@@ -62,11 +123,12 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void block_norm_kernel(const
 #pragma unroll
             for (int e = 0; e < 8; e++) sq = __builtin_fmaf(v[i][e], v[i][e], sq);
         const float inv = rsqrtf(row_sum<TPR>(sq, part) * inv_h + g.eps);
+        if constexpr (!AHEAD) load_weights(g.post_weight, post_w);
 #pragma unroll
         for (int i = 0; i < NC; i++) {
             float w[8] = {1, 1, 1, 1, 1, 1, 1, 1};
             if (g.post_weight) {
-                load_row_f32(g.post_weight, (tid + TPR * i) * 8, g.H, w);
+                post_w[i].get(w);
 #pragma unroll
                 for (int e = 0; e < 8; e++) w[e] = w[e] + g.offset;
             }
@@ -74,37 +136,30 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void block_norm_kernel(const
             for (int e = 0; e < 8; e++) v[i][e] = v[i][e] * inv * w[e];
         }
     }
+    if constexpr (!AHEAD) load_weights(g.gate ? g.gate + m * g.ld_gate : nullptr, gate);
     float sq = 0.0f;
 #pragma unroll
     for (int i = 0; i < NC; i++) {
-        const int at = (tid + TPR * i) * 8;
-        float s[8];
-        if (g.gate) {
-            load_row_f32(g.gate + m * g.ld_gate, at, g.H, s);
-#pragma unroll
-            for (int e = 0; e < 8; e++) s[e] = s[e] * g.scale;
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; e++) s[e] = g.scale;
-        }
-        float old[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-        if (g.residual) load_row_f32(static_cast<const TR*>(g.residual) + m * g.ld_residual, at, g.H, old);
+        float s[8] = {1, 1, 1, 1, 1, 1, 1, 1}, r[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (g.gate) gate[i].get(s);
+        if (g.residual) old[i].get(r);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             // (past the end of the row everything loaded is zero)
-            v[i][e] = __builtin_fmaf(v[i][e], s[e], old[e]);
+            v[i][e] = __builtin_fmaf(v[i][e], s[e] * g.scale, r[e]);
             sq = __builtin_fmaf(v[i][e], v[i][e], sq);
         }
-        if (g.r) store8(static_cast<TR*>(g.r) + m * g.ld_r, at, g.H, v[i]);
+        if (g.r) store8(static_cast<TR*>(g.r) + m * g.ld_r, at_of(i), g.H, v[i]);
     }
     if (!g.z) return;
+    if constexpr (!AHEAD) load_weights(g.pre_weight, pre_w);
     const float inv = g.pre ? rsqrtf(row_sum<TPR>(sq, part) * inv_h + g.eps) : 1.0f;
 #pragma unroll
     for (int i = 0; i < NC; i++) {
-        const int at = (tid + TPR * i) * 8;
+        const int at = at_of(i);
         float w[8] = {1, 1, 1, 1, 1, 1, 1, 1};
         if (g.pre_weight) {
-            load_row_f32(g.pre_weight, at, g.H, w);
+            pre_w[i].get(w);
 #pragma unroll
             for (int e = 0; e < 8; e++) w[e] = w[e] + g.offset;
         }
@@ -130,19 +185,23 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void block_norm_kernel(const
     }
 }
 
+// (us with and without: 1 x 4096 3.5 / 3.9, 200 x 8192 5.4 / 6.5, 391 x 1000 4.1 / 4.6; 512 threads at 2048 x 4096 14.6 / 13.6)
+constexpr int FEW = 256, MANY = 512;
 template <typename TR>
 static int launch_norm(const NormArgs& g, hipStream_t st) {
 #define MMX_NORM(TPR, NC)                                                                                                                              \
     hipLaunchKernelGGL((block_norm_kernel<TR, TPR, NC>), dim3((unsigned)((g.M + (TPR >= 256 ? 1 : 256 / TPR) - 1) / (TPR >= 256 ? 1 : 256 / TPR))), \
                        dim3(TPR > 256 ? TPR : 256), 0, st, g)
+    // few rows: more threads for each, since they wait for memory and for each other only
     if (g.H <= 512) MMX_NORM(64, 1);
-    else if (g.H <= 1024) MMX_NORM(64, 2);
+    else if (g.H <= 1024 && g.M > MANY) MMX_NORM(64, 2);
     else if (g.H <= 2048) MMX_NORM(256, 1);
+    else if (g.H <= 4096 && g.M <= FEW) MMX_NORM(512, 1);
     else if (g.H <= 4096) MMX_NORM(256, 2);
+    else if (g.H <= 8192 && g.M <= FEW) MMX_NORM(1024, 1);
     else if (g.H <= 8192) MMX_NORM(256, 4);
     else if (g.H <= 16384) MMX_NORM(1024, 2);
-    else if (g.H <= 32768) MMX_NORM(1024, 4);
-    else MMX_NORM(1024, 8);
+    else MMX_NORM(1024, 4);
 #undef MMX_NORM
     return check_hip(hipGetLastError(), "block_norm_kernel launch");
 }

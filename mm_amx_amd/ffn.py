@@ -344,7 +344,7 @@ def block_norm(f, residual=None, *, post=False, post_weight=None, gate=None, sca
         z = r, or with pre   r / sqrt(mean(r^2) + eps) * (weight_offset + pre_weight)
 
     -> (r, z).  residual [M, H] bf16 or fp32, r like it (bf16 without one); gate bf16 [H], or [M, H] for a gate per row; weights bf16 [H] or None.
-    z is bf16, or with quantize Fp8Rows.  r, z: where to put them (r may be residual itself)."""
+    z is bf16, or with quantize Fp8Rows.  r, z: where to put them (r may be residual itself; False: r is not wanted, and None in its place)."""
     if L._native is not None and L._initialised and z is None:
         made = L._made(L._native.block_norm, f, residual, post, post_weight, gate, scale, pre, pre_weight, eps, weight_offset, quantize, r)
         if made is not None:
@@ -371,6 +371,8 @@ def block_norm(f, residual=None, *, post=False, post_weight=None, gate=None, sca
         ld_gate = 0 if gate.dim() == 1 or gate.shape[0] == 1 else gate.stride(0) * 2
     if r is None:
         r = torch.empty((M, H), dtype=stream, device=f.device)
+    elif r is False:
+        r = None
     elif _gpu(r, "r", (stream,), 2).shape != f.shape:
         raise MmxError(f"r is {tuple(r.shape)}, f {tuple(f.shape)}")
     if z is None:
@@ -384,7 +386,7 @@ def block_norm(f, residual=None, *, post=False, post_weight=None, gate=None, sca
         zp, ldz = _gpu(z, "z", (torch.bfloat16,), 2).data_ptr(), _rows(z)
     if M:
         args = L._BlockNorm(f.data_ptr(), _rows(f), _ptr(residual), 0 if residual is None else _rows(residual), _ptr(post_weight), _ptr(gate), ld_gate, _ptr(pre_weight),
-                            r.data_ptr(), _rows(r), zp, ldz, zs, ld_zs, L.F32 if stream == torch.float32 else L.BF16, L.F8 if quantize else L.BF16, int(post), int(pre),
+                            _ptr(r), 0 if r is None else _rows(r), zp, ldz, zs, ld_zs, L.F32 if stream == torch.float32 else L.BF16, L.F8 if quantize else L.BF16, int(post), int(pre),
                             scale, eps, weight_offset)
         L._check(L.lib().mmx_block_norm(C.byref(args), M, H, L._stream()))
     return r, z

@@ -5,14 +5,17 @@ Follows torch-ext/test.py:176-218 (``perf_llama7b_MLP``: 32 layers, per-layer ti
 closeness of the two results) and torch-ext/mlp_llama.py:6-19 (the module).  Every layer has its own
 weights (32 x 270 MB stay resident in HBM), as in the reference's deep-copied stack.
 
-    python -m mm_amx_amd.mlp_llama --M 256 --layers 32 --rounds 10
+With ``fp8`` the same stack runs a third time over e4m3 weights, its norms and quantisation in one kernel in front of each MLP
+(no counterpart in the reference).
+
+    python -m mm_amx_amd.mlp_llama --M 256 --layers 32 --rounds 10 --fp8
 """
 import argparse
 import time
 
 import torch
 
-from . import ops
+from . import ffn, ops
 
 
 class LlamaRMSNorm(torch.nn.Module):
@@ -51,6 +54,15 @@ class LlamaMLP(torch.nn.Module):
     def numel(self, M):
         return 3 * self.hidden_size * self.intermediate_size
 
+    def compress(self):
+        """Adds the MLP over e4m3 weights."""
+        self.fp8 = ops.MLP()
+        self.fp8.setup(self.w_gate, self.w_up, self.w_down, compress="fp8")
+
+    def forward_fp8(self, x):
+        """LlamaRMSNorm and the MLP: the normed rows go quantised from the one to the other."""
+        return self.fp8.run(ffn.block_norm(x, eps=1e-6, quantize=True, r=False)[1])
+
     def forward(self, x):
         if self.opt:
             return self.fused.run(x)
@@ -58,7 +70,7 @@ class LlamaMLP(torch.nn.Module):
         return F.linear(F.silu(F.linear(x, self.w_gate)) * F.linear(x, self.w_up), self.w_down)
 
 
-def perf_llama7b_MLP(M=256, num_layers=32, rounds=10, hidden_size=4096, intermediate_size=11008, verbose=True, graph=False):
+def perf_llama7b_MLP(M=256, num_layers=32, rounds=10, hidden_size=4096, intermediate_size=11008, verbose=True, graph=False, fp8=False):
     layers = []
     for i in range(num_layers):
         layers += [LlamaRMSNorm(), LlamaMLP(hidden_size, intermediate_size, seed=i)]
@@ -109,6 +121,27 @@ def perf_llama7b_MLP(M=256, num_layers=32, rounds=10, hidden_size=4096, intermed
                 print(f"{'graph':>11}: per-layer dt {dt * 1e6:9.1f} us   GFlops {out['mm_amx_amd_graph']['GFlops']:10.0f}   "
                       f"GB/s {out['mm_amx_amd_graph']['GBps']:8.0f}")
             del gr
+        if fp8:
+            def stack(y):
+                for m in mlps:
+                    y = m.forward_fp8(y)
+                return y
+            for m in mlps:
+                m.compress()
+            stack(x)  # warm-up
+            torch.cuda.synchronize()
+            t0 = time.time()
+            for _ in range(rounds):
+                stack(x)
+            torch.cuda.synchronize()
+            dt = (time.time() - t0) / rounds / num_layers
+            out["fp8"] = {"per_layer_us": dt * 1e6, "GFlops": mlps[0].flops(M) * 1e-9 / dt, "GBps": mlps[0].numel(M) * 1e-9 / dt}
+            mlps[0].opt = False
+            want = mlps[0](layers[0](x)).float()
+            out["rel_err_fp8_one_layer"] = (torch.linalg.norm(mlps[0].forward_fp8(x).float() - want) / torch.linalg.norm(want)).item()
+            if verbose:
+                print(f"{'fp8':>11}: per-layer dt {dt * 1e6:9.1f} us   GFlops {out['fp8']['GFlops']:10.0f}   "
+                      f"GB/s {out['fp8']['GBps']:8.0f}   relative difference to torch's bf16, one layer {out['rel_err_fp8_one_layer']:.2e}")
     y0, y1 = out.pop("y_torch"), out.pop("y_mm_amx_amd")
     out["rel_err"] = (torch.linalg.norm(y1 - y0) / torch.linalg.norm(y0)).item()
     # one layer on the same input: the stack has no residual connections, so rounding differences of
@@ -132,6 +165,7 @@ if __name__ == "__main__":
     ap.add_argument("--layers", type=int, default=32)
     ap.add_argument("--rounds", type=int, default=10)
     ap.add_argument("--graph", action="store_true", help="also replay the stack from a HIP graph")
+    ap.add_argument("--fp8", action="store_true", help="also run the stack over e4m3 weights, norms fused with the quantisation")
     a = ap.parse_args()
     ops.L.init(0)
-    perf_llama7b_MLP(a.M, a.layers, a.rounds, graph=a.graph)
+    perf_llama7b_MLP(a.M, a.layers, a.rounds, graph=a.graph, fp8=a.fp8)

@@ -16,20 +16,26 @@ from safetensors.torch import save_file
 from . import _lib as L
 
 FORMAT = "mm_amx_amd.packed_b/1"
-_DT = {"bf16": L.BF16, "int8": L.I8, "int4": L.I4}
+_DT = {"bf16": L.BF16, "int8": L.I8, "int4": L.I4, "fp8": L.F8}
 
 
 def save_packed(path, packed, dtype, K, N, scales=None, layout="b", extra=None):
-    """packed: uint8 tensor from repack_b / repack_gate_up / quantize_pack_int4; dtype 'bf16', 'int8' or 'int4'; K, N: the logical [K, N]
-    of the packed matrix (for a gate/up pair N is 2 x the projection width, layout='gate_up');
-    scales: optional fp32 [N] per-output-channel dequantisation scales."""
+    """packed: uint8 tensor from repack_b / repack_gate_up / quantize_pack_int4 / quantize_pack_fp8 / pack_fp8 / pack_gate_up_fp8; dtype 'bf16', 'int8', 'int4'
+    or 'fp8'; K, N: the logical [K, N] of the packed matrix (for a gate/up pair N is 2 x the projection width, layout='gate_up');
+    scales: optional fp32 [N] per-output-channel dequantisation scales; of 'fp8' weights the scales of their blocks [rows, ceil(K / 128)]."""
     if dtype not in _DT:
-        raise L.MmxError("dtype must be 'bf16', 'int8' or 'int4'")
+        raise L.MmxError("dtype must be 'bf16', 'int8', 'int4' or 'fp8'")
     if packed.dtype != torch.uint8 or packed.numel() != L.packed_b_bytes(_DT[dtype], K, N):
         raise L.MmxError("packed does not have the size of a packed [K, N] matrix of this dtype")
+    if dtype == "fp8" and scales is None:
+        raise L.MmxError("e4m3 weights come with scales")
     tensors = {"packed": packed.detach().cpu().contiguous()}
     if scales is not None:
-        if scales.numel() != N:
+        if dtype == "fp8":
+            rows = 2 * -(-N // 256) if layout == "gate_up" else -(-N // 128)
+            if tuple(scales.shape) != (rows, -(-K // 128)):
+                raise L.MmxError(f"scales of the blocks must be [{rows}, {-(-K // 128)}]")
+        elif scales.numel() != N:
             raise L.MmxError("scales must have one entry per output channel")
         tensors["scales"] = scales.detach().to(torch.float32).cpu().contiguous()
     meta = {"format": FORMAT, "dtype": dtype, "K": str(K), "N": str(N), "layout": layout,

@@ -51,7 +51,8 @@ def test_products(lib):
 
     for bad, word in ((dict(dt=2), "dtype"), (dict(A=None), "NULL"), (dict(s=None), "NULL"), (dict(A=P + 8), "16-byte"), (dict(lda=128), "apart"), (dict(lda=1 << 24), "8 MiB"),
                       (dict(lds=3), "scales"), (dict(B=None), "NULL"), (dict(B=P + 8), "16-byte"), (dict(bs=None), "NULL"), (dict(K=0), "positive"), (dict(M=-1), "negative"),
-                      (dict(dt=1, lda=512), "e4m3 activations only"), (dict(dt=1, s=None, lda=512), "scratch"), (dict(dt=1, s=None, lda=512, scratch=P + 16, n=1 << 20), "256-byte"),
+                      (dict(dt=1, lda=512), "e4m3 activations only"), (dict(dt=0, s=None, lda=1024), "scratch"), (dict(dt=0, s=None, lda=1024, scratch=P + 16, n=1 << 20), "256-byte"),
+                      (dict(dt=1, M=40, lds=40, s=None, lda=512), "scratch"),
                       (dict(ep=epilogue(out=2)), "dtype"), (dict(ep=epilogue(steps=1)), "DEQUANT"), (dict(ep=epilogue(steps=8)), "QUANT"), (dict(ep=epilogue(steps=2)), "bias"),
                       (dict(ep=epilogue(C_=None)), "NULL"), (dict(ep=epilogue(ld=126)), "row"), (dict(N=32, ep=epilogue(steps=16)), "64"),
                       (dict(ep=epilogue(steps=18, bias=P)), "SILU_GATE"), (dict(ep=epilogue(steps=64)), "unknown")):
@@ -59,7 +60,8 @@ def test_products(lib):
         refused(gemm(ep, **bad), word)
     assert gemm(M=0, A=None) == 0
     assert lib.mmx_gemm_fp8_scratch_bytes(6, 4, 256, 64) == 0 and lib.mmx_gemm_fp8_scratch_bytes(1, 0, 256, 64) == 0
-    assert lib.mmx_gemm_fp8_scratch_bytes(1, 4, 200, 64) >= 4 * 256 + 2 * 4 * 4
+    assert lib.mmx_gemm_fp8_scratch_bytes(0, 4, 200, 64) >= 4 * 256 + 2 * 4 * 4
+    assert lib.mmx_gemm_fp8_scratch_bytes(1, 400, 200, 64) >= 400 * 256 + 2 * 400 * 4
 
     need = lib.mmx_mlp_fp8_scratch_bytes(6, 4, 256, 64)
     mlp = lambda **k: lib.mmx_mlp_fp8(*{**dict(dt=6, x=P, ldx=256, s=P, lds=4, gu=P, gs=P, d=P, ds=P, yt=1, y=P, ldy=512, M=4, K=256, N=64, scratch=P, n=need, st=None), **k}.values())  # noqa: E731
@@ -137,3 +139,19 @@ def test_the_definitions_against_torch():
     x = torch.cat([torch.randn(20000, generator=torch.Generator().manual_seed(1)) * 100, torch.linspace(-20, 20, 4001) / 16, torch.tensor([0.0, 448.0, -448.0, 17.0, 19.0])]).clamp(-448, 448)
     assert np.array_equal(u.encode(x.double().numpy()), x.to(torch.float8_e4m3fn).view(torch.uint8).numpy())
     assert list(u.scale_of(np.array([0.0, 448.0, 449.0, 1.75, np.inf]))) [:4] == [2.0 ** -126, 1.0, 2.0, 2.0 ** -8]
+
+
+def test_packed_weights_on_disk(tmp_path):
+    from mm_amx_amd import packed_io
+    K, N = 300, 160
+    packed = torch.arange(L.packed_b_bytes(L.F8, K, N), dtype=torch.int64).to(torch.uint8)
+    scales = torch.rand((2, 3))
+    path = str(tmp_path / "w.safetensors")
+    packed_io.save_packed(path, packed, "fp8", K, N, scales=scales)
+    w = packed_io.load_packed(path, device="cpu")
+    assert torch.equal(w["packed"], packed) and torch.equal(w["scales"], scales) and (w["dtype"], w["K"], w["N"]) == ("fp8", K, N)
+    pair = torch.zeros(L.packed_b_bytes(L.F8, K, 320), dtype=torch.uint8)
+    packed_io.save_packed(path, pair, "fp8", K, 320, scales=torch.rand((4, 3)), layout="gate_up")
+    for bad in (dict(scales=None), dict(scales=scales[:1]), dict(scales=torch.rand(160)), dict(packed=packed[:-1])):
+        with pytest.raises(mx.MmxError):
+            packed_io.save_packed(path, **{**dict(packed=packed, dtype="fp8", K=K, N=N, scales=scales), **bad})

@@ -96,6 +96,12 @@ def test_in_place_strides_and_rows_behind():
             mask = torch.ones_like(old, dtype=torch.bool)
             mask[at] = False
             assert torch.equal(got[mask], old[mask])
+    # r not wanted
+    for q in (False, True):
+        a, b = mx.block_norm(f[at], None, pre_weight=w, quantize=q), mx.block_norm(f[at], None, pre_weight=w, quantize=q, r=False)
+        c = mx.block_norm(f[at], None, pre_weight=w, quantize=q, r=False, z=a[1])  # (a z of its own: the Python form)
+        bits = lambda v: (v.q if q else v).contiguous().view(torch.uint8)  # noqa: E731
+        assert b[0] is None and c[0] is None and torch.equal(bits(a[1]), bits(b[1])) and torch.equal(bits(a[1]), bits(c[1]))
     # one row of gate for all, as a view too
     f, res, gate = normal((M, H), 1), normal((M, H), 2), normal((H,), 3)
     a = mx.block_norm(f, res, gate=gate)
@@ -176,3 +182,10 @@ def test_refusals_on_the_gpu():
             mx.block_norm(**{**dict(f=f, residual=res), **bad})
     with pytest.raises(mx.MmxError):
         mx.block_norm(normal((1, 40000), 1))
+
+
+def test_the_stack_of_the_demo():
+    """Three layers of the MLP demo over e4m3 weights beside torch's: x, the weights and the intermediate are each quantised to 4 significant bits (2^-4 at most)."""
+    from mm_amx_amd import mlp_llama
+    out = mlp_llama.perf_llama7b_MLP(M=5, num_layers=2, rounds=1, hidden_size=256, intermediate_size=704, verbose=False, fp8=True)
+    assert out["fp8"]["per_layer_us"] > 0 and out["rel_err_fp8_one_layer"] < 4 * 2.0 ** -4

@@ -218,6 +218,7 @@ __global__ __launch_bounds__(512) void fp8_rows_kernel(const Fp8Gemm g) {
 // columns' fragments, which it holds in registers.  The one barrier per stage stands in front of the last 16 rows: all of this
 // stage has been read into registers then, so its slot is free for the loads of stage kb + R (issued during the next stage), and the next stage has landed, so its
 // first fragments are fetched beside the last rows' products.
+// KG groups of NW wavefronts, each with a ring of its own, take the blocks of k in turn where there are fewer tiles than CUs; their sums are added in LDS, in order.
 // What bounds it: at 4096 x 8192 x 4096 the matrix cores are busy for 56 % of a stage's cycles, and the chip's power holds the clock at 2.0 GHz; a loop of nothing but these
 // products and multiply-adds runs at 3.2 PFLOP/s on random values, 4.3 on zeros.
 // Where the chunks of a row of A lie in LDS: chunk ^ turn(row), 0 ... 7.  An LDS cycle serves 16 lanes of a ds_read_b128, 256 bytes, and takes them as
@@ -228,13 +229,14 @@ __device__ __forceinline__ int turn(int row) {
     const int x = row >> 1 & 7;
     return ((x >> 2 ^ x >> 1) & 1) << 2 | (x >> 2) << 1 | (x & 1);
 }
-template <int BM, int BN, int NW, int WGM, int R>
+template <int BM, int BN, int NW, int WGM, int R, int KG>
 struct Fp8Tile {
     static constexpr int WGN = NW / WGM, WM = BM / WGM, WN = BN / WGN;
     static constexpr int MI = WM / 16, NJ = WN / 16;
     static constexpr int A_B = BM * 128, B_B = BN * 128, SA_B = BM * 4, SB_B = 256;
     static constexpr int STAGE = A_B + B_B + SA_B + SB_B;
-    static constexpr int BYTES = R * STAGE;
+    static constexpr int RING = R * STAGE, BYTES = KG * RING;
+    static_assert((KG - 1) * BM * BN * 4 <= BYTES, "the groups' sums fit where the stages were");
     static constexpr int PIECES = (A_B + B_B) / 1024, LOADS = PIECES / NW;  // loads of 1 KiB: of a stage, of a wavefront
     static constexpr int A_LOADS = BM / 8 / NW;  // of them of A, the first ones
     static_assert(PIECES % NW == 0 && BM / 8 % NW == 0 && BM % 64 == 0, "every wavefront issues the same number of loads");
@@ -242,10 +244,10 @@ struct Fp8Tile {
     static_assert(BM / 64 < NW, "a wavefront is left for B's scales");
 };
 
-template <int BM, int BN, int NW, int WGM, int R>
-__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void fp8_tile_kernel(const Fp8Gemm g, int tiles_m, int total,
+template <int BM, int BN, int NW, int WGM, int R, int KG>
+__global__ __launch_bounds__(NW * KG * 64) __attribute__((amdgpu_waves_per_eu(NW * KG > 8 ? NW * KG / 4 : 2, NW * KG > 8 ? NW * KG / 4 : 2))) void fp8_tile_kernel(const Fp8Gemm g, int tiles_m, int total,
                                                                                                           int per_xcd) {
-    using T = Fp8Tile<BM, BN, NW, WGM, R>;
+    using T = Fp8Tile<BM, BN, NW, WGM, R, KG>;
     constexpr int MI = T::MI, NJ = T::NJ, STAGE = T::STAGE, LOADS = T::LOADS;
     using lds_u32x4 = __attribute__((address_space(3))) const u32x4;
     using lds_float = __attribute__((address_space(3))) const float;
@@ -255,16 +257,17 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     if (L >= total) return;
     const int tn = L / tiles_m, tm = L - tn * tiles_m;
     const int m0 = tm * BM, panel0 = tn * (BN / 32);
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int lane = threadIdx.x & 63, all_waves = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = all_waves % NW, group = all_waves / NW;
     const int wm = wave / T::WGN, wn = wave % T::WGN;
     const int c = lane & 15, quad = lane >> 4;
     const int nkb = g.nkb;
     const bool younger = wave >= NW / 2;
+    const int steps = (nkb - group + KG - 1) / KG, most = (nkb + KG - 1) / KG;  // of this group, of any: blocks group, group + KG, ...
 
     // ---- loads: this wavefront's pieces of 1 KiB of a stage, as offsets from the stage's place in A and B
     const char* const a_base = g.A + (int64_t)m0 * g.lda;
     const char* const b_base = g.Bp + (int64_t)panel0 * g.panel_stride;
-    const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem);
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem) + group * T::RING;
     auto panel_off = [&](int p) __attribute__((always_inline)) {  // of the tile's panel p; a tile may reach past the last panel: that one again, never stored
         const int panel = panel0 + p < g.npanels ? panel0 + p : g.npanels - 1;
         return (uint32_t)(panel - panel0) * (uint32_t)g.panel_stride;
@@ -319,10 +322,11 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
         s_step = 4;
         s_dst = T::A_B + T::B_B + T::SA_B;
     }
-    // Number ic of this wavefront's loads of stage kb, the last of which is the scales.  lanes: all (-1), or none (0) past the last stage - such a load brings
+    // Number ic of this wavefront's loads of its group's stage t, the last of which is the scales.  lanes: all (-1), or none (0) past the last stage - such a load brings
     // nothing and counts like any other, so the counts that are waited for are the same throughout.
-    auto load = [&](auto ic, int kb, int slot, int lanes) __attribute__((always_inline)) {
+    auto load = [&](auto ic, int t, int slot, int lanes) __attribute__((always_inline)) {
         constexpr int i = decltype(ic)::value;
+        const int kb = group + KG * t;
         const uint32_t st = lds0 + slot * STAGE;
         lanes = __builtin_amdgcn_readfirstlane(lanes);
         if constexpr (i < LOADS) {
@@ -366,7 +370,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 
     unrolled<0, R - 1>([&](auto rc) __attribute__((always_inline)) {
         constexpr int r = decltype(rc)::value;
-        unrolled<0, LOADS + 1>([&](auto ic) __attribute__((always_inline)) { load(ic, r, r, __builtin_amdgcn_readfirstlane((r - nkb) >> 31)); });
+        unrolled<0, LOADS + 1>([&](auto ic) __attribute__((always_inline)) { load(ic, r, r, (r - steps) >> 31); });
     });
     asm volatile("s_waitcnt vmcnt(%0)" : : "n"((R - 2) * (LOADS + 1)) : "memory");
     __builtin_amdgcn_s_barrier();
@@ -395,7 +399,7 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     auto stage = [&](auto turn_c, int kb) __attribute__((always_inline)) {
         constexpr int F = decltype(turn_c)::value * MI % 3;  // the first rows' operands: the three sets go round
         const int next = slot + 1 < R ? slot + 1 : 0;
-        const int more = __builtin_amdgcn_readfirstlane((kb + R - 1 - nkb) >> 31), free_slot = slot > 0 ? slot - 1 : R - 1;
+        const int more = (kb + R - 1 - steps) >> 31, free_slot = slot > 0 ? slot - 1 : R - 1;
         float sb_next[NJ];
         unrolled<0, SLOTS + LAG>([&](auto tc) __attribute__((always_inline)) {
             constexpr int t = decltype(tc)::value, i = t / NJ, j = t % NJ;
@@ -466,11 +470,34 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     // stages in turn until the sets of registers are where they were
     constexpr int TURN = MI % 3 ? 3 : 1;
     int kb = 0;
-    for (; kb + TURN <= nkb; kb += TURN) unrolled<0, TURN>([&](auto pc) __attribute__((always_inline)) { stage(pc, kb + decltype(pc)::value); });
+    for (; kb + TURN <= steps; kb += TURN) unrolled<0, TURN>([&](auto pc) __attribute__((always_inline)) { stage(pc, kb + decltype(pc)::value); });
     unrolled<0, TURN - 1>([&](auto pc) __attribute__((always_inline)) {
-        if (kb + decltype(pc)::value < nkb) stage(pc, kb + decltype(pc)::value);
+        if (kb + decltype(pc)::value < steps) stage(pc, kb + decltype(pc)::value);
     });
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if constexpr (KG > 1) {
+        if (steps < most) __builtin_amdgcn_s_barrier();  // (the others have one stage more)
+        __syncthreads();
+        f32x4* const sums = reinterpret_cast<f32x4*>(smem) + threadIdx.x % (NW * 64);
+        if (group > 0) {
+#pragma unroll
+            for (int i = 0; i < MI; i++)
+#pragma unroll
+                for (int j = 0; j < NJ; j++) sums[(((group - 1) * MI + i) * NJ + j) * (NW * 64)] = acc[i][j];
+        }
+        __syncthreads();
+        if (group > 0) return;
+#pragma unroll
+        for (int o = 0; o < KG - 1; o++)
+#pragma unroll
+            for (int i = 0; i < MI; i++)
+#pragma unroll
+                for (int j = 0; j < NJ; j++) {
+                    const f32x4 v = sums[((o * MI + i) * NJ + j) * (NW * 64)];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[i][j][e] += v[e];
+                }
+    }
 
     // ---- post-op: a lane holds columns n + 0..3 of row m of each 16 x 16 tile
 #pragma unroll
@@ -501,17 +528,17 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     }
 }
 
-template <int BM, int BN, int NW, int WGM, int R>
+template <int BM, int BN, int NW, int WGM, int R, int KG = 1>
 static int launch_tile(const Fp8Gemm& g, hipStream_t st, const char* name) {
-    using T = Fp8Tile<BM, BN, NW, WGM, R>;
+    using T = Fp8Tile<BM, BN, NW, WGM, R, KG>;
     static std::atomic<uint64_t> done{0};
-    const auto kernel = fp8_tile_kernel<BM, BN, NW, WGM, R>;
+    const auto kernel = fp8_tile_kernel<BM, BN, NW, WGM, R, KG>;
     const int rc = ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), T::BYTES, done);
     if (rc) return rc;
     const int64_t tiles_m = (g.M + BM - 1) / BM, tiles_n = (g.npanels * 32 + BN - 1) / BN, total = tiles_m * tiles_n, per_xcd = (total + 7) / 8;
     if (per_xcd * 8 > 0x7fffffff) return set_error(MMX_E_INVALID, "mmx_gemm_fp8: too many tiles for one launch");
     note_kernel(name);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(per_xcd * 8)), dim3(NW * 64), T::BYTES, st, g, (int)tiles_m, (int)total, (int)per_xcd);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(per_xcd * 8)), dim3(NW * KG * 64), T::BYTES, st, g, (int)tiles_m, (int)total, (int)per_xcd);
     return check_hip(hipGetLastError(), "fp8_tile_kernel launch");
 }
 
@@ -528,29 +555,32 @@ static int launch_rows(const Fp8Gemm& g, hipStream_t st, const char* name) {
     return check_hip(hipGetLastError(), "fp8_rows_kernel launch");
 }
 
-// Which tile: the least of rounds * (fixed + blocks of k * stage), a round being as many tiles as fit on the chip, with the constants below fitted to
-// 4096 x 8192 x 4096, 1024 x 11008 x 4096, 2048 x 4096 x 11008, 512 x 4096 x 4096 and 256 x 4096 x 11008 (us; "fixed" holds the first loads and the post-op).
-// us at 2048 x 4096 x 11008 / 1024 x 11008 x 4096 / 512 x 4096 x 4096 / 391 x 1000 x 3001:
-//     256x192   114 / 102 / 44 / 18.6        128x128   144 / 63 / 23 / 10.1
-//      64x128   145 /  65 / 17 /  7.4         64x64    203 / 85 / 18 /  7.4
+// Which tile: the least of rounds * (fixed + blocks of k * stage), a round being as many tiles as fit on the chip; one that is not full leaves each of its tiles more of the chip, down to
+// `least` of the time.  The constants are fitted to these measurements, us at 2048 x 4096 x 11008 / 1024 x 11008 x 4096 / 512 x 4096 x 4096 / 256 x 11008 x 4096 / 391 x 1000 x 3001 /
+// 128 x 4096 x 4096 / 100 x 8192 x 1024 ("fixed" holds the first loads and the post-op):
+//     256 x 192           114 / 102 / 44 / 101 / 18.6 / 41 / 77
+//     128 x 128           144 /  63 / 23 /  50 / 10.1 / 22 / 37
+//      64 x 128           145 /  65 / 17 /  35 /  7.4 / 15 / 26
+//      64 x 64            203 /  85 / 18 /  31 /  7.3 / 13 / 21
+//      64 x 64, K shared   -  /  -  / 20 /  24 /  9.7 / 11 / 16
 struct TileCost {
     int bm, bn, per_cu;
-    float fixed_us, stage_us;
+    float fixed_us, stage_us, least;
 };
-static constexpr TileCost TILES[4] = {{256, 192, 1, 9.0f, 1.34f}, {128, 128, 1, 5.2f, 0.67f}, {64, 128, 2, 5.5f, 0.66f}, {64, 64, 2, 2.9f, 0.46f}};
+enum { T_256_192, T_128_128, T_64_128, T_64_64, T_64_64_SHARED, TILES };
+static constexpr TileCost COSTS[TILES] = {{256, 192, 1, 9.0f, 1.34f, 0.9f}, {128, 128, 1, 5.2f, 0.67f, 0.75f}, {64, 128, 2, 5.5f, 0.66f, 0.55f}, {64, 64, 2, 2.9f, 0.46f, 0.55f}, {64, 64, 1, 2.5f, 0.26f, 0.85f}};
 
 static int choose_tile(const Fp8Gemm& g) {
     int best = 0;
-    double least = 0;
-    for (int i = 0; i < 4; i++) {
-        const TileCost& t = TILES[i];
+    double fastest = 0;
+    for (int i = 0; i < TILES; i++) {
+        const TileCost& t = COSTS[i];
         const int64_t tiles = (int64_t)((g.M + t.bm - 1) / t.bm) * ((g.npanels * 32 + t.bn - 1) / t.bn), at_once = (int64_t)num_cus() * t.per_cu;
-        // (a round that is not full leaves each of its tiles more of the chip)
         const double full = (double)(tiles / at_once), rest = (double)(tiles % at_once) / at_once;
-        const double us = (full + (rest > 0 ? 0.55 + 0.45 * rest : 0)) * (t.fixed_us + g.nkb * t.stage_us);
-        if (i == 0 || us < least) {
+        const double us = (full + (rest > 0 ? t.least + (1 - t.least) * rest : 0)) * (t.fixed_us + g.nkb * t.stage_us);
+        if (i == 0 || us < fastest) {
             best = i;
-            least = us;
+            fastest = us;
         }
     }
     return best;
@@ -569,11 +599,12 @@ int launch_gemm_fp8(const Fp8Gemm& g, hipStream_t st) {
     if (g.M <= 32 && !pair && 2 * g.npanels <= num_cus()) return launch_rows<2, 1, false>(g, st, "fp8_rows_32");
     if (g.M <= 32) return pair ? launch_rows<2, 2, true>(g, st, "fp8_rows_32_pair") : launch_rows<2, 2, false>(g, st, "fp8_rows_32");
     switch (choose_tile(g)) {
-    case 0:  // (a wavefront of a pair needs as many gate columns as up's: 64 x 96 of the tile instead of 128 x 48)
+    case T_256_192:  // (a wavefront of a pair needs as many gate columns as up's: 64 x 96 of the tile instead of 128 x 48)
         return pair ? launch_tile<256, 192, 8, 4, 2>(g, st, "fp8_256x192_pair") : launch_tile<256, 192, 8, 2, 2>(g, st, "fp8_256x192");
-    case 1: return launch_tile<128, 128, 8, 2, 4>(g, st, "fp8_128x128");
-    case 2: return launch_tile<64, 128, 4, 1, 3>(g, st, "fp8_64x128");
-    default: return launch_tile<64, 64, 4, 2, 4>(g, st, "fp8_64x64");
+    case T_128_128: return launch_tile<128, 128, 8, 2, 4>(g, st, "fp8_128x128");
+    case T_64_128: return launch_tile<64, 128, 4, 1, 3>(g, st, "fp8_64x128");
+    case T_64_64: return launch_tile<64, 64, 4, 2, 4>(g, st, "fp8_64x64");
+    default: return launch_tile<64, 64, 4, 2, 3, 2>(g, st, "fp8_64x64_shared_k");
     }
 }
 

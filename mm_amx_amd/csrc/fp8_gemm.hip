@@ -242,6 +242,7 @@ struct Fp8Tile {
     static_assert(PIECES % NW == 0 && BM / 8 % NW == 0 && BM % 64 == 0, "every wavefront issues the same number of loads");
     // wavefront w < BM / 64 brings 64 rows' scales, the others B's (again): one load each
     static_assert(BM / 64 < NW, "a wavefront is left for B's scales");
+    static_assert(MI >= 2 && NJ >= 1, "the loads of a stage go in front of its last 16 rows");
 };
 
 template <int BM, int BN, int NW, int WGM, int R, int KG>
@@ -322,8 +323,8 @@ __global__ __launch_bounds__(NW * KG * 64) __attribute__((amdgpu_waves_per_eu(NW
         s_step = 4;
         s_dst = T::A_B + T::B_B + T::SA_B;
     }
-    // Number ic of this wavefront's loads of its group's stage t, the last of which is the scales.  lanes: all (-1), or none (0) past the last stage - such a load brings
-    // nothing and counts like any other, so the counts that are waited for are the same throughout.
+    // Number ic of this wavefront's loads of its group's stage t, the last of which is the scales.  lanes: all (-1), or none (0) past the last stage, where nothing is to be loaded
+    // (and nobody counts on how many loads there were).
     auto load = [&](auto ic, int t, int slot, int lanes) __attribute__((always_inline)) {
         constexpr int i = decltype(ic)::value;
         const int kb = group + KG * t;
@@ -372,7 +373,8 @@ __global__ __launch_bounds__(NW * KG * 64) __attribute__((amdgpu_waves_per_eu(NW
         constexpr int r = decltype(rc)::value;
         unrolled<0, LOADS + 1>([&](auto ic) __attribute__((always_inline)) { load(ic, r, r, (r - steps) >> 31); });
     });
-    asm volatile("s_waitcnt vmcnt(%0)" : : "n"((R - 2) * (LOADS + 1)) : "memory");
+    if (R > 2 && steps >= R - 1) asm volatile("s_waitcnt vmcnt(%0)" : : "n"((R - 2) * (LOADS + 1)) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     places(0);
@@ -405,7 +407,9 @@ __global__ __launch_bounds__(NW * KG * 64) __attribute__((amdgpu_waves_per_eu(NW
             constexpr int t = decltype(tc)::value, i = t / NJ, j = t % NJ;
             if constexpr (t == SLOTS - NJ) {
                 // in front of the last rows: everything of this stage is in registers (their operands arrive now), and the next one has landed
-                asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"((R - 2) * (LOADS + 1)) : "memory");
+                // (R - 2 younger stages may be on their way; where there are no more to load, all that are)
+                if (R > 2 && more) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"((R - 2) * (LOADS + 1)) : "memory");
+                else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
                 __builtin_amdgcn_s_barrier();
                 asm volatile("" ::: "memory");
                 places(next);

@@ -242,7 +242,7 @@ struct Fp8Tile {
     static_assert(PIECES % NW == 0 && BM / 8 % NW == 0 && BM % 64 == 0, "every wavefront issues the same number of loads");
     // wavefront w < BM / 64 brings 64 rows' scales, the others B's (again): one load each
     static_assert(BM / 64 < NW, "a wavefront is left for B's scales");
-    static_assert(MI >= 2 && NJ >= 1, "the loads of a stage go in front of its last 16 rows");
+    static_assert(MI >= 2 && NJ >= 2, "the loads of a stage go in front of its last 16 rows; a row's two halves are read in two slots");
 };
 
 template <int BM, int BN, int NW, int WGM, int R, int KG>
@@ -323,24 +323,20 @@ __global__ __launch_bounds__(NW * KG * 64) __attribute__((amdgpu_waves_per_eu(NW
         s_step = 4;
         s_dst = T::A_B + T::B_B + T::SA_B;
     }
-    // Number ic of this wavefront's loads of its group's stage t, the last of which is the scales.  lanes: all (-1), or none (0) past the last stage, where nothing is to be loaded
-    // (and nobody counts on how many loads there were).
-    auto load = [&](auto ic, int t, int slot, int lanes) __attribute__((always_inline)) {
+    // Number ic of this wavefront's loads of its group's stage t, the last of which is the scales.
+    auto load = [&](auto ic, int t, int slot) __attribute__((always_inline)) {
         constexpr int i = decltype(ic)::value;
         const int kb = group + KG * t;
         const uint32_t st = lds0 + slot * STAGE;
-        lanes = __builtin_amdgcn_readfirstlane(lanes);
         if constexpr (i < LOADS) {
             const int piece = i * NW + wave;
             const char* const src = i < T::A_LOADS ? a_base + (int64_t)kb * 128 : b_base + (int64_t)kb * 4096;
             const uint32_t to = st + piece * 1024, from = off[i];
-            asm volatile("s_mov_b32 m0, %0\n\ts_mov_b32 exec_lo, %3\n\ts_mov_b32 exec_hi, %3\n\tglobal_load_lds_dwordx4 %1, %2\n\ts_mov_b64 exec, -1"
-                         : : "s"(to), "v"(from), "s"(src), "s"(lanes) : "memory");
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(to), "v"(from), "s"(src) : "memory");
         } else {
             const char* const src = s_base + kb * s_step;
             const uint32_t to = st + s_dst, from = s_off;
-            asm volatile("s_mov_b32 m0, %0\n\ts_mov_b32 exec_lo, %3\n\ts_mov_b32 exec_hi, %3\n\tglobal_load_lds_dword %1, %2\n\ts_mov_b64 exec, -1"
-                         : : "s"(to), "v"(from), "s"(src), "s"(lanes) : "memory");
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, %2" : : "s"(to), "v"(from), "s"(src) : "memory");
         }
     };
 
@@ -371,7 +367,7 @@ __global__ __launch_bounds__(NW * KG * 64) __attribute__((amdgpu_waves_per_eu(NW
 
     unrolled<0, R - 1>([&](auto rc) __attribute__((always_inline)) {
         constexpr int r = decltype(rc)::value;
-        unrolled<0, LOADS + 1>([&](auto ic) __attribute__((always_inline)) { load(ic, r, r, (r - steps) >> 31); });
+        unrolled<0, LOADS + 1>([&](auto ic) __attribute__((always_inline)) { if (r < steps) load(ic, r, r); });
     });
     if (R > 2 && steps >= R - 1) asm volatile("s_waitcnt vmcnt(%0)" : : "n"((R - 2) * (LOADS + 1)) : "memory");
     else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -394,14 +390,15 @@ __global__ __launch_bounds__(NW * KG * 64) __attribute__((amdgpu_waves_per_eu(NW
     // One slot per MFMA, in this order and no other (the compiler would gather the multiply-adds behind the last of them): the MFMA; the multiply-adds of
     // the one LAG slots before, whose result is there by now; an LDS read for the rows or the stage to come; a load.
     // The loads are spread over the slots in front of the barrier: issued behind one another they hold up the wavefronts, the products and all, until the address unit has taken them.
-    constexpr int LAG = 2, SLOTS = MI * NJ, SPAN = MI > 2 ? (MI - 2) * NJ : MI > 1 ? NJ : 1;
+    constexpr int LAG = 2, SLOTS = MI * NJ, SPAN = MI > 2 ? (MI - 2) * NJ : NJ;
     f32x4 p[LAG + 1];
     float s[LAG + 1];
     int slot = 0;
     auto stage = [&](auto turn_c, int kb) __attribute__((always_inline)) {
         constexpr int F = decltype(turn_c)::value * MI % 3;  // the first rows' operands: the three sets go round
         const int next = slot + 1 < R ? slot + 1 : 0;
-        const int more = (kb + R - 1 - steps) >> 31, free_slot = slot > 0 ? slot - 1 : R - 1;
+        const bool more = kb + R - 1 < steps;
+        const int free_slot = slot > 0 ? slot - 1 : R - 1;
         float sb_next[NJ];
         unrolled<0, SLOTS + LAG>([&](auto tc) __attribute__((always_inline)) {
             constexpr int t = decltype(tc)::value, i = t / NJ, j = t % NJ;
@@ -435,17 +432,14 @@ __global__ __launch_bounds__(NW * KG * 64) __attribute__((amdgpu_waves_per_eu(NW
             }
             if constexpr (t < SLOTS) {
                 unrolled<0, LOADS + 1>([&](auto ic) __attribute__((always_inline)) {
-                    if constexpr (decltype(ic)::value * SPAN / (LOADS + 1) == t) load(ic, kb + R - 1, free_slot, more);
+                    if constexpr (decltype(ic)::value * SPAN / (LOADS + 1) == t) {
+                        if (more) load(ic, kb + R - 1, free_slot);
+                    }
                 });
                 if constexpr (i < MI - 2) {
                     constexpr int n = (F + i + 2) % 3;
                     if constexpr (j == 0) sa[n] = read_sa(i + 2);
-                    if constexpr (NJ == 1) {
-                        fa[n][0] = read_a(i + 2, 0);
-                        fa[n][1] = read_a(i + 2, 1);
-                    } else if constexpr (j < 2) {
-                        fa[n][j] = read_a(i + 2, j);
-                    }
+                    if constexpr (j < 2) fa[n][j] = read_a(i + 2, j);
                 } else if constexpr (i == MI - 1) {
                     // (past the last stage these read what an earlier one left there: never used)
                     constexpr int n0 = (F + MI) % 3, n1 = (F + MI + 1) % 3;
@@ -562,11 +556,11 @@ static int launch_rows(const Fp8Gemm& g, hipStream_t st, const char* name) {
 // Which tile: the least of rounds * (fixed + blocks of k * stage), a round being as many tiles as fit on the chip; one that is not full leaves each of its tiles more of the chip, down to
 // `least` of the time.  The constants are fitted to these measurements, us at 2048 x 4096 x 11008 / 1024 x 11008 x 4096 / 512 x 4096 x 4096 / 256 x 11008 x 4096 / 391 x 1000 x 3001 /
 // 128 x 4096 x 4096 / 100 x 8192 x 1024 ("fixed" holds the first loads and the post-op):
-//     256 x 192           114 / 102 / 44 / 101 / 18.6 / 41 / 77
-//     128 x 128           144 /  63 / 23 /  50 / 10.1 / 22 / 37
-//      64 x 128           145 /  65 / 17 /  35 /  7.4 / 15 / 26
-//      64 x 64            203 /  85 / 18 /  31 /  7.3 / 13 / 21
-//      64 x 64, K shared   -  /  -  / 20 /  24 /  9.7 / 11 / 16
+//     256 x 192           112 / 101 / 43 / 100 / 18.9 / 40 / 72
+//     128 x 128           149 /  66 / 24 /  52 / 10.3 / 22 / 39
+//      64 x 128           144 /  66 / 18 /  35 /  7.2 / 15 / 26
+//      64 x 64            199 /  85 / 18 /  30 /  7.0 / 13 / 22
+//      64 x 64, K shared  248 /  93 / 21 /  24 /  9.4 / 11 / 16
 struct TileCost {
     int bm, bn, per_cu;
     float fixed_us, stage_us, least;

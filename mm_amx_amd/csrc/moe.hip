@@ -399,7 +399,8 @@ __global__ __launch_bounds__(512) void moe_up_kernel(const MoeArgs g, int col_un
                 for (int e = 0; e < 4; e++) {
                     const float v = weight * (silu32(gate[e]) * up[e]);
                     hi[e] = to_bf16(v);
-                    lo[e] = to_bf16(v - from_bf16(hi[e]));
+                    const float rest = v - from_bf16(hi[e]);
+                    lo[e] = abs_bits(rest) < 0x7f800000u ? to_bf16(rest) : 0;  // (an infinity, or a NaN, is all in the first)
                 }
                 __builtin_memcpy(__builtin_assume_aligned(h, 8), hi, 8);
                 __builtin_memcpy(__builtin_assume_aligned(h + g.I, 8), lo, 8);

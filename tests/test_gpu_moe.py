@@ -179,6 +179,21 @@ def test_a_bad_token_is_its_own():
     assert torch.equal(y[others], clean[others]) and torch.isnan(y[11]).all()
 
 
+@pytest.mark.parametrize("f8", [False, True])
+def test_values_past_the_largest_are_infinite(f8):
+    E, H, I = 2, 128, 64
+    big = torch.full((E, I, H), 256.0, device="cuda")
+    wd = torch.ones((E, H, I), device="cuda")
+    wd[:, 1::2] = -1
+    moe = mx.MoE(1)
+    moe.setup(torch.zeros((E, H), dtype=torch.bfloat16, device="cuda"), *(w.to(torch.bfloat16) for w in (big, big, wd)), compress="fp8" if f8 else None)
+    x = torch.zeros((3, H), dtype=torch.bfloat16, device="cuda")
+    x[0, 0], x[1, 0] = 2.0 ** 60, 1  # gate = up = 2^68: their product is past 2^128; and 2^16 of 64 of them
+    y = moe.run(x).cpu().float()
+    assert (y[0, ::2] == float("inf")).all() and (y[0, 1::2] == -float("inf")).all()
+    assert (y[1, ::2] == 2.0 ** 22).all() and (y[1, 1::2] == -2.0 ** 22).all() and (y[2] == 0).all()
+
+
 def test_compressed_from_bf16_weights():
     E, H, I = 4, 256, 128
     wg, wu, wd, _, _ = experts(E, H, I, False)

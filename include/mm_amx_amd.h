@@ -261,7 +261,7 @@ int mmx_mlp_splitk(const void* x, int64_t ldx_bytes, const void* w_gate_up, cons
  * scales[n / 128][k / 128], contiguous; any values.  In a gate/up pair gate's rows of scales come first, then up's.
  * Rows of quantised activations are 16-byte aligned and lie a multiple of 16 bytes apart; they hold ceil(K / 128) * 128 bytes, and
  * the bytes from K on must be zero (every entry point here that writes such rows writes them so).
- * With M (or T) = 0 these calls do nothing. */
+ * With M (or T) = 0 these calls do nothing.  M < 2^22, N <= 2^26, K <= 2^22. */
 
 /* x [M, K] (MMX_BF16 or MMX_F32) -> q, scales: scales[kb][m] is the least power of two, 2^-126 at least, with which the block's
  * largest magnitude is at most 448; q = x / scale to nearest even.  (x / scale is exact, so the result does not depend on how it is computed.)  A block that

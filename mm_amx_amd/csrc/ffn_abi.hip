@@ -56,12 +56,12 @@ static int check_scratch(const char* who, const void* scratch, size_t have, size
     return MMX_OK;
 }
 
-// K and N within what the kernels address with 32 bits
-constexpr int MOST_K = 1 << 22, MOST_N = 1 << 26, MOST_M = 1 << 26;
+// K and N within what the kernels address with 32 bits; M such that a launch of up to 1024 threads for each row has fewer than 2^32 of them
+constexpr int MOST_K = 1 << 22, MOST_N = 1 << 26, MOST_M = (1 << 22) - 1;
 static int check_sizes(const char* who, int M, int K, int N) {
     if (M < 0 || K <= 0 || N <= 0) return set_error(MMX_E_INVALID, "%s: K and N must be positive and M not negative (got %d, %d, %d)", who, M, K, N);
     if (K > MOST_K || N > MOST_N || M > MOST_M)
-        return set_error(MMX_E_UNSUPPORTED, "%s: M and N up to %d and K up to %d (got %d, %d, %d)", who, MOST_N, MOST_K, M, K, N);
+        return set_error(MMX_E_UNSUPPORTED, "%s: M up to %d, N up to %d and K up to %d (got %d, %d, %d)", who, MOST_M, MOST_N, MOST_K, M, K, N);
     return MMX_OK;
 }
 

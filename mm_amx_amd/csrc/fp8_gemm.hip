@@ -534,7 +534,7 @@ static int launch_tile(const Fp8Gemm& g, hipStream_t st, const char* name) {
     const int rc = ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), T::BYTES, done);
     if (rc) return rc;
     const int64_t tiles_m = (g.M + BM - 1) / BM, tiles_n = (g.npanels * 32 + BN - 1) / BN, total = tiles_m * tiles_n, per_xcd = (total + 7) / 8;
-    if (per_xcd * 8 > 0x7fffffff) return set_error(MMX_E_INVALID, "mmx_gemm_fp8: too many tiles for one launch");
+    if (per_xcd * 8 * (NW * KG * 64) > 0xffffffffll) return set_error(MMX_E_INVALID, "mmx_gemm_fp8: too many tiles for one launch");
     note_kernel(name);
     hipLaunchKernelGGL(kernel, dim3((unsigned)(per_xcd * 8)), dim3(NW * KG * 64), T::BYTES, st, g, (int)tiles_m, (int)total, (int)per_xcd);
     return check_hip(hipGetLastError(), "fp8_tile_kernel launch");

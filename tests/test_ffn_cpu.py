@@ -28,7 +28,7 @@ def test_quantisers(lib):
     rows = lambda **k: lib.mmx_quantize_rows_fp8(*{**dict(dt=1, x=P, ldx=512, M=4, K=256, q=P, ldq=256, s=P, lds=4, st=None), **k}.values())  # noqa: E731
     for bad, word in ((dict(dt=2), "dtype"), (dict(M=-1), "negative"), (dict(K=0), "positive"), (dict(x=None), "NULL"), (dict(x=P + 1), "aligned"), (dict(ldx=510), "apart"),
                       (dict(ldx=513), "aligned"), (dict(q=P + 8), "16-byte"), (dict(ldq=264), "16-byte"), (dict(ldq=240), "apart"), (dict(s=None), "NULL"),
-                      (dict(s=P + 2), "aligned"), (dict(lds=3), "scales"), (dict(K=1 << 23), "up to"), (dict(dt=0), "apart")):
+                      (dict(s=P + 2), "aligned"), (dict(lds=3), "scales"), (dict(K=1 << 23), "up to"), (dict(dt=0), "apart"), (dict(M=1 << 22, lds=1 << 22), "up to")):
         refused(rows(**bad), word)
     assert rows(M=0, x=None, q=None) == 0
     pack = lambda **k: lib.mmx_quantize_pack_fp8(*{**dict(W=P, ldw=512, K=256, N=64, t=1, pair=0, packed=P, s=P, st=None), **k}.values())  # noqa: E731

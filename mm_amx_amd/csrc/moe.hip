@@ -163,8 +163,9 @@ struct MoeArgs {
     char* y;
     int64_t ldy;
     int y_f32;
-    float* parts;         // [splits][T][H] sums of a part of the experts each, or NULL: straight to y
-    int splits;
+    int splits;           // workgroups that share 16 columns of y
+    float* parts;         // splits > 1: their sums, [splits][T][H]
+    int* arrived;         //             and how many of them are there, for each group of tokens and 16 columns; zeroed by the gate/up kernel
 };
 
 // The experts that the tokens [t0, t0 + n / k) chose, in ascending order.  flags: LDS, E bytes.
@@ -258,6 +259,10 @@ __global__ __launch_bounds__(512) void moe_up_kernel(const MoeArgs g, int col_un
     const int t0 = blockIdx.y * MOE_GROUP, tokens = g.T - t0 < MOE_GROUP ? g.T - t0 : MOE_GROUP;
     const int first = t0 * g.k, n = tokens * g.k;
     const int a = blockIdx.x / col_units, u = blockIdx.x - a * col_units;
+    if (g.splits > 1 && blockIdx.x == 0) {
+        const int tiles = (g.H + 15) / 16;
+        for (int i = threadIdx.x; i < tiles; i += NW * 64) g.arrived[blockIdx.y * tiles + i] = 0;
+    }
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int expert, count;
     if (tokens == 1) {  // its slots are the chosen experts themselves
@@ -423,7 +428,7 @@ __global__ __launch_bounds__(1024) void moe_down_kernel(const MoeArgs g) {
     __shared__ uint16_t named[SLOTS], expert_at[SLOTS];  // a slot's expert as it is named, and NONE for a slot that does not count
     __shared__ uint16_t sorted[SLOTS], start[SLOTS + 1]; // the slots by expert, and where each expert's begin
     __shared__ uint8_t begins[SLOTS];
-    __shared__ int chosen;
+    __shared__ int chosen, last;
     __shared__ __attribute__((aligned(16))) float part[NW][TOKENS][16];
     const int t0 = blockIdx.y * MOE_GROUP, tokens = g.T - t0 < MOE_GROUP ? g.T - t0 : MOE_GROUP;
     const int first = t0 * g.k, n = tokens * g.k;
@@ -544,6 +549,15 @@ __global__ __launch_bounds__(1024) void moe_down_kernel(const MoeArgs g) {
         }
     }
     __syncthreads();
+    auto store_y = [&](int t, int n0, const float (&r)[4]) __attribute__((always_inline)) {
+        char* const row = g.y + (int64_t)(t0 + t) * g.ldy;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            if (n0 + e >= g.H) break;
+            if (g.y_f32) reinterpret_cast<float*>(row)[n0 + e] = r[e];
+            else reinterpret_cast<uint16_t*>(row)[n0 + e] = to_bf16(r[e]);
+        }
+    };
     if (threadIdx.x < TOKENS * 4) {
         const int t = threadIdx.x >> 2, n0 = u * 16 + (threadIdx.x & 3) * 4;
         if (t < tokens) {
@@ -554,45 +568,53 @@ __global__ __launch_bounds__(1024) void moe_down_kernel(const MoeArgs g) {
 #pragma unroll
                 for (int e = 0; e < 4; e++) r[e] += v[e];
             }
-            char* const row = g.y + (int64_t)(t0 + t) * g.ldy;
-            float* const to = g.parts ? g.parts + ((int64_t)blockIdx.z * g.T + t0 + t) * g.H : reinterpret_cast<float*>(row);
+            if (g.splits == 1) {
+                store_y(t, n0, r);
+            } else {
+                float* const to = g.parts + ((int64_t)blockIdx.z * g.T + t0 + t) * g.H;
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                if (n0 + e >= g.H) break;
-                if (g.parts || g.y_f32) to[n0 + e] = r[e];
-                else reinterpret_cast<uint16_t*>(row)[n0 + e] = to_bf16(r[e]);
+                for (int e = 0; e < 4; e++)
+                    if (n0 + e < g.H) __hip_atomic_store(to + n0 + e, r[e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
         }
     }
+    if (g.splits == 1) return;
+    // Whoever comes last adds all sums, in the order of the workgroups; nobody waits.  The sums are written and read past the L2, which another XCD does not see, and have arrived before
+    // this workgroup counts itself.  (With ordinary stores and __threadfence(), which writes back all of the L2, in each wavefront: 1 x 2048 x 1024, 8 of 64 experts, 115 us instead of 27.)
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0)
+        last = __hip_atomic_fetch_add(g.arrived + blockIdx.y * gridDim.x + u, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == g.splits - 1;
+    __syncthreads();
+    if (!last) return;
+    const int t = threadIdx.x >> 2, n0 = u * 16 + (threadIdx.x & 3) * 4;
+    if (t < tokens) {
+        float v[MOE_SPLITS][4], r[4];
+#pragma unroll
+        for (int z = 0; z < MOE_SPLITS; z++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[z][e] = z < g.splits && n0 + e < g.H ? __hip_atomic_load(g.parts + ((int64_t)z * g.T + t0 + t) * g.H + n0 + e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            r[e] = v[0][e];
+#pragma unroll
+            for (int z = 1; z < MOE_SPLITS; z++) r[e] += v[z][e];
+        }
+        store_y(t, n0, r);
+    }
 }
 
-// y = the splits' sums, in their order
-__global__ __launch_bounds__(256) void moe_add_kernel(const MoeArgs g) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, all = (int64_t)g.T * g.H;
-    if (i >= all) return;
-    float v[MOE_SPLITS];
-#pragma unroll
-    for (int z = 0; z < MOE_SPLITS; z++) v[z] = z < g.splits ? g.parts[z * all + i] : 0.0f;
-    float sum = v[0];
-#pragma unroll
-    for (int z = 1; z < MOE_SPLITS; z++) sum += v[z];
-    const int64_t t = i / g.H;
-    char* const row = g.y + t * g.ldy;
-    if (g.y_f32) reinterpret_cast<float*>(row)[i - t * g.H] = sum;
-    else reinterpret_cast<uint16_t*>(row)[i - t * g.H] = to_bf16(sum);
-}
-
-// Into how many workgroups the down products of 16 columns are split: a narrow layer's columns are a workgroup each for a part of the CUs only.  The sums then go through memory
-// and one more launch, which has to be worth it (32 tokens, 2 of 16 experts, 1000 x 1376: 30.5 us whole,
-// 16.7 + 2.5 in four; of 2048 columns, 128 workgroups, the whole kernel takes 11 us for 33 MB).
+// Into how many workgroups the down products of 16 columns are split: a narrow layer's columns are a workgroup each for a part of the CUs only.  The sums then go through memory, some 2 us,
+// for which there have to be CUs without work (us whole / split, experts' calls: in two 4 x 2048 x 768, 8 of 128, 72 / 68; 32 x 2048 x 1024, 8 of 64, 219 / 190;
+// 1 x 2048 x 1024, 8 of 64, 27 / 27; the down products alone in four 32 x 1000 x 1376, 2 of 16, 30.5 / 19).
 static int moe_splits(int T, int H) {
     const int64_t tiles = (int64_t)((H + 15) / 16) * ((T + MOE_GROUP - 1) / MOE_GROUP), cus = num_cus();
-    return tiles * 3 > cus ? 1 : tiles * MOE_SPLITS <= cus ? MOE_SPLITS : 2;
+    return tiles * MOE_SPLITS <= cus ? MOE_SPLITS : tiles * 2 <= cus ? 2 : 1;
 }
 static size_t moe_h_bytes(int T, int I, int k) { return ((size_t)T * k * 2 * I * 2 + 255) & ~(size_t)255; }
 size_t moe_scratch_bytes(int T, int H, int I, int k) {
     const int splits = moe_splits(T, H);
-    return moe_h_bytes(T, I, k) + (splits > 1 ? (size_t)splits * T * H * 4 : 0);
+    return moe_h_bytes(T, I, k) + (splits > 1 ? (size_t)splits * T * H * 4 + (size_t)((T + MOE_GROUP - 1) / MOE_GROUP) * ((H + 15) / 16) * 4 : 0);
 }
 
 int launch_moe_experts(bool f8, const void* x, int64_t ldx_bytes, const int* ids, const float* weights, int T, int H, int I, int E, int k,
@@ -608,6 +630,9 @@ int launch_moe_experts(bool f8, const void* x, int64_t ldx_bytes, const int* ids
     g.y = static_cast<char*>(y);
     g.ldy = ldy;
     g.y_f32 = y_f32;
+    g.splits = moe_splits(T, H);
+    g.parts = reinterpret_cast<float*>(static_cast<char*>(h) + moe_h_bytes(T, I, k));
+    g.arrived = reinterpret_cast<int*>(g.parts + (int64_t)g.splits * T * H);
     const int64_t ku_h = f8 ? (H + 127) / 128 : (H + 63) / 64, ku_i = f8 ? (I + 127) / 128 : (I + 63) / 64;
     const unsigned groups = (unsigned)((T + MOE_GROUP - 1) / MOE_GROUP);
     const int most = (T < MOE_GROUP ? T : MOE_GROUP) * k, units = I / 16;
@@ -627,14 +652,9 @@ int launch_moe_experts(bool f8, const void* x, int64_t ldx_bytes, const int* ids
     g.expert_bytes = g.panel_stride * ((H + 31) / 32);
     g.scales = s_down;
     g.scale_rows = (H + 127) / 128;
-    g.splits = moe_splits(T, H);
-    g.parts = g.splits > 1 ? reinterpret_cast<float*>(static_cast<char*>(h) + moe_h_bytes(T, I, k)) : nullptr;
     const auto down = T <= 16 ? (f8 ? moe_down_kernel<W_fp8, 1> : moe_down_kernel<W_bf16, 1>) : f8 ? moe_down_kernel<W_fp8, 2> : moe_down_kernel<W_bf16, 2>;
     hipLaunchKernelGGL(down, dim3((unsigned)((H + 15) / 16), groups, (unsigned)g.splits), dim3(1024), 0, st, g);
-    rc = check_hip(hipGetLastError(), "moe_down_kernel launch");
-    if (rc || g.splits == 1) return rc;
-    hipLaunchKernelGGL(moe_add_kernel, dim3((unsigned)(((int64_t)T * H + 255) / 256)), dim3(256), 0, st, g);
-    return check_hip(hipGetLastError(), "moe_add_kernel launch");
+    return check_hip(hipGetLastError(), "moe_down_kernel launch");
 }
 
 }  // namespace mmx

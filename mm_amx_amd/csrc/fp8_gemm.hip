@@ -219,8 +219,9 @@ __global__ __launch_bounds__(512) void fp8_rows_kernel(const Fp8Gemm g) {
 // stage has been read into registers then, so its slot is free for the loads of stage kb + R (issued during the next stage), and the next stage has landed, so its
 // first fragments are fetched beside the last rows' products.
 // KG groups of NW wavefronts, each with a ring of its own, take the blocks of k in turn where there are fewer tiles than CUs; their sums are added in LDS, in order.
-// What bounds it: at 4096 x 8192 x 4096 the matrix cores are busy for 56 % of a stage's cycles, and the chip's power holds the clock at 2.0 GHz; a loop of nothing but these
-// products and multiply-adds runs at 3.2 PFLOP/s on random values, 4.3 on zeros.
+// What bounds it: beside a product of 32 cycles each of a SIMD's two wavefronts issues 6 or 7 vector instructions of 4 cycles, and the chip's power holds the clock at 2.0 GHz; a loop of
+// nothing but these products and multiply-adds runs at 3.2 PFLOP/s on random values, 4.3 on zeros.  8192 x 8192 x 8192 runs at 2.0, 4096 x 4096 x 4096 at 1.9, 2048 x 4096 x 11008, whose tiles
+// leave a fifth of the second round empty, at 1.65.  (Workgroups that walk over tiles, the next one's first loads on their way while results are stored: 0 to 2 %.)
 // Where the chunks of a row of A lie in LDS: chunk ^ turn(row), 0 ... 7.  An LDS cycle serves 16 lanes of a ds_read_b128, 256 bytes, and takes them as
 // lanes 0-3, 12-15, 20-23, 24-27 (and 4-11, 16-19, 28-31, and the same of the other half): eight rows' chunk c and the other eight's c ^ 2.  Two rows lie in
 // 256 bytes, so row / 2 has to be spread over the eight positions, the first eight's and the second's without a common one: {0, 1, 6, 7} go to {0, 1, 2, 3},
@@ -246,17 +247,19 @@ struct Fp8Tile {
 };
 
 template <int BM, int BN, int NW, int WGM, int R, int KG>
-__global__ __launch_bounds__(NW * KG * 64) __attribute__((amdgpu_waves_per_eu(NW * KG > 8 ? NW * KG / 4 : 2, NW * KG > 8 ? NW * KG / 4 : 2))) void fp8_tile_kernel(const Fp8Gemm g, int tiles_m, int total,
+__global__ __launch_bounds__(NW * KG * 64) __attribute__((amdgpu_waves_per_eu(NW * KG > 8 ? NW * KG / 4 : 2, NW * KG > 8 ? NW * KG / 4 : 2))) void fp8_tile_kernel(const Fp8Gemm g, int tiles_m, int tiles_n, int total,
                                                                                                           int per_xcd) {
     using T = Fp8Tile<BM, BN, NW, WGM, R, KG>;
     constexpr int MI = T::MI, NJ = T::NJ, STAGE = T::STAGE, LOADS = T::LOADS;
     using lds_u32x4 = __attribute__((address_space(3))) const u32x4;
     using lds_float = __attribute__((address_space(3))) const float;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
-    // neighbouring workgroups go to different XCDs: each XCD gets a run of tiles, rows fastest, which share their columns' weights
+    // Neighbouring workgroups go to different XCDs: each XCD gets a run of tiles, eight rows of them at a time and those fastest, so that the 32 it works on share both operands
+    // in its L2 (all rows of tiles fastest: 8192 x 8192 x 8192 700 us in 256 x 192 and 582 in 128 x 256, now 596 and 553).
     const int L = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
     if (L >= total) return;
-    const int tn = L / tiles_m, tm = L - tn * tiles_m;
+    const int band = L / (8 * tiles_n), in_band = L - band * (8 * tiles_n), high = tiles_m - band * 8 < 8 ? tiles_m - band * 8 : 8;
+    const int tn = in_band / high, tm = band * 8 + in_band - tn * high;
     const int m0 = tm * BM, panel0 = tn * (BN / 32);
     const int lane = threadIdx.x & 63, all_waves = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = all_waves % NW, group = all_waves / NW;
     const int wm = wave / T::WGN, wn = wave % T::WGN;
@@ -414,7 +417,7 @@ __global__ __launch_bounds__(NW * KG * 64) __attribute__((amdgpu_waves_per_eu(NW
             if constexpr (NW > 4 && t < SLOTS && j == 0) {
                 // Of a SIMD's two wavefronts the older one is served first: it was at the barrier 670 of a stage's 3300 cycles before the other,
                 // which then had the SIMD to itself and could not fill it.  The younger one is served first for the first half.
-                // (256 x 192, 4096 x 8192 x 4096: 186 -> 183 us; 256 x 256: 130 -> 125.)
+                // (256 x 192, 4096 x 8192 x 4096: 186 -> 183 us.)
                 if constexpr (i == 0 || i == MI / 2) {
                     if (younger) __builtin_amdgcn_s_setprio(i == 0 ? 1 : 0);
                 }
@@ -536,7 +539,7 @@ static int launch_tile(const Fp8Gemm& g, hipStream_t st, const char* name) {
     const int64_t tiles_m = (g.M + BM - 1) / BM, tiles_n = (g.npanels * 32 + BN - 1) / BN, total = tiles_m * tiles_n, per_xcd = (total + 7) / 8;
     if (per_xcd * 8 * (NW * KG * 64) > 0xffffffffll) return set_error(MMX_E_INVALID, "mmx_gemm_fp8: too many tiles for one launch");
     note_kernel(name);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(per_xcd * 8)), dim3(NW * KG * 64), T::BYTES, st, g, (int)tiles_m, (int)total, (int)per_xcd);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(per_xcd * 8)), dim3(NW * KG * 64), T::BYTES, st, g, (int)tiles_m, (int)tiles_n, (int)total, (int)per_xcd);
     return check_hip(hipGetLastError(), "fp8_tile_kernel launch");
 }
 
@@ -554,19 +557,20 @@ static int launch_rows(const Fp8Gemm& g, hipStream_t st, const char* name) {
 }
 
 // Which tile: the least of rounds * (fixed + blocks of k * stage), a round being as many tiles as fit on the chip; one that is not full leaves each of its tiles more of the chip, down to
-// `least` of the time.  The constants are fitted to these measurements, us at 2048 x 4096 x 11008 / 1024 x 11008 x 4096 / 512 x 4096 x 4096 / 256 x 11008 x 4096 / 391 x 1000 x 3001 /
-// 128 x 4096 x 4096 / 100 x 8192 x 1024 ("fixed" holds the first loads and the post-op):
-//     256 x 192           112 / 101 / 43 / 100 / 18.9 / 40 / 72
-//     128 x 128           149 /  66 / 24 /  52 / 10.3 / 22 / 39
-//      64 x 128           144 /  66 / 18 /  35 /  7.2 / 15 / 26
-//      64 x 64            199 /  85 / 18 /  30 /  7.0 / 13 / 22
-//      64 x 64, K shared  248 /  93 / 21 /  24 /  9.4 / 11 / 16
+// `least` of the time.  The constants are fitted to these measurements, us at 2048 x 4096 x 11008 / 4096 x 8192 x 4096 / 8192 x 8192 x 8192 / 1024 x 11008 x 4096 / 512 x 4096 x 4096 /
+// 256 x 11008 x 4096 / 391 x 1000 x 3001 / 128 x 4096 x 4096 ("fixed" holds the first loads and the post-op):
+//     256 x 192           108 / 194 /  596 / 103 / 43 / 100 / 18.9 / 40
+//     128 x 256           115 / 152 /  553 /  80 / 33 /  75 / 14.7 / 32
+//      64 x 128           144 / 198 /   -  /  66 / 18 /  35 /  7.2 / 15
+//      64 x 64            199 / 305 /   -  /  85 / 18 /  30 /  7.0 / 13
+//      64 x 64, K shared  248 / 322 /   -  /  93 / 21 /  24 /  9.4 / 11
+// Over 60 products of 33 to 6000 rows, 200 to 11008 k and 200 to 16000 columns the tile chosen was 1.4 % behind the fastest on average, 12 % at most.
 struct TileCost {
     int bm, bn, per_cu;
     float fixed_us, stage_us, least;
 };
-enum { T_256_192, T_128_128, T_64_128, T_64_64, T_64_64_SHARED, TILES };
-static constexpr TileCost COSTS[TILES] = {{256, 192, 1, 9.0f, 1.34f, 0.9f}, {128, 128, 1, 5.2f, 0.67f, 0.75f}, {64, 128, 2, 5.5f, 0.66f, 0.55f}, {64, 64, 2, 2.9f, 0.46f, 0.55f}, {64, 64, 1, 2.5f, 0.26f, 0.85f}};
+enum { T_256_192, T_128_256, T_64_128, T_64_64, T_64_64_SHARED, TILES };
+static constexpr TileCost COSTS[TILES] = {{256, 192, 1, 9.0f, 1.45f, 0.7f}, {128, 256, 1, 6.0f, 1.03f, 0.78f}, {64, 128, 2, 5.5f, 0.66f, 0.55f}, {64, 64, 2, 2.9f, 0.46f, 0.55f}, {64, 64, 1, 2.5f, 0.26f, 0.85f}};
 
 static int choose_tile(const Fp8Gemm& g) {
     int best = 0;
@@ -599,7 +603,7 @@ int launch_gemm_fp8(const Fp8Gemm& g, hipStream_t st) {
     switch (choose_tile(g)) {
     case T_256_192:  // (a wavefront of a pair needs as many gate columns as up's: 64 x 96 of the tile instead of 128 x 48)
         return pair ? launch_tile<256, 192, 8, 4, 2>(g, st, "fp8_256x192_pair") : launch_tile<256, 192, 8, 2, 2>(g, st, "fp8_256x192");
-    case T_128_128: return launch_tile<128, 128, 8, 2, 4>(g, st, "fp8_128x128");
+    case T_128_256: return launch_tile<128, 256, 8, 2, 3>(g, st, pair ? "fp8_128x256_pair" : "fp8_128x256");
     case T_64_128: return launch_tile<64, 128, 4, 1, 3>(g, st, "fp8_64x128");
     case T_64_64: return launch_tile<64, 64, 4, 2, 4>(g, st, "fp8_64x64");
     default: return launch_tile<64, 64, 4, 2, 3, 2>(g, st, "fp8_64x64_shared_k");

@@ -172,6 +172,29 @@ def test_gate_up(M, K, N, dtype):
     assert (wide[:, N:] == 9.0).all()
 
 
+@pytest.mark.parametrize("M,K,N,pair,tile", [(640, 300, 11000, False, "128x256"), (1200, 260, 5999, False, "128x256"), (640, 300, 11008, True, "128x256"), (1200, 260, 6016, True, "128x256"),
+                                             (2300, 700, 3900, False, "256x192"), (2300, 700, 3904, True, "256x192")])
+def test_large_tiles(M, K, N, pair, tile):
+    """The two tiles that smaller products do not choose, their last rows and columns in part, over one band of eight rows of tiles and more.  N: packed columns."""
+    x = normal((M, K), 1)
+    rows = mx.quantize_fp8(x)
+    a = u.value_rows(bits(rows.q), u.f64(rows.scales))
+    if pair:
+        (g, gs), (v, vs) = weight(N // 2, K, 2), weight(N // 2, K, 3)
+        gs, vs = gs * 0.1, vs * 0.1
+        packed, s = mx.pack_gate_up_fp8(g, v, (gs, vs))
+        want, bound = u.gated(*u.product(a, u.f64(g) * u.spread(u.f64(gs), N // 2, K), 8), *u.product(a, u.f64(v) * u.spread(u.f64(vs), N // 2, K), 8))
+    else:
+        w, sw = weight(N, K, 2)
+        packed, s = mx.pack_fp8(w, sw)
+        want, bound = u.product(a, u.f64(w) * u.spread(u.f64(sw), N, K), 8)
+    y, wide = in_wide(torch.empty((M, want.shape[1]), device="cuda"), 3, 9.0)
+    mx.gemm_fp8(rows, packed, s, N, mx.Epilogue(y, mx.PP_SILU_GATE if pair else mx.PP_NONE))
+    assert mx.last_kernel() == f"fp8_{tile}" + ("_pair" if pair else "")
+    u.close(y, want, bound, torch.float32, mx.last_kernel())
+    assert (wide[:, want.shape[1]:] == 9.0).all()
+
+
 @pytest.mark.parametrize("M", [1, 16, 33, 100, 300])
 def test_rows_do_not_touch_each_other(M):
     """A row of infinities and NaN, and blocks of zeros, leave the other rows' bits as they are; the rows behind the last are not written."""

@@ -182,9 +182,10 @@ __device__ __forceinline__ void mark_experts(const MoeArgs& g, int first, int n,
 // Whether slot i (its token's j-th choice) is the first of its token with that expert: a later one only adds its weight.
 __device__ __forceinline__ bool first_of_token(const int* ids, int i, int k) {
     const int e = ids[i], begin = i - i % k;
-    for (int o = begin; o < i; o++)
-        if (ids[o] == e) return false;
-    return true;
+    bool first = true;
+#pragma unroll 4
+    for (int o = 0; o < k; o++) first &= ids[begin + o] != e || begin + o >= i;  // (no way out before the end: the loads do not wait for one another)
+    return first;
 }
 
 // How a wavefront reads 16 columns x KU of k of packed weights, and the tokens' values beside them: each step is one
@@ -266,8 +267,9 @@ __global__ __launch_bounds__(512) void moe_up_kernel(const MoeArgs g, int col_un
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int expert, count;
     if (tokens == 1) {  // its slots are the chosen experts themselves
-        expert = a < n ? g.ids[first + a] : -1;
-        if ((unsigned)expert >= (unsigned)g.E || !first_of_token(g.ids + first, a, g.k)) expert = -1;
+        const int mine = lane < n ? g.ids[first + lane] : -1;
+        expert = a < n ? __builtin_amdgcn_readlane(mine, a) : -1;
+        if ((unsigned)expert >= (unsigned)g.E || __builtin_amdgcn_ballot_w64(lane < a && mine == expert)) expert = -1;
         count = 1;
         if (threadIdx.x == 0) list[0] = (uint16_t)a;
     } else {
@@ -379,6 +381,16 @@ __global__ __launch_bounds__(512) void moe_up_kernel(const MoeArgs g, int col_un
                 red[wave][2 * i + 1][lane] = acc[i][1];
             }
         }
+        // (fetched while the other wavefronts finish)
+        float weight = 0.0f;
+        if (threadIdx.x < 64 * MT && i0 + (int)(threadIdx.x >> 6) * 16 + c < count) {
+            const int slot = list[i0 + (threadIdx.x >> 6) * 16 + c], begin = first + slot - slot % g.k;
+#pragma unroll 4
+            for (int j = 0; j < g.k; j++) {
+                const float w = g.weights[begin + j];
+                weight += g.ids[begin + j] == expert ? w : 0.0f;
+            }
+        }
         __syncthreads();
         // 64 lanes per 16 tokens: tile i, lane l holds columns 4 (l / 16) + 0..3 of its token l % 16
         if (threadIdx.x < 64 * MT) {
@@ -395,9 +407,6 @@ __global__ __launch_bounds__(512) void moe_up_kernel(const MoeArgs g, int col_un
                     }
                 }
                 const int slot = list[s];
-                float weight = 0.0f;
-                for (int o = slot - slot % g.k, j = 0; j < g.k; j++)
-                    if (g.ids[first + o + j] == expert) weight += g.weights[first + o + j];
                 uint16_t* const h = g.h + (int64_t)(first + slot) * 2 * g.I + u * 16 + quad * 4;
                 uint16_t hi[4], lo[4];
 #pragma unroll
@@ -433,51 +442,68 @@ __global__ __launch_bounds__(1024) void moe_down_kernel(const MoeArgs g) {
     const int t0 = blockIdx.y * MOE_GROUP, tokens = g.T - t0 < MOE_GROUP ? g.T - t0 : MOE_GROUP;
     const int first = t0 * g.k, n = tokens * g.k;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    for (int i = threadIdx.x; i < n; i += NW * 64) {
-        const int e = g.ids[first + i];
-        named[i] = (unsigned)e < (unsigned)g.E ? (uint16_t)e : NONE;  // (-1 or anything else out of range: no expert)
-        begins[i] = 0;
-    }
     for (int i = lane; i < TOKENS * 16; i += 64) (&part[wave][0][0])[i] = 0.0f;
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += NW * 64) {
-        uint16_t e = named[i];
-        for (int o = i - i % g.k; o < i; o++)
-            if (named[o] == e) e = NONE;  // (its token has named it before: that slot has both weights)
-        expert_at[i] = e;
-    }
-    __syncthreads();
-    for (int i = threadIdx.x; i < n; i += NW * 64) {
-        const uint16_t e = expert_at[i];
-        if (e != NONE) {
-            int before = 0, same = 0;
-#pragma unroll 4
-            for (int o = 0; o < n; o++) {
-                const uint16_t other = expert_at[o];
-                before += other < e;
-                same += other == e && o < i;
+    int experts;
+    if (tokens == 1) {  // every wavefront finds and writes all of it, the same, and waits for nobody
+        const int e = lane < n ? g.ids[first + lane] : -1;
+        bool counts = (unsigned)e < (unsigned)g.E;
+        for (int o = 0; o < n; o++) counts &= __builtin_amdgcn_readlane(e, o) != e || o >= lane;
+        const uint64_t all = __builtin_amdgcn_ballot_w64(counts);
+        const int place = __builtin_popcountll(all & ((1ull << lane) - 1));
+        experts = __builtin_popcountll(all);
+        if (counts) {
+            sorted[place] = (uint16_t)lane;
+            expert_at[lane] = (uint16_t)e;
+        }
+        if (lane <= experts) start[lane] = (uint16_t)lane;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    } else {
+        for (int i = threadIdx.x; i < n; i += NW * 64) {
+            const int e = g.ids[first + i];
+            named[i] = (unsigned)e < (unsigned)g.E ? (uint16_t)e : NONE;  // (-1 or anything else out of range: no expert)
+            begins[i] = 0;
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < n; i += NW * 64) {
+            uint16_t e = named[i];
+            for (int o = i - i % g.k; o < i; o++)
+                if (named[o] == e) e = NONE;  // (its token has named it before: that slot has both weights)
+            expert_at[i] = e;
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < n; i += NW * 64) {
+            const uint16_t e = expert_at[i];
+            if (e != NONE) {
+                int before = 0, same = 0;
+#pragma unroll 16
+                for (int o = 0; o < n; o++) {
+                    const uint16_t other = expert_at[o];
+                    before += other < e;
+                    same += other == e && o < i;
+                }
+                sorted[before + same] = (uint16_t)i;
+                if (same == 0) begins[before] = 1;
             }
-            sorted[before + same] = (uint16_t)i;
-            if (same == 0) begins[before] = 1;
         }
+        __syncthreads();
+        if (wave == 0) {
+            int count = 0, valid = 0;
+            for (int i0 = 0; i0 < n; i0 += 64) {
+                const bool is = i0 + lane < n && begins[i0 + lane];
+                const uint64_t has = __builtin_amdgcn_ballot_w64(is);
+                if (is) start[count + __builtin_popcountll(has & ((1ull << lane) - 1))] = (uint16_t)(i0 + lane);
+                count += __builtin_popcountll(has);
+                valid += __builtin_popcountll(__builtin_amdgcn_ballot_w64(i0 + lane < n && expert_at[i0 + lane] != NONE));
+            }
+            if (lane == 0) {
+                start[count] = (uint16_t)valid;
+                chosen = count;
+            }
+        }
+        __syncthreads();
+        experts = chosen;
     }
-    __syncthreads();
-    if (wave == 0) {
-        int count = 0, valid = 0;
-        for (int i0 = 0; i0 < n; i0 += 64) {
-            const bool is = i0 + lane < n && begins[i0 + lane];
-            const uint64_t has = __builtin_amdgcn_ballot_w64(is);
-            if (is) start[count + __builtin_popcountll(has & ((1ull << lane) - 1))] = (uint16_t)(i0 + lane);
-            count += __builtin_popcountll(has);
-            valid += __builtin_popcountll(__builtin_amdgcn_ballot_w64(i0 + lane < n && expert_at[i0 + lane] != NONE));
-        }
-        if (lane == 0) {
-            start[count] = (uint16_t)valid;
-            chosen = count;
-        }
-    }
-    __syncthreads();
-    const int experts = chosen;
 
     const int c = lane & 15, quad = lane >> 4, u = blockIdx.x, half = u & 1;
     const int kunits = (g.I + W::KU - 1) / W::KU;

@@ -116,12 +116,18 @@ __global__ void moe_topk_kernel(const double* __restrict__ logits, int E, int k,
     keys[e] = key;
     if (e < k) chosen[e] = 0.0f;
     __syncthreads();
+    // (equal ones go by their index: those of the wavefronts before this one are in front, of the later ones behind)
+    const int low = wave * 64, high = low + 64 < E ? low + 64 : E;
     int before = 0;
 #pragma unroll 8
-    for (int o = 0; o < E; o++) {
+    for (int o = 0; o < low; o++) before += keys[o] >= key;
+#pragma unroll 8
+    for (int o = low; o < high; o++) {
         const double other = keys[o];
         before += other > key || (other == key && o < e);
     }
+#pragma unroll 8
+    for (int o = high; o < E; o++) before += keys[o] > key;
     const bool mine = e < E && before < k;
     if (mine) chosen[before] = u;
     __syncthreads();

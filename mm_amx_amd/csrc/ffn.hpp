@@ -8,7 +8,6 @@
 namespace mmx {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
-typedef float f4 __attribute__((ext_vector_type(4)));
 
 // compile-time loop: f(integral_constant<int, B>) ... f(integral_constant<int, E - 1>), for arrays that have to stay in registers
 template <int B, int E, typename F>

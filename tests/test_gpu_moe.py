@@ -194,6 +194,27 @@ def test_values_past_the_largest_are_infinite(f8):
     assert (y[1, ::2] == 2.0 ** 22).all() and (y[1, 1::2] == -2.0 ** 22).all() and (y[2] == 0).all()
 
 
+@pytest.mark.parametrize("T,H", [(1, 200), (5, 1100), (40, 200), (33, 1100)])
+def test_scratch_of_any_contents_and_the_same_bits_each_time(T, H):
+    """Workgroups that share columns count in the scratch who is there: whatever it held, and in whichever order they come, the sums are the same."""
+    from mm_amx_amd import _lib as L
+    I, E, k = 96, 6, 3
+    moe, _ = layer(E, H, I, False, k)
+    x = normal((T, H), 5)
+    ids, w = mx.moe_route(x, moe.router, k)
+    want = mx.moe_experts(x, ids, w, moe.gate_up, moe.down, E, I)
+    need = L.lib().mmx_moe_experts_scratch_bytes(T, H, I, k)
+    y = torch.empty_like(x)
+    scratch = torch.empty(need + 64, dtype=torch.uint8, device="cuda")
+    for fill in (0, 1, 3, 0x7f, 0xff):
+        for _ in range(4):
+            scratch.fill_(fill)
+            y.fill_(7)
+            assert L.lib().mmx_moe_experts(L.BF16, x.data_ptr(), H * 2, ids.data_ptr(), w.data_ptr(), T, H, I, E, k, moe.gate_up.data_ptr(), None, moe.down.data_ptr(), None,
+                                           L.BF16, y.data_ptr(), H * 2, scratch.data_ptr(), need, torch.cuda.current_stream().cuda_stream) == 0
+            assert torch.equal(y, want) and (scratch[need:] == fill).all()
+
+
 def test_compressed_from_bf16_weights():
     E, H, I = 4, 256, 128
     wg, wu, wd, _, _ = experts(E, H, I, False)

@@ -112,6 +112,8 @@ class Matmul:
     def __call__(self, matA, matB, n0=None, n1=None, ppkernel=None):
         if ppkernel is None:
             raise L.MmxError("Matmul needs a post-op (BiasGeluStore)")
+        if torch.float8_e4m3fn in (matA.dtype, matB.dtype):
+            raise L.MmxError("Matmul: operands must be bf16, int8 or uint8 (e4m3 weights have scales: LinearFp8)")
         M, K = matA.shape
         Kb, N = (matB.shape[1], matB.shape[0]) if self.transposeB else matB.shape
         if K != Kb:

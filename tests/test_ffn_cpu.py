@@ -115,6 +115,20 @@ def test_python_refuses_what_is_not_on_the_gpu():
         mx.MLP().setup(w, w, w.t(), compress="int8")
 
 
+def test_the_other_operators_refuse_e4m3(lib):
+    for a in (torch.bfloat16, torch.int8, torch.uint8, torch.float8_e4m3fn):
+        A, B = torch.zeros((64, 128), dtype=a), torch.zeros((128, 64)).to(torch.float8_e4m3fn)
+        for const in (False, True):
+            with pytest.raises(mx.MmxError, match="e4m3"):
+                mx.Matmul(constB=const)(A, B, ppkernel=mx.BiasGeluStore(torch.zeros((64, 64))))
+    ep = L._Epilogue(0, 1, P, 1024, None, 1.0, None, 0.0, None)
+    for a, b in ((6, 6), (1, 6), (6, 1), (2, 6), (6, 2)):
+        refused(lib.mmx_gemm(a, b, P, 1024, P, 64, 128, 64, 0, 64, C.byref(ep), None), "dtype")
+    refused(lib.mmx_matvec(6, P, 1024, P, P, 64, 128, None), "dtype")
+    ep.out_dtype = 6
+    refused(lib.mmx_gemm(1, 1, P, 1024, P, 64, 128, 64, 0, 64, C.byref(ep), None), "dtype")
+
+
 def test_rows_from_elsewhere_are_padded():
     q = torch.arange(-60, 60, dtype=torch.float32).view(3, 40).to(torch.float8_e4m3fn)
     s = torch.ones((1, 3))

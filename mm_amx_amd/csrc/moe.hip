@@ -86,22 +86,24 @@ __global__ void moe_topk_kernel(const double* __restrict__ logits, int E, int k,
                                 int* __restrict__ ids, float* __restrict__ weights) {
     __shared__ double keys[MOE_EXPERTS];
     __shared__ double tops[MOE_EXPERTS / 64];
-    __shared__ float totals[MOE_EXPERTS / 64], chosen[MOE_TOP_K];
+    __shared__ float totals[MOE_EXPERTS / 64];
+    __shared__ double chosen[MOE_TOP_K];
     const int e = threadIdx.x, lane = e & 63, wave = e >> 6, waves = blockDim.x >> 6;
     const int64_t t = blockIdx.x;
     const double l = e < E ? logits[t * E + e] : -__builtin_inf();
     double top = l;
-    float total = 1.0f, u;
-    if (sigmoid) {
-        u = 1.0f / (1.0f + expf(-(float)l));
+    float total = 1.0f;
+    double u;
+    if (sigmoid) {  // (in 64 bits: in 32 all of a token's p are zero where its logits are below -104, and their shares 0 / 0)
+        u = 1.0 / (1.0 + exp(-l));
     } else {  // softmax's terms against the largest logit
 #pragma unroll
         for (int d = 32; d >= 1; d >>= 1) top = __builtin_fmax(top, __shfl_xor(top, d));
         if (lane == 0) tops[wave] = top;
         __syncthreads();
         for (int w = 0; w < waves; w++) top = __builtin_fmax(top, tops[w]);
-        u = e < E ? expf((float)(l - top)) : 0.0f;
-        total = u;
+        total = e < E ? expf((float)(l - top)) : 0.0f;
+        u = total;
 #pragma unroll
         for (int d = 32; d >= 1; d >>= 1) total += __shfl_xor(total, d);
         if (lane == 0) totals[wave] = total;
@@ -111,10 +113,10 @@ __global__ void moe_topk_kernel(const double* __restrict__ logits, int E, int k,
     }
     // (without a bias the logits have the order of the p, and no two of them meet in rounding)
     double key = l;
-    if (bias && e < E) key = (sigmoid ? 1.0 / (1.0 + exp(-l)) : exp(l - top) / (double)total) + (double)bias[e];
+    if (bias && e < E) key = (sigmoid ? u : exp(l - top) / (double)total) + (double)bias[e];
     if (!(key == key)) key = -__builtin_inf();
     keys[e] = key;
-    if (e < k) chosen[e] = 0.0f;
+    if (e < k) chosen[e] = 0.0;
     __syncthreads();
     // (equal ones go by their index: those of the wavefronts before this one are in front, of the later ones behind)
     const int low = wave * 64, high = low + 64 < E ? low + 64 : E;
@@ -132,10 +134,10 @@ __global__ void moe_topk_kernel(const double* __restrict__ logits, int E, int k,
     if (mine) chosen[before] = u;
     __syncthreads();
     if (mine) {
-        float sum = 0.0f;
+        double sum = 0.0;
         for (int j = 0; j < k; j++) sum += chosen[j];
         ids[t * k + before] = e;
-        weights[t * k + before] = scale * u / (renormalize ? sum : total);
+        weights[t * k + before] = (float)(scale * u / (renormalize ? sum : (double)total));
     }
 }
 

@@ -98,6 +98,16 @@ def test_route_ties_go_to_the_lowest_index():
     assert mx.moe_route(x, r, 4, scoring="sigmoid", bias=b)[0].cpu().tolist() == [[5, 70, 129, 0]] * 3
 
 
+def test_shares_of_small_sigmoids():
+    x, r = torch.ones((2, 64), dtype=torch.bfloat16, device="cuda"), torch.full((5, 64), -4.0, dtype=torch.bfloat16, device="cuda")
+    r[3, 0] = -3.0  # logits -256, and -255 for expert 3: p is e^-256 and e^-255
+    for bias in (None, torch.zeros(5, device="cuda")):
+        ids, w = mx.moe_route(x, r, 2, scoring="sigmoid", bias=bias)
+        assert ids.cpu().tolist() == [[3, 0]] * 2
+        want = torch.tensor([1 / (1 + np.exp(-1.0)), 1 / (1 + np.exp(1.0))]).float()
+        assert ((w.cpu() - want).abs() <= 2.0 ** -23 * want).all()
+
+
 def test_route_with_nan_stays_in_range():
     x, r = normal((4, 64), 1), normal((40, 64), 2, 0.2)
     want = mx.moe_route(x, r, 3)[0]

@@ -274,7 +274,7 @@ __global__ __launch_bounds__(512) void moe_up_kernel(const MoeArgs g, int col_un
     }
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int expert, count;
-    if (tokens == 1) {  // its slots are the chosen experts themselves
+    if (tokens == 1) {  // its slots are the chosen experts themselves (there are places for all of them)
         const int mine = lane < n ? g.ids[first + lane] : -1;
         expert = a < n ? __builtin_amdgcn_readlane(mine, a) : -1;
         if ((unsigned)expert >= (unsigned)g.E || __builtin_amdgcn_ballot_w64(lane < a && mine == expert)) expert = -1;
@@ -315,7 +315,7 @@ __global__ __launch_bounds__(512) void moe_up_kernel(const MoeArgs g, int col_un
         expert = found[0];
         count = found[1];
     }
-    if (expert < 0) return;  // (fewer experts were chosen than there are workgroups for)
+    if (expert < 0) return;  // (fewer experts were chosen than there are places for)
     expert = __builtin_amdgcn_readfirstlane(expert);
 
     const int c = lane & 15, quad = lane >> 4, half = u & 1;
@@ -669,8 +669,9 @@ int launch_moe_experts(bool f8, const void* x, int64_t ldx_bytes, const int* ids
     g.arrived = reinterpret_cast<int*>(g.parts + (int64_t)g.splits * T * H);
     const int64_t ku_h = f8 ? (H + 127) / 128 : (H + 63) / 64, ku_i = f8 ? (I + 127) / 128 : (I + 63) / 64;
     const unsigned groups = (unsigned)((T + MOE_GROUP - 1) / MOE_GROUP);
-    const int most = (T < MOE_GROUP ? T : MOE_GROUP) * k, units = I / 16;
-    const int64_t grid = (int64_t)(most < E ? most : E) * units;
+    // a place for each expert that a group's tokens can choose, and for each slot of a token alone in its group, which names experts more than once, or none, where k > E
+    const int most = (T < MOE_GROUP ? T : MOE_GROUP) * k, distinct = most < E ? most : E, units = I / 16;
+    const int64_t grid = (int64_t)(distinct > k ? distinct : k) * units;
     if (grid > 0x7fffffff || groups > 65535) return set_error(MMX_E_INVALID, "mmx_moe_experts: too many experts, columns or tokens for one launch");
     g.W = static_cast<const char*>(w_gate_up);
     g.panel_stride = ku_h * 4096;

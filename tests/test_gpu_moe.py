@@ -159,6 +159,41 @@ def test_choices_of_no_expert_the_same_twice_and_all_of_one(f8):
     assert (none == 0).all()
 
 
+def in_scratch_of(fill, moe, x, ids, w, E, H, I):
+    """moe_experts in scratch memory that holds these bytes, with a guard behind it."""
+    from mm_amx_amd import _lib as L
+    T, k = ids.shape
+    f8 = isinstance(moe.gate_up, tuple)
+    need = L.lib().mmx_moe_experts_scratch_bytes(T, H, I, k)
+    scratch = torch.full((need + 64,), fill, dtype=torch.uint8, device="cuda")
+    y = torch.empty((T, H), device="cuda")
+    gu, gs, d, ds = (*moe.gate_up, *moe.down) if f8 else (moe.gate_up, None, moe.down, None)
+    at = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    assert L.lib().mmx_moe_experts(L.F8 if f8 else L.BF16, x.data_ptr(), H * 2, ids.data_ptr(), w.data_ptr(), T, H, I, E, k, at(gu), at(gs), at(d), at(ds), L.F32, y.data_ptr(),
+                                   H * 4, scratch.data_ptr(), need, torch.cuda.current_stream().cuda_stream) == 0
+    assert (scratch[need:] == fill).all()
+    return y
+
+
+@pytest.mark.parametrize("T,E,choices", [
+    (1, 2, [-1, -1, 0, 1]), (1, 2, [0, 0, 1]), (1, 1, [-1, 5, 0]), (1, 1, [0, 0, 0]), (1, 3, [7, 1, 1, -1, 2, 0, 0, 1 << 30, 2]), (1, 6, [-1, 5, 5, 2]), (1, 6, [-1, -1]), (1, 16, [3] * 16),
+    (33, 2, [-1, -1, 0, 1]), (33, 2, [1, 1, 0]), (33, 3, [-1, -1, -1, 2, 2, 1]), (33, 8, [-1, 7, 7]), (2, 2, [-1, 1, 1, 0]), (65, 1, [-1, 0])])
+@pytest.mark.parametrize("f8", [False, True])
+def test_no_expert_and_the_same_twice_for_a_token_alone_in_its_group(T, E, choices, f8):
+    """Also where a token names more experts than there are, as a shard of a few of a layer's experts is asked: what one of them is not chosen for, the scratch's
+    old contents are not taken for."""
+    H, I, k = 72, 64, len(choices)
+    moe, full = layer(E, H, I, f8, 1)
+    x = normal((T, H), 5)
+    g = torch.Generator().manual_seed(6)
+    ids = torch.randint(-1, E + 1, (T, k), generator=g, dtype=torch.int32)
+    ids[0] = ids[T - 1] = torch.tensor(choices, dtype=torch.int32)
+    ids, w = ids.cuda(), torch.rand((T, k), generator=g).cuda()
+    want, bound = definition(u.f64(x), ids.cpu().numpy(), u.f64(w), full)
+    for fill in (0xff, 0x7f, 0):  # (0xffff is a NaN in bf16, 0x7f7f a large value)
+        u.close(in_scratch_of(fill, moe, x, ids, w, E, H, I), want, bound * 2, torch.float32, f"scratch {fill:#x}")
+
+
 @pytest.mark.parametrize("f8", [False, True])
 @pytest.mark.parametrize("T", [1, 5, 40])
 def test_layer(T, f8):

@@ -86,24 +86,22 @@ __global__ void moe_topk_kernel(const double* __restrict__ logits, int E, int k,
                                 int* __restrict__ ids, float* __restrict__ weights) {
     __shared__ double keys[MOE_EXPERTS];
     __shared__ double tops[MOE_EXPERTS / 64];
-    __shared__ float totals[MOE_EXPERTS / 64];
-    __shared__ double chosen[MOE_TOP_K];
+    __shared__ double totals[MOE_EXPERTS / 64];
+    __shared__ double chosen[MOE_TOP_K], chosen_l[MOE_TOP_K];  // their p (of softmax less the division) and their logits
     const int e = threadIdx.x, lane = e & 63, wave = e >> 6, waves = blockDim.x >> 6;
     const int64_t t = blockIdx.x;
     const double l = e < E ? logits[t * E + e] : -__builtin_inf();
-    double top = l;
-    float total = 1.0f;
-    double u;
-    if (sigmoid) {  // (in 64 bits: in 32 all of a token's p are zero where its logits are below -104, and their shares 0 / 0)
-        u = 1.0 / (1.0 + exp(-l));
+    double top = l, total = 1.0, u;
+    if (sigmoid) {
+        const double far = exp(-__builtin_fabs(l));  // (1 / (1 + e^-l) would be zero below -709)
+        u = (l < 0.0 ? far : 1.0) / (1.0 + far);
     } else {  // softmax's terms against the largest logit
 #pragma unroll
         for (int d = 32; d >= 1; d >>= 1) top = __builtin_fmax(top, __shfl_xor(top, d));
         if (lane == 0) tops[wave] = top;
         __syncthreads();
         for (int w = 0; w < waves; w++) top = __builtin_fmax(top, tops[w]);
-        total = e < E ? expf((float)(l - top)) : 0.0f;
-        u = total;
+        u = total = e < E ? exp(l - top) : 0.0;
 #pragma unroll
         for (int d = 32; d >= 1; d >>= 1) total += __shfl_xor(total, d);
         if (lane == 0) totals[wave] = total;
@@ -113,10 +111,9 @@ __global__ void moe_topk_kernel(const double* __restrict__ logits, int E, int k,
     }
     // (without a bias the logits have the order of the p, and no two of them meet in rounding)
     double key = l;
-    if (bias && e < E) key = (sigmoid ? u : exp(l - top) / (double)total) + (double)bias[e];
+    if (bias && e < E) key = u / total + (double)bias[e];
     if (!(key == key)) key = -__builtin_inf();
     keys[e] = key;
-    if (e < k) chosen[e] = 0.0;
     __syncthreads();
     // (equal ones go by their index: those of the wavefronts before this one are in front, of the later ones behind)
     const int low = wave * 64, high = low + 64 < E ? low + 64 : E;
@@ -131,13 +128,28 @@ __global__ void moe_topk_kernel(const double* __restrict__ logits, int E, int k,
 #pragma unroll 8
     for (int o = high; o < E; o++) before += keys[o] > key;
     const bool mine = e < E && before < k;
-    if (mine) chosen[before] = u;
+    if (mine) {
+        chosen[before] = u;
+        chosen_l[before] = l;
+    }
     __syncthreads();
     if (mine) {
-        double sum = 0.0;
-        for (int j = 0; j < k; j++) sum += chosen[j];
+        if (renormalize) {
+            // Shares are ratios, and a bias can choose experts whose p 32 bits cannot hold (from e^-104 on), nor 64 (e^-745).  Where even their sum is below 2^-700 every p is
+            // e^l times what all experts of the token share, to far more than 64 bits, and the terms are formed against the largest chosen logit.  Above that, a term
+            // that is no longer exact (below 2^-1022) is less than 2^-322 of the sum.
+            total = 0.0;
+            for (int j = 0; j < k; j++) total += chosen[j];
+            if (total < 0x1p-700) {
+                double largest = chosen_l[0];
+                for (int j = 1; j < k; j++) largest = __builtin_fmax(largest, chosen_l[j]);
+                u = exp(l - largest);
+                total = 0.0;
+                for (int j = 0; j < k; j++) total += exp(chosen_l[j] - largest);
+            }
+        }
         ids[t * k + before] = e;
-        weights[t * k + before] = (float)(scale * u / (renormalize ? sum : (double)total));
+        weights[t * k + before] = (float)(scale * u / total);
     }
 }
 

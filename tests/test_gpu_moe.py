@@ -108,6 +108,45 @@ def test_shares_of_small_sigmoids():
         assert ((w.cpu() - want).abs() <= 2.0 ** -23 * want).all()
 
 
+@pytest.mark.parametrize("logits,masked", [((0.0, -110.0, -112.0), 0), ((0.0, -102.0, -102.5), 0), ((3.0, -88.0, -90.0, -87.0), 0), ((0.0, -800.0, -801.0), 0),
+                                           ((300.0, -500.0, -501.0, -499.0), 0), ((0.0, -1.0, -2.0), 0), ((0.0, -30000.0, -30000.0), 0), ((-50.0, -50.0, 0.0), 2)])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("mask", [-float("inf"), -2.0])
+def test_shares_of_choices_far_below_the_largest(logits, masked, scoring, mask):
+    """A bias keeps the expert of the largest logit out: the shares of the others are what they are among themselves, however small their p.  e^x in 64 bits and
+    a sum of a few terms are off by less than 2^-45, so what counts is the rounding of a weight to 32 bits, half a step of 2^-24."""
+    E, k = len(logits), len(logits) - 1
+    x = torch.zeros((2, 64), dtype=torch.bfloat16, device="cuda")
+    x[:, 0] = x[:, 1] = 1
+    r = torch.zeros((E, 64), dtype=torch.bfloat16, device="cuda")
+    for e, l in enumerate(logits):  # (two summands of at most 8 bits each)
+        r[e, 0] = l
+        r[e, 1] = l - float(r[e, 0])
+    assert [float(v) for v in r.double().sum(1)] == list(logits)
+    bias = torch.zeros(E, device="cuda")
+    bias[masked] = mask
+    ids, w = mx.moe_route(x, r, k, scoring, True, 2.5, bias)
+    l = np.array(logits)
+    chosen = [e for e in range(E) if e != masked]
+    # log p but for what all experts of a token have in common
+    log_p = l if scoring == "softmax" else np.where(l < 0, l - np.log1p(np.exp(-np.abs(l))), -np.log1p(np.exp(-np.abs(l))))
+    share = np.exp(log_p - log_p[chosen].max())
+    share = 2.5 * share / share[chosen].sum()
+    for t in range(2):
+        assert sorted(ids[t].tolist()) == chosen
+        assert (np.abs(u.f64(w)[t] - share[ids[t].tolist()]) <= 2.0 ** -23 * share[ids[t].tolist()] + 2.0 ** -149).all(), (w[t], share[ids[t].tolist()])
+
+
+def test_shares_of_sigmoids_that_64_bits_cannot_hold():
+    x = torch.ones((2, 64), dtype=torch.bfloat16, device="cuda")
+    r = torch.zeros((5, 64), dtype=torch.bfloat16, device="cuda")
+    r[:, 0] = -2048.0
+    r[3, 1] = 1.0  # logits -2048, and -2047 for expert 3: e^-l is past the largest double
+    ids, w = mx.moe_route(x, r, 2, scoring="sigmoid")
+    want = torch.tensor([1 / (1 + np.exp(-1.0)), 1 / (1 + np.exp(1.0))]).float()
+    assert ids.cpu().tolist() == [[3, 0]] * 2 and ((w.cpu() - want).abs() <= 2.0 ** -23 * want).all()
+
+
 def test_route_with_nan_stays_in_range():
     x, r = normal((4, 64), 1), normal((40, 64), 2, 0.2)
     want = mx.moe_route(x, r, 3)[0]

@@ -307,7 +307,7 @@ int mmx_moe_route(const void* x, int64_t ldx_bytes, const void* router, int64_t 
 /* y[t] = sum over j of weights[t][j] * down_e( silu(gate_e . x[t]) * (up_e . x[t]) ), e = ids[t][j]; an id outside [0, E) stands for no
  * expert, one that a token names twice counts with both weights.  w_dtype MMX_BF16 (scales NULL) or MMX_F8; the weights of the experts lie one behind the
  * other: w_gate_up E times a pair of [H, 2 I] (mmx_repack_gate_up / _fp8, mmx_quantize_pack_fp8), w_down E times [I, H]
- * (mmx_repack_b of the torch layout [H, I] with transpose = 1), scales likewise.  I % 32 == 0.  x stays bf16, sums are
+ * (mmx_repack_b of the torch layout [H, I] with transpose = 1), scales likewise.  I % 32 == 0, and max(min(32 top_k, E), top_k) * I < 2^27.  x stays bf16, sums are
  * fp32, the intermediate enters the second product with 16 bits of mantissa.  Every chosen expert's weights are read once per 32 tokens:
  * for many tokens gather them by expert and use mmx_gemm.  scratch: 256-byte aligned device memory,
  * mmx_moe_experts_scratch_bytes() bytes, free to reuse once the call's work on `stream` has finished.  y MMX_BF16 or MMX_F32. */

@@ -15,6 +15,7 @@ constexpr int MOE_TOP_K = 16;   // experts of a token at most
 constexpr int MOE_EXPERTS = 1024;
 constexpr int MOE_SLOTS = MOE_GROUP * MOE_TOP_K;
 constexpr int MOE_SPLITS = 4;
+constexpr int MOST_GRID_Y = 65535;
 
 int num_cus();
 
@@ -158,12 +159,16 @@ int launch_moe_route(const void* x, int64_t ldx, const void* Wr, int64_t ldr, in
     const auto xp = static_cast<const uint16_t*>(x), wp = static_cast<const uint16_t*>(Wr);
     const unsigned gx = (unsigned)((E + 3) / 4);
     const int tb = (int64_t)T * E <= 2048 ? 1 : 4;  // (wavefronts for all CUs first, then less of the router read again)
-    const unsigned gy = (unsigned)((T + tb - 1) / tb);
-    if (gy > 65535) return set_error(MMX_E_INVALID, "mmx_moe_route: too many tokens for one launch");
-    if (tb == 1) hipLaunchKernelGGL(moe_logits_kernel<1>, dim3(gx, gy), dim3(256), 0, st, xp, ldx / 2, wp, ldr / 2, T, H, E, logits);
-    else hipLaunchKernelGGL(moe_logits_kernel<4>, dim3(gx, gy), dim3(256), 0, st, xp, ldx / 2, wp, ldr / 2, T, H, E, logits);
-    const int rc = check_hip(hipGetLastError(), "moe_logits_kernel launch");
-    if (rc) return rc;
+    for (int t0 = 0; t0 < T; t0 += MOST_GRID_Y * tb) {  // (one launch up to 262140 tokens)
+        const int n = T - t0 < MOST_GRID_Y * tb ? T - t0 : MOST_GRID_Y * tb;
+        const uint16_t* const from = xp + t0 * (ldx / 2);
+        double* const to = logits + (int64_t)t0 * E;
+        const dim3 grid(gx, (unsigned)((n + tb - 1) / tb));
+        if (tb == 1) hipLaunchKernelGGL(moe_logits_kernel<1>, grid, dim3(256), 0, st, from, ldx / 2, wp, ldr / 2, n, H, E, to);
+        else hipLaunchKernelGGL(moe_logits_kernel<4>, grid, dim3(256), 0, st, from, ldx / 2, wp, ldr / 2, n, H, E, to);
+        const int rc = check_hip(hipGetLastError(), "moe_logits_kernel launch");
+        if (rc) return rc;
+    }
     hipLaunchKernelGGL(moe_topk_kernel, dim3((unsigned)T), dim3((unsigned)((E + 63) / 64 * 64)), 0, st, logits, E, k, sigmoid, renormalize, scale, bias, ids, weights);
     return check_hip(hipGetLastError(), "moe_topk_kernel launch");
 }
@@ -663,9 +668,9 @@ size_t moe_scratch_bytes(int T, int H, int I, int k) {
     return moe_h_bytes(T, I, k) + (splits > 1 ? (size_t)splits * T * H * 4 + (size_t)((T + MOE_GROUP - 1) / MOE_GROUP) * ((H + 15) / 16) * 4 : 0);
 }
 
-int launch_moe_experts(bool f8, const void* x, int64_t ldx_bytes, const int* ids, const float* weights, int T, int H, int I, int E, int k,
-                       const void* w_gate_up, const float* s_gate_up, const void* w_down, const float* s_down, void* h, void* y, int64_t ldy, int y_f32,
-                       hipStream_t st) {
+static int launch_experts(bool f8, const void* x, int64_t ldx_bytes, const int* ids, const float* weights, int T, int H, int I, int E, int k,
+                          const void* w_gate_up, const float* s_gate_up, const void* w_down, const float* s_down, void* h, void* y, int64_t ldy, int y_f32,
+                          hipStream_t st) {
     MoeArgs g;
     g.x = static_cast<const uint16_t*>(x);
     g.ldx = ldx_bytes / 2;
@@ -684,7 +689,7 @@ int launch_moe_experts(bool f8, const void* x, int64_t ldx_bytes, const int* ids
     // a place for each expert that a group's tokens can choose, and for each slot of a token alone in its group, which names experts more than once, or none, where k > E
     const int most = (T < MOE_GROUP ? T : MOE_GROUP) * k, distinct = most < E ? most : E, units = I / 16;
     const int64_t grid = (int64_t)(distinct > k ? distinct : k) * units;
-    if (grid > 0x7fffffff || groups > 65535) return set_error(MMX_E_INVALID, "mmx_moe_experts: too many experts, columns or tokens for one launch");
+    if (grid * 512 > 0xffffffffll) return set_error(MMX_E_UNSUPPORTED, "mmx_moe_experts: %d experts at a time of I = %d columns are too many for one launch", (int)(grid / units), I);
     g.W = static_cast<const char*>(w_gate_up);
     g.panel_stride = ku_h * 4096;
     g.expert_bytes = g.panel_stride * (I / 32 * 2);
@@ -702,6 +707,19 @@ int launch_moe_experts(bool f8, const void* x, int64_t ldx_bytes, const int* ids
     const auto down = T <= 16 ? (f8 ? moe_down_kernel<W_fp8, 1> : moe_down_kernel<W_bf16, 1>) : f8 ? moe_down_kernel<W_fp8, 2> : moe_down_kernel<W_bf16, 2>;
     hipLaunchKernelGGL(down, dim3((unsigned)((H + 15) / 16), groups, (unsigned)g.splits), dim3(1024), 0, st, g);
     return check_hip(hipGetLastError(), "moe_down_kernel launch");
+}
+
+// One pair of launches up to 2097120 tokens.  The pairs take the scratch from its start, one behind the other on the stream; sums of split down products, which only the last
+// of them can have, are a megabyte at most behind its own rows of h, and there the scratch has the rows of the pairs before it.
+int launch_moe_experts(bool f8, const void* x, int64_t ldx_bytes, const int* ids, const float* weights, int T, int H, int I, int E, int k,
+                       const void* w_gate_up, const float* s_gate_up, const void* w_down, const float* s_down, void* h, void* y, int64_t ldy, int y_f32,
+                       hipStream_t st) {
+    constexpr int MOST = MOST_GRID_Y * MOE_GROUP;
+    int rc = MMX_OK;
+    for (int t0 = 0; t0 < T && !rc; t0 += MOST)
+        rc = launch_experts(f8, static_cast<const char*>(x) + t0 * ldx_bytes, ldx_bytes, ids + (int64_t)t0 * k, weights + (int64_t)t0 * k, T - t0 < MOST ? T - t0 : MOST, H, I, E, k,
+                            w_gate_up, s_gate_up, w_down, s_down, h, static_cast<char*>(y) + t0 * ldy, ldy, y_f32, st);
+    return rc;
 }
 
 }  // namespace mmx

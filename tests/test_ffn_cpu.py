@@ -88,6 +88,12 @@ def test_experts(lib):
     assert ex(T=0) == 0
 
 
+def test_experts_that_one_launch_cannot_take(lib):
+    """512 places of 2^14 workgroups of 512 threads are 2^32 of them."""
+    T, H, I, E, k = 32, 1, 1 << 18, 512, 16
+    refused(lib.mmx_moe_experts(1, P, 2, P, P, T, H, I, E, k, P, None, P, None, 1, P, 2, P, 1 << 62, None), "too many")
+
+
 def test_block_norm(lib):
     base = dict(f=P, ldf=256, res=P, ldres=256, pw=None, gate=None, ldg=0, nw=None, r=P, ldr=256, z=P, ldz=256, zs=None, ldzs=0, rt=1, zt=1, post=0, pre=1, scale=1.0, eps=1e-6, off=0.0)
 

@@ -299,6 +299,23 @@ def test_scratch_of_any_contents_and_the_same_bits_each_time(T, H):
             assert torch.equal(y, want) and (scratch[need:] == fill).all()
 
 
+def test_more_tokens_than_a_grid_has_rows():
+    """Launches are made for 262140 tokens (routing) and 2097120 (experts) at a time: the tokens on both sides of those borders, and the last ones."""
+    T, H, E, I = 2097120 + 33, 8, 4, 32
+    moe, full = layer(E, H, I, False, 1)
+    x = torch.randn((T, H), device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)).to(torch.bfloat16)
+    ids, w = mx.moe_route(x, moe.router, 1, renormalize=False)
+    y = mx.moe_experts(x, ids, w, moe.gate_up, moe.down, E, I)
+    at = torch.tensor([t for b in (4, 262140, 524280, 2097120, T) for t in range(b - 4, min(b + 4, T))])
+    xs, got = u.f64(x[at]), ids[at].cpu().numpy()
+    _, want_w, key = routing(xs, u.f64(moe.router), 1, "softmax", False, 1.0, None)
+    slack = 2 * 8 * u.U * (np.abs(xs) @ np.abs(u.f64(moe.router)).T).max()
+    assert (np.abs(np.take_along_axis(key, got, 1) - key.max(1, keepdims=True)) <= slack).all()
+    assert (np.abs(u.f64(w[at]) - want_w) <= 1e-5 * want_w + slack).all()
+    want, bound = definition(xs, got, u.f64(w[at]), full)
+    u.close(y[at], want, bound, torch.bfloat16)
+
+
 def test_compressed_from_bf16_weights():
     E, H, I = 4, 256, 128
     wg, wu, wd, _, _ = experts(E, H, I, False)

@@ -256,10 +256,15 @@ class MoE:
         if any(not isinstance(w, torch.Tensor) or w.dim() != 3 for w in (w_gate, w_up, w_down)):
             raise L.MmxError("setup: w_gate, w_up and w_down must be 3-D tensors, an expert each along the first")
         E, I, H = w_gate.shape
-        if tuple(w_up.shape) != (E, I, H) or tuple(w_down.shape) != (E, H, I) or tuple(router.shape) != (E, H):
+        if tuple(w_up.shape) != (E, I, H) or tuple(w_down.shape) != (E, H, I) or tuple(getattr(router, "shape", ())) != (E, H):
             raise L.MmxError("setup: w_up must be shaped as w_gate [E, I, H], w_down [E, H, I], router [E, H]")
         if I % 32 or 0 in (E, I, H):
             raise L.MmxError(f"setup: experts of {I} columns (a positive multiple of 32 is needed)")
+        if E > 1024 or not isinstance(self.top_k, int) or not 1 <= self.top_k <= min(E, 16):
+            raise L.MmxError(f"setup: top_k = {self.top_k} of {E} experts (up to 16 of up to 1024)")
+        ffn._gpu(router, "router", (torch.bfloat16,), 2)
+        if bias is not None and ffn._gpu(bias, "bias", (torch.float32,), 1).numel() != E:
+            raise L.MmxError(f"setup: bias holds {bias.numel()} values for {E} experts")
         if compress not in (None, "fp8") or (compress and scales is not None):
             raise L.MmxError("setup: compress is 'fp8', for weights that come without scales")
         f8 = scales is not None or compress == "fp8"

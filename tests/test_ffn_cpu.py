@@ -121,6 +121,15 @@ def test_python_refuses_what_is_not_on_the_gpu():
         mx.MLP().setup(w, w, w.t(), compress="int8")
 
 
+def test_the_experts_setup_refuses_what_run_could_not_take():
+    E, H, I = 4, 64, 32
+    w = [torch.zeros(s, dtype=torch.bfloat16) for s in ((E, I, H), (E, I, H), (E, H, I))]
+    router = torch.zeros((E, H), dtype=torch.bfloat16)
+    for top_k, r, word in ((2, router.float(), "router must be"), (2, [[0.0] * H] * E, "router"), (5, router, "top_k"), (0, router, "top_k"), (2.0, router, "top_k")):
+        with pytest.raises(mx.MmxError, match=word):
+            mx.MoE(top_k).setup(r, *w)
+
+
 def test_the_other_operators_refuse_e4m3(lib):
     for a in (torch.bfloat16, torch.int8, torch.uint8, torch.float8_e4m3fn):
         A, B = torch.zeros((64, 128), dtype=a), torch.zeros((128, 64)).to(torch.float8_e4m3fn)

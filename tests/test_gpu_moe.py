@@ -355,6 +355,16 @@ def test_graph_and_streams():
                 assert torch.equal(y, w) and torch.equal(eager, w)
 
 
+def test_setup_refuses_a_bias_that_run_could_not_take():
+    E, H, I = 4, 128, 64
+    wg, wu, wd, _, _ = experts(E, H, I, False)
+    router, b = normal((E, H), 1), torch.zeros(E, device="cuda")
+    for bias in (b.double(), b.half(), b[:3], b[None], b.cpu(), [0.0] * E):
+        with pytest.raises(mx.MmxError, match="bias"):
+            mx.MoE(2).setup(router, wg, wu, wd, bias=bias)
+    mx.MoE(2).setup(router, wg, wu, wd, bias=b)
+
+
 def test_refusals_on_the_gpu():
     E, H, I = 4, 128, 64
     moe, _ = layer(E, H, I, False)

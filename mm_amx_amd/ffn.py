@@ -133,7 +133,7 @@ def _given_scales(scales, what, N, K):
     _gpu(scales, f"{what}'s scales", (torch.float32,), 2)
     if tuple(scales.shape) != (_blocks(N), _blocks(K)):
         raise MmxError(f"{what}'s scales must be [{_blocks(N)}, {_blocks(K)}] for [{N}, {K}] weights, a block of 128 x 128 each")
-    return scales.contiguous()
+    return scales.detach().contiguous()  # (of a parameter: what is packed holds no graph)
 
 
 def pack_fp8(w, scales=None, out=None):

@@ -248,6 +248,27 @@ def test_linear_layer_takes_both_kinds_of_weights():
     assert torch.equal(y, y2)
 
 
+def test_scales_that_are_parameters():
+    """torch.nn.Parameter requires a gradient unless told otherwise: what is packed is not part of a graph, and layers over it can be copied."""
+    K, N = 256, 160
+    x, (w, s), (d, ds) = normal((3, K), 1), weight(N, K, 2), weight(K, N, 3)
+    p, dp = torch.nn.Parameter(s), torch.nn.Parameter(ds)
+    assert p.requires_grad
+    for packed, scales in (mx.pack_fp8(w, p), mx.pack_gate_up_fp8(w, w, (p, p))):
+        assert not packed.requires_grad and not scales.requires_grad
+    one, other = mx.LinearFp8(), mx.LinearFp8()
+    one.set_weight(w, p)
+    other.set_weight(w, s)
+    y, y2 = torch.empty((3, N), device="cuda"), torch.empty((3, N), device="cuda")
+    copy.deepcopy(one).forward(x, y)
+    other.forward(x, y2)
+    assert torch.equal(y, y2)
+    mlp, same = mx.MLP(), mx.MLP()
+    mlp.setup(w, w, d, scales=(p, p, dp))
+    same.setup(w, w, d, scales=(s, s, ds))
+    assert torch.equal(copy.deepcopy(mlp).run(x), same.run(x))
+
+
 @pytest.mark.parametrize("M,K,N", [(1, 256, 96), (7, 300, 352), (16, 1024, 512), (30, 640, 256), (100, 512, 384), (200, 260, 160), (513, 384, 1056)])
 def test_mlp(M, K, N):
     """Stage by stage: the intermediate that the gate/up product gives in fp32 is quantised to the same bits as by the quantiser.  Over both stages only

@@ -289,8 +289,8 @@ class MoE:
     def run(self, x, y=None):
         if self.gate_up is None:
             raise L.MmxError("run: setup has not been called")
-        if x.dim() != 2 or x.shape[1] != self.H:
-            raise L.MmxError(f"run: x must be [T, {self.H}]")
+        if type(x) is ffn.Fp8Rows or x.dim() != 2 or x.shape[1] != self.H:
+            raise L.MmxError(f"run: x must be a bf16 tensor [T, {self.H}] (quantised rows go to LinearFp8 and MLP)")
         return ffn.moe(x, self.router, self.top_k, self.gate_up, self.down, self.I, self.scoring, self.renormalize, self.scale, self.bias, y)
 
 

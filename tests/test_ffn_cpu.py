@@ -130,6 +130,13 @@ def test_the_experts_setup_refuses_what_run_could_not_take():
             mx.MoE(top_k).setup(r, *w)
 
 
+def test_the_experts_refuse_quantised_rows():
+    moe = mx.MoE(2)
+    moe.H, moe.gate_up = 128, torch.zeros(1, dtype=torch.uint8)
+    with pytest.raises(mx.MmxError, match="quantised rows"):
+        moe.run(mx.Fp8Rows.of(torch.zeros((3, 128), dtype=torch.uint8).view(torch.float8_e4m3fn), torch.ones((1, 3))))
+
+
 def test_the_other_operators_refuse_e4m3(lib):
     for a in (torch.bfloat16, torch.int8, torch.uint8, torch.float8_e4m3fn):
         A, B = torch.zeros((64, 128), dtype=a), torch.zeros((128, 64)).to(torch.float8_e4m3fn)

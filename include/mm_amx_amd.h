@@ -258,7 +258,9 @@ int mmx_mlp_splitk(const void* x, int64_t ldx_bytes, const void* w_gate_up, cons
 /* ==== the feed-forward block in 8-bit floating point (no counterpart in the reference) ==========================
  * Numbers of MMX_F8 (e4m3: 4 bits of exponent, 3 of mantissa, NaN, no infinities) come with fp32 scales, one for each block of
  * 128.  Activations [M, K]: scales[k / 128][m], rows of scales ld_scales (>= M) elements apart.  Weights [N, K]:
- * scales[n / 128][k / 128], contiguous; any values.  In a gate/up pair gate's rows of scales come first, then up's.
+ * scales[n / 128][k / 128], contiguous.  In a gate/up pair gate's rows of scales come first, then up's.  Both may have any values whose
+ * product is a normal number of fp32: the products multiply the two scales of a block first, so that one from 2^128 on is infinite (a NaN, where
+ * the block's sum is zero), and one below 2^-126 is rounded to a multiple of 2^-149, which is off by less than 2^-124 in the result.
  * Rows of quantised activations are 16-byte aligned and lie a multiple of 16 bytes apart; they hold ceil(K / 128) * 128 bytes, and
  * the bytes from K on must be zero (every entry point here that writes such rows writes them so).
  * With M (or T) = 0 these calls do nothing.  M < 2^22, N <= 2^26, K <= 2^22. */

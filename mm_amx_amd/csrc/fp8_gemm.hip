@@ -2,7 +2,7 @@
 //
 // v_mfma_f32_16x16x128_f8f6f4 multiplies one block of 128 k in one instruction, so its result, started from zero, is what the
 // two scales are applied to; the sums over the blocks are kept in 32 bits by vector instructions, 4 fused multiply-adds per MFMA
-// of 32 cycles.  The weights are the first operand: a lane then holds four neighbouring columns of one row of C, and its row's
+// of 32 cycles.  (By the product of both scales, a multiplication for each MFMA: one after the other would be four more of them.)  The weights are the first operand: a lane then holds four neighbouring columns of one row of C, and its row's
 // scale is one register for all of them.
 #include "ffn.hpp"
 

@@ -212,7 +212,7 @@ def _result(y, what, M, N):
 def gemm_fp8(A, Bpacked, b_scales, N, ep):
     """C = PP(A . B) in e4m3 with a scale for each block of 128: A [M, K] is Fp8Rows, or bf16 / fp32 and quantised on the way;
     Bpacked and b_scales from quantize_pack_fp8, pack_fp8 or, with PP_SILU_GATE, pack_gate_up_fp8 (N then counts both halves).
-    ep: PP_BIAS, PP_GELU or both, or PP_SILU_GATE alone, into bf16 or fp32."""
+    ep: PP_BIAS, PP_GELU or both, or PP_SILU_GATE alone, into bf16 or fp32.  The product of the scales that meet in a block is to be a normal number of fp32."""
     if not isinstance(ep, L.Epilogue):
         raise MmxError("ep must be an Epilogue")
     if L._native is not None and L._initialised and len(getattr(A, "shape", ())) == 2:

@@ -214,6 +214,22 @@ def test_rows_do_not_touch_each_other(M):
     assert (out[M // 2] == 0).all()
 
 
+@pytest.mark.parametrize("M", [1, 16, 20, 40, 100, 600])
+def test_scales_whose_products_are_at_the_ends_of_32_bits(M):
+    """Products of scales from 1.75 * 2^-126 to 1.5 * 2^127, bit for bit: values that are small multiples of 2^-9, so that a block's sum is exact and what is rounded is
+    its one product with the scales (subnormal for the least of them)."""
+    K, N = 128, 384
+    g = torch.Generator().manual_seed(M)
+    q, w = torch.randint(1, 8, (M, K), generator=g, dtype=torch.uint8), torch.randint(1, 8, (N, K), generator=g, dtype=torch.uint8)  # (codes of subnormals of e4m3)
+    sA = torch.tensor([2.0 ** 100, 2.0 ** -100, 1.0])[torch.arange(M) % 3][None]
+    sB = torch.tensor([[1.5 * 2.0 ** 27], [1.75 * 2.0 ** -26], [3.0]])
+    packed, scales = mx.pack_fp8(w.view(E4).cuda(), sB.cuda())
+    y = torch.empty((M, N), device="cuda")
+    mx.gemm_fp8(mx.Fp8Rows.of(q.view(E4).cuda(), sA.cuda()), packed, scales, N, mx.Epilogue(y, mx.PP_NONE))
+    sums = (q.double() @ w.double().t()) * 2.0 ** -18
+    assert torch.equal(y.cpu(), (sums * (sA.double().t() * sB.double()[:, 0].repeat_interleave(128))).float())
+
+
 def test_rows_from_elsewhere():
     """Values and scales that the quantiser did not make: any scales, rows of any stride and length."""
     g = torch.Generator().manual_seed(3)

@@ -195,6 +195,33 @@ def test_large_tiles(M, K, N, pair, tile):
     assert (wide[:, want.shape[1]:] == 9.0).all()
 
 
+@pytest.mark.parametrize("M,K,N,pair,kernel", [
+    (513, 1000, 4001, False, "64x128"), (700, 300, 2999, False, "64x128"), (200, 500, 11000, False, "64x128"), (513, 1000, 4032, True, "64x128"), (300, 260, 9024, True, "64x128"),
+    (129, 129, 15936, True, "64x128"), (65, 3100, 705, False, "64x64_shared_k"), (33, 2950, 130, False, "64x64_shared_k"), (33, 3100, 704, True, "64x64_shared_k"),
+    (70, 2950, 128, True, "64x64_shared_k"), (129, 1000, 300, False, "64x64"), (40, 1152, 576, True, "64x64"), (70, 130, 320, True, "64x64"),
+    (20, 300, 9000, False, "rows_32"), (31, 515, 70, False, "rows_32"), (17, 300, 640, True, "rows_32_pair"), (16, 1000, 65, False, "rows_16"), (9, 1000, 192, True, "rows_16_pair")])
+def test_every_kernel_that_products_choose(M, K, N, pair, kernel):
+    """Sizes with rows, k and columns left over, an even and an odd number of blocks of k.  N: packed columns."""
+    x = normal((M, K), 1)
+    rows = mx.quantize_fp8(x)
+    a = u.value_rows(bits(rows.q), u.f64(rows.scales))
+    if pair:
+        (g, gs), (v, vs) = weight(N // 2, K, 2), weight(N // 2, K, 3)
+        gs, vs = gs * 0.1, vs * 0.1
+        packed, s = mx.pack_gate_up_fp8(g, v, (gs, vs))
+        want, bound = u.gated(*u.product(a, u.f64(g) * u.spread(u.f64(gs), N // 2, K), 8), *u.product(a, u.f64(v) * u.spread(u.f64(vs), N // 2, K), 8))
+    else:
+        w, sw = weight(N, K, 2)
+        packed, s = mx.pack_fp8(w, sw)
+        want, bound = u.product(a, u.f64(w) * u.spread(u.f64(sw), N, K), 8)
+    for dtype in (torch.float32, torch.bfloat16):
+        y, wide = in_wide(torch.empty((M, want.shape[1]), dtype=dtype, device="cuda"), 3, 9.0)
+        mx.gemm_fp8(rows, packed, s, N, mx.Epilogue(y, mx.PP_SILU_GATE if pair else mx.PP_NONE))
+        assert mx.last_kernel() == f"fp8_{kernel}"
+        u.close(y, want, bound, dtype, kernel)
+        assert (wide[:, want.shape[1]:] == 9.0).all()
+
+
 @pytest.mark.parametrize("M", [1, 16, 33, 100, 300])
 def test_rows_do_not_touch_each_other(M):
     """A row of infinities and NaN, and blocks of zeros, leave the other rows' bits as they are; the rows behind the last are not written."""

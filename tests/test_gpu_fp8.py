@@ -334,6 +334,28 @@ def test_mlp(M, K, N):
     assert torch.equal(y32.to(torch.bfloat16), y)
 
 
+@pytest.mark.parametrize("M,K,N", [(1, 256, 96), (16, 300, 352), (30, 640, 256), (200, 260, 160), (513, 384, 1056)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_mlp_is_its_two_products_with_the_intermediate_quantised_from_32_bits(M, K, N, dtype):
+    """Step by step through the public calls, bit for bit.  (Rounded to bf16 on the way, a value of the intermediate may come to lie on the border between two of e4m3: some in a
+    hundred of them would go to the other one.)"""
+    x = mx.quantize_fp8(normal((M, K), 1))
+    ws = [weight(*shape, 5 + i) for i, shape in enumerate(((N, K), (N, K), (K, N)))]
+    (g, gs), (v, vs), (d, ds) = [(w, s * 0.2) for w, s in ws]
+    mlp = mx.MLP()
+    mlp.setup(g, v, d, scales=(gs, vs, ds))
+    y = mlp.run(x, torch.empty((M, K), dtype=dtype, device="cuda"))
+    h = torch.empty((M, N), device="cuda")
+    mx.gemm_fp8(x, *mx.pack_gate_up_fp8(g, v, (gs, vs)), 2 * N, mx.Epilogue(h, mx.PP_SILU_GATE))
+    hq, want = mx.quantize_fp8(h), torch.empty_like(y)
+    mx.gemm_fp8(hq, *mx.pack_fp8(d, ds), K, mx.Epilogue(want, mx.PP_NONE))
+    assert torch.equal(y, want)
+    value, bound = u.product(u.value_rows(bits(hq.q), u.f64(hq.scales)), u.f64(d) * u.spread(u.f64(ds), K, N), 8)
+    u.close(y, value, bound, dtype)
+    if M * N > 4000:
+        assert not torch.equal(mx.quantize_fp8(h.to(torch.bfloat16)).q.view(torch.uint8), hq.q.view(torch.uint8))
+
+
 def test_mlp_from_bf16_weights():
     M, K, N = 24, 256, 192
     x, w = normal((M, K), 1), [normal(s, 2 + i, 0.05) for i, s in enumerate(((N, K), (N, K), (K, N)))]

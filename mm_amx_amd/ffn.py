@@ -136,6 +136,15 @@ def _given_scales(scales, what, N, K):
     return scales.detach().contiguous()  # (of a parameter: what is packed holds no graph)
 
 
+def _packed_into(out, w, K, N, rows):
+    """The caller's (packed, scales), checked, or new ones."""
+    if out is None:
+        return torch.empty(L._packed_bytes_host(L.F8, K, N), dtype=torch.uint8, device=w.device), torch.empty((rows, _blocks(K)), device=w.device)
+    packed, scales = out
+    _packed(packed, scales, "out", K, N, rows)
+    return packed, scales
+
+
 def pack_fp8(w, scales=None, out=None):
     """Weights w [N, K] in torch's layout, bf16 (quantised here) or e4m3 with the scales [ceil(N / 128), ceil(K / 128)] they came with
     -> (packed, scales); out: where to put both."""
@@ -145,7 +154,7 @@ def pack_fp8(w, scales=None, out=None):
         _gpu(w, "weights with scales", (_E4M3,), 2)
         scales = _given_scales(scales, "weights", *w.shape)
     N, K = w.shape
-    packed, s = out or (torch.empty(L._packed_bytes_host(L.F8, K, N), dtype=torch.uint8, device=w.device), torch.empty((_blocks(N), _blocks(K)), device=w.device))
+    packed, s = _packed_into(out, w, K, N, _blocks(N))
     if scales is None:
         L._check(L.lib().mmx_quantize_pack_fp8(w.data_ptr(), _rows(w), K, N, 1, 0, packed.data_ptr(), s.data_ptr(), L._stream()))
     else:
@@ -166,7 +175,7 @@ def pack_gate_up_fp8(w_gate, w_up, scales=None, out=None):
     if scales is not None:
         scales = [_given_scales(s, n, N, K) for s, n in zip(scales, ("w_gate", "w_up"))]
     nb = _blocks(N)
-    packed, s = out or (torch.empty(L._packed_bytes_host(L.F8, K, 2 * N), dtype=torch.uint8, device=w_gate.device), torch.empty((2 * nb, _blocks(K)), device=w_gate.device))
+    packed, s = _packed_into(out, w_gate, K, 2 * N, 2 * nb)
     if scales is None:
         for pair, w in ((1, w_gate), (2, w_up)):
             L._check(L.lib().mmx_quantize_pack_fp8(w.data_ptr(), _rows(w), K, N, 1, pair, packed.data_ptr(), s.data_ptr(), L._stream()))

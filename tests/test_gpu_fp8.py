@@ -405,6 +405,24 @@ def test_nothing_to_do():
     mx.gemm_fp8(mx.quantize_fp8(x), packed, scales, 64, mx.Epilogue(torch.empty((0, 64), device="cuda"), mx.PP_NONE))
 
 
+def test_packing_into_what_is_too_small_or_of_another_kind_is_refused():
+    N, K = 96, 200
+    (w, s), b = weight(N, K, 1), normal((N, K), 2)
+    room = lambda n, rows: (torch.full((mx.packed_b_bytes(mx.F8, K, n) + 64,), 7, dtype=torch.uint8, device="cuda"), torch.zeros((rows, 2), device="cuda"))  # noqa: E731
+    for pack, given, n, rows in ((lambda out: mx.pack_fp8(w, s, out=out), mx.pack_fp8(w, s), N, 1), (lambda out: mx.pack_fp8(b, out=out), mx.pack_fp8(b), N, 1),
+                                 (lambda out: mx.pack_gate_up_fp8(w, w, (s, s), out=out), mx.pack_gate_up_fp8(w, w, (s, s)), 2 * N, 2),
+                                 (lambda out: mx.pack_gate_up_fp8(b, b, out=out), mx.pack_gate_up_fp8(b, b), 2 * N, 2)):
+        p, sc = room(n, rows)
+        need = p.numel() - 64
+        for bad in ((p[:need - 1], sc), (p[8:], sc), (p.view(torch.int8), sc), (p[:need].cpu(), sc), (p, sc[:, :1]), (p, sc.double()), (p, sc.t()[:, :1] if rows == 1 else sc.t()),
+                    (p, torch.zeros((rows, 4), device="cuda")[:, ::2])):
+            with pytest.raises(mx.MmxError):
+                pack(bad)
+        assert (p == 7).all()
+        pack((p, sc))
+        assert torch.equal(p[:need], given[0]) and (p[need:] == 7).all() and torch.equal(sc, given[1])
+
+
 def test_refusals_on_the_gpu():
     w, s = weight(96, 256, 1)
     packed, scales = mx.pack_fp8(w, s)

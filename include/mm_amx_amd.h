@@ -325,7 +325,8 @@ int mmx_moe_experts(int w_dtype, const void* x, int64_t ldx_bytes, const int32_t
  * f, gate and the weights are bf16, rows of f [M, H]; residual and r are both residual_dtype, MMX_BF16 or MMX_F32; z is MMX_BF16, or MMX_F8 with scales as
  * mmx_quantize_rows_fp8 gives them (of z in fp32).  NULL: residual (zero), gate (one), post_weight / pre_weight (the norm without weights), r or z (not
  * wanted; one of them is).  ld_gate_bytes = 0: one row of gate for all.  r may be residual itself; apart from that outputs overlap nothing.
- * H <= 32768. */
+ * H <= 32768.  The sums of squares are fp32: a row whose squares come to 2^128 or more (values of some 2^64 / sqrt(H)) is normed to zeros, and with
+ * eps = 0 one whose squares are too small for fp32 to infinities or NaN. */
 typedef struct mmx_block_norm_args {
     const void* f;
     int64_t ldf_bytes;

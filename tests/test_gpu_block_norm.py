@@ -124,6 +124,22 @@ def test_rows_do_not_touch_each_other(H):
     assert torch.isnan(z[3]).all() and torch.isnan(z[5]).all() and (z[7] == 0).all() and (r[7] == 0).all()
 
 
+@pytest.mark.parametrize("H", [128, 1000, 4096, 20000])
+def test_rows_whose_squares_32_bits_cannot_hold(H):
+    f, res = normal((6, H), 1), normal((6, H), 2, 1.0, torch.float32)
+    clean = mx.block_norm(f, res, post=True)
+    f[1] = 2.0 ** 64  # a square of 2^128 alone
+    f[4] = 0
+    f[4, H // 2] = -(2.0 ** 63)  # 2^126: not yet
+    r, z = mx.block_norm(f, res, post=True)
+    others = [0, 2, 3, 5]
+    assert torch.equal(r[others], clean[0][others]) and torch.equal(z[others], clean[1][others])
+    assert torch.equal(r[1], res[1])  # (what the norm made zeros of, added)
+    want = definition(u.f64(f), u.f64(res), True, None, None, 1.0, True, None, 1e-6, 0.0)
+    u.close(r[4:5], want[0][4:5], want[1][4:5], torch.float32)
+    u.close(z[4:5], want[2][4:5], want[3][4:5], torch.bfloat16)
+
+
 def test_a_block_as_it_is_used():
     """Norm and quantise, MLP on the quantised rows, the seam to a mixture of experts, and the last seam: each step against the step's own
     definition on what the step before it gave."""

@@ -300,7 +300,9 @@ int mmx_mlp_fp8(int x_dtype, const void* x, int64_t ldx_bytes, const float* x_sc
 /* ---- a mixture-of-experts layer for a few tokens -------------------------------------------------------------
  * Routing of T tokens x [T, H] bf16 over E experts, router [E, H] bf16: logits l = x . router^T, p = softmax(l) or, with MMX_MOE_SIGMOID, 1 / (1 + e^-l);
  * ids[t][0..top_k) = the experts of the largest p + bias (bias [E] or NULL), in descending order, the lowest index of equal ones (a NaN counts as the least);
- * weights[t][j] = scale * p, with MMX_MOE_RENORMALIZE divided by the sum of the chosen p.  1 <= top_k <= min(E, 16), E <= 1024.
+ * weights[t][j] = scale * p, with MMX_MOE_RENORMALIZE divided by the sum of the chosen p (also where the p themselves are too small for their type).
+ * A logit is a sum in 64 bits of sums of eight neighbouring h in fp32, everything behind it is in 64 bits: keys nearer to each other than what those eights are off can change places.
+ * 1 <= top_k <= min(E, 16), E <= 1024.
  * logits: scratch of T * E doubles. */
 enum { MMX_MOE_SIGMOID = 1, MMX_MOE_RENORMALIZE = 2 };
 int mmx_moe_route(const void* x, int64_t ldx_bytes, const void* router, int64_t ldr_bytes, int T, int H, int E, int top_k, int flags,
@@ -311,7 +313,7 @@ int mmx_moe_route(const void* x, int64_t ldx_bytes, const void* router, int64_t 
  * other: w_gate_up E times a pair of [H, 2 I] (mmx_repack_gate_up / _fp8, mmx_quantize_pack_fp8), w_down E times [I, H]
  * (mmx_repack_b of the torch layout [H, I] with transpose = 1), scales likewise.  I % 32 == 0, and max(min(32 top_k, E), top_k) * I < 2^27.  x stays bf16, sums are
  * fp32, the intermediate enters the second product with 16 bits of mantissa.  Every chosen expert's weights are read once per 32 tokens:
- * for many tokens gather them by expert and use mmx_gemm.  scratch: 256-byte aligned device memory,
+ * for many tokens gather them by expert, use mmx_gemm or mmx_gemm_fp8 and add up what comes out: nothing here does that.  scratch: 256-byte aligned device memory,
  * mmx_moe_experts_scratch_bytes() bytes, free to reuse once the call's work on `stream` has finished.  y MMX_BF16 or MMX_F32. */
 size_t mmx_moe_experts_scratch_bytes(int T, int H, int I, int top_k);
 int mmx_moe_experts(int w_dtype, const void* x, int64_t ldx_bytes, const int32_t* ids, const float* weights, int T, int H, int I, int E,

@@ -6,8 +6,9 @@ namespace mmx {
 // ---- activations ------------------------------------------------------------------------------------------------------
 // q[m][k] = e4m3(x[m][k] / s), s = scales[k / 128][m] the least power of two with which the block's largest magnitude is at most 448.
 // Eight lanes take a block of 128, 16 values each; neighbouring groups of lanes take neighbouring rows, so that a wavefront's eight scales are neighbours in memory too.  Past
-// the end of a row the bytes are zero up to the next multiple of 128: the products read whole blocks.  (2048 x 4096 bf16 7.4 us, 1024 x 11008 fp32 11.0 us, 5.1 TB/s, of which 2
-// are there for one row; four blocks of a row per group of lanes, to have more on its way, 7.4 and 11.0 too.)
+// the end of a row the bytes are zero up to the next multiple of 128: the products read whole blocks.  (Medians of a kernel trace: 2048 x 4096 bf16 8.3 us, or 10.0 from memory behind a
+// product that fills the caches; 1024 x 11008 fp32 11.1 us just after it was written, 5.1 TB/s, and 15.4 from memory; one row 2.6.  Four blocks of a row per group of lanes, to have more on
+// its way, were no faster.)
 template <typename T>
 __global__ __launch_bounds__(256) void quantize_rows_fp8_kernel(const T* __restrict__ x, int64_t ldx, int M, int K, char* __restrict__ q, int64_t ldq,
                                                                 float* __restrict__ scales, int64_t ld_s) {

@@ -220,8 +220,8 @@ __global__ __launch_bounds__(512) void fp8_rows_kernel(const Fp8Gemm g) {
 // first fragments are fetched beside the last rows' products.
 // KG groups of NW wavefronts, each with a ring of its own, take the blocks of k in turn where there are fewer tiles than CUs; their sums are added in LDS, in order.
 // What bounds it: beside a product of 32 cycles each of a SIMD's two wavefronts issues 6 or 7 vector instructions of 4 cycles, and the chip's power holds the clock at 2.0 GHz; a loop of
-// nothing but these products and multiply-adds runs at 3.2 PFLOP/s on random values, 4.3 on zeros.  8192 x 8192 x 8192 runs at 2.0, 4096 x 4096 x 4096 at 1.9, 2048 x 4096 x 11008, whose tiles
-// leave a fifth of the second round empty, at 1.65.  (Workgroups that walk over tiles, the next one's first loads on their way while results are stored: 0 to 2 %.)
+// nothing but these products and multiply-adds runs at 3.2 PFLOP/s on random values, 4.3 on zeros.  By card 8192 x 8192 x 8192 runs at 1.9 to 2.0, 4096 x 4096 x 4096 at 1.75 to 1.9, 2048 x 4096 x 11008,
+// whose tiles leave a fifth of the second round empty, at 1.6 (115 us; 100 to 107 where the operands stay in the caches, 7 more with a bias).  (Workgroups that walk over tiles, the next one's first loads on their way while results are stored: 0 to 2 %.)
 // Where the chunks of a row of A lie in LDS: chunk ^ turn(row), 0 ... 7.  An LDS cycle serves 16 lanes of a ds_read_b128, 256 bytes, and takes them as
 // lanes 0-3, 12-15, 20-23, 24-27 (and 4-11, 16-19, 28-31, and the same of the other half): eight rows' chunk c and the other eight's c ^ 2.  Two rows lie in
 // 256 bytes, so row / 2 has to be spread over the eight positions, the first eight's and the second's without a common one: {0, 1, 6, 7} go to {0, 1, 2, 3},
@@ -564,7 +564,8 @@ static int launch_rows(const Fp8Gemm& g, hipStream_t st, const char* name) {
 //      64 x 128           144 / 198 /   -  /  66 / 18 /  35 /  7.2 / 15
 //      64 x 64            199 / 305 /   -  /  85 / 18 /  30 /  7.0 / 13
 //      64 x 64, K shared  248 / 322 /   -  /  93 / 21 /  24 /  9.4 / 11
-// Over 60 products of 33 to 6000 rows, 200 to 11008 k and 200 to 16000 columns the tile chosen was 1.4 % behind the fastest on average, 12 % at most.
+// Over 60 products of 33 to 6000 rows, 200 to 11008 k and 200 to 16000 columns the tile chosen was 1.4 % behind the fastest on average, 12 % at most; over 66 gate/up pairs of 40 to 2048 rows, 300 to
+// 11008 k and 1408 to 22016 packed columns 0.5 %, 10 % at most (64 x 4096 x 22016 21.0 us, 19.1 in 64 x 128).
 struct TileCost {
     int bm, bn, per_cu;
     float fixed_us, stage_us, least;

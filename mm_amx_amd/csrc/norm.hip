@@ -77,7 +77,8 @@ struct Raw8 {
 };
 
 // TPR threads per row, each NC chunks of 8 neighbouring values: chunk threadIdx + TPR * i.  A block of 128 is 16 neighbouring threads.
-// Everything is asked for before the first sum: behind it, and the barrier in it, each of them would be one more trip to memory (one row of 4096 4.7 -> 3.9 us, 8192 rows 51 -> 44, 6.0 TB/s).
+// Everything is asked for before the first sum: behind it, and the barrier in it, each of them would be one more trip to memory (one row of 4096 1.2 times as long,
+// 8192 rows 1.15 times; now 3.2 and 47 us in a kernel trace, the latter 5.7 TB/s).
 template <typename TR, int TPR, int NC>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void block_norm_kernel(const NormArgs g) {
     constexpr int ROWS = TPR >= 256 ? 1 : 256 / TPR;

@@ -130,8 +130,9 @@ def test_shares_of_choices_far_below_the_largest(logits, masked, scoring, mask):
     chosen = [e for e in range(E) if e != masked]
     # log p but for what all experts of a token have in common
     log_p = l if scoring == "softmax" else np.where(l < 0, l - np.log1p(np.exp(-np.abs(l))), -np.log1p(np.exp(-np.abs(l))))
-    share = np.exp(log_p - log_p[chosen].max())
-    share = 2.5 * share / share[chosen].sum()
+    share = np.zeros(E)
+    share[chosen] = np.exp(log_p[chosen] - log_p[chosen].max())
+    share *= 2.5 / share.sum()
     for t in range(2):
         assert sorted(ids[t].tolist()) == chosen
         assert (np.abs(u.f64(w)[t] - share[ids[t].tolist()]) <= 2.0 ** -23 * share[ids[t].tolist()] + 2.0 ** -149).all(), (w[t], share[ids[t].tolist()])

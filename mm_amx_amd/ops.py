@@ -263,8 +263,6 @@ class MoE:
             raise L.MmxError("setup: w_up must be shaped as w_gate [E, I, H], w_down [E, H, I], router [E, H]")
         if I % 32 or 0 in (E, I, H):
             raise L.MmxError(f"setup: experts of {I} columns (a positive multiple of 32 is needed)")
-        if E > 1024 or not isinstance(self.top_k, int) or not 1 <= self.top_k <= min(E, 16):
-            raise L.MmxError(f"setup: top_k = {self.top_k} of {E} experts (up to 16 of up to 1024)")
         ffn._gpu(router, "router", (torch.bfloat16,), 2)
         if bias is not None and ffn._gpu(bias, "bias", (torch.float32,), 1).numel() != E:
             raise L.MmxError(f"setup: bias holds {bias.numel()} values for {E} experts")

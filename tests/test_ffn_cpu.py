@@ -125,9 +125,9 @@ def test_the_experts_setup_refuses_what_run_could_not_take():
     E, H, I = 4, 64, 32
     w = [torch.zeros(s, dtype=torch.bfloat16) for s in ((E, I, H), (E, I, H), (E, H, I))]
     router = torch.zeros((E, H), dtype=torch.bfloat16)
-    for top_k, r, word in ((2, router.float(), "router must be"), (2, [[0.0] * H] * E, "router"), (5, router, "top_k"), (0, router, "top_k"), (2.0, router, "top_k")):
+    for r, word in ((router.float(), "router must be"), ([[0.0] * H] * E, "router")):
         with pytest.raises(mx.MmxError, match=word):
-            mx.MoE(top_k).setup(r, *w)
+            mx.MoE(2).setup(r, *w)
 
 
 def test_the_experts_refuse_quantised_rows():

@@ -317,6 +317,20 @@ def test_more_tokens_than_a_grid_has_rows():
     u.close(y[at], want, bound, torch.bfloat16)
 
 
+@pytest.mark.parametrize("T", [1, 3, 33])
+def test_a_shard_of_a_layers_experts(T):
+    """Experts 4 to 6 of 12, packed by a layer of their own, whose tokens have eight choices each: ids less 4, and what is not theirs out of range."""
+    E, H, I, k = 12, 136, 64, 8
+    wg, wu, wd, _, full = experts(E, H, I, False)
+    router, x = normal((E, H), 9, 0.1), normal((T, H), 5)
+    shard = mx.MoE(k)
+    shard.setup(router[4:7], wg[4:7], wu[4:7], wd[4:7])
+    ids, w = mx.moe_route(x, router, k)
+    y = mx.moe_experts(x, ids - 4, w, shard.gate_up, shard.down, 3, I)
+    want, bound = definition(u.f64(x), ids.cpu().numpy() - 4, u.f64(w), [f[4:7] for f in full])
+    u.close(y, want, bound, torch.bfloat16)
+
+
 def test_compressed_from_bf16_weights():
     E, H, I = 4, 256, 128
     wg, wu, wd, _, _ = experts(E, H, I, False)

@@ -24,7 +24,8 @@ extern "C" {
 /* element types */
 enum { MMX_F32 = 0, MMX_BF16 = 1, MMX_I8 = 2, MMX_I32 = 3, MMX_I4 = 4 /* packed weights only */,
        MMX_U8 = 5 /* unsigned bytes: mmx_repack_b, mmx_gemm_u8, mmx_matvec_u8 only */,
-       MMX_F8 = 6 /* 8-bit floating point, e4m3 (largest value 448): mmx_repack_b and the entry points named fp8 or moe, mmx_block_norm */ };
+       MMX_F8 = 6 /* 8-bit floating point, e4m3 (largest value 448): mmx_repack_b and the entry points named fp8 or moe, mmx_block_norm */,
+       MMX_F4 = 7 /* microscaled 4-bit floating point, e2m1 with a scale for each 32: the entry points named mxfp4, mmx_block_norm */ };
 
 /* error codes */
 enum {
@@ -325,7 +326,7 @@ int mmx_moe_experts(int w_dtype, const void* x, int64_t ldx_bytes, const int32_t
  *     r = residual + scale * gate * u
  *     z = r (as it is in fp32)                                  or, with pre,   r / sqrt(mean(r^2) + eps) * (weight_offset + pre_weight)
  * f, gate and the weights are bf16, rows of f [M, H]; residual and r are both residual_dtype, MMX_BF16 or MMX_F32; z is MMX_BF16, or MMX_F8 with scales as
- * mmx_quantize_rows_fp8 gives them (of z in fp32).  NULL: residual (zero), gate (one), post_weight / pre_weight (the norm without weights), r or z (not
+ * mmx_quantize_rows_fp8 gives them (of z in fp32), or MMX_F4: mmx_mxfp4_bytes(M, H) bytes as mmx_quantize_mxfp4 writes them (ldz_bytes and z_scales are not used).  NULL: residual (zero), gate (one), post_weight / pre_weight (the norm without weights), r or z (not
  * wanted; one of them is).  ld_gate_bytes = 0: one row of gate for all.  r may be residual itself; apart from that outputs overlap nothing.
  * H <= 32768.  The sums of squares are fp32: a row whose squares come to 2^128 or more (values of some 2^64 / sqrt(H)) is normed to zeros, and with
  * eps = 0 one whose squares are too small for fp32 to infinities or NaN. */
@@ -349,6 +350,41 @@ typedef struct mmx_block_norm_args {
     float scale, eps, weight_offset;
 } mmx_block_norm_args;
 int mmx_block_norm(const mmx_block_norm_args* args, int M, int H, void* stream);
+
+/* ==== microscaled 4-bit floating point (no counterpart in the reference) ========================================
+ * Numbers of MMX_F4 are e2m1 (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), with a scale 2^(b - 127), b a byte (255: NaN), for each row and 32 of k.
+ * Activations [M, K] and weights [N, K] are laid out alike, "packed": a panel of 32 rows after the other; in it a chunk of 256 k after the other, 4352 bytes each:
+ * 4 steps of 64 k x 64 lanes x 16 bytes, where lane = row % 32 + 32 * ((k % 64) / 32) holds its 32 values two a byte, the first in the low half; then 64 lanes x 4 bytes,
+ * byte u the lane's b of step u.  Memory is mmx_mxfp4_bytes() bytes, 16-byte aligned; values from K up to the end of the chunk are zero with a scale that is not NaN (every
+ * entry point here that packs writes them so); rows from M up in the last panel may hold anything, and are not written.
+ * With M = 0 these calls do nothing.  M < 2^22 (weights: N <= 2^26), K <= 2^22. */
+size_t mmx_mxfp4_bytes(int64_t rows, int K);
+
+/* x [M, K] (MMX_BF16 or MMX_F32) -> packed: b is that of the least power of two, 2^-126 at least, with which the block's largest magnitude is less than 7, so that it
+ * rounds to 6 at most; values are x / scale to nearest even.  (x / scale is exact, so the result does not depend on how it is computed.)  A block that holds an
+ * infinity or a NaN gets the scale NaN; a magnitude from 3.5 * 2^126 on rounds to 2^128, which 32 bits cannot hold.  pair: 0; or 1 / 2: x is the gate / up half of a pair of M rows each (M % 32 == 0) and packed the whole pair's,
+ * mmx_mxfp4_bytes(2 M, K) bytes, in which gate's panels and up's alternate. */
+int mmx_quantize_mxfp4(int x_dtype, const void* x, int64_t ldx_bytes, int M, int K, int pair, void* packed, void* stream);
+/* The same from values and scales as checkpoints hold them: q [M, ceil(K / 2)] bytes, the value of the lower k in the low half, and scales [M, ceil(K / 32)] bytes; rows
+ * ldq_bytes and ld_scales_bytes apart.  And back (of a pair nothing: pair = 0). */
+int mmx_repack_mxfp4(const void* q, int64_t ldq_bytes, const void* scales, int64_t ld_scales_bytes, int M, int K, int pair, void* packed, void* stream);
+int mmx_unpack_mxfp4(const void* packed, int M, int K, void* q, int64_t ldq_bytes, void* scales, int64_t ld_scales_bytes, void* stream);
+/* packed -> the values in y [M, K], MMX_BF16 or MMX_F32 (rounded to nearest even where the type cannot hold them). */
+int mmx_dequantize_mxfp4(const void* packed, int M, int K, int y_dtype, void* y, int64_t ldy_bytes, void* stream);
+
+/* C = PP( A . B ), A [M, K] packed (MMX_F4; lda_bytes is not used), or MMX_BF16 / MMX_F32 rows, quantised as by mmx_quantize_mxfp4 on the way; B the packed weights [N, K].
+ * Sums are fp32 in the matrix cores, which apply the scales: a result is good to some 2^-20 of its largest partial sum.  ep: any of BIAS, GELU, or SILU_GATE
+ * alone (then B is a pair, N counts both and is a multiple of 64, and C has N / 2 columns); C fp32 or bf16.  scratch: 256-byte aligned device memory,
+ * mmx_gemm_mxfp4_scratch_bytes() bytes (0: none needed), free to reuse once the call's work on `stream` has finished.  C must not overlap A. */
+size_t mmx_gemm_mxfp4_scratch_bytes(int a_dtype, int M, int K, int N);
+int mmx_gemm_mxfp4(int a_dtype, const void* A, int64_t lda_bytes, const void* Bpacked, int M, int K, int N, const mmx_epilogue* ep, void* scratch,
+                   size_t scratch_bytes, void* stream);
+
+/* mmx_mlp over such weights: y [M, K] = down( silu(x . gate) * (x . up) ), both products as mmx_gemm_mxfp4; the fp32 result of the first is quantised without being
+ * rounded to bf16 in between.  x as A above; w_gate_up the pair of two [N, K], w_down [K, N], N % 32 == 0; y MMX_BF16 or MMX_F32. */
+size_t mmx_mlp_mxfp4_scratch_bytes(int x_dtype, int M, int K, int N);
+int mmx_mlp_mxfp4(int x_dtype, const void* x, int64_t ldx_bytes, const void* w_gate_up, const void* w_down, int y_dtype, void* y, int64_t ldy_bytes, int M, int K,
+                  int N, void* scratch, size_t scratch_bytes, void* stream);
 
 /* ---- introspection / tuning (no reference counterpart) --------------------------------------- */
 /* Force the MFMA tile shape ("256x256", "256x192", "128x256", "128x192", "128x128", "128x64", "64x128" (aligned

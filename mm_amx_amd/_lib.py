@@ -9,7 +9,7 @@ import warnings
 
 import torch
 
-F32, BF16, I8, I32, I4, U8, F8 = 0, 1, 2, 3, 4, 5, 6
+F32, BF16, I8, I32, I4, U8, F8, F4 = 0, 1, 2, 3, 4, 5, 6, 7
 PP_NONE, PP_DEQUANT, PP_BIAS, PP_GELU, PP_QUANT, PP_SILU_GATE = 0, 1, 2, 4, 8, 16
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -23,7 +23,9 @@ EXPORTS = ["mmx_last_error", "mmx_init", "mmx_packed_b_bytes", "mmx_repack_b", "
            "mmx_gemm_u8_scratch_bytes", "mmx_gemm_u8", "mmx_matvec_u8", "mmx_matvec", "mmx_mlp", "mmx_mlp_splitk", "mmx_set_tile",
            "mmx_set_option", "mmx_last_kernel",
            "mmx_quantize_rows_fp8", "mmx_quantize_pack_fp8", "mmx_repack_gate_up_fp8", "mmx_gemm_fp8_scratch_bytes", "mmx_gemm_fp8",
-           "mmx_mlp_fp8_scratch_bytes", "mmx_mlp_fp8", "mmx_moe_route", "mmx_moe_experts_scratch_bytes", "mmx_moe_experts", "mmx_block_norm"]
+           "mmx_mlp_fp8_scratch_bytes", "mmx_mlp_fp8", "mmx_moe_route", "mmx_moe_experts_scratch_bytes", "mmx_moe_experts", "mmx_block_norm",
+           "mmx_mxfp4_bytes", "mmx_quantize_mxfp4", "mmx_repack_mxfp4", "mmx_unpack_mxfp4", "mmx_dequantize_mxfp4", "mmx_gemm_mxfp4_scratch_bytes", "mmx_gemm_mxfp4",
+           "mmx_mlp_mxfp4_scratch_bytes", "mmx_mlp_mxfp4"]
 # measurement aids (include/mm_amx_amd_bench.h)
 BENCH_EXPORTS = ["mmx_time_gemm", "mmx_probe_mfma", "mmx_probe_read"]
 
@@ -74,7 +76,8 @@ def _host_module(l):
         l.mmx_gemm_splitk, l.mmx_gemm_workspace_bytes, l.mmx_gemm_unpacked, l.mmx_gemm_unpacked_workspace_bytes, l.mmx_matvec,
         l.mmx_packed_b_bytes, l.mmx_repack_b, l.mmx_quantize_weights_scratch, l.mmx_quantize_weights_scaled, l.mmx_quantize_pack_int4,
         l.mmx_quantize_pack_scaled, l.mmx_quantize_rows_fp8, l.mmx_gemm_fp8_scratch_bytes, l.mmx_gemm_fp8, l.mmx_mlp_fp8_scratch_bytes, l.mmx_mlp_fp8,
-        l.mmx_moe_route, l.mmx_moe_experts_scratch_bytes, l.mmx_moe_experts, l.mmx_block_norm)))
+        l.mmx_moe_route, l.mmx_moe_experts_scratch_bytes, l.mmx_moe_experts, l.mmx_block_norm,
+        l.mmx_mxfp4_bytes, l.mmx_quantize_mxfp4, l.mmx_gemm_mxfp4_scratch_bytes, l.mmx_gemm_mxfp4, l.mmx_mlp_mxfp4_scratch_bytes, l.mmx_mlp_mxfp4)))
     return _host_call
 
 
@@ -146,6 +149,15 @@ def lib():
         l.mmx_moe_experts_scratch_bytes.argtypes = [i, i, i, i]
         l.mmx_moe_experts.argtypes = [i, p, n, p, p, i, i, i, i, i, p, p, p, p, i, p, n, p, z, p]
         l.mmx_block_norm.argtypes = [C.POINTER(_BlockNorm), i, i, p]
+        l.mmx_mxfp4_bytes.restype = l.mmx_gemm_mxfp4_scratch_bytes.restype = l.mmx_mlp_mxfp4_scratch_bytes.restype = z  # (of mxfp4.py)
+        l.mmx_mxfp4_bytes.argtypes = [n, i]
+        l.mmx_quantize_mxfp4.argtypes = [i, p, n, i, i, i, p, p]
+        l.mmx_repack_mxfp4.argtypes = [p, n, p, n, i, i, i, p, p]
+        l.mmx_unpack_mxfp4.argtypes = [p, i, i, p, n, p, n, p]
+        l.mmx_dequantize_mxfp4.argtypes = [p, i, i, i, p, n, p]
+        l.mmx_gemm_mxfp4_scratch_bytes.argtypes = l.mmx_mlp_mxfp4_scratch_bytes.argtypes = [i, i, i, i]
+        l.mmx_gemm_mxfp4.argtypes = [i, p, n, p, i, i, i, C.POINTER(_Epilogue), p, z, p]
+        l.mmx_mlp_mxfp4.argtypes = [i, p, n, p, p, i, p, n, i, i, i, p, z, p]
         global _native
         _native = _host_module(l)
         _lib = l

@@ -100,6 +100,43 @@ __device__ __forceinline__ u32x4 to_fp8x16(const float (&v)[16], float inv) {
     return w;
 }
 
+// C[m][n .. n + 3] = PP(r); the caller has checked m < M.  n1: columns of the result.
+__device__ __forceinline__ void store4(const Epilogue& ep, int m, int n, int n1, const float (&r)[4]) {
+    char* const row = ep.C + (int64_t)m * ep.ldc;
+    if (ep.out_dtype == MMX_F32) {
+        float* const p = reinterpret_cast<float*>(row) + n;
+        if (n + 4 <= n1) {
+            const u32x4 w = {f2u(r[0]), f2u(r[1]), f2u(r[2]), f2u(r[3])};
+            __builtin_memcpy(__builtin_assume_aligned(p, 4), &w, 16);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (n + e < n1) p[e] = r[e];
+        }
+    } else {
+        uint16_t* const p = reinterpret_cast<uint16_t*>(row) + n;
+        if (n + 4 <= n1) {
+            const uint16_t w[4] = {to_bf16(r[0]), to_bf16(r[1]), to_bf16(r[2]), to_bf16(r[3])};
+            __builtin_memcpy(__builtin_assume_aligned(p, 2), w, 8);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (n + e < n1) p[e] = to_bf16(r[e]);
+        }
+    }
+}
+// bias and GELU of four neighbouring columns
+__device__ __forceinline__ void post4(const Epilogue& ep, int n, int n1, float (&r)[4]) {
+    if (ep.steps & MMX_PP_BIAS) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) r[e] = r[e] + ep.bias[n + e < n1 ? n + e : n1 - 1];
+    }
+    if (ep.steps & MMX_PP_GELU) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) r[e] = gelu_erf_minimax(r[e]);
+    }
+}
+
 // What the products in 8-bit floating point are made of.  A: rows of e4m3, lda bytes apart, 16-byte aligned, zero from K up to the
 // next multiple of 128; sA[kb * ld_sA + m].  Or, where fp8_takes_bf16(M, K), rows of K bf16 that lie anywhere, and sA = NULL.  B: packed as mmx_repack_b packs bytes; sB[row of B's scales][kb].
 struct Fp8Gemm {
@@ -138,7 +175,7 @@ struct NormArgs {
     int64_t ld_scales;
     float scale, eps, offset;
     int M, H;
-    int post, pre, z_f8;
+    int post, pre, z_type;  // of z: MMX_BF16, MMX_F8 or MMX_F4 (packed)
 };
 
 bool fp8_takes_bf16(int M, int K);

@@ -1,7 +1,7 @@
 // C ABI of the feed-forward block's operators: argument validation, scratch layout, dispatch.
 #include <string.h>
 
-#include "ffn.hpp"
+#include "mxfp4.hpp"
 
 namespace mmx {
 
@@ -18,6 +18,10 @@ int launch_moe_experts(bool f8, const void* x, int64_t ldx_bytes, const int* ids
                        hipStream_t st);
 size_t moe_scratch_bytes(int T, int H, int I, int k);
 int launch_block_norm(const NormArgs& g, bool residual_f32, hipStream_t st);
+int launch_quantize_mxfp4(bool f32, const void* x, int64_t ldx_bytes, int M, int K, int pair, void* out, hipStream_t st);
+int launch_dequantize_mxfp4(const void* in, int M, int K, bool f32, void* y, int64_t ldy_bytes, hipStream_t st);
+int launch_repack_mxfp4(bool to_layout, void* q, int64_t ldq, void* scales, int64_t lds, int M, int K, int pair, void* packed, hipStream_t st);
+int launch_gemm_mxfp4(const Mxfp4Gemm& g, hipStream_t st);
 
 static bool misaligned(const void* p, int to) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(to - 1)) != 0; }
 static int64_t padded_k(int K) { return ((int64_t)K + BLOCK - 1) / BLOCK * BLOCK; }
@@ -111,6 +115,52 @@ static int check_a(const char* who, int dtype, const void* A, int64_t lda, const
     if (dtype != MMX_BF16 && dtype != MMX_F32) return set_error(MMX_E_INVALID, "%s: activations of dtype %d (bf16, fp32 and e4m3 exist)", who, dtype);
     if (scales) return set_error(MMX_E_INVALID, "%s: scales come with e4m3 activations only", who);
     return check_rows(who, "A", A, lda, M, K, dtype == MMX_F32 ? 4 : 2);
+}
+
+// ---- microscaled 4-bit floating point
+static int check_mxfp4(const char* who, const char* what, const void* packed) {
+    if (!packed) return set_error(MMX_E_INVALID, "%s: %s is NULL", who, what);
+    if (misaligned(packed, 16)) return set_error(MMX_E_INVALID, "%s: %s must be 16-byte aligned", who, what);
+    return MMX_OK;
+}
+static int check_a_mxfp4(const char* who, int dtype, const void* A, int64_t lda, int M, int K) {
+    if (dtype == MMX_F4) return check_mxfp4(who, "A", A);
+    if (dtype != MMX_BF16 && dtype != MMX_F32) return set_error(MMX_E_INVALID, "%s: activations of dtype %d (bf16, fp32 and packed e2m1 exist)", who, dtype);
+    return check_rows(who, "A", A, lda, M, K, dtype == MMX_F32 ? 4 : 2);
+}
+static int check_pair_mxfp4(const char* who, int pair, int M) {
+    if (pair < 0 || pair > 2 || (pair && M % 32)) return set_error(MMX_E_INVALID, "%s: pair = %d, %d rows (a half of a pair has a multiple of 32)", who, pair, M);
+    return MMX_OK;
+}
+static int check_sizes_mxfp4(const char* who, int64_t rows, int K) {
+    if (rows < 0 || K <= 0) return set_error(MMX_E_INVALID, "%s: K must be positive and the rows not negative (got %lld x %d)", who, (long long)rows, K);
+    if (rows > MOST_N || K > MOST_K) return set_error(MMX_E_UNSUPPORTED, "%s: up to %d rows and K up to %d (got %lld x %d)", who, MOST_N, MOST_K, (long long)rows, K);
+    return MMX_OK;
+}
+// codes and scales as checkpoints hold them
+static int check_codes(const char* who, const void* q, int64_t ldq, const void* scales, int64_t lds, int M, int K) {
+    const int rc = check_rows(who, "q", q, ldq, M, ((int64_t)K + 1) / 2, 1);
+    return rc ? rc : check_rows(who, "scales", scales, lds, M, ((int64_t)K + MX_BLOCK - 1) / MX_BLOCK, 1);
+}
+// A packed: as given, or made in scratch; or as bf16 rows that the product quantises itself
+static int packed_rows(int dtype, const void* A, int64_t lda, int M, int K, void* scratch, Mxfp4Gemm* g, hipStream_t st) {
+    g->a_bf16 = dtype == MMX_BF16 && mx_takes_bf16(M, K);
+    g->A = static_cast<const char*>(A);
+    g->lda = g->a_bf16 ? lda : mx_bytes(32, K);
+    if (dtype == MMX_F4 || g->a_bf16) return MMX_OK;
+    g->A = static_cast<const char*>(scratch);
+    return launch_quantize_mxfp4(dtype == MMX_F32, A, lda, M, K, 0, scratch, st);
+}
+static void weights_mxfp4(const void* Bp, int M, int K, int N, bool pair, const Epilogue& ep, Mxfp4Gemm* g) {
+    g->B = static_cast<const char*>(Bp);
+    g->ldb = mx_bytes(32, K);
+    g->M = M, g->N = N, g->K = K;
+    g->chunks = (int)mx_chunks(K);
+    g->npanels = (N + 31) / 32;
+    g->pair = pair;
+    g->packed_out = nullptr;
+    g->ld_out = 0;
+    g->ep = ep;
 }
 
 }  // namespace mmx
@@ -270,7 +320,8 @@ int mmx_block_norm(const mmx_block_norm_args* a, int M, int H, void* stream) {
     if (rc) return rc;
     if (H > 32768) return set_error(MMX_E_UNSUPPORTED, "%s: H = %d, 32768 at most", who, H);
     if (a->residual_dtype != MMX_BF16 && a->residual_dtype != MMX_F32) return set_error(MMX_E_INVALID, "%s: residual of dtype %d (bf16 and fp32 exist)", who, a->residual_dtype);
-    if (a->z && a->z_dtype != MMX_BF16 && a->z_dtype != MMX_F8) return set_error(MMX_E_INVALID, "%s: z of dtype %d (bf16 and e4m3 exist)", who, a->z_dtype);
+    if (a->z && a->z_dtype != MMX_BF16 && a->z_dtype != MMX_F8 && a->z_dtype != MMX_F4)
+        return set_error(MMX_E_INVALID, "%s: z of dtype %d (bf16, e4m3 and packed e2m1 exist)", who, a->z_dtype);
     if (!a->r && !a->z) return set_error(MMX_E_INVALID, "%s: neither r nor z is wanted", who);
     if ((a->post_weight && !a->post) || (a->pre_weight && !a->pre)) return set_error(MMX_E_INVALID, "%s: weights of a norm that is off", who);
     if (M == 0) return MMX_OK;
@@ -282,6 +333,7 @@ int mmx_block_norm(const mmx_block_norm_args* a, int M, int H, void* stream) {
     if (misaligned(a->post_weight, 2) || misaligned(a->pre_weight, 2)) return set_error(MMX_E_INVALID, "%s: weights are not aligned to their element size", who);
     if (a->z && a->z_dtype == MMX_BF16 && (rc = check_rows(who, "z", a->z, a->ldz_bytes, M, H, 2))) return rc;
     if (a->z && a->z_dtype == MMX_F8 && (rc = check_rows_fp8(who, "z", a->z, a->ldz_bytes, a->z_scales, a->ld_z_scales, M, H))) return rc;
+    if (a->z && a->z_dtype == MMX_F4 && misaligned(a->z, 16)) return set_error(MMX_E_INVALID, "%s: packed z must be 16-byte aligned", who);
     NormArgs g;
     g.f = static_cast<const uint16_t*>(a->f);
     g.ld_f = a->ldf_bytes / 2;
@@ -300,8 +352,106 @@ int mmx_block_norm(const mmx_block_norm_args* a, int M, int H, void* stream) {
     g.scale = a->scale, g.eps = a->eps, g.offset = a->weight_offset;
     g.M = M, g.H = H;
     g.post = a->post, g.pre = a->pre;
-    g.z_f8 = a->z && a->z_dtype == MMX_F8;
+    g.z_type = a->z_dtype;
+    if (a->z && a->z_dtype == MMX_F4) g.ld_z = mx_bytes(32, H);
     return launch_block_norm(g, a->residual_dtype == MMX_F32, static_cast<hipStream_t>(stream));
+}
+
+size_t mmx_mxfp4_bytes(int64_t rows, int K) { return rows <= 0 || K <= 0 ? 0 : (size_t)mx_bytes(rows, K); }
+
+int mmx_quantize_mxfp4(int x_dtype, const void* x, int64_t ldx_bytes, int M, int K, int pair, void* packed, void* stream) {
+    const char* const who = "mmx_quantize_mxfp4";
+    if (x_dtype != MMX_BF16 && x_dtype != MMX_F32) return set_error(MMX_E_INVALID, "%s: x of dtype %d (bf16 and fp32 exist)", who, x_dtype);
+    int rc = check_sizes_mxfp4(who, M, K);
+    if (rc || (rc = check_pair_mxfp4(who, pair, M)) || M == 0) return rc;
+    if ((rc = check_rows(who, "x", x, ldx_bytes, M, K, x_dtype == MMX_F32 ? 4 : 2)) || (rc = check_mxfp4(who, "packed", packed))) return rc;
+    return launch_quantize_mxfp4(x_dtype == MMX_F32, x, ldx_bytes, M, K, pair, packed, static_cast<hipStream_t>(stream));
+}
+
+int mmx_repack_mxfp4(const void* q, int64_t ldq_bytes, const void* scales, int64_t ld_scales_bytes, int M, int K, int pair, void* packed, void* stream) {
+    const char* const who = "mmx_repack_mxfp4";
+    int rc = check_sizes_mxfp4(who, M, K);
+    if (rc || (rc = check_pair_mxfp4(who, pair, M)) || M == 0) return rc;
+    if ((rc = check_codes(who, q, ldq_bytes, scales, ld_scales_bytes, M, K)) || (rc = check_mxfp4(who, "packed", packed))) return rc;
+    return launch_repack_mxfp4(true, const_cast<void*>(q), ldq_bytes, const_cast<void*>(scales), ld_scales_bytes, M, K, pair, packed, static_cast<hipStream_t>(stream));
+}
+
+int mmx_unpack_mxfp4(const void* packed, int M, int K, void* q, int64_t ldq_bytes, void* scales, int64_t ld_scales_bytes, void* stream) {
+    const char* const who = "mmx_unpack_mxfp4";
+    int rc = check_sizes_mxfp4(who, M, K);
+    if (rc || M == 0) return rc;
+    if ((rc = check_codes(who, q, ldq_bytes, scales, ld_scales_bytes, M, K)) || (rc = check_mxfp4(who, "packed", packed))) return rc;
+    return launch_repack_mxfp4(false, q, ldq_bytes, scales, ld_scales_bytes, M, K, 0, const_cast<void*>(packed), static_cast<hipStream_t>(stream));
+}
+
+int mmx_dequantize_mxfp4(const void* packed, int M, int K, int y_dtype, void* y, int64_t ldy_bytes, void* stream) {
+    const char* const who = "mmx_dequantize_mxfp4";
+    if (y_dtype != MMX_BF16 && y_dtype != MMX_F32) return set_error(MMX_E_INVALID, "%s: y of dtype %d (bf16 and fp32 exist)", who, y_dtype);
+    int rc = check_sizes_mxfp4(who, M, K);
+    if (rc || M == 0) return rc;
+    if ((rc = check_rows(who, "y", y, ldy_bytes, M, K, y_dtype == MMX_F32 ? 4 : 2)) || (rc = check_mxfp4(who, "packed", packed))) return rc;
+    return launch_dequantize_mxfp4(packed, M, K, y_dtype == MMX_F32, y, ldy_bytes, static_cast<hipStream_t>(stream));
+}
+
+size_t mmx_gemm_mxfp4_scratch_bytes(int a_dtype, int M, int K, int N) {
+    if (M <= 0 || K <= 0 || N <= 0 || (a_dtype != MMX_BF16 && a_dtype != MMX_F32) || (a_dtype == MMX_BF16 && mx_takes_bf16(M, K))) return 0;
+    return round256((size_t)mx_bytes(M, K));
+}
+
+int mmx_gemm_mxfp4(int a_dtype, const void* A, int64_t lda_bytes, const void* Bpacked, int M, int K, int N, const mmx_epilogue* ep_in, void* scratch,
+                   size_t scratch_bytes, void* stream) {
+    const char* const who = "mmx_gemm_mxfp4";
+    int rc = check_sizes(who, M, K, N);
+    if (rc || M == 0) return rc;
+    if ((rc = check_a_mxfp4(who, a_dtype, A, lda_bytes, M, K)) || (rc = check_mxfp4(who, "Bpacked", Bpacked))) return rc;
+    Epilogue ep;
+    if ((rc = make_epilogue(ep_in, MMX_BF16, MMX_F4, M, 0, N, &ep))) return rc;
+    if (ep.steps & (MMX_PP_DEQUANT | MMX_PP_QUANT)) return set_error(MMX_E_INVALID, "%s: the scales of the blocks take the place of DEQUANT, and there is no QUANT", who);
+    if (ep.out_dtype != MMX_F32 && ep.out_dtype != MMX_BF16) return set_error(MMX_E_INVALID, "%s: output dtype %d (bf16 and fp32 exist)", who, ep.out_dtype);
+    const bool pair = ep.steps & MMX_PP_SILU_GATE;
+    if (pair && (N % 64 || ep.steps != MMX_PP_SILU_GATE)) return set_error(MMX_E_INVALID, "%s: SILU_GATE stands alone and needs N %% 64 == 0 (got %d)", who, N);
+    if ((rc = check_scratch(who, scratch, scratch_bytes, mmx_gemm_mxfp4_scratch_bytes(a_dtype, M, K, N)))) return rc;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    Mxfp4Gemm g;
+    weights_mxfp4(Bpacked, M, K, N, pair, ep, &g);
+    if ((rc = packed_rows(a_dtype, A, lda_bytes, M, K, scratch, &g, st))) return rc;
+    return launch_gemm_mxfp4(g, st);
+}
+
+size_t mmx_mlp_mxfp4_scratch_bytes(int x_dtype, int M, int K, int N) {
+    if (M <= 0 || K <= 0 || N <= 0) return 0;
+    return mmx_gemm_mxfp4_scratch_bytes(x_dtype, M, K, N) + round256((size_t)mx_bytes(M, N));
+}
+
+int mmx_mlp_mxfp4(int x_dtype, const void* x, int64_t ldx_bytes, const void* w_gate_up, const void* w_down, int y_dtype, void* y, int64_t ldy_bytes, int M, int K,
+                  int N, void* scratch, size_t scratch_bytes, void* stream) {
+    const char* const who = "mmx_mlp_mxfp4";
+    int rc = check_sizes(who, M, K, N);
+    if (rc || M == 0) return rc;
+    if (N % 32 || N > MOST_K) return set_error(MMX_E_INVALID, "%s: N = %d must be a multiple of 32, %d at most", who, N, MOST_K);
+    if ((rc = check_a_mxfp4(who, x_dtype, x, ldx_bytes, M, K)) || (rc = check_mxfp4(who, "w_gate_up", w_gate_up)) || (rc = check_mxfp4(who, "w_down", w_down))) return rc;
+    if (y_dtype != MMX_F32 && y_dtype != MMX_BF16) return set_error(MMX_E_INVALID, "%s: output dtype %d (bf16 and fp32 exist)", who, y_dtype);
+    if ((rc = check_scratch(who, scratch, scratch_bytes, mmx_mlp_mxfp4_scratch_bytes(x_dtype, M, K, N)))) return rc;
+    mmx_epilogue e;
+    memset(&e, 0, sizeof e);
+    e.out_dtype = y_dtype;
+    e.C = y;
+    e.ldc_bytes = ldy_bytes;
+    Epilogue out;
+    if ((rc = make_epilogue(&e, MMX_BF16, MMX_F4, M, 0, K, &out))) return rc;
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    char* const h = static_cast<char*>(scratch) + mmx_gemm_mxfp4_scratch_bytes(x_dtype, M, K, N);
+    Epilogue mid;
+    memset(&mid, 0, sizeof mid);
+    mid.steps = MMX_PP_SILU_GATE;
+    Mxfp4Gemm g;
+    weights_mxfp4(w_gate_up, M, K, 2 * N, true, mid, &g);
+    g.packed_out = h;
+    g.ld_out = mx_bytes(32, N);
+    if ((rc = packed_rows(x_dtype, x, ldx_bytes, M, K, scratch, &g, st)) || (rc = launch_gemm_mxfp4(g, st))) return rc;
+    weights_mxfp4(w_down, M, N, K, false, out, &g);
+    if ((rc = packed_rows(MMX_F4, h, 0, M, N, nullptr, &g, st))) return rc;
+    return launch_gemm_mxfp4(g, st);
 }
 
 }  // extern "C"

@@ -10,43 +10,6 @@ namespace mmx {
 
 int num_cus();
 
-// C[m][n .. n + 3] = PP(r); the caller has checked m < M.  n1: columns of the result.
-__device__ __forceinline__ void store4(const Epilogue& ep, int m, int n, int n1, const float (&r)[4]) {
-    char* const row = ep.C + (int64_t)m * ep.ldc;
-    if (ep.out_dtype == MMX_F32) {
-        float* const p = reinterpret_cast<float*>(row) + n;
-        if (n + 4 <= n1) {
-            const u32x4 w = {f2u(r[0]), f2u(r[1]), f2u(r[2]), f2u(r[3])};
-            __builtin_memcpy(__builtin_assume_aligned(p, 4), &w, 16);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (n + e < n1) p[e] = r[e];
-        }
-    } else {
-        uint16_t* const p = reinterpret_cast<uint16_t*>(row) + n;
-        if (n + 4 <= n1) {
-            const uint16_t w[4] = {to_bf16(r[0]), to_bf16(r[1]), to_bf16(r[2]), to_bf16(r[3])};
-            __builtin_memcpy(__builtin_assume_aligned(p, 2), w, 8);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (n + e < n1) p[e] = to_bf16(r[e]);
-        }
-    }
-}
-// bias and GELU of four neighbouring columns
-__device__ __forceinline__ void post4(const Epilogue& ep, int n, int n1, float (&r)[4]) {
-    if (ep.steps & MMX_PP_BIAS) {
-#pragma unroll
-        for (int e = 0; e < 4; e++) r[e] = r[e] + ep.bias[n + e < n1 ? n + e : n1 - 1];
-    }
-    if (ep.steps & MMX_PP_GELU) {
-#pragma unroll
-        for (int e = 0; e < 4; e++) r[e] = gelu_erf_minimax(r[e]);
-    }
-}
-
 __device__ __forceinline__ i32x8 join(u32x4 a, u32x4 b) {
     return i32x8{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
 }

@@ -400,6 +400,12 @@ decltype(&mmx_moe_route) call_moe_route = nullptr;
 decltype(&mmx_moe_experts_scratch_bytes) call_moe_need = nullptr;
 decltype(&mmx_moe_experts) call_moe_experts = nullptr;
 decltype(&mmx_block_norm) call_block_norm = nullptr;
+decltype(&mmx_mxfp4_bytes) call_mxfp4_bytes = nullptr;
+decltype(&mmx_quantize_mxfp4) call_quantize_mxfp4 = nullptr;
+decltype(&mmx_gemm_mxfp4_scratch_bytes) call_gemm_mxfp4_need = nullptr;
+decltype(&mmx_gemm_mxfp4) call_gemm_mxfp4 = nullptr;
+decltype(&mmx_mlp_mxfp4_scratch_bytes) call_mlp_mxfp4_need = nullptr;
+decltype(&mmx_mlp_mxfp4) call_mlp_mxfp4 = nullptr;
 
 int64_t blocks(int64_t n) { return (n + 127) / 128; }
 
@@ -573,13 +579,100 @@ PyObject* moe(PyObject*, PyObject* const* a, Py_ssize_t count) {
     }
 }
 
-// block_norm(f, residual, post, post_weight, gate, scale, pre, pre_weight, eps, offset, quantize, r, device, stream) -> (r, z) or (r, padded rows of z, scales)
-//   r: where to put it, None: made here, False: not wanted
+// ---- microscaled 4-bit floating point: rows of bf16 or fp32 with (None, None), or packed rows with their (M, K)
+struct Rows4 {
+    const at::Tensor* t;
+    int dtype, M, K;
+    const void* data;
+    int64_t ld;
+};
+Rows4 rows4(PyObject* const* a, int device) {
+    if (a[1] == Py_None) {
+        const Matrix x = matrix(a[0], device);
+        return {x.t, float_code(*x.t), x.rows, x.cols, x.data, x.ld};
+    }
+    Rows4 r = {&tensor_on(a[0], device), MMX_F4, 0, 0, nullptr, 0};
+    if (!whole_number(a[1], 1, 1 << 30, r.M) || !whole_number(a[2], 1, 1 << 22, r.K)) throw Leave();
+    r.data = packed_bytes(a[0], device, (int64_t)call_mxfp4_bytes(r.M, r.K));
+    return r;
+}
+
+// quantize_mxfp4(x, device, stream) -> packed rows
+PyObject* quantize_mxfp4(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    if (count != 3 || !call_quantize_mxfp4) Py_RETURN_NONE;
+    try {
+        int device, rc = 0;
+        if (!whole_number(a[1], 0, 1 << 20, device)) throw Leave();
+        const Matrix x = matrix(a[0], device);
+        const int dt = float_code(*x.t);
+        void* const stream = stream_of(a[2]);
+        at::Tensor packed;
+        if (!unlocked([&] {
+                packed = make({(int64_t)call_mxfp4_bytes(x.rows, x.cols)}, at::kByte, *x.t);
+                rc = call_quantize_mxfp4(dt, x.data, x.ld, x.rows, x.cols, 0, packed.mutable_data_ptr(), stream);
+            })) throw Leave();
+        return rc ? PyLong_FromLong(rc) : THPVariable_Wrap(packed);
+    } catch (...) {
+        Py_RETURN_NONE;
+    }
+}
+
+// gemm_mxfp4(x, M, K, packed, N, device, stream, C, steps, bias, deq, deq_per_oc, q, q_per_oc)
+PyObject* gemm_mxfp4(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    if (count != 14 || !call_gemm_mxfp4) Py_RETURN_NONE;
+    int rc = 0;
+    try {
+        int N, device;
+        if (!whole_number(a[5], 0, 1 << 20, device) || !whole_number(a[4], 1, 1 << 30, N)) throw Leave();
+        const Rows4 x = rows4(a, device);
+        const mmx_epilogue e = epilogue_of(a + 7, device, x.M, N);
+        const at::Tensor& C = tensor_on(a[7], device);
+        if (C.size(0) != x.M || C.size(1) != (e.steps & MMX_PP_SILU_GATE ? N / 2 : N) || (a[9] != Py_None && tensor_on(a[9], device).numel() != N)) throw Leave();
+        const void* const w = packed_bytes(a[3], device, (int64_t)call_mxfp4_bytes(N, x.K));
+        void* const stream = stream_of(a[6]);
+        if (!unlocked([&] {
+                const size_t need = call_gemm_mxfp4_need(x.dtype, x.M, x.K, N);
+                at::Tensor scratch;
+                if (need) scratch = make({(int64_t)need}, at::kByte, *x.t);
+                rc = call_gemm_mxfp4(x.dtype, x.data, x.ld, w, x.M, x.K, N, &e, need ? scratch.mutable_data_ptr() : nullptr, need, stream);
+            })) throw Leave();
+    } catch (...) {
+        Py_RETURN_NONE;
+    }
+    return PyLong_FromLong(rc);
+}
+
+// mlp_mxfp4(x, M, K, gate_up, down, N, y, device, stream) -> y
+PyObject* mlp_mxfp4(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    if (count != 9 || !call_mlp_mxfp4) Py_RETURN_NONE;
+    try {
+        int N, device, rc = 0;
+        if (!whole_number(a[7], 0, 1 << 20, device) || !whole_number(a[5], 1, 1 << 29, N) || N % 32) throw Leave();
+        const Rows4 x = rows4(a, device);
+        const void* const gu = packed_bytes(a[3], device, (int64_t)call_mxfp4_bytes(2 * (int64_t)N, x.K));
+        const void* const d = packed_bytes(a[4], device, (int64_t)call_mxfp4_bytes(x.K, N));
+        void* const stream = stream_of(a[8]);
+        at::Tensor y = result(a[6], device, x.M, x.K);
+        if (!unlocked([&] {
+                if (!y.defined()) y = make({x.M, x.K}, at::kBFloat16, *x.t);
+                const size_t need = call_mlp_mxfp4_need(x.dtype, x.M, x.K, N);
+                const at::Tensor scratch = make({(int64_t)need}, at::kByte, *x.t);
+                rc = call_mlp_mxfp4(x.dtype, x.data, x.ld, gu, d, code_of(y.scalar_type()), y.mutable_data_ptr(), row_stride_bytes(y), x.M, x.K, N, scratch.mutable_data_ptr(), need,
+                                    stream);
+            })) throw Leave();
+        return rc ? PyLong_FromLong(rc) : THPVariable_Wrap(y);
+    } catch (...) {
+        Py_RETURN_NONE;
+    }
+}
+
+// block_norm(f, residual, post, post_weight, gate, scale, pre, pre_weight, eps, offset, quantize, r, device, stream) -> (r, z), (r, padded rows of z, scales) or (r, packed z)
+//   quantize: False, True (e4m3) or 2 (packed e2m1); r: where to put it, None: made here, False: not wanted
 PyObject* block_norm(PyObject*, PyObject* const* a, Py_ssize_t count) {
     if (count != 14 || !call_block_norm) Py_RETURN_NONE;
     try {
         int device, rc = 0;
-        if (!whole_number(a[12], 0, 1 << 20, device) || !PyBool_Check(a[2]) || !PyBool_Check(a[6]) || !PyBool_Check(a[10]) || !PyFloat_CheckExact(a[5]) ||
+        if (!whole_number(a[12], 0, 1 << 20, device) || !PyBool_Check(a[2]) || !PyBool_Check(a[6]) || !PyFloat_CheckExact(a[5]) ||
             !PyFloat_CheckExact(a[8]) || !PyFloat_CheckExact(a[9])) throw Leave();
         const Matrix f = matrix(a[0], device);
         const int64_t M = f.rows, H = f.cols;
@@ -621,7 +714,9 @@ PyObject* block_norm(PyObject*, PyObject* const* a, Py_ssize_t count) {
         n.scale = (float)PyFloat_AS_DOUBLE(a[5]);
         n.eps = (float)PyFloat_AS_DOUBLE(a[8]);
         n.weight_offset = (float)PyFloat_AS_DOUBLE(a[9]);
-        const bool quantize = a[10] == Py_True;
+        int two = 0;
+        if (!PyBool_Check(a[10]) && !whole_number(a[10], 2, 2, two)) throw Leave();
+        const bool quantize = a[10] == Py_True, packed = two == 2;
         const at::ScalarType stream_type = n.residual_dtype == MMX_F32 ? at::kFloat : at::kBFloat16;
         const bool keep = a[11] != Py_False;
         if (keep && a[11] != Py_None && same(a[11]).t->scalar_type() != stream_type) throw Leave();
@@ -634,7 +729,10 @@ PyObject* block_norm(PyObject*, PyObject* const* a, Py_ssize_t count) {
                     n.r = r.mutable_data_ptr();
                     n.ldr_bytes = row_stride_bytes(r);
                 }
-                if (quantize) {
+                if (packed) {
+                    z = make({(int64_t)call_mxfp4_bytes(M, (int)H)}, at::kByte, *f.t);
+                    n.z_dtype = MMX_F4;
+                } else if (quantize) {
                     const int64_t p = blocks(H) * 128;
                     z = make({M, p % 2048 ? p : p + 128}, at::kFloat8_e4m3fn, *f.t).narrow(1, 0, p);
                     s = make({blocks(H), M}, at::kFloat, *f.t);
@@ -658,11 +756,11 @@ PyObject* block_norm(PyObject*, PyObject* const* a, Py_ssize_t count) {
     }
 }
 
-// bind(addresses of the twenty entry points, in the order below)
+// bind(addresses of the entry points, in the order below)
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t count) {
-    constexpr int ENTRIES = 20;
+    constexpr int ENTRIES = 26;
     if (count != ENTRIES) {
-        PyErr_SetString(PyExc_TypeError, "bind takes twenty addresses");
+        PyErr_SetString(PyExc_TypeError, "bind takes an address for each entry point");
         return nullptr;
     }
     void* at[ENTRIES];
@@ -690,13 +788,20 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t count) {
     set(call_moe_need);
     set(call_moe_experts);
     set(call_block_norm);
+    set(call_mxfp4_bytes);
+    set(call_quantize_mxfp4);
+    set(call_gemm_mxfp4_need);
+    set(call_gemm_mxfp4);
+    set(call_mlp_mxfp4_need);
+    set(call_mlp_mxfp4);
     Py_RETURN_NONE;
 }
 
 #define METHOD(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {METHOD(gemm), METHOD(gemm_unpacked), METHOD(gemm_packing), METHOD(matvec), METHOD(repack), METHOD(quantize), METHOD(quantize_scaled),
                          METHOD(quantize_pack_int4), METHOD(quantize_pack_scaled), METHOD(quantize_fp8),
-                         METHOD(gemm_fp8), METHOD(mlp_fp8), METHOD(moe), METHOD(block_norm), METHOD(bind), {nullptr, nullptr, 0, nullptr}};
+                         METHOD(gemm_fp8), METHOD(mlp_fp8), METHOD(moe), METHOD(block_norm),
+                         METHOD(quantize_mxfp4), METHOD(gemm_mxfp4), METHOD(mlp_mxfp4), METHOD(bind), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host_call", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -1,0 +1,484 @@
+// Products in microscaled 4-bit floating point: C = PP( sum over blocks kb of 32 k of sA[m][kb] sB[n][kb] (A_kb . B_kb) ).
+//
+// The matrix cores apply both scales themselves, so all sums stay in them.  The weights are the first operand: a lane then holds neighbouring columns of one row of C.  An instruction's
+// sum came out within 2^-20 of its largest term over random values and scales, and exact wherever it can be held in 24 bits; scales of 255 make a NaN of their row, products from 2^128 on an infinity.
+#include "mxfp4.hpp"
+
+namespace mmx {
+
+int num_cus();
+
+typedef int i32x2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ i32x8 mx_operand(u32x4 a) { return i32x8{(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0}; }
+
+// ---- few rows: every wavefront multiplies its own chunks of k --------------------------------------------------------------
+// A workgroup computes 16 NT columns of 16 MT rows; its eight wavefronts take chunks of 256 k in turn, straight from memory into registers, and add their sums in LDS in the order of the
+// wavefronts.  The 16 x 16 x 128 form of the instruction (half the rate of the other, which does not matter here) lets a workgroup have half a panel.
+// PAIR: the four column tiles are both halves of a gate panel and of its up panel, 32 columns of the result, a whole block of it.
+// QUANTIZE: A is bf16 rows, which every workgroup quantises into LDS while its first weights are on their way.
+template <int MT, int NT, bool PAIR, bool QUANTIZE>
+__global__ __launch_bounds__(512) void mxfp4_rows_kernel(const Mxfp4Gemm g) {
+    static_assert(!PAIR || NT == 4, "both halves of a gate and an up panel");
+    constexpr int NW = 8;
+    __shared__ __attribute__((aligned(16))) f32x4 red[NW][MT * NT][64];
+    extern __shared__ __attribute__((aligned(16))) char rows[];  // QUANTIZE: M rows of pitch bytes, then their scales, M rows of 8 chunks bytes
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = lane & 15, quad = lane >> 4;
+    const int m0 = blockIdx.y * (16 * MT);
+    const int pitch = g.chunks * 128 + 16;  // (16 bytes more: neighbouring rows in other banks)
+    // this lane's place in a chunk: of its row c, block 4 kk + quad for the instructions kk = 0, 1
+    const uint32_t place = (quad >> 1) * 1024 + (quad & 1) * 512 + c * 16, scale_place = MX_SCALES_AT + (quad & 1) * 128 + c * 4;
+    const int turn = 8 * (quad >> 1);
+
+    const char* w_at[NT];
+#pragma unroll
+    for (int j = 0; j < NT; j++) {
+        const int tile = PAIR ? blockIdx.x * 4 + j : blockIdx.x * NT + j;
+        const int panel = tile >> 1 < g.npanels ? tile >> 1 : g.npanels - 1;
+        w_at[j] = g.B + (int64_t)panel * g.ldb + (tile & 1) * 256;  // (its scales: 64 bytes on)
+    }
+    const int w_scale = (int)scale_place;
+    const char* x_at[MT];
+#pragma unroll
+    for (int i = 0; i < MT; i++) {
+        int m = m0 + i * 16 + c;
+        m = m < g.M ? m : g.M - 1;
+        // (a row past the last one: the last again, never stored)
+        x_at[i] = QUANTIZE ? rows + m * pitch + quad * 16 : g.A + (int64_t)(m >> 5) * g.lda + ((m & 31) - c) * 16 + place;
+    }
+    f32x4 acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+        for (int j = 0; j < NT; j++) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    // U chunks: ch, ch + NW, ...
+    constexpr int U = MT * NT <= 2 ? 2 : 1;
+    auto load = [&](auto n_c, int ch, u32x4 (&w)[U][NT][2], uint32_t (&sw)[U][NT]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < decltype(n_c)::value; u++)
+#pragma unroll
+            for (int j = 0; j < NT; j++) {
+                const char* const p = w_at[j] + (int64_t)(ch + u * NW) * MX_CHUNK_BYTES;
+                w[u][j][0] = *reinterpret_cast<const u32x4*>(p + place);
+                w[u][j][1] = *reinterpret_cast<const u32x4*>(p + place + 2048);
+                const int half = (PAIR ? j : blockIdx.x * NT + j) & 1;
+                sw[u][j] = *reinterpret_cast<const uint32_t*>(p + w_scale - half * 192) >> turn;
+            }
+    };
+    auto multiply = [&](auto n_c, int ch, const u32x4 (&w)[U][NT][2], const uint32_t (&sw)[U][NT]) __attribute__((always_inline)) {
+        constexpr int N = decltype(n_c)::value;
+        u32x4 x[N][MT][2];
+        uint32_t sx[N][MT];
+#pragma unroll
+        for (int u = 0; u < N; u++)
+#pragma unroll
+            for (int i = 0; i < MT; i++) {
+                if constexpr (QUANTIZE) {
+                    int m = m0 + i * 16 + c;
+                    m = m < g.M ? m : g.M - 1;
+                    x[u][i][0] = *reinterpret_cast<const u32x4*>(x_at[i] + (ch + u * NW) * 128);
+                    x[u][i][1] = *reinterpret_cast<const u32x4*>(x_at[i] + (ch + u * NW) * 128 + 64);
+                    // bytes 0 and 2 are the ones that are taken
+                    const char* const s = rows + g.M * pitch + (m * g.chunks + ch + u * NW) * 8 + quad;
+                    sx[u][i] = (uint32_t)(uint8_t)s[0] | (uint32_t)(uint8_t)s[4] << 16;
+                } else {
+                    const char* const p = x_at[i] + (int64_t)(ch + u * NW) * MX_CHUNK_BYTES;
+                    x[u][i][0] = *reinterpret_cast<const u32x4*>(p);
+                    x[u][i][1] = *reinterpret_cast<const u32x4*>(p + 2048);
+                    int m = m0 + i * 16 + c;
+                    m = m < g.M ? m : g.M - 1;
+                    sx[u][i] = *reinterpret_cast<const uint32_t*>(p - place - ((m & 31) - c) * 12 + scale_place) >> turn;
+                }
+            }
+#pragma unroll
+        for (int u = 0; u < N; u++)
+#pragma unroll
+            for (int i = 0; i < MT; i++)
+#pragma unroll
+                for (int j = 0; j < NT; j++) {
+                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(w[u][j][0]), mx_operand(x[u][i][0]), acc[i][j], 4, 4, 0, (int)sw[u][j], 0, (int)sx[u][i]);
+                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(w[u][j][1]), mx_operand(x[u][i][1]), acc[i][j], 4, 4, 2, (int)sw[u][j], 2, (int)sx[u][i]);
+                }
+    };
+    typedef std::integral_constant<int, U> all_c;
+    typedef std::integral_constant<int, 1> one_c;
+    u32x4 w[U][NT][2];
+    uint32_t sw[U][NT];
+    int ch = wave;
+    if constexpr (QUANTIZE) {
+        const bool ahead = ch + (U - 1) * NW < g.chunks;
+        if (ahead) load(all_c(), ch, w, sw);
+        // four lanes a block
+        for (int b = threadIdx.x >> 2; b < g.M * g.chunks * 8; b += NW * 16) {
+            const int m = b / (g.chunks * 8), kb = b - m * (g.chunks * 8), part = threadIdx.x & 3;
+            float v[8];
+            load_row_f32(reinterpret_cast<const uint16_t*>(g.A + m * g.lda), kb * MX_BLOCK + part * 8, g.K, v);
+            uint32_t top = 0;
+#pragma unroll
+            for (int e = 0; e < 8; e++) top = umax(top, abs_bits(v[e]));
+#pragma unroll
+            for (int d = 1; d < 4; d *= 2) top = umax(top, (uint32_t)__shfl_xor((int)top, d));
+            const uint32_t s = mx_scale_of(top);
+            *reinterpret_cast<uint32_t*>(rows + m * pitch + kb * 16 + part * 4) = to_fp4x8(v, mx_value_of(s));
+            if (part == 0) rows[g.M * pitch + b] = (char)s;
+        }
+        __syncthreads();
+        if (ahead) {
+            multiply(all_c(), ch, w, sw);
+            ch += U * NW;
+        }
+    }
+    for (; ch + (U - 1) * NW < g.chunks; ch += U * NW) {
+        load(all_c(), ch, w, sw);
+        multiply(all_c(), ch, w, sw);
+    }
+    for (; ch < g.chunks; ch += NW) {
+        load(one_c(), ch, w, sw);
+        multiply(one_c(), ch, w, sw);
+    }
+
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+        for (int j = 0; j < NT; j++) red[wave][i * NT + j][lane] = acc[i][j];
+    __syncthreads();
+    auto sum = [&](int t, int l, float (&r)[4]) __attribute__((always_inline)) {
+        f32x4 s = red[0][t][l];
+#pragma unroll
+        for (int w = 1; w < NW; w++) {
+            const f32x4 a = red[w][t][l];
+#pragma unroll
+            for (int e = 0; e < 4; e++) s[e] = s[e] + a[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) r[e] = s[e];
+    };
+    if constexpr (PAIR) {
+        // 16 rows x 32 columns of the result: a row's columns 4 q ... 4 q + 3 of half h in lane l = 16 q + row % 16 of tile h; eight neighbouring threads take a row's eight fours
+        for (int t = threadIdx.x; t < MT * 128; t += NW * 64) {
+            const int row = t >> 3, part = t & 7, i = row >> 4, l = (part & 3) * 16 + (row & 15), half = part >> 2;
+            const int m = m0 + row;
+            float r[4], up[4];
+            sum(i * NT + half, l, r);
+            sum(i * NT + 2 + half, l, up);
+#pragma unroll
+            for (int e = 0; e < 4; e++) r[e] = silu32(r[e]) * up[e];
+            if (!g.packed_out) {
+                if (m < g.M) store4(g.ep, m, blockIdx.x * 32 + part * 4, g.N / 2, r);
+                continue;
+            }
+            uint32_t top = 0;
+#pragma unroll
+            for (int e = 0; e < 4; e++) top = umax(top, abs_bits(r[e]));
+#pragma unroll
+            for (int d = 1; d < 8; d *= 2) top = umax(top, (uint32_t)__shfl_xor((int)top, d));
+            const uint32_t s = mx_scale_of(top);
+            if (m < g.M) {
+                char* const panel = g.packed_out + (int64_t)(m >> 5) * g.ld_out;
+                const uint16_t w = (uint16_t)to_fp4x4(r[0], r[1], r[2], r[3], mx_value_of(s));
+                *reinterpret_cast<uint16_t*>(panel + mx_piece(m, blockIdx.x) + part * 2) = w;
+                if (part == 0) panel[mx_scale_at(m, blockIdx.x)] = (char)s;
+                if (blockIdx.x + 1 == gridDim.x) {  // what is left of the last chunk
+                    for (int kb = blockIdx.x + 1; kb & 7; kb++) {
+                        *reinterpret_cast<uint16_t*>(panel + mx_piece(m, kb) + part * 2) = 0;
+                        if (part == 0) panel[mx_scale_at(m, kb)] = 127;
+                    }
+                }
+            }
+        }
+    } else {
+        for (int u = threadIdx.x; u < MT * NT * 64; u += NW * 64) {
+            const int t = u >> 6, l = u & 63;
+            const int m = m0 + (t / NT) * 16 + (l & 15);
+            float r[4];
+            sum(t, l, r);
+            const int n = (blockIdx.x * NT + t % NT) * 16 + (l >> 4) * 4;
+            if (m < g.M && n < g.N) {
+                post4(g.ep, n, g.N, r);
+                store4(g.ep, m, n, g.N, r);
+            }
+        }
+    }
+}
+
+// ---- many rows: tiles ------------------------------------------------------------------------------------------------------
+// A workgroup computes 32 PM WGM rows x 32 PN WGN columns, a wavefront PM x PN panels of them.  A stage is a chunk of 256 k: all the tile's panels' 4 KiB of values one behind the other,
+// then their 256 bytes of scales, straight from memory into one of R slots of LDS; with the operands in the instruction's own order every LDS read is a KiB in a row.  A stage has four steps of 64 k;
+// the operands of a step are read during the one before.  The one barrier per stage stands in front of its last step: all of it has been read into registers then, so its slot is free for
+// stage t + R, whose loads are spread over the last step and the next stage's first two, and stage t + 1 has landed.
+template <int PM, int PN, int WGM, int WGN, int R>
+struct Mxfp4Tile {
+    static constexpr int NW = WGM * WGN, BM = 32 * PM * WGM, BN = 32 * PN * WGN;
+    static constexpr int PANELS = PM * WGM + PN * WGN;
+    static constexpr int SCALES = PANELS * 4096;          // their place in a stage
+    static constexpr int STAGE = SCALES + (PANELS + 3) / 4 * 1024;
+    static constexpr int BYTES = R * STAGE;
+    static constexpr int PIECES = PANELS * 4;             // KiB of values
+    static constexpr int DATA_LOADS = PIECES / NW, SCALE_LOADS = ((PANELS + 3) / 4 + NW - 1) / NW, LOADS = DATA_LOADS + SCALE_LOADS;
+    static_assert(PIECES % NW == 0 && BYTES <= 160 * 1024 && (R - 1) * LOADS < 64, "every wavefront issues the same number of loads, which a wait can count");
+};
+
+template <int PM, int PN, int WGM, int WGN, int R>
+__global__ __launch_bounds__(WGM * WGN * 64) void mxfp4_tile_kernel(const Mxfp4Gemm g, int tiles_m, int tiles_n, int total, int per_xcd) {
+    using T = Mxfp4Tile<PM, PN, WGM, WGN, R>;
+    constexpr int NW = T::NW, STAGE = T::STAGE, LOADS = T::LOADS, DATA = T::DATA_LOADS;
+    using lds_u32x4 = __attribute__((address_space(3))) const u32x4;
+    using lds_u32 = __attribute__((address_space(3))) const uint32_t;
+    extern __shared__ __attribute__((aligned(1024))) char smem[];
+    // Neighbouring workgroups go to different XCDs: each XCD gets a run of tiles, eight rows of them at a time and those fastest, so that the ones it works on share both operands in its L2.
+    const int L = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+    if (L >= total) return;
+    const int band = L / (8 * tiles_n), in_band = L - band * (8 * tiles_n), high = tiles_m - band * 8 < 8 ? tiles_m - band * 8 : 8;
+    const int tn = in_band / high, tm = band * 8 + in_band - tn * high;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wm = wave / WGN, wn = wave % WGN;
+    const int half = lane >> 5, c = lane & 31;
+    const int panel_m0 = tm * (PM * WGM), panel_n0 = tn * (PN * WGN), panels_m = (g.M + 31) >> 5;
+    const int steps = g.chunks;
+
+    // ---- loads: this wavefront's KiB of a stage.  A tile may reach past the last panel: that one again, never stored.
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem);
+    auto panel_at = [&](int p) __attribute__((always_inline)) {
+        if (p < PM * WGM) {
+            const int panel = panel_m0 + p < panels_m ? panel_m0 + p : panels_m - 1;
+            return g.A + (int64_t)panel * g.lda;
+        }
+        p -= PM * WGM;
+        const int panel = panel_n0 + p < g.npanels ? panel_n0 + p : g.npanels - 1;
+        return g.B + (int64_t)panel * g.ldb;
+    };
+    const char* from[LOADS];  // (uniform for values, each lane's own for scales)
+    uint32_t to[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; i++) {
+        if (i < DATA) {
+            const int piece = i * NW + wave;
+            from[i] = panel_at(piece >> 2) + (piece & 3) * 1024;
+            to[i] = lds0 + piece * 1024;
+        } else {
+            // 16 lanes a panel's scales; what is past the last group of four panels again
+            int group = (i - DATA) * NW + wave;
+            group = group < (T::PANELS + 3) / 4 ? group : (T::PANELS + 3) / 4 - 1;
+            const int p = group * 4 + (lane >> 4);
+            from[i] = panel_at(p < T::PANELS ? p : T::PANELS - 1) + MX_SCALES_AT + (lane & 15) * 16;
+            to[i] = lds0 + T::SCALES + group * 1024;
+        }
+    }
+    const uint32_t lane16 = lane * 16;
+    auto load = [&](auto ic, int t, int slot) __attribute__((always_inline)) {
+        constexpr int i = decltype(ic)::value;
+        const uint32_t dst = __builtin_amdgcn_readfirstlane(to[i] + slot * STAGE);
+        if constexpr (i < DATA) {
+            const char* const src = from[i] + (int64_t)t * MX_CHUNK_BYTES;
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(dst), "v"(lane16), "s"(src) : "memory");
+        } else {
+            const char* const src = from[i] + (int64_t)t * MX_CHUNK_BYTES;
+            asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(dst), "v"(src) : "memory");
+        }
+    };
+
+    f32x16 acc[PM][PN];
+#pragma unroll
+    for (int i = 0; i < PM; i++)
+#pragma unroll
+        for (int j = 0; j < PN; j++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) acc[i][j][e] = 0.0f;
+    u32x4 fa[2][PM], fb[2][PN];  // a step's operands, now and next
+    uint32_t sa[2][PM], sb[2][PN];
+    const uint32_t a_lane = wm * PM * 4096 + lane * 16, b_lane = (PM * WGM + wn * PN) * 4096 + lane * 16;
+    const uint32_t sa_lane = T::SCALES + wm * PM * 256 + lane * 4, sb_lane = T::SCALES + (PM * WGM + wn * PN) * 256 + lane * 4;
+    uint32_t at_a, at_b, at_sa, at_sb;
+    auto places = [&](int slot) __attribute__((always_inline)) {
+        const uint32_t st = lds0 + slot * STAGE;
+        at_a = st + a_lane, at_b = st + b_lane, at_sa = st + sa_lane, at_sb = st + sb_lane;
+        asm volatile("" : "+v"(at_a), "+v"(at_b), "+v"(at_sa), "+v"(at_sb));
+    };
+    auto read_a = [&](int i, int u) __attribute__((always_inline)) { return *reinterpret_cast<lds_u32x4*>(at_a + i * 4096 + u * 1024); };
+    auto read_b = [&](int j, int u) __attribute__((always_inline)) { return *reinterpret_cast<lds_u32x4*>(at_b + j * 4096 + u * 1024); };
+    auto read_sa = [&](int i) __attribute__((always_inline)) { return *reinterpret_cast<lds_u32*>(at_sa + i * 256); };
+    auto read_sb = [&](int j) __attribute__((always_inline)) { return *reinterpret_cast<lds_u32*>(at_sb + j * 256); };
+
+    unrolled<0, R>([&](auto rc) __attribute__((always_inline)) {
+        constexpr int r = decltype(rc)::value;
+        unrolled<0, LOADS>([&](auto ic) __attribute__((always_inline)) { if (r < steps) load(ic, r, r); });
+    });
+    if (steps >= R) asm volatile("s_waitcnt vmcnt(%0)" : : "n"((R - 1) * LOADS) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    places(0);
+#pragma unroll
+    for (int i = 0; i < PM; i++) {
+        fa[0][i] = read_a(i, 0);
+        sa[0][i] = read_sa(i);
+    }
+#pragma unroll
+    for (int j = 0; j < PN; j++) {
+        fb[0][j] = read_b(j, 0);
+        sb[0][j] = read_sb(j);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+
+    // One slot per MFMA, in this order and no other: the MFMA, an LDS read for the next step, a load.
+    constexpr int PER = PM * PN, READS = PM + PN;
+    int slot = 0;
+    // ODD: which set of scales the stage has
+    auto stage = [&](auto odd_c, int t) __attribute__((always_inline)) {
+        constexpr int S = decltype(odd_c)::value;
+        const int next = slot + 1 < R ? slot + 1 : 0, before = slot > 0 ? slot - 1 : R - 1;
+        const bool more_before = t > 0 && t - 1 + R < steps, more = t + R < steps;
+        unrolled<0, 4 * PER>([&](auto xc) __attribute__((always_inline)) {
+            constexpr int x = decltype(xc)::value, u = x / PER, y = x % PER, i = y / PN, j = y % PN;
+            if constexpr (x == 3 * PER) {
+                // all of this stage is in registers (its last step's operands arrive now); the next one has landed, R - 2 younger ones may be on their way
+                if (R > 2 && t + R - 1 < steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"((R - 2) * LOADS) : "memory");
+                else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                places(next);
+            }
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand(fb[u & 1][j]), mx_operand(fa[u & 1][i]), acc[i][j], 4, 4, u, (int)sb[S][j], u, (int)sa[S][i]);
+            asm volatile("" : "+v"(acc[i][j]));  // (else the compiler gathers the products behind the branches of the loads)
+            // the next step's operands (past the last stage what an earlier one left there: never used)
+            unrolled<0, READS>([&](auto rc) __attribute__((always_inline)) {
+                constexpr int r = decltype(rc)::value;
+                if constexpr (r * PER / READS == y) {
+                    // in the order in which the step uses them
+                    if constexpr (r == 0) fa[(u + 1) & 1][0] = read_a(0, (u + 1) & 3);
+                    else if constexpr (r <= PN) fb[(u + 1) & 1][r - 1] = read_b(r - 1, (u + 1) & 3);
+                    else fa[(u + 1) & 1][r - PN] = read_a(r - PN, (u + 1) & 3);
+                    if constexpr (u == 3) {
+                        if constexpr (r == 0) sa[S ^ 1][0] = read_sa(0);
+                        else if constexpr (r <= PN) sb[S ^ 1][r - 1] = read_sb(r - 1);
+                        else sa[S ^ 1][r - PN] = read_sa(r - PN);
+                    }
+                }
+            });
+            // stage t + R from the last step on; the rest of t - 1 + R before
+            unrolled<0, LOADS>([&](auto lc) __attribute__((always_inline)) {
+                constexpr int l = decltype(lc)::value, when = l * 3 * PER / LOADS;  // of three steps, the first of which is a stage's last
+                if constexpr (when < PER) {
+                    if constexpr (x == 3 * PER + when) {
+                        if (more) load(lc, t + R, slot);
+                    }
+                } else if constexpr (x == when - PER) {
+                    if (more_before) load(lc, t - 1 + R, before);
+                }
+            });
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        slot = next;
+    };
+    int t = 0;
+    for (; t + 2 <= steps; t += 2) {
+        stage(std::integral_constant<int, 0>(), t);
+        stage(std::integral_constant<int, 1>(), t + 1);
+    }
+    if (t < steps) stage(std::integral_constant<int, 0>(), t);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+
+    // ---- post-op: a lane holds columns 8 q + 4 half + 0..3, q = 0..3, of row c of each panel of 32 columns
+#pragma unroll
+    for (int i = 0; i < PM; i++) {
+        const int m = (panel_m0 + wm * PM + i) * 32 + c;
+        if (g.pair) {
+            if constexpr (PN % 2 == 0) {
+#pragma unroll
+                for (int j = 0; j < PN / 2; j++) {
+                    const int block = (panel_n0 + wn * PN) / 2 + j;  // of 32 columns of the result
+                    float r[16];
+#pragma unroll
+                    for (int e = 0; e < 16; e++) r[e] = silu32(acc[i][2 * j][e]) * acc[i][2 * j + 1][e];
+                    if (block * 64 >= g.N) continue;
+                    if (!g.packed_out) {
+                        if (m < g.M) {
+#pragma unroll
+                            for (int q = 0; q < 4; q++) {
+                                const float r4[4] = {r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]};
+                                store4(g.ep, m, block * 32 + q * 8 + half * 4, g.N / 2, r4);
+                            }
+                        }
+                        continue;
+                    }
+                    uint32_t top = 0;
+#pragma unroll
+                    for (int e = 0; e < 16; e++) top = umax(top, abs_bits(r[e]));
+                    top = umax(top, (uint32_t)__shfl_xor((int)top, 32));
+                    const uint32_t b = mx_scale_of(top);
+                    const float s = mx_value_of(b);
+                    uint32_t mine[2], other[2];
+#pragma unroll
+                    for (int q = 0; q < 2; q++)
+                        mine[q] = to_fp4x4(r[8 * q], r[8 * q + 1], r[8 * q + 2], r[8 * q + 3], s) | to_fp4x4(r[8 * q + 4], r[8 * q + 5], r[8 * q + 6], r[8 * q + 7], s) << 16;
+#pragma unroll
+                    for (int q = 0; q < 2; q++) other[q] = (uint32_t)__shfl_xor((int)mine[q], 32);
+                    if (half == 0 && m < g.M) {
+                        char* const panel = g.packed_out + (int64_t)(m >> 5) * g.ld_out;
+                        *reinterpret_cast<u32x4*>(panel + mx_piece(m, block)) =
+                            u32x4{(mine[0] & 0xffffu) | other[0] << 16, mine[0] >> 16 | (other[0] & 0xffff0000u), (mine[1] & 0xffffu) | other[1] << 16, mine[1] >> 16 | (other[1] & 0xffff0000u)};
+                        panel[mx_scale_at(m, block)] = (char)b;
+                        if ((block + 1) * 64 == g.N) {  // what is left of the last chunk
+                            for (int kb = block + 1; kb & 7; kb++) {
+                                *reinterpret_cast<u32x4*>(panel + mx_piece(m, kb)) = u32x4{0, 0, 0, 0};
+                                panel[mx_scale_at(m, kb)] = 127;
+                            }
+                        }
+                    }
+                }
+            }
+        } else if (m < g.M) {
+#pragma unroll
+            for (int j = 0; j < PN; j++) {
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const int n = (panel_n0 + wn * PN + j) * 32 + q * 8 + half * 4;
+                    if (n >= g.N) continue;
+                    float r[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+                    post4(g.ep, n, g.N, r);
+                    store4(g.ep, m, n, g.N, r);
+                }
+            }
+        }
+    }
+}
+
+template <int PM, int PN, int WGM, int WGN, int R>
+static int launch_tile(const Mxfp4Gemm& g, hipStream_t st, const char* name) {
+    using T = Mxfp4Tile<PM, PN, WGM, WGN, R>;
+    static std::atomic<uint64_t> done{0};
+    const auto kernel = mxfp4_tile_kernel<PM, PN, WGM, WGN, R>;
+    const int rc = ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), T::BYTES, done);
+    if (rc) return rc;
+    const int64_t tiles_m = (g.M + T::BM - 1) / T::BM, tiles_n = ((int64_t)g.npanels * 32 + T::BN - 1) / T::BN, total = tiles_m * tiles_n, per_xcd = (total + 7) / 8;
+    if (per_xcd * 8 * (T::NW * 64) > 0xffffffffll) return set_error(MMX_E_INVALID, "mmx_gemm_mxfp4: too many tiles for one launch");
+    note_kernel(name);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(per_xcd * 8)), dim3(T::NW * 64), T::BYTES, st, g, (int)tiles_m, (int)tiles_n, (int)total, (int)per_xcd);
+    return check_hip(hipGetLastError(), "mxfp4_tile_kernel launch");
+}
+
+static size_t quantized_in_lds(int M, int K) {
+    const size_t chunks = (size_t)mx_chunks(K);
+    return (size_t)M * (chunks * 128 + 16) + (size_t)M * chunks * 8;
+}
+template <int MT, int NT, bool PAIR, bool QUANTIZE = false>
+static int launch_rows(const Mxfp4Gemm& g, hipStream_t st, const char* name) {
+    note_kernel(name);
+    const unsigned cols = PAIR ? (unsigned)g.npanels / 2 : (unsigned)((g.N + 16 * NT - 1) / (16 * NT));
+    hipLaunchKernelGGL((mxfp4_rows_kernel<MT, NT, PAIR, QUANTIZE>), dim3(cols, (unsigned)((g.M + 16 * MT - 1) / (16 * MT))), dim3(512), QUANTIZE ? quantized_in_lds(g.M, g.K) : 0, st, g);
+    return check_hip(hipGetLastError(), "mxfp4_rows_kernel launch");
+}
+
+// Whether the kernel for few rows quantises bf16 rows on the way
+bool mx_takes_bf16(int M, int K) { return M <= 8 && (int64_t)M * K <= 16384; }
+
+int launch_gemm_mxfp4(const Mxfp4Gemm& g, hipStream_t st) {
+    if (g.a_bf16) return g.pair ? launch_rows<1, 4, true, true>(g, st, "mxfp4_rows_16_pair_bf16") : launch_rows<1, 1, false, true>(g, st, "mxfp4_rows_16_bf16");
+    if (g.M <= 16) return g.pair ? launch_rows<1, 4, true>(g, st, "mxfp4_rows_16_pair") : launch_rows<1, 1, false>(g, st, "mxfp4_rows_16");
+    if (g.M <= 32) return g.pair ? launch_rows<2, 4, true>(g, st, "mxfp4_rows_32_pair") : launch_rows<2, 1, false>(g, st, "mxfp4_rows_32");
+    return launch_tile<4, 2, 2, 4, 2>(g, st, "mxfp4_256x256");
+}
+
+}  // namespace mmx

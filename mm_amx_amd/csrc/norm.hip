@@ -2,11 +2,11 @@
 //
 //   u = f,  or  f / sqrt(mean(f^2) + eps) * (offset + post)          the norm behind the block that made f
 //   r = residual + scale * gate * u                                  its gate and the residual stream
-//   z = r / sqrt(mean(r^2) + eps) * (offset + pre)                   the norm in front of the next block, bf16 or e4m3 with scales
+//   z = r / sqrt(mean(r^2) + eps) * (offset + pre)                   the norm in front of the next block, bf16, e4m3 with scales or packed e2m1 with theirs
 //
 // Bound: HBM - f, residual and a gate per row are read once, r and z are written once.  A row stays in registers between its two
 // sums of squares; r goes on into the second norm as it is in 32 bits, not as it is stored.
-#include "ffn.hpp"
+#include "mxfp4.hpp"
 
 namespace mmx {
 
@@ -166,8 +166,21 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void block_norm_kernel(const
         }
 #pragma unroll
         for (int e = 0; e < 8; e++) v[i][e] = at + e < g.H ? v[i][e] * inv * w[e] : 0.0f;
-        if (!g.z_f8) {
+        if (g.z_type == MMX_BF16) {
             store8(reinterpret_cast<uint16_t*>(g.z + m * g.ld_z), at, g.H, v[i]);
+        } else if (g.z_type == MMX_F4) {
+            uint32_t top = 0;
+#pragma unroll
+            for (int e = 0; e < 8; e++) top = umax(top, abs_bits(v[i][e]));
+#pragma unroll
+            for (int d = 1; d < 4; d *= 2) top = umax(top, (uint32_t)__shfl_xor((int)top, d));
+            const uint32_t b = mx_scale_of(top);
+            const int kb = at / MX_BLOCK;
+            if (kb < (int)mx_chunks(g.H) * 8) {  // (the last chunk is written whole, zero behind the end of the row)
+                char* const panel = g.z + (int64_t)(m >> 5) * g.ld_z;
+                *reinterpret_cast<uint32_t*>(panel + mx_piece(m, kb) + (at & (MX_BLOCK - 1)) / 2) = to_fp4x8(v[i], mx_value_of(b));
+                if ((at & (MX_BLOCK - 1)) == 0) panel[mx_scale_at(m, kb)] = (char)b;
+            }
         } else {
             uint32_t top = 0;
 #pragma unroll

@@ -353,11 +353,16 @@ def block_norm(f, residual=None, *, post=False, post_weight=None, gate=None, sca
         z = r, or with pre   r / sqrt(mean(r^2) + eps) * (weight_offset + pre_weight)
 
     -> (r, z).  residual [M, H] bf16 or fp32, r like it (bf16 without one); gate bf16 [H], or [M, H] for a gate per row; weights bf16 [H] or None.
-    z is bf16, or with quantize Fp8Rows.  r, z: where to put them (r may be residual itself; False: r is not wanted, and None in its place)."""
+    z is bf16, or quantised: with quantize True or "fp8" Fp8Rows, with "mxfp4" Mxfp4Rows.  r, z: where to put them (r may be residual itself; False: r is not wanted, and None in its place)."""
+    mx4 = quantize == "mxfp4"
+    if quantize == "fp8":
+        quantize = True
+    elif isinstance(quantize, str) and not mx4:
+        raise MmxError("quantize is False, True ('fp8') or 'mxfp4'")
     if L._native is not None and L._initialised and z is None:
-        made = L._made(L._native.block_norm, f, residual, post, post_weight, gate, scale, pre, pre_weight, eps, weight_offset, quantize, r)
+        made = L._made(L._native.block_norm, f, residual, post, post_weight, gate, scale, pre, pre_weight, eps, weight_offset, 2 if mx4 else quantize, r)
         if made is not None:
-            return (made[0], Fp8Rows(made[1], made[2], f.shape[1])) if quantize else made
+            return (made[0], Mxfp4Rows(made[1], *f.shape)) if mx4 else (made[0], Fp8Rows(made[1], made[2], f.shape[1])) if quantize else made
     _gpu(f, "f", (torch.bfloat16,), 2)
     M, H = f.shape
     if H == 0:
@@ -384,18 +389,24 @@ def block_norm(f, residual=None, *, post=False, post_weight=None, gate=None, sca
         r = None
     elif _gpu(r, "r", (stream,), 2).shape != f.shape:
         raise MmxError(f"r is {tuple(r.shape)}, f {tuple(f.shape)}")
+    rows = Mxfp4Rows if mx4 else Fp8Rows
     if z is None:
-        z = Fp8Rows.empty(M, H, f.device) if quantize else torch.empty((M, H), dtype=torch.bfloat16, device=f.device)
-    elif isinstance(z, Fp8Rows) != bool(quantize) or z.shape != f.shape:
-        raise MmxError(f"z must be {'Fp8Rows' if quantize else 'a bf16 tensor'} of {tuple(f.shape)}")
+        z = rows.empty(M, H, f.device) if quantize else torch.empty((M, H), dtype=torch.bfloat16, device=f.device)
+    elif not isinstance(z, rows if quantize else torch.Tensor) or z.shape != f.shape:
+        raise MmxError(f"z must be {rows.__name__ if quantize else 'a bf16 tensor'} of {tuple(f.shape)}")
     zs, ld_zs = None, 0
-    if quantize:
+    if mx4:
+        zp, ldz = z._args("z"), 0
+    elif quantize:
         zp, ldz, zs, ld_zs = z._args("z")
     else:
         zp, ldz = _gpu(z, "z", (torch.bfloat16,), 2).data_ptr(), _rows(z)
     if M:
         args = L._BlockNorm(f.data_ptr(), _rows(f), _ptr(residual), 0 if residual is None else _rows(residual), _ptr(post_weight), _ptr(gate), ld_gate, _ptr(pre_weight),
-                            _ptr(r), 0 if r is None else _rows(r), zp, ldz, zs, ld_zs, L.F32 if stream == torch.float32 else L.BF16, L.F8 if quantize else L.BF16, int(post), int(pre),
+                            _ptr(r), 0 if r is None else _rows(r), zp, ldz, zs, ld_zs, L.F32 if stream == torch.float32 else L.BF16, L.F4 if mx4 else L.F8 if quantize else L.BF16, int(post), int(pre),
                             scale, eps, weight_offset)
         L._check(L.lib().mmx_block_norm(C.byref(args), M, H, L._stream()))
     return r, z
+
+
+from .mxfp4 import Mxfp4Rows  # noqa: E402  (which takes its helpers from here)

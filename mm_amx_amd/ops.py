@@ -11,7 +11,7 @@ import enum
 import torch
 
 from . import _lib as L
-from . import ffn
+from . import ffn, mxfp4
 
 _I8, _U8, _E4M3 = torch.int8, torch.uint8, torch.float8_e4m3fn  # (torch's dtypes are one object each; looked up in torch they cost a small call 0.2 us)
 
@@ -241,6 +241,36 @@ class LinearFp8:
         return other
 
 
+class LinearMxfp4:
+    """LinearNxN over weights in microscaled 4-bit floating point, e2m1 with a scale for each column and 32 of K: ``set_weight(w)`` takes bf16
+    weights [N, K], which are quantised, or codes uint8 [N, K/2] (the lower k in a byte's low half) with their ``scales`` uint8 [N, K/32] (rounded up);
+    ``forward(x[M,K], y[M,N])`` quantises x in the same way (or takes it quantised: Mxfp4Rows) and writes into the caller's y, bf16 or fp32.  N is any, and K
+    where the weights are bf16.  With a ``bias`` (fp32 [N]) it is added before y is rounded."""
+
+    def __init__(self):
+        self.name = ""
+        self.m_N = self.m_K = 0
+        self._packed = None
+
+    def set_weight(self, weight, scales=None):
+        packed = mxfp4.pack_mxfp4(weight, scales)
+        self.m_N, self.m_K = weight.shape[0], weight.shape[1] * (1 if scales is None else 2)
+        self._packed = packed
+
+    def forward(self, x, y, bias=None):
+        if self._packed is None:
+            raise L.MmxError("forward: set_weight has not been called")
+        if len(x.shape) != 2 or x.shape[1] != self.m_K:
+            raise L.MmxError(f"forward: x must be [M, {self.m_K}]")
+        mxfp4.gemm_mxfp4(x, self._packed, self.m_N, L.Epilogue(y, L.PP_NONE if bias is None else L.PP_BIAS, bias=bias))
+
+    def __deepcopy__(self, memo):
+        other = LinearMxfp4()
+        other.name, other.m_N, other.m_K = self.name, self.m_N, self.m_K
+        other._packed = copy.deepcopy(self._packed)
+        return other
+
+
 class MoE:
     """A mixture-of-experts layer for a few tokens.  ``setup(router[E,H], w_gate[E,I,H], w_up[E,I,H], w_down[E,H,I])`` packs the experts'
     weights: bf16; with ``compress="fp8"`` bf16 weights quantised to e4m3 with a scale for each block of 128 x 128; or e4m3 weights with
@@ -290,7 +320,7 @@ class MoE:
     def run(self, x, y=None):
         if self.gate_up is None:
             raise L.MmxError("run: setup has not been called")
-        if type(x) is ffn.Fp8Rows or x.dim() != 2 or x.shape[1] != self.H:
+        if type(x) in (ffn.Fp8Rows, mxfp4.Mxfp4Rows) or x.dim() != 2 or x.shape[1] != self.H:
             raise L.MmxError(f"run: x must be a bf16 tensor [T, {self.H}] (quantised rows go to LinearFp8 and MLP)")
         return ffn.moe(x, self.router, self.top_k, self.gate_up, self.down, self.I, self.scoring, self.renormalize, self.scale, self.bias, y)
 
@@ -301,19 +331,30 @@ class MLP:
     bf16(silu(x·Wg^T) * (x·Wu^T)) fused in the gate/up epilogue, then the down projection.
 
     With ``compress="fp8"`` the bf16 weights are quantised to e4m3, with ``scales`` (gate's, up's and down's, a block of 128 x 128 each) they are e4m3 already;
-    run then quantises x and the intermediate per row and 128 columns, or takes x as Fp8Rows."""
+    run then quantises x and the intermediate per row and 128 columns, or takes x as Fp8Rows.  With ``compress="mxfp4"``, or codes uint8 [.., .. / 2] with ``scales``
+    uint8 for each 32, the weights are microscaled 4-bit floating point (see LinearMxfp4), and x is quantised likewise or taken as Mxfp4Rows."""
 
     def __init__(self):
         self.m_N = self.m_K = 0
         self.gate_up = self.down = None
         self.actUp = None
+        self.mx4 = False
 
     def setup(self, w_gate, w_up, w_down, scales=None, compress=None):
+        mx4 = compress == "mxfp4" or (scales is not None and w_gate.dtype in mxfp4._BYTES)
         N, K = w_gate.shape
-        if tuple(w_down.shape) != (K, N):
+        if mx4 and scales is not None:
+            K *= 2  # (two codes a byte)
+        if tuple(w_down.shape) != (K, N // 2 if mx4 and scales is not None else N):
             raise L.MmxError("setup: w_down must be [K, N]")
-        if compress not in (None, "fp8") or (compress and scales is not None):
-            raise L.MmxError("setup: compress is 'fp8', for weights that come without scales")
+        if compress not in (None, "fp8", "mxfp4") or (compress and scales is not None):
+            raise L.MmxError("setup: compress is 'fp8' or 'mxfp4', for weights that come without scales")
+        if mx4:
+            gate_up = mxfp4.pack_gate_up_mxfp4(w_gate, w_up, None if scales is None else scales[:2])
+            self.down = mxfp4.pack_mxfp4(w_down, None if scales is None else scales[2])
+            self.gate_up, self.m_N, self.m_K, self.mx4 = gate_up, N, K, True
+            return
+        self.mx4 = False
         if scales is not None or compress:
             gate_up = ffn.pack_gate_up_fp8(w_gate, w_up, None if scales is None else scales[:2])
             self.down = ffn.pack_fp8(w_down, None if scales is None else scales[2])
@@ -328,6 +369,8 @@ class MLP:
             raise L.MmxError("run: setup has not been called")
         if len(x.shape) != 2 or x.shape[1] != self.m_K:
             raise L.MmxError(f"run: x must be [M, {self.m_K}]")
+        if self.mx4:
+            return mxfp4.mlp_mxfp4(x, self.gate_up, self.down, self.m_N, y=y)
         if isinstance(self.gate_up, tuple):
             return ffn.mlp_fp8(x, self.gate_up, self.down, self.m_N, y=y)
         M = x.shape[0]
@@ -338,6 +381,6 @@ class MLP:
 
     def __deepcopy__(self, memo):
         other = MLP()
-        other.m_N, other.m_K = self.m_N, self.m_K
+        other.m_N, other.m_K, other.mx4 = self.m_N, self.m_K, self.mx4
         other.gate_up, other.down = copy.deepcopy(self.gate_up), copy.deepcopy(self.down)
         return other

@@ -386,6 +386,34 @@ size_t mmx_mlp_mxfp4_scratch_bytes(int x_dtype, int M, int K, int N);
 int mmx_mlp_mxfp4(int x_dtype, const void* x, int64_t ldx_bytes, const void* w_gate_up, const void* w_down, int y_dtype, void* y, int64_t ldy_bytes, int M, int K,
                   int N, void* scratch, size_t scratch_bytes, void* stream);
 
+/* ==== drawing tokens (no counterpart in the reference) ============================================================
+ * One token for each row of logits [B, V] (MMX_BF16 or MMX_F32), given a random number u of [0, 1) for each:
+ *     w_i = e^((l_i - max l) / temperature)
+ *     order: descending l, the lowest index of equal ones first
+ *     top_k (0: off) keeps the first k of it; top_p (1 or more: off) of those the shortest run that holds top_p of their weight at least, one token at least; min_p (0: off) of
+ *     those what has w >= min_p (the largest always)
+ *     ids[b] = the first index, in the order of the vocabulary, up to which the weights that were kept come to more than u times their sum.
+ * A temperature of 0 takes the largest (the lowest index of equal ones).  -inf (a masked token) and NaN are never drawn; a row of nothing else gives -1.  Beside +inf nothing else has
+ * weight.  Weights and sums are in 64 bits, or whole numbers of 2^-39 at least where a run is sought, so the same inputs give the same token every time.
+ * temperature, top_k, top_p and min_p are the same for all rows, or come as fp32 / int32 [B] (the pointers _of, on the device; what is out of range there is taken as the
+ * nearest that is not, NaN as off, a temperature that is NaN as 0).  u of 1 or more takes the last token that is kept, NaN or below 0 the first.
+ * B <= 65535, V <= 2^22.  scratch: 256-byte aligned device memory, mmx_sample_scratch_bytes() bytes, free to reuse once the call's work on `stream` has finished. */
+typedef struct mmx_sample_args {
+    const void* logits;
+    int64_t ld_bytes;
+    const float* u;
+    const float* temperature_of; /* or NULL: temperature, and likewise below */
+    const int32_t* top_k_of;
+    const float* top_p_of;
+    const float* min_p_of;
+    double temperature, top_p, min_p;
+    int32_t* ids;
+    int32_t top_k;
+    int32_t dtype;
+} mmx_sample_args;
+size_t mmx_sample_scratch_bytes(int B, int V);
+int mmx_sample(const mmx_sample_args* args, int B, int V, void* scratch, size_t scratch_bytes, void* stream);
+
 /* ---- introspection / tuning (no reference counterpart) --------------------------------------- */
 /* Force the MFMA tile shape ("256x256", "256x192", "128x256", "128x192", "128x128", "128x64", "64x128" (aligned
  * operands and no SILU_GATE only; otherwise 128x128 is used), "" = automatic)

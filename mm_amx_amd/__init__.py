@@ -11,6 +11,7 @@ from ._lib import (BF16, F32, F4, F8, I4, I8, I32, U8, gemm_u8, matvec_u8, PP_BI
                    quantize_pack_int4, quantize_weights, quantize_weights_scaled, probe_mfma, probe_read, repack_b, repack_gate_up, set_option, set_tile, time_gemm, workspace, release_workspaces)
 from .ffn import Fp8Rows, block_norm, gemm_fp8, mlp_fp8, moe, moe_experts, moe_route, pack_fp8, pack_gate_up_fp8, quantize_fp8, quantize_pack_fp8
 from .mxfp4 import Mxfp4Rows, dequantize_mxfp4, gemm_mxfp4, mlp_mxfp4, pack_gate_up_mxfp4, pack_mxfp4, quantize_mxfp4
+from .sampling import sample
 from .ops import MLP, BiasGeluStore, LinearFp8, LinearMxfp4, MoE, GemAvB, LinearNxN, Matmul, MatmulVector, Steps, repackB_1x2, repackB_1xL
 
 __all__ = [
@@ -20,5 +21,5 @@ __all__ = [
     "BiasGeluStore", "Matmul", "MatmulVector", "GemAvB", "repackB_1x2", "repackB_1xL", "LinearNxN", "MLP",
     "F8", "Fp8Rows", "quantize_fp8", "quantize_pack_fp8", "pack_fp8", "pack_gate_up_fp8", "gemm_fp8", "mlp_fp8", "moe", "moe_route", "moe_experts", "block_norm",
     "LinearFp8", "MoE",
-    "F4", "Mxfp4Rows", "quantize_mxfp4", "dequantize_mxfp4", "pack_mxfp4", "pack_gate_up_mxfp4", "gemm_mxfp4", "mlp_mxfp4", "LinearMxfp4",
+    "F4", "Mxfp4Rows", "quantize_mxfp4", "dequantize_mxfp4", "pack_mxfp4", "pack_gate_up_mxfp4", "gemm_mxfp4", "mlp_mxfp4", "LinearMxfp4", "sample",
 ]

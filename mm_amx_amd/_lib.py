@@ -25,7 +25,7 @@ EXPORTS = ["mmx_last_error", "mmx_init", "mmx_packed_b_bytes", "mmx_repack_b", "
            "mmx_quantize_rows_fp8", "mmx_quantize_pack_fp8", "mmx_repack_gate_up_fp8", "mmx_gemm_fp8_scratch_bytes", "mmx_gemm_fp8",
            "mmx_mlp_fp8_scratch_bytes", "mmx_mlp_fp8", "mmx_moe_route", "mmx_moe_experts_scratch_bytes", "mmx_moe_experts", "mmx_block_norm",
            "mmx_mxfp4_bytes", "mmx_quantize_mxfp4", "mmx_repack_mxfp4", "mmx_unpack_mxfp4", "mmx_dequantize_mxfp4", "mmx_gemm_mxfp4_scratch_bytes", "mmx_gemm_mxfp4",
-           "mmx_mlp_mxfp4_scratch_bytes", "mmx_mlp_mxfp4"]
+           "mmx_mlp_mxfp4_scratch_bytes", "mmx_mlp_mxfp4", "mmx_sample_scratch_bytes", "mmx_sample"]
 # measurement aids (include/mm_amx_amd_bench.h)
 BENCH_EXPORTS = ["mmx_time_gemm", "mmx_probe_mfma", "mmx_probe_read"]
 
@@ -49,6 +49,12 @@ class _BlockNorm(C.Structure):
                 ("gate", C.c_void_p), ("ld_gate_bytes", C.c_int64), ("pre_weight", C.c_void_p), ("r", C.c_void_p), ("ldr_bytes", C.c_int64),
                 ("z", C.c_void_p), ("ldz_bytes", C.c_int64), ("z_scales", C.c_void_p), ("ld_z_scales", C.c_int64), ("residual_dtype", C.c_int32),
                 ("z_dtype", C.c_int32), ("post", C.c_int32), ("pre", C.c_int32), ("scale", C.c_float), ("eps", C.c_float), ("weight_offset", C.c_float)]
+
+
+class _Sample(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("ld_bytes", C.c_int64), ("u", C.c_void_p), ("temperature_of", C.c_void_p), ("top_k_of", C.c_void_p), ("top_p_of", C.c_void_p),
+                ("min_p_of", C.c_void_p), ("temperature", C.c_double), ("top_p", C.c_double), ("min_p", C.c_double), ("ids", C.c_void_p), ("top_k", C.c_int32),
+                ("dtype", C.c_int32)]
 
 
 _lib = None
@@ -77,7 +83,8 @@ def _host_module(l):
         l.mmx_packed_b_bytes, l.mmx_repack_b, l.mmx_quantize_weights_scratch, l.mmx_quantize_weights_scaled, l.mmx_quantize_pack_int4,
         l.mmx_quantize_pack_scaled, l.mmx_quantize_rows_fp8, l.mmx_gemm_fp8_scratch_bytes, l.mmx_gemm_fp8, l.mmx_mlp_fp8_scratch_bytes, l.mmx_mlp_fp8,
         l.mmx_moe_route, l.mmx_moe_experts_scratch_bytes, l.mmx_moe_experts, l.mmx_block_norm,
-        l.mmx_mxfp4_bytes, l.mmx_quantize_mxfp4, l.mmx_gemm_mxfp4_scratch_bytes, l.mmx_gemm_mxfp4, l.mmx_mlp_mxfp4_scratch_bytes, l.mmx_mlp_mxfp4)))
+        l.mmx_mxfp4_bytes, l.mmx_quantize_mxfp4, l.mmx_gemm_mxfp4_scratch_bytes, l.mmx_gemm_mxfp4, l.mmx_mlp_mxfp4_scratch_bytes, l.mmx_mlp_mxfp4,
+        l.mmx_sample_scratch_bytes, l.mmx_sample)))
     return _host_call
 
 
@@ -157,6 +164,9 @@ def lib():
         l.mmx_dequantize_mxfp4.argtypes = [p, i, i, i, p, n, p]
         l.mmx_gemm_mxfp4_scratch_bytes.argtypes = l.mmx_mlp_mxfp4_scratch_bytes.argtypes = [i, i, i, i]
         l.mmx_gemm_mxfp4.argtypes = [i, p, n, p, i, i, i, C.POINTER(_Epilogue), p, z, p]
+        l.mmx_sample_scratch_bytes.restype = z  # (of sampling.py)
+        l.mmx_sample_scratch_bytes.argtypes = [i, i]
+        l.mmx_sample.argtypes = [C.POINTER(_Sample), i, i, p, z, p]
         l.mmx_mlp_mxfp4.argtypes = [i, p, n, p, p, i, p, n, i, i, i, p, z, p]
         global _native
         _native = _host_module(l)

@@ -26,8 +26,8 @@ SOURCES = ["abi.hip", "gemm_bf16.hip", "gemm_i8.hip", "gemm_w8.hip",
            "gemm_bf16_out_bf16.hip", "gemm_bf16_out_f32.hip", "gemm_bf16_out_i8.hip",
            "gemm_i8_out_i8.hip", "gemm_i8_out_i32.hip", "gemm_i8_out_f32.hip", "gemm_i8_out_bf16.hip",
            "skinny.hip", "wave_ring.hip", "unpacked.hip", "repack.hip", "probe.hip", "u8.hip", "fp8.hip", "fp8_gemm.hip", "moe.hip", "norm.hip",
-           "mxfp4.hip", "mxfp4_gemm.hip", "ffn_abi.hip"]
-HEADERS = ["common.hpp", "gemm_tile.hpp", "ffn.hpp", "mxfp4.hpp", os.path.join("..", "..", "include", "mm_amx_amd.h"),
+           "mxfp4.hip", "mxfp4_gemm.hip", "sample.hip", "ffn_abi.hip"]
+HEADERS = ["common.hpp", "gemm_tile.hpp", "ffn.hpp", "mxfp4.hpp", "sample.hpp", os.path.join("..", "..", "include", "mm_amx_amd.h"),
            os.path.join("..", "..", "include", "mm_amx_amd_bench.h")]
 # -ffp-contract=off: the epilogues reproduce the reference's separately rounded mul/add sequence;
 # fused operations are spelled fmaf().  Packed fp32 VALU instructions stay disabled.

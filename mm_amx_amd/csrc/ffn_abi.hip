@@ -1,7 +1,8 @@
-// C ABI of the feed-forward block's operators: argument validation, scratch layout, dispatch.
+// C ABI of the feed-forward block's operators and of drawing tokens: argument validation, scratch layout, dispatch.
 #include <string.h>
 
 #include "mxfp4.hpp"
+#include "sample.hpp"
 
 namespace mmx {
 
@@ -22,6 +23,8 @@ int launch_quantize_mxfp4(bool f32, const void* x, int64_t ldx_bytes, int M, int
 int launch_dequantize_mxfp4(const void* in, int M, int K, bool f32, void* y, int64_t ldy_bytes, hipStream_t st);
 int launch_repack_mxfp4(bool to_layout, void* q, int64_t ldq, void* scales, int64_t lds, int M, int K, int pair, void* packed, hipStream_t st);
 int launch_gemm_mxfp4(const Mxfp4Gemm& g, hipStream_t st);
+size_t sample_scratch_bytes(int B, int V);
+int launch_sample(const SampleArgs& a, int B, bool f32, hipStream_t st);
 
 static bool misaligned(const void* p, int to) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(to - 1)) != 0; }
 static int64_t padded_k(int K) { return ((int64_t)K + BLOCK - 1) / BLOCK * BLOCK; }
@@ -61,6 +64,7 @@ static int check_scratch(const char* who, const void* scratch, size_t have, size
 }
 
 // K and N within what the kernels address with 32 bits; M such that a launch of up to 1024 threads for each row has fewer than 2^32 of them
+constexpr int MOST_V = 1 << 22;  // of a vocabulary
 constexpr int MOST_K = 1 << 22, MOST_N = 1 << 26, MOST_M = (1 << 22) - 1;
 static int check_sizes(const char* who, int M, int K, int N) {
     if (M < 0 || K <= 0 || N <= 0) return set_error(MMX_E_INVALID, "%s: K and N must be positive and M not negative (got %d, %d, %d)", who, M, K, N);
@@ -452,6 +456,39 @@ int mmx_mlp_mxfp4(int x_dtype, const void* x, int64_t ldx_bytes, const void* w_g
     weights_mxfp4(w_down, M, N, K, false, out, &g);
     if ((rc = packed_rows(MMX_F4, h, 0, M, N, nullptr, &g, st))) return rc;
     return launch_gemm_mxfp4(g, st);
+}
+
+size_t mmx_sample_scratch_bytes(int B, int V) { return B <= 0 || V <= 0 || B > 65535 || V > MOST_V ? 0 : sample_scratch_bytes(B, V); }
+
+int mmx_sample(const mmx_sample_args* a, int B, int V, void* scratch, size_t scratch_bytes, void* stream) {
+    const char* const who = "mmx_sample";
+    if (!a) return set_error(MMX_E_INVALID, "%s: NULL arguments", who);
+    if (B < 0 || V <= 0) return set_error(MMX_E_INVALID, "%s: V must be positive and B not negative (got %d x %d)", who, B, V);
+    if (B > 65535 || V > MOST_V) return set_error(MMX_E_UNSUPPORTED, "%s: up to 65535 rows of up to %d (got %d x %d)", who, MOST_V, B, V);
+    if (a->dtype != MMX_BF16 && a->dtype != MMX_F32) return set_error(MMX_E_INVALID, "%s: logits of dtype %d (bf16 and fp32 exist)", who, a->dtype);
+    if (!a->temperature_of && !(a->temperature >= 0)) return set_error(MMX_E_INVALID, "%s: temperature %g", who, a->temperature);
+    if (!a->top_p_of && !(a->top_p >= 0)) return set_error(MMX_E_INVALID, "%s: top_p %g", who, a->top_p);
+    if (!a->min_p_of && !(a->min_p >= 0 && a->min_p <= 1)) return set_error(MMX_E_INVALID, "%s: min_p %g", who, a->min_p);
+    if (!a->top_k_of && a->top_k < 0) return set_error(MMX_E_INVALID, "%s: top_k %d", who, a->top_k);
+    if (B == 0) return MMX_OK;
+    int rc;
+    if ((rc = check_rows(who, "logits", a->logits, a->ld_bytes, B, V, a->dtype == MMX_F32 ? 4 : 2))) return rc;
+    if (!a->u || !a->ids) return set_error(MMX_E_INVALID, "%s: NULL pointer", who);
+    if (misaligned(a->u, 4) || misaligned(a->ids, 4) || misaligned(a->temperature_of, 4) || misaligned(a->top_k_of, 4) || misaligned(a->top_p_of, 4) || misaligned(a->min_p_of, 4))
+        return set_error(MMX_E_INVALID, "%s: an operand is not aligned to its element size", who);
+    if ((rc = check_scratch(who, scratch, scratch_bytes, mmx_sample_scratch_bytes(B, V)))) return rc;
+    SampleArgs g;
+    g.logits = static_cast<const char*>(a->logits);
+    g.ld = a->ld_bytes;
+    g.u = a->u;
+    g.temperature = a->temperature_of, g.top_p = a->top_p_of, g.min_p = a->min_p_of, g.top_k = a->top_k_of;
+    g.temperature_all = a->temperature, g.top_p_all = a->top_p, g.min_p_all = a->min_p, g.top_k_all = a->top_k;
+    g.V = V;
+    g.shift = 61;
+    while ((int64_t)1 << (61 - g.shift) < V) g.shift--;
+    g.ids = a->ids;
+    g.scratch = static_cast<char*>(scratch);
+    return launch_sample(g, B, a->dtype == MMX_F32, static_cast<hipStream_t>(stream));
 }
 
 }  // extern "C"

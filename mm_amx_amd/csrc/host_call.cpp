@@ -406,6 +406,8 @@ decltype(&mmx_gemm_mxfp4_scratch_bytes) call_gemm_mxfp4_need = nullptr;
 decltype(&mmx_gemm_mxfp4) call_gemm_mxfp4 = nullptr;
 decltype(&mmx_mlp_mxfp4_scratch_bytes) call_mlp_mxfp4_need = nullptr;
 decltype(&mmx_mlp_mxfp4) call_mlp_mxfp4 = nullptr;
+decltype(&mmx_sample_scratch_bytes) call_sample_need = nullptr;
+decltype(&mmx_sample) call_sample = nullptr;
 
 int64_t blocks(int64_t n) { return (n + 127) / 128; }
 
@@ -756,9 +758,49 @@ PyObject* block_norm(PyObject*, PyObject* const* a, Py_ssize_t count) {
     }
 }
 
+// sample(logits, u, temperature, top_k, top_p, min_p, device, stream) -> ids; each of the four a number or a tensor with one for each row
+PyObject* sample(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    if (count != 8 || !call_sample) Py_RETURN_NONE;
+    try {
+        int device, rc = 0;
+        if (!whole_number(a[6], 0, 1 << 20, device)) throw Leave();
+        const Matrix l = matrix(a[0], device);
+        mmx_sample_args s = {};
+        s.logits = l.data;
+        s.ld_bytes = l.ld;
+        s.dtype = float_code(*l.t);
+        s.u = floats(a[1], device, {l.rows});
+        const auto asked = [&](PyObject* o, const float*& of, double& all) {
+            if (PyFloat_CheckExact(o)) all = PyFloat_AS_DOUBLE(o);
+            else of = floats(o, device, {l.rows});
+        };
+        asked(a[2], s.temperature_of, s.temperature);
+        asked(a[4], s.top_p_of, s.top_p);
+        asked(a[5], s.min_p_of, s.min_p);
+        if (!whole_number(a[3], 0, INT32_MAX, s.top_k)) {
+            const at::Tensor& k = tensor_on(a[3], device);
+            if (k.scalar_type() != at::kInt || k.dim() != 1 || k.size(0) != l.rows || !k.is_contiguous()) throw Leave();
+            s.top_k_of = static_cast<const int32_t*>(k.mutable_data_ptr());
+        }
+        void* const stream = stream_of(a[7]);
+        at::Tensor ids;
+        if (!unlocked([&] {
+                ids = make({l.rows}, at::kInt, *l.t);
+                s.ids = static_cast<int32_t*>(ids.mutable_data_ptr());
+                const size_t need = call_sample_need(l.rows, l.cols);
+                at::Tensor scratch;
+                if (need) scratch = make({(int64_t)need}, at::kByte, *l.t);
+                rc = call_sample(&s, l.rows, l.cols, need ? scratch.mutable_data_ptr() : nullptr, need, stream);
+            })) throw Leave();
+        return rc ? PyLong_FromLong(rc) : THPVariable_Wrap(ids);
+    } catch (...) {
+        Py_RETURN_NONE;
+    }
+}
+
 // bind(addresses of the entry points, in the order below)
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t count) {
-    constexpr int ENTRIES = 26;
+    constexpr int ENTRIES = 28;
     if (count != ENTRIES) {
         PyErr_SetString(PyExc_TypeError, "bind takes an address for each entry point");
         return nullptr;
@@ -794,6 +836,8 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t count) {
     set(call_gemm_mxfp4);
     set(call_mlp_mxfp4_need);
     set(call_mlp_mxfp4);
+    set(call_sample_need);
+    set(call_sample);
     Py_RETURN_NONE;
 }
 
@@ -801,7 +845,7 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t count) {
 PyMethodDef methods[] = {METHOD(gemm), METHOD(gemm_unpacked), METHOD(gemm_packing), METHOD(matvec), METHOD(repack), METHOD(quantize), METHOD(quantize_scaled),
                          METHOD(quantize_pack_int4), METHOD(quantize_pack_scaled), METHOD(quantize_fp8),
                          METHOD(gemm_fp8), METHOD(mlp_fp8), METHOD(moe), METHOD(block_norm),
-                         METHOD(quantize_mxfp4), METHOD(gemm_mxfp4), METHOD(mlp_mxfp4), METHOD(bind), {nullptr, nullptr, 0, nullptr}};
+                         METHOD(quantize_mxfp4), METHOD(gemm_mxfp4), METHOD(mlp_mxfp4), METHOD(sample), METHOD(bind), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host_call", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

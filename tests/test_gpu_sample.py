@@ -1,0 +1,221 @@
+"""Drawing tokens from logits, against the definition in 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+import sample_util as su
+
+pytestmark = pytest.mark.gpu
+
+import mm_amx_amd as mx  # noqa: E402
+
+
+def logits(B, V, seed, std=2.0, dtype=torch.float32, peaks=12):
+    g = torch.Generator().manual_seed(seed)
+    l = torch.randn((B, V), generator=g) * std
+    l += 10 * (torch.rand((B, V), generator=g) < peaks / V) * torch.rand((B, V), generator=g)
+    return l.to(dtype), torch.rand(B, generator=g)
+
+
+def check(l, u, T=1.0, k=0, p=1.0, m=0.0):
+    """Numbers, or a list with one for each row."""
+    B = l.shape[0]
+    rows = [[v] * B if not isinstance(v, list) else v for v in (T, k, p, m)]
+    give = [torch.tensor(v, dtype=torch.int32 if i == 1 else torch.float32).cuda() if isinstance(v, list) else v for i, v in enumerate((T, k, p, m))]
+    got = mx.sample(l.cuda(), u.cuda(), *give)
+    assert got.dtype == torch.int32 and got.shape == (B,)
+    exact = lambda v, of: float(np.float32(v)) if isinstance(of, list) else v  # noqa: E731 (tensors hold 32 bits)
+    want = [su.token(l[b].double().numpy(), float(u[b]), exact(rows[0][b], T), rows[1][b], exact(rows[2][b], p), exact(rows[3][b], m)) for b in range(B)]
+    assert got.tolist() == want
+    return got
+
+
+FILTERS = [(1.0, 0, 1.0, 0.0), (0.8, 50, 0.9, 0.0), (1.0, 0, 0.95, 0.0), (1.3, 0, 0.5, 0.0), (0.7, 20, 1.0, 0.0), (1.0, 0, 1.0, 0.05), (1.0, 2, 1.0, 0.0), (1.1, 700, 0.99, 0.001), (1.0, 3000, 1.0, 0.0),
+           (1.0, 5000, 0.8, 0.0), (0.2, 0, 0.999, 0.0), (5.0, 0, 0.9, 0.3), (1.0, 1, 1.0, 0.0), (0.0, 40, 0.9, 0.0), (1.0, 0, 0.0, 0.0), (1.0, 100, 0.7, 1.0), (0.05, 0, 0.9, 0.0), (30.0, 0, 0.9, 0.0)]
+
+
+@pytest.mark.parametrize("V", [1, 2, 63, 1000, 1024, 1025, 8191, 32000, 50001])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_filters(V, dtype):
+    l, u = logits(7, V, V, dtype=dtype)
+    for T, k, p, m in FILTERS:
+        check(l, u, T, k, p, m)
+
+
+@pytest.mark.parametrize("B,V", [(1, 131072), (33, 100003), (64, 20000), (300, 999)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_each_row_asks_for_its_own(B, V, dtype):
+    l, u = logits(B, V, B, dtype=dtype)
+    rows = [FILTERS[b % len(FILTERS)] for b in range(B)]
+    check(l, u, *([r[i] for r in rows] for i in range(4)))
+
+
+def test_large_vocabularies_and_flat_rows():
+    for V, std in ((1 << 20, 2.0), ((1 << 22) - 5, 0.1)):
+        l, u = logits(2, V, 3, std=std)
+        for f in ((1.0, 0, 1.0, 0.0), (1.0, 0, 0.9, 0.0), (1.0, 100, 0.9, 0.0), (1.0, 100000, 0.9, 0.0), (1.0, 0, 1.0, 0.2)):
+            check(l, u, *f)
+
+
+@pytest.mark.parametrize("V", [5, 1000, 3000, 70000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_equal_logits_go_by_their_index(V, dtype):
+    """All equal, and two values only: the run that stays ends among equal ones."""
+    g = torch.Generator().manual_seed(V)
+    u = torch.tensor([0.0, 0.3, 0.6, 0.999, 0.5, 0.9])
+    same = torch.zeros((6, V), dtype=dtype)
+    two = (torch.rand((6, V), generator=g) < 0.5).to(dtype)
+    signs = torch.where(torch.rand((6, V), generator=g) < 0.5, 0.0, -0.0).to(dtype)  # (the two zeros are equal)
+    for l in (same, two, signs):
+        for f in ((1.0, 0, 1.0, 0.0), (1.0, 3, 1.0, 0.0), (1.0, V // 2 + 1, 1.0, 0.0), (1.0, 0, 0.37, 0.0), (1.0, V // 3 + 1, 0.41, 0.0), (1.0, 0, 0.77, 0.4), (0.0, 0, 1.0, 0.0)):
+            check(l, u, *f)
+    assert mx.sample(same.cuda(), u.cuda(), temperature=0.0).tolist() == [0] * 6
+
+
+@pytest.mark.parametrize("V", [4, 1500, 40000])
+@pytest.mark.parametrize("f", [(1.0, 0, 1.0, 0.0), (1.0, 50, 0.9, 0.0), (0.7, 0, 0.8, 0.0), (0.0, 0, 1.0, 0.0), (1.0, 0, 1.0, 0.1), (1.0, 1, 1.0, 0.0)])
+def test_masks_infinities_and_nan(V, f):
+    l, u = logits(12, V, 1)
+    inf = float("inf")
+    l[0] = -inf                               # nothing is left
+    l[1] = float("nan")
+    l[2], l[2, V // 2] = -inf, -3.0           # one is
+    l[3, ::2] = -inf
+    l[4, 1::2] = float("nan")
+    l[5, 1] = inf                             # beside it nothing has weight
+    l[6, 0], l[6, V - 1] = inf, inf
+    l[7] = torch.finfo(torch.float32).min     # masks of the lowest value: all equal
+    l[8], l[8, 1] = torch.finfo(torch.float32).min, 2.0
+    l[9] = inf
+    l[10, 0], l[10, 1] = 3e38, -3e38
+    l[11] = l[11] * 1e-30
+    got = check(l, u, *f).tolist()
+    assert got[0] == got[1] == -1 and got[2] == V // 2 and got[5] == 1 and got[6] in (0, V - 1) and got[8] == 1 and got[10] == 0
+
+
+def test_the_ends_of_u():
+    l, _ = logits(6, 3000, 2)
+    l[:, 0] = l[:, 2999] = -float("inf")
+    u = torch.tensor([0.0, 1.0, -1.0, float("nan"), 1.0 - 2.0 ** -24, 7.0])
+    for f in ((1.0, 0, 1.0, 0.0), (1.0, 20, 1.0, 0.0), (1.0, 0, 0.9, 0.0), (1.0, 0, 1.0, 0.01)):
+        got = mx.sample(l.cuda(), u.cuda(), *f).tolist()
+        for b in range(6):
+            at, w = su.kept(l[b].double().numpy(), *f)
+            live = at[w > 0]
+            assert got[b] == (live[0] if b in (0, 2, 3) else live[-1] if b in (1, 5) else su.token(l[b].double().numpy(), float(u[b]), *f)), (f, b)
+
+
+def test_out_of_range_in_tensors_is_taken_as_the_nearest():
+    l, u = logits(4, 2000, 3)
+    nan, inf = float("nan"), float("inf")
+    give = lambda v, t=torch.float32: torch.tensor(v, dtype=t).cuda()  # noqa: E731
+    base = lambda **k: mx.sample(l.cuda(), u.cuda(), **k).tolist()  # noqa: E731
+    assert base(temperature=give([-1.0, nan, 0.0, -inf])) == base(temperature=0.0)
+    assert base(top_k=give([-5, 0, 2000, 2 ** 31 - 1], torch.int32)) == base()
+    assert base(top_p=give([nan, 1.5, inf, 1.0])) == base() and base(top_p=give([-1.0, 0.0, -inf, 0.0])) == base(top_p=0.0)
+    assert base(min_p=give([nan, -1.0, 0.0, -inf])) == base() and base(min_p=give([1.5, inf, 1.0, 2.0])) == base(min_p=1.0)
+    assert base(temperature=inf, top_k=3) == [su.token(l[b].double().numpy(), float(u[b]), inf, 3) for b in range(4)]
+
+
+@pytest.mark.parametrize("f", [(1.0, 0, 1.0, 0.0), (0.9, 30, 0.9, 0.0), (1.0, 0, 0.9, 0.0)])
+def test_rows_of_any_stride_and_alignment(f):
+    base, u = logits(20, 3333, 4, dtype=torch.bfloat16)
+    wide = base.cuda()
+    for sub in ((slice(None), slice(1, 3001)), (slice(0, None, 2), slice(3, 3300)), (slice(5, 6), slice(7, 3333))):
+        l = wide[sub]
+        want = [su.token(r.double().numpy(), float(x), *f) for r, x in zip(base[sub], u[:l.shape[0]])]
+        assert mx.sample(l, u[:l.shape[0]].cuda(), *f).tolist() == want
+    out = torch.full((22,), 77, dtype=torch.int32, device="cuda")
+    assert mx.sample(wide, u.cuda(), *f, out=out[:20]).data_ptr() == out.data_ptr()
+    assert out[:20].tolist() == mx.sample(wide, u.cuda(), *f).tolist() and out[20:].tolist() == [77, 77]
+
+
+def test_frequencies_are_the_weights():
+    """20000 draws from eight tokens: each one's count is within 6 standard deviations of what its share makes it."""
+    l = torch.tensor([0.0, 1.0, -1.0, 2.0, 0.5, -3.0, 1.5, 0.0])
+    n = 20000
+    u = torch.rand(n, generator=torch.Generator().manual_seed(5)).cuda()
+    ids = mx.sample(l.expand(n, 8).contiguous().cuda(), u, temperature=0.7, top_k=6)
+    at, w = su.kept(l.double().numpy(), 0.7, 6)
+    share = np.zeros(8)
+    share[at] = w / w.sum()
+    count = np.bincount(ids.cpu().numpy(), minlength=8)
+    assert (np.abs(count - n * share) <= 6 * np.sqrt(n * share * (1 - share)) + 1e-9).all()
+
+
+def test_graphs_and_streams():
+    """Replays of captured draws with other logits and random numbers in place, beside eager ones on another stream."""
+    l, u = logits(9, 30000, 6)
+    l, u = l.cuda(), u.cuda()
+    fs = ((1.0, 0, 1.0, 0.0), (0.9, 30, 0.9, 0.0), (1.0, 0, 0.9, 0.0), (1.0, 0, 1.0, 0.05))
+    side = torch.cuda.Stream()
+    graphs = []
+    for f in fs:
+        with torch.cuda.stream(side):
+            mx.sample(l, u, *f)
+            side.synchronize()
+            gr = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(gr, stream=side):
+                ids = mx.sample(l, u, *f)
+            graphs.append((gr, ids))
+    for i in range(4):
+        a, b = logits(9, 30000, 20 + i)
+        torch.cuda.synchronize()
+        l.copy_(a), u.copy_(b)
+        want = [mx.sample(l, u, *f) for f in fs]
+        torch.cuda.synchronize()
+        for (gr, ids), f, w in zip(graphs, fs, want):
+            with torch.cuda.stream(side):
+                gr.replay()
+            eager = mx.sample(l, u, *f)
+            torch.cuda.synchronize()
+            assert torch.equal(ids, w) and torch.equal(eager, w)
+
+
+def test_block_head_and_token_together():
+    """A norm into packed rows, an MLP, the norm in front of the head, the head and the draw, as a decode step runs them, against the same in 64 bits from its logits."""
+    M, K, N, V = 5, 512, 768, 5000
+    g = torch.Generator().manual_seed(7)
+    t = lambda *s, std=1.0: (torch.randn(s, generator=g) * std).to(torch.bfloat16).cuda()  # noqa: E731
+    f, r = t(M, K), t(M, K)
+    mlp, head = mx.MLP(), mx.LinearMxfp4()
+    mlp.setup(t(N, K, std=0.05), t(N, K, std=0.05), t(K, N, std=0.05), compress="mxfp4")
+    head.set_weight(t(V, K, std=0.1))
+    u = torch.rand(M, generator=g).cuda()
+
+    def step():
+        r1, z = mx.block_norm(f, r, quantize="mxfp4")
+        y = mlp.run(z)
+        _, z = mx.block_norm(y, r1, quantize="mxfp4", r=False)
+        l = torch.empty((M, V), device="cuda")
+        head.forward(z, l)
+        return l, mx.sample(l, u, temperature=0.8, top_k=40, top_p=0.9)
+
+    l, ids = step()
+    assert ids.tolist() == [su.token(l[b].double().cpu().numpy(), float(u[b]), 0.8, 40, 0.9) for b in range(M)]
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step()
+        side.synchronize()
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr, stream=side):
+            lg, ig = step()
+    for _ in range(3):
+        torch.cuda.synchronize()
+        lg.zero_(), ig.zero_()
+        torch.cuda.synchronize()
+        gr.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(lg, l) and torch.equal(ig, ids)
+
+
+def test_nothing_to_do_and_refusals():
+    l, u = logits(4, 100, 8)
+    l, u = l.cuda(), u.cuda()
+    assert mx.sample(l[:0], u[:0]).shape == (0,)
+    for bad in (dict(logits=l.half()), dict(logits=l[0]), dict(logits=l[:, :0]), dict(logits=l.t()), dict(logits=l.cpu()), dict(u=u[:3]), dict(u=u.double()), dict(u=u.cpu()), dict(temperature=-1.0),
+                dict(temperature=float("nan")), dict(top_k=-1), dict(top_k=2.0), dict(top_p=-0.1), dict(min_p=1.1), dict(min_p=float("nan")), dict(top_k=u), dict(temperature=u[:2]),
+                dict(top_p=u.double()), dict(min_p=u.cpu()), dict(temperature="1"), dict(top_p=torch.stack((u, u), 1)[:, 0]), dict(out=torch.empty(3, dtype=torch.int32, device="cuda")),
+                dict(out=torch.empty(4, device="cuda")), dict(u=torch.stack((u, u), 1)[:, 0])):
+        with pytest.raises(mx.MmxError):
+            mx.sample(**{**dict(logits=l, u=u), **bad})

@@ -394,7 +394,7 @@ int mmx_mlp_mxfp4(int x_dtype, const void* x, int64_t ldx_bytes, const void* w_g
  *     those what has w >= min_p (the largest always)
  *     ids[b] = the first index, in the order of the vocabulary, up to which the weights that were kept come to more than u times their sum.
  * A temperature of 0 takes the largest (the lowest index of equal ones).  -inf (a masked token) and NaN are never drawn; a row of nothing else gives -1.  Beside +inf nothing else has
- * weight.  Weights and sums are in 64 bits, or whole numbers of 2^-39 at least where a run is sought, so the same inputs give the same token every time.
+ * weight.  Weights and sums are in 64 bits, or whole numbers of 2^-34 of the largest where the end of a run is sought, so the same inputs give the same token every time.
  * temperature, top_k, top_p and min_p are the same for all rows, or come as fp32 / int32 [B] (the pointers _of, on the device; what is out of range there is taken as the
  * nearest that is not, NaN as off, a temperature that is NaN as 0).  u of 1 or more takes the last token that is kept, NaN or below 0 the first.
  * B <= 65535, V <= 2^22.  scratch: 256-byte aligned device memory, mmx_sample_scratch_bytes() bytes, free to reuse once the call's work on `stream` has finished. */

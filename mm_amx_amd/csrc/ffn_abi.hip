@@ -24,7 +24,7 @@ int launch_dequantize_mxfp4(const void* in, int M, int K, bool f32, void* y, int
 int launch_repack_mxfp4(bool to_layout, void* q, int64_t ldq, void* scales, int64_t lds, int M, int K, int pair, void* packed, hipStream_t st);
 int launch_gemm_mxfp4(const Mxfp4Gemm& g, hipStream_t st);
 size_t sample_scratch_bytes(int B, int V);
-int launch_sample(const SampleArgs& a, int B, bool f32, hipStream_t st);
+int launch_sample(SampleArgs a, int B, bool f32, hipStream_t st);
 
 static bool misaligned(const void* p, int to) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(to - 1)) != 0; }
 static int64_t padded_k(int K) { return ((int64_t)K + BLOCK - 1) / BLOCK * BLOCK; }
@@ -487,6 +487,7 @@ int mmx_sample(const mmx_sample_args* a, int B, int V, void* scratch, size_t scr
     g.shift = 61;
     while ((int64_t)1 << (61 - g.shift) < V) g.shift--;
     g.ids = a->ids;
+    g.slice = 0;
     g.scratch = static_cast<char*>(scratch);
     return launch_sample(g, B, a->dtype == MMX_F32, static_cast<hipStream_t>(stream));
 }

@@ -8,9 +8,9 @@
 // What stays is a run of the order whatever the filters are, so it is held as its last element: a key (the bits of l, made to order like l) and, among equal keys, an index.
 // A row is cut into segments of 1024 neighbours, one wavefront's 16 values a lane, whose maxima and sums are what the draw goes by: it finds its segment, then its token in it.
 //
-// Three kernels.  One workgroup for each slice of 16 segments reads the logits: segments' maxima; without filters their sums too; with top_k or top_p a histogram of the slice, counts and weights by
-// l / T in steps of 1 / 16, on one grid for the row.  With filters the slices' workgroups add up the row's histograms, which shows the bin in which the run ends, and collect what lies in it and above, or,
-// where that is more than a list holds, what lies in it and the sums of what lies above.  One workgroup a row finishes: it sorts the list, which settles the run, and draws.
+// Three kernels.  A workgroup for each slice of a row reads the logits: segments' maxima; without filters their sums too; with top_k or top_p a histogram of the slice, counts and weights by
+// l / T in steps of 1 / 16, on one grid for the row.  With filters workgroups of four segments add the row's histograms up, which shows the bin in which the run ends, and collect what lies in it and above; or,
+// where that is more than a list holds, what lies in it, and the segments' sums of what lies above.  A workgroup a row sorts out from the list where the run ends, and draws.
 // Rows that this does not suit (more than a list of equal or nearly equal logits in the last bin, 2^50 bins and more) are worked on by that one workgroup alone, a pass over the row for every eight bits of the key.
 #include "sample.hpp"
 
@@ -18,17 +18,18 @@
 
 namespace mmx {
 
-constexpr int SEG = 1024, SLICE = 16;     // logits of a segment, segments of a slice
-constexpr int BINS = 512;                 // the last one: everything below
+constexpr int SEG = 1024;                 // logits of a segment
+constexpr int BINS = 512;                 // the last one: everything below, e^-31.9 of the largest weight or less, which top_p's run takes for nothing
 constexpr double PER_UNIT = 16;           // bins of a unit of l / T
 constexpr int LIST = 4096;                // entries
+constexpr int MOST_SLICES = 256;          // of a row
 constexpr int MOST_SUMS = 1024;           // segments of a row whose sums fit beside a list
 constexpr double GRID = 1125899906842624.0;  // 2^50: up to here bins are exact
 constexpr float NEVER = -__builtin_huge_valf();
 
 // What a row asks for
 struct RowAsks {
-    double T, p, min_p;
+    double T, per, p, min_p;  // per: 1 / T
     int k;
     bool greedy, top_k, top_p, min;
     __device__ __forceinline__ bool filtered() const { return !greedy && (top_k || top_p); }
@@ -36,6 +37,7 @@ struct RowAsks {
 __device__ __forceinline__ RowAsks asks_of(const SampleArgs& a, int row) {
     RowAsks r;
     r.T = a.temperature ? (double)a.temperature[row] : a.temperature_all;
+    r.per = 1.0 / r.T;
     r.k = a.top_k ? a.top_k[row] : a.top_k_all;
     r.p = a.top_p ? (double)a.top_p[row] : a.top_p_all;
     r.min_p = a.min_p ? (double)a.min_p[row] : a.min_p_all;
@@ -54,9 +56,30 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 __device__ __forceinline__ float of_key(uint32_t k) { return u2f(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 __device__ __forceinline__ float settled(float x) { return x != x ? NEVER : x + 0.0f; }
 
-__device__ __forceinline__ double weight_of(float l, float top, double T) {
-    if (l == top) return 1.0;  // (an infinite one too: the others have no weight beside it)
-    return l == NEVER ? 0.0 : exp(((double)l - (double)top) / T);
+// e^x for x <= 0: 2^n times the series of e^r to its eleventh power, |r| <= ln 2 / 2, whose rest is r^12 / 12! = 6e-15.  (The library's exp, with a division by the temperature, took most of
+// the time: 256 rows of 131072 62 us, so 26; 1 row of 32000 12.8, so 5.)
+__device__ __forceinline__ double exp_of(double x) {
+    x = fmax(x, -1000.0);  // (NaN, which +inf beside +inf makes, too: it has no weight)
+    const double n = rint(x * 1.4426950408889634);
+    const double r = __builtin_fma(n, -0.6931471805599453, x);
+    double p = 1.0 / 39916800;
+    p = __builtin_fma(p, r, 1.0 / 3628800);
+    p = __builtin_fma(p, r, 1.0 / 362880);
+    p = __builtin_fma(p, r, 1.0 / 40320);
+    p = __builtin_fma(p, r, 1.0 / 5040);
+    p = __builtin_fma(p, r, 1.0 / 720);
+    p = __builtin_fma(p, r, 1.0 / 120);
+    p = __builtin_fma(p, r, 1.0 / 24);
+    p = __builtin_fma(p, r, 1.0 / 6);
+    p = __builtin_fma(p, r, 0.5);
+    p = __builtin_fma(p, r, 1.0);
+    p = __builtin_fma(p, r, 1.0);
+    return ldexp(p, (int)n);
+}
+// per: 1 / temperature
+__device__ __forceinline__ double weight_of(float l, float top, double per) {
+    const double w = exp_of(((double)l - (double)top) * per);
+    return l == top ? 1.0 : l == NEVER ? 0.0 : w;  // (an infinite one too: the others have no weight beside it)
 }
 
 __device__ __forceinline__ float value_at(const uint16_t* row, int64_t i) { return settled(from_bf16(row[i])); }
@@ -67,13 +90,20 @@ template <typename TL>
 struct Lane16 {
     static constexpr int PER = 16 / (int)sizeof(TL);  // values of a piece
     float v[16];
+    u32x4 w[16 / PER];  // as they are in memory, so that several segments can be on their way
+    bool whole;
     __device__ __forceinline__ static int at(int e) { return (e / PER) * (64 * PER) + (threadIdx.x & 63) * PER + e % PER; }
-    __device__ __forceinline__ void load(const TL* row, int V, int seg) {
+    __device__ __forceinline__ void ask(const TL* row, int V, int seg) {
         const int64_t base = (int64_t)seg * SEG;
-        if (base + SEG <= V) {
-            u32x4 w[16 / PER];
+        whole = base + SEG <= V;
+        if (whole) {
 #pragma unroll
             for (int c = 0; c < 16 / PER; c++) __builtin_memcpy(&w[c], __builtin_assume_aligned(row + base + at(c * PER), sizeof(TL)), 16);  // (the hardware takes any address)
+        }
+    }
+    __device__ __forceinline__ void get(const TL* row, int V, int seg) {
+        const int64_t base = (int64_t)seg * SEG;
+        if (whole) {
 #pragma unroll
             for (int e = 0; e < 16; e++) {
                 const uint32_t x = w[e / PER][(e % PER) * (int)sizeof(TL) / 4];
@@ -85,6 +115,10 @@ struct Lane16 {
             for (int e = 0; e < 16; e++) v[e] = base + at(e) < V ? value_at(row, base + at(e)) : NEVER;
         }
     }
+    __device__ __forceinline__ void load(const TL* row, int V, int seg) {
+        ask(row, V, seg);
+        get(row, V, seg);
+    }
 };
 
 template <typename T>
@@ -93,9 +127,13 @@ __device__ __forceinline__ T wave_sum(T v) {
     for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d);
     return v;
 }
-__device__ __forceinline__ float wave_max(float v) {
+template <typename T>
+__device__ __forceinline__ T wave_max(T v) {
 #pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) v = fmaxf(v, __shfl_xor(v, d));
+    for (int d = 32; d >= 1; d >>= 1) {
+        const T o = __shfl_xor(v, d);
+        v = o > v ? o : v;
+    }
     return v;
 }
 
@@ -107,17 +145,30 @@ struct Cut {       // what stays: keys above, and of the equal ones indexes up t
     __device__ __forceinline__ bool holds(uint32_t k, int i) const { return k > key || (k == key && i <= index); }
 };
 
-// What a slice's workgroup leaves
+// What a slice's workgroup leaves beside its histogram
 struct Slice {
     double bin;  // of its largest logit
-    unsigned long long mass;
-    float top;
-    uint32_t count;
+    uint32_t count, pad;
 };
+// Weights by bins: l / T = (bin + f) / PER_UNIT with f in [0, 1), so a weight is e^(f / PER_UNIT) times what all of the bin have in common.  A bin's word has its count above bit 49 and the sum
+// of those factors, at most 1.065 each, as whole numbers of 2^-34 below (up to 2^14 of them).
+constexpr int MASS_BITS = 49;
+constexpr double FACTOR_SCALE = 17179869184.0;  // 2^34
+// e^(f / 16) - 1 for f from [0, 1): the series to its seventh power, the rest is 6e-15
+__device__ __forceinline__ double factor_less_1(double f) {
+    const double x = f * (1.0 / PER_UNIT);
+    double p = 1.0 / 5040;
+    p = __builtin_fma(p, x, 1.0 / 720);
+    p = __builtin_fma(p, x, 1.0 / 120);
+    p = __builtin_fma(p, x, 1.0 / 24);
+    p = __builtin_fma(p, x, 1.0 / 6);
+    p = __builtin_fma(p, x, 0.5);
+    p = __builtin_fma(p, x, 1.0);
+    return p * x;
+}
 enum { BY_LIST, BY_SUMS, ALONE };
 struct State {
-    uint32_t entries, path, before_count;
-    float top;
+    uint32_t entries, path, before_count, pad;
     double before_mass, mass;  // of what lies above the last bin, and of everything
 };
 // A row's scratch
@@ -127,26 +178,25 @@ struct Scratch {
     Slice* slices;
     State* state;
     unsigned long long* list;
-    unsigned long long* mass;  // histograms, a slice's behind the other
-    uint32_t* count;
-    int segs, n_slices;
+    unsigned long long* bins;  // histograms, a slice's behind the other
+    int segs, slice, n_slices;
 };
-__host__ __device__ inline size_t row_bytes(int V) {
-    const size_t segs = ((size_t)V + SEG - 1) / SEG, slices = (segs + SLICE - 1) / SLICE;
-    return (segs * 12 + slices * (sizeof(Slice) + BINS * 12) + LIST * 8 + sizeof(State) + 255) & ~(size_t)255;
+__host__ __device__ inline size_t row_bytes(int V, int slice) {
+    const size_t segs = ((size_t)V + SEG - 1) / SEG, slices = (segs + slice - 1) / slice;
+    return (segs * 12 + slices * (sizeof(Slice) + BINS * 8) + LIST * 8 + sizeof(State) + 255) & ~(size_t)255;
 }
 __device__ __forceinline__ Scratch scratch_of(const SampleArgs& a, int row) {
     Scratch r;
     r.segs = (a.V + SEG - 1) / SEG;
-    r.n_slices = (r.segs + SLICE - 1) / SLICE;
-    char* p = a.scratch + (int64_t)row * row_bytes(a.V);
+    r.slice = a.slice;
+    r.n_slices = (r.segs + r.slice - 1) / r.slice;
+    char* p = a.scratch + (int64_t)row * row_bytes(a.V, r.slice);
     r.list = reinterpret_cast<unsigned long long*>(p), p += LIST * 8;
     r.state = reinterpret_cast<State*>(p), p += sizeof(State);
     r.slices = reinterpret_cast<Slice*>(p), p += r.n_slices * sizeof(Slice);
-    r.mass = reinterpret_cast<unsigned long long*>(p), p += (int64_t)r.n_slices * BINS * 8;
+    r.bins = reinterpret_cast<unsigned long long*>(p), p += (int64_t)r.n_slices * BINS * 8;
     r.sums = reinterpret_cast<double*>(p), p += (int64_t)r.segs * 8;
-    r.seg_top = reinterpret_cast<float*>(p), p += (int64_t)r.segs * 4;
-    r.count = reinterpret_cast<uint32_t*>(p);
+    r.seg_top = reinterpret_cast<float*>(p);
     return r;
 }
 static_assert(sizeof(Slice) % 8 == 0 && sizeof(State) % 8 == 0, "what lies behind them stays aligned");
@@ -166,6 +216,7 @@ struct Shared {
 };
 
 // A value of each thread: the sum over the threads before it, and over all
+template <int WAVES = NW>
 __device__ __forceinline__ double scan_before(double v, double* part, double* all) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     double run = v;
@@ -179,7 +230,7 @@ __device__ __forceinline__ double scan_before(double v, double* part, double* al
     __syncthreads();
     double before = 0, total = 0;
 #pragma unroll
-    for (int w = 0; w < NW; w++) {
+    for (int w = 0; w < WAVES; w++) {
         before += w < wave ? part[w] : 0.0;
         total += part[w];
     }
@@ -190,7 +241,7 @@ __device__ __forceinline__ double scan_before(double v, double* part, double* al
 // The cut that keeps the first `want_count` of what `limit` holds (by_mass: the shortest run of it that holds `want_mass`): its key by eight bits at a time from the top, over the whole row each time,
 // then, if not all of the equal keys stay, the index.  Masses are whole numbers of 2^-shift, whose sums do not depend on their order.
 template <typename TL>
-__device__ Cut select(const TL* row, int V, float top, double T, double scale, Cut limit, bool by_mass, uint32_t want_count, unsigned long long want_mass, Shared& s) {
+__device__ Cut select(const TL* row, int V, float top, double per, double scale, Cut limit, bool by_mass, uint32_t want_count, unsigned long long want_mass, Shared& s) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, segs = (V + SEG - 1) / SEG;
     uint32_t prefix = 0;
     unsigned long long mass_before = 0;
@@ -207,7 +258,7 @@ __device__ Cut select(const TL* row, int V, float top, double T, double scale, C
                 const uint32_t k = key_of(x.v[e]);
                 if (x.v[e] == NEVER || !limit.holds(k, g * SEG + x.at(e)) || (shift < 24 && (k >> (shift + 8)) != (prefix >> (shift + 8)))) continue;
                 atomicAdd(&s.count[k >> shift & 255], 1u);
-                if (by_mass) atomicAdd(&s.mass[k >> shift & 255], whole(weight_of(x.v[e], top, T), scale));
+                if (by_mass) atomicAdd(&s.mass[k >> shift & 255], whole(weight_of(x.v[e], top, per), scale));
             }
         }
         __syncthreads();
@@ -230,7 +281,7 @@ __device__ Cut select(const TL* row, int V, float top, double T, double scale, C
     }
     uint32_t stay = want_count - count_before;
     if (by_mass) {
-        const unsigned long long each = whole(weight_of(of_key(prefix), top, T), scale);
+        const unsigned long long each = whole(weight_of(of_key(prefix), top, per), scale);
         const unsigned long long n = each ? (want_mass - mass_before + each - 1) / each : equal;
         stay = want_mass <= mass_before ? 1 : n < equal ? (uint32_t)n : equal;
     }
@@ -273,333 +324,551 @@ __device__ Cut select(const TL* row, int V, float top, double T, double scale, C
 }
 
 // ---- the slices -----------------------------------------------------------------------------------------------------------------
-template <typename TL>
-__global__ __launch_bounds__(THREADS) void sample_slices_kernel(const SampleArgs a) {
-    __shared__ unsigned long long mass[BINS], total_mass;
-    __shared__ uint32_t count[BINS], total_count;
-    __shared__ float tops[NW];
+// (the first thread whose condition holds, as a ballot a wavefront: atomics of all lanes on one word took 20 cycles a lane)
+__device__ __forceinline__ void first_of(bool holds, uint32_t* first) {
+    const uint64_t m = __ballot(holds);
+    if (m && (threadIdx.x & 63) == 0) atomicMin(first, (uint32_t)(threadIdx.x + __builtin_ctzll(m)));
+}
+__device__ __forceinline__ void last_of(bool holds, uint32_t* last) {
+    const uint64_t m = __ballot(holds);
+    if (m && (threadIdx.x & 63) == 0) atomicMax(last, (uint32_t)(threadIdx.x + 63 - __builtin_clzll(m)));
+}
+
+// SLICE wavefronts, a segment each
+template <typename TL, int SLICE>
+__global__ __launch_bounds__(SLICE * 64) void sample_slices_kernel(const SampleArgs a) {
+    constexpr int WG = SLICE * 64;
+    __shared__ unsigned long long bins[BINS];
+    __shared__ uint32_t last;
+    __shared__ double part[SLICE];
+    __shared__ float tops[SLICE];
+    __shared__ uint32_t counts[SLICE];
     const int row_at = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const Scratch sc = scratch_of(a, row_at);
-    const RowAsks r = asks_of(a, row_at);
     const int g = blockIdx.x * SLICE + wave;
     const bool here = g < sc.segs;
     Lane16<TL> x;
-    float top = NEVER;
+    if (here) x.load(reinterpret_cast<const TL*>(a.logits + (int64_t)row_at * a.ld), a.V, g);
+    const RowAsks r = asks_of(a, row_at);
+    float mine = NEVER;
     if (here) {
-        x.load(reinterpret_cast<const TL*>(a.logits + (int64_t)row_at * a.ld), a.V, g);
 #pragma unroll
-        for (int e = 0; e < 16; e++) top = fmaxf(top, x.v[e]);
-        top = wave_max(top);
-        if (lane == 0) sc.seg_top[g] = top;
+        for (int e = 0; e < 16; e++) mine = fmaxf(mine, x.v[e]);
     }
+    float top = wave_max(mine);
+    if (here && lane == 0) sc.seg_top[g] = top;
     if (!r.filtered()) {
         if (!here || r.greedy || r.min) return;
         double w = 0;
 #pragma unroll
-        for (int e = 0; e < 16; e++) w += weight_of(x.v[e], top, r.T);
+        for (int e = 0; e < 16; e++) w += weight_of(x.v[e], top, r.per);
         w = wave_sum(top == NEVER ? 0.0 : w);
         if (lane == 0) sc.sums[g] = w;
         return;
     }
     if (lane == 0) tops[wave] = top;
-    for (int i = threadIdx.x; i < BINS; i += THREADS) mass[i] = 0, count[i] = 0;
-    if (threadIdx.x == 0) total_mass = 0, total_count = 0;
+    for (int i = threadIdx.x; i < BINS; i += WG) bins[i] = 0;
+    if (threadIdx.x == 0) last = BINS;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < NW; w++) top = fmaxf(top, tops[w]);
-    const double per = PER_UNIT / r.T, bin = floor((double)top * per), scale = (double)(1ull << a.shift);
+    for (int w = 0; w < SLICE; w++) top = fmaxf(top, tops[w]);
+    const double per = PER_UNIT * r.per, bin = floor((double)top * per);
+    auto bin_of = [&](double t) __attribute__((always_inline)) {
+        const double d = bin - t;
+        return d < BINS - 1 ? (int)d : BINS - 1;  // (NaN too: the last)
+    };
+    int until = BINS;  // bins from here on are of no interest
+    if (r.top_k && r.k <= WG) {
+        // The lanes' maxima alone: where k of them lie is a bin below which nothing can be among the first k.
+        if (mine != NEVER) atomicAdd(&bins[bin_of(floor((double)mine * per))], 1ull);
+        __syncthreads();
+        constexpr int EACH = BINS / WG > 0 ? BINS / WG : 1;
+        double n[EACH], all, sum = 0;
+#pragma unroll
+        for (int i = 0; i < EACH; i++) {
+            const int b = threadIdx.x * EACH + i;
+            n[i] = b < BINS ? (double)bins[b] : 0.0;
+            sum += n[i];
+        }
+        double run = scan_before<SLICE>(sum, part, &all);
+        bool enough = false;
+        uint32_t at = 0;
+#pragma unroll
+        for (int i = 0; i < EACH; i++) {
+            run += n[i];
+            if (!enough && run >= (double)r.k) enough = true, at = threadIdx.x * EACH + i;
+        }
+        const uint64_t m = __ballot(enough && threadIdx.x * EACH < BINS);
+        const uint32_t first = __shfl(at, m ? __builtin_ctzll(m) : 0);
+        if (m && lane == 0) atomicMin(&last, first);
+        __syncthreads();
+        until = (int)last + 1;
+        for (int i = threadIdx.x; i < BINS; i += WG) bins[i] = 0;
+        __syncthreads();
+    }
+    uint32_t n = 0;
     if (top != NEVER && here) {
-        unsigned long long m = 0;
-        uint32_t n = 0;
 #pragma unroll
         for (int e = 0; e < 16; e++) {
+            const double t = (double)x.v[e] * per, low = floor(t);
+            const int at = bin_of(low);
             if (x.v[e] == NEVER) continue;
-            const double d = bin - floor((double)x.v[e] * per);
-            const int at = d < BINS - 1 ? (int)d : BINS - 1;
-            const unsigned long long w = whole(weight_of(x.v[e], top, r.T), scale);
-            atomicAdd(&count[at], 1u);
-            atomicAdd(&mass[at], w);
-            m += w, n++;
+            n++;
+            if (at >= until) continue;
+            unsigned long long w = 1ull << MASS_BITS;
+            if (!r.top_k) w += (1ull << 34) + (uint32_t)(factor_less_1(t - low) * FACTOR_SCALE + 0.5);  // (top_k goes by counts)
+            atomicAdd(&bins[at], w);
         }
-        m = wave_sum(m), n = wave_sum(n);
-        if (lane == 0) atomicAdd(&total_mass, m), atomicAdd(&total_count, n);
     }
+    n = wave_sum(n);
+    if (lane == 0) counts[wave] = n;
     __syncthreads();
-    for (int i = threadIdx.x; i < BINS; i += THREADS) {
-        sc.mass[(int64_t)blockIdx.x * BINS + i] = mass[i];
-        sc.count[(int64_t)blockIdx.x * BINS + i] = count[i];
-    }
+    for (int i = threadIdx.x; i < BINS; i += WG) sc.bins[(int64_t)blockIdx.x * BINS + i] = bins[i];
     if (threadIdx.x == 0) {
-        sc.slices[blockIdx.x] = Slice{bin, total_mass, top, total_count};
+        uint32_t all = 0;
+#pragma unroll
+        for (int w = 0; w < SLICE; w++) all += counts[w];
+        sc.slices[blockIdx.x] = Slice{bin, all, 0};
         if (blockIdx.x == 0) sc.state->entries = 0;
     }
 }
 
-// ---- what the filters leave -----------------------------------------------------------------------------------------------------
-__device__ __forceinline__ float row_top(const Scratch& sc, float* part) {
-    float top = NEVER;
-    for (int i = threadIdx.x; i < sc.segs; i += THREADS) top = fmaxf(top, sc.seg_top[i]);
+// ---- what the filters leave: workgroups of four segments ---------------------------------------------------------------------------
+// the largest of all (first: this thread's own of the row's segments' maxima)
+template <int WAVES>
+__device__ __forceinline__ float row_top(const Scratch& sc, float first, float* part) {
+    float top = first;
+    for (int i = WAVES * 64 + threadIdx.x; i < sc.segs; i += WAVES * 64) top = fmaxf(top, sc.seg_top[i]);
     top = wave_max(top);
-    __syncthreads();
     if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = top;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < NW; w++) top = fmaxf(top, part[w]);
+    for (int w = 0; w < WAVES; w++) top = fmaxf(top, part[w]);
     return top;
 }
 
+// the least logit whose bin is `at` or more
+__device__ __forceinline__ float least_of(double at, double per) {
+    uint32_t k = key_of(settled((float)(at / per)));
+    while (floor((double)of_key(k) * per) >= at) k--;
+    while (floor((double)of_key(k) * per) < at) k++;
+    return settled(of_key(k));
+}
+
 template <typename TL>
-__global__ __launch_bounds__(THREADS) void sample_filter_kernel(const SampleArgs a) {
-    __shared__ double part[NW];
-    __shared__ float fpart[NW];
-    __shared__ uint32_t found, entries, base, n_last, n_run;
-    __shared__ double before_mass, before_count;
+__global__ __launch_bounds__(256) void sample_filter_kernel(const SampleArgs a) {
+    constexpr int WAVES = 4, HALF = 256;
+    static_assert(BINS == 2 * HALF, "two bins a thread");
+    __shared__ double part[WAVES][4], before_mass, before_count;
+    __shared__ int slice_ahead[MOST_SLICES];
+    __shared__ float fpart[WAVES];
+    __shared__ uint32_t found, last_bin, base, n_last, n_run, taken[WAVES], all_count;
     const int row_at = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const Scratch sc = scratch_of(a, row_at);
-    const RowAsks r = asks_of(a, row_at);
-    if (r.greedy || !(r.filtered() || r.min)) return;
-    const float top = row_top(sc, fpart);
-    if (top == NEVER) return;
-    const int g = blockIdx.x * SLICE + wave;
+    const int g = blockIdx.x * WAVES + wave;
     const TL* const row = reinterpret_cast<const TL*>(a.logits + (int64_t)row_at * a.ld);
     const bool here = g < sc.segs;
+    // (everything that does not wait for something else first)
+    const float first_top = (int)threadIdx.x < sc.segs ? sc.seg_top[threadIdx.x] : NEVER;
     const float seg_top = here ? sc.seg_top[g] : NEVER;
+    const RowAsks r = asks_of(a, row_at);
+    if (r.greedy || !(r.filtered() || r.min)) return;
+    Slice own = {0.0, 0, 0};
+    if (r.filtered() && (int)threadIdx.x < sc.n_slices) own = sc.slices[threadIdx.x];
+    Lane16<TL> x;
+    if (here) x.ask(row, a.V, g);
+    const float top = row_top<WAVES>(sc, first_top, fpart);
+    if (top == NEVER) return;
+    auto weight = [&](float l) __attribute__((always_inline)) {
+        const double v = weight_of(l, top, r.per);
+        return v < r.min_p && l != top ? 0.0 : v;
+    };
     if (!r.filtered()) {
         if (!here) return;
         double w = 0;
         if (seg_top != NEVER) {
-            Lane16<TL> x;
-            x.load(row, a.V, g);
+            x.get(row, a.V, g);
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const double v = weight_of(x.v[e], top, r.T);
-                w += v < r.min_p && x.v[e] != top ? 0.0 : v;
-            }
+            for (int e = 0; e < 16; e++) w += weight(x.v[e]);
             w = wave_sum(w);
         }
         if (lane == 0) sc.sums[g] = w;
         return;
     }
-    // the row's histogram, a bin a thread
-    double bin = -__builtin_huge_val(), all_mass = 0, all_count = 0;
-    for (int i = 0; i < sc.n_slices; i++) {
-        const Slice s = sc.slices[i];
-        if (s.count) bin = fmax(bin, s.bin);
+    const double per = PER_UNIT * r.per, bin = floor((double)top * per);
+    const bool odd = !(fabs(bin) <= GRID) || !(per <= 1e300) || per < 1e-30;
+    if (threadIdx.x == 0) found = BINS, last_bin = 0, all_count = 0;
+    __syncthreads();
+    if ((int)threadIdx.x < sc.n_slices) {
+        // (a slice that lies below the grid, or holds nothing, has nothing in the row's other bins)
+        const double ahead = bin - own.bin;
+        slice_ahead[threadIdx.x] = ahead < BINS ? (int)ahead : BINS;
     }
-    const double per = PER_UNIT / r.T;
-    const bool odd = !(fabs(bin) <= GRID) || !(per <= 1e300);  // (a slice that lies below the grid has all it holds in the last bin)
-    const double scale = 1.0 / (double)(1ull << a.shift);
+    const uint32_t held = wave_sum(own.count);
+    if (lane == 0 && held) atomicAdd(&all_count, held);
+    __syncthreads();
+    // The row's histogram, bins b and b + 256 a thread; four slices at a time, so that nothing waits for one load after the other.
     const int b = threadIdx.x;
-    double mass = 0, count = 0;
+    unsigned long long mass[2] = {0, 0};
+    uint32_t count[2] = {0, 0};
     if (!odd) {
-        for (int i = 0; i < sc.n_slices; i++) {
-            const Slice s = sc.slices[i];
-            if (!s.count) continue;
-            const double f = weight_of(s.top, top, r.T) * scale;
-            all_mass += f * (double)s.mass, all_count += s.count;
-            const double at = b - (bin - s.bin);
-            if (b < BINS - 1 && at >= 0.0) {
-                const int64_t o = (int64_t)i * BINS + (int)at;
-                mass += f * (double)sc.mass[o];
-                count += sc.count[o];
+        for (int i0 = 0; i0 < sc.n_slices; i0 += 8) {
+            unsigned long long v[8][2];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const int at = i0 + i < sc.n_slices ? b - slice_ahead[i0 + i] : -BINS;
+                const unsigned long long* const p = sc.bins + (int64_t)(i0 + i) * BINS + at;
+                v[i][0] = at >= 0 ? p[0] : 0ull;
+                v[i][1] = at + HALF >= 0 && b + HALF < BINS - 1 ? p[HALF] : 0ull;
             }
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    mass[h] += v[i][h] & ((1ull << MASS_BITS) - 1);
+                    count[h] += (uint32_t)(v[i][h] >> MASS_BITS);
+                }
         }
     }
-    double sum_mass, sum_count;
-    double run_mass = scan_before(mass, part, &sum_mass), run_count = scan_before(count, part, &sum_count);
-    if (b == BINS - 1) mass = fmax(all_mass - sum_mass, 0.0), count = all_count - sum_count;
+    double m[2], v[4], run[4], all[4];
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+        m[h] = r.top_k ? 0.0 : (double)mass[h] / FACTOR_SCALE * exp_of((bin - (b + h * HALF) - (double)top * per) * (1.0 / PER_UNIT));
+        v[h] = m[h], v[2 + h] = count[h];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        run[k] = v[k];
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const double o = __shfl_up(run[k], d);
+            if (lane >= d) run[k] += o;
+        }
+        if (lane == 63) part[wave][k] = run[k];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        double before = 0;
+        all[k] = 0;
+#pragma unroll
+        for (int w = 0; w < WAVES; w++) {
+            before += w < wave ? part[w][k] : 0.0;
+            all[k] += part[w][k];
+        }
+        run[k] += before;  // (up to this bin and with it)
+    }
+    run[1] += all[0], run[3] += all[2];
+    const double all_mass = all[0] + all[1];
+    if (b + HALF == BINS - 1) run[3] = all_count, v[3] = run[3] - all[2] - all[3], count[1] = (uint32_t)v[3];
     // the bin in which the run ends: of top_k the first whose count is enough, of top_p alone the first whose mass is (of both: top_p's share is of what top_k leaves, which only the list tells)
+#pragma unroll
+    for (int h = 1; h >= 0; h--) {
+        const uint64_t e = __ballot(r.top_k ? run[2 + h] >= (double)r.k : run[h] >= r.p * all_mass), o = __ballot(count[h] > 0);
+        if (lane == 0) {
+            if (e) atomicMin(&found, (uint32_t)(b + h * HALF + __builtin_ctzll(e)));
+            if (o) atomicMax(&last_bin, (uint32_t)(b + h * HALF + 63 - __builtin_clzll(o)));
+        }
+    }
     __syncthreads();
-    if (threadIdx.x == 0) found = BINS - 1;
-    __syncthreads();
-    if (b < BINS && (r.top_k ? run_count + count >= (double)r.k : run_mass + mass >= r.p * all_mass)) atomicMin(&found, (uint32_t)b);
-    __syncthreads();
-    const int cut = found;
-    if (b == cut) before_mass = run_mass, before_count = run_count, n_last = (uint32_t)count, n_run = (uint32_t)(run_count + count);
-    if (threadIdx.x == 0) entries = 0;
+    const int cut = found < BINS ? (int)found : (int)last_bin;  // (none: fewer tokens than top_k, or sums that were rounded)
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+        if (b + h * HALF == cut) before_mass = run[h] - m[h], before_count = run[2 + h] - v[2 + h], n_last = count[h], n_run = (uint32_t)run[2 + h];
     __syncthreads();
     const uint32_t path = odd ? ALONE : n_run <= LIST ? BY_LIST : (r.top_k && r.top_p) || n_last > LIST || sc.segs > MOST_SUMS ? ALONE : BY_SUMS;
     if (blockIdx.x == 0 && threadIdx.x == 0) {
         State* const s = sc.state;
-        s->path = path, s->before_count = (uint32_t)before_count, s->top = top, s->before_mass = before_mass, s->mass = all_mass;
+        s->path = path, s->before_count = (uint32_t)before_count, s->before_mass = before_mass, s->mass = all_mass;
     }
     if (path == ALONE) return;
-    // this slice's: into the list what lies in the bin (BY_LIST: and above it), into the sums what lies above
-    Lane16<TL> x;
+    // into the list what lies in the bin, or in it and above
+    const float from = cut == BINS - 1 ? of_key(key_of(NEVER) + 1) : least_of(bin - cut, per), to = path == BY_SUMS && cut > 0 ? least_of(bin - cut + 1, per) : __builtin_huge_valf();
     uint32_t takes = 0;
-    const bool some = here && seg_top != NEVER && bin - floor((double)seg_top * per) <= cut;
     double w = 0;
-    if (some) {
-        x.load(row, a.V, g);
+    if (here && seg_top >= from) {
+        x.get(row, a.V, g);
 #pragma unroll
         for (int e = 0; e < 16; e++) {
-            if (x.v[e] == NEVER) continue;
-            const double d = fmin(bin - floor((double)x.v[e] * per), BINS - 1.0);
-            if (d == cut || (path == BY_LIST && d < cut)) takes |= 1u << e;
-            if (path == BY_SUMS && d < cut) {
-                const double v = weight_of(x.v[e], top, r.T);
-                w += v < r.min_p && x.v[e] != top ? 0.0 : v;
-            }
+            takes |= x.v[e] >= from && x.v[e] < to ? 1u << e : 0;
+            if (path == BY_SUMS && __any(x.v[e] >= to)) w += x.v[e] >= to ? weight(x.v[e]) : 0.0;
         }
     }
     if (path == BY_SUMS && here) {
         w = wave_sum(w);
         if (lane == 0) sc.sums[g] = w;
     }
-    uint32_t at = 0;
-    if (takes) at = atomicAdd(&entries, (uint32_t)__popc(takes));
-    __syncthreads();
-    if (threadIdx.x == 0 && entries) base = atomicAdd(&sc.state->entries, entries);
-    __syncthreads();
-    if (takes) {
-        at += base;
+    uint32_t at = __popc(takes);
+    const uint32_t mine = at;
 #pragma unroll
-        for (int e = 0; e < 16; e++)
-            if (takes >> e & 1) sc.list[at++] = (unsigned long long)key_of(x.v[e]) << 32 | (0xffffffffu - (uint32_t)(g * SEG + x.at(e)));
+    for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t o = __shfl_up(at, d);
+        if (lane >= d) at += o;
     }
+    if (lane == 63) taken[wave] = at;
+    __syncthreads();
+    uint32_t every = 0, before = 0;
+#pragma unroll
+    for (int i = 0; i < WAVES; i++) {
+        before += i < wave ? taken[i] : 0;
+        every += taken[i];
+    }
+    if (every == 0) return;
+    if (threadIdx.x == 0) base = atomicAdd(&sc.state->entries, every);
+    __syncthreads();
+    at += base + before - mine;
+#pragma unroll
+    for (int e = 0; e < 16; e++)
+        if (takes >> e & 1) {
+            if (at < LIST) sc.list[at] = (unsigned long long)key_of(x.v[e]) << 32 | (0xffffffffu - (uint32_t)(g * SEG + x.at(e)));
+            at++;
+        }
 }
 
-// ---- the draw: a workgroup a row -------------------------------------------------------------------------------------------------
-// n entries of the list, largest first; returns the place of them
-__device__ unsigned long long* sorted(unsigned long long* e, unsigned long long* room, int n) {
-    if (n <= THREADS) {  // by counting
-        const unsigned long long mine = (int)threadIdx.x < n ? e[threadIdx.x] : 0;
-        int rank = 0;
-        if ((int)threadIdx.x < n)
-            for (int i = 0; i < n; i++) rank += e[i] > mine;
-        if ((int)threadIdx.x < n) room[rank] = mine;
+// ---- where the run ends, a workgroup a row --------------------------------------------------------------------------------------------
+constexpr int MINE = LIST / THREADS, BUCKETS = 1024, FEW = 128;
+struct Room {
+    unsigned long long mass[BUCKETS];
+    uint32_t count[BUCKETS];
+    unsigned long long few[FEW], few_mass[FEW];
+    unsigned long long low, high, best, part[NW], before_mass;
+    uint32_t cpart[NW], first, last;
+};
+static_assert(BUCKETS == THREADS && FEW * 8 == THREADS, "a bucket a thread; eight threads for each that is left");
+
+// Of the entries (a thread's c, no two alike; 0: none) in descending order: the first up to which there are `want` of them, or whose masses m come to `want` (STRICT: to more); the last if none does.
+// The range of what is left is cut into 1024 buckets until one of them holds few, and those are compared with each other.
+enum { BY_COUNT, BY_MASS, BY_MASS_STRICT };
+// most: entries lie in the first `most` places.
+__device__ __forceinline__ unsigned long long pick(const unsigned long long (&c)[MINE], const unsigned long long (&m)[MINE], int most, int mode, unsigned long long want, Room& o) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    unsigned long long low = 1, high = ~0ull, before = 0;  // of the entries from low to high; what lies above them
+    int n;
+    for (;;) {
+        unsigned long long lo = ~0ull, hi = 0;
+        uint32_t here = 0;
+#pragma unroll
+        for (int i = 0; i < MINE; i++)
+            if (i * THREADS < most && c[i] >= low && c[i] <= high) {
+                here++;
+                lo = c[i] < lo ? c[i] : lo;
+                hi = c[i] > hi ? c[i] : hi;
+            }
+        uint32_t at = here;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t v = __shfl_up(at, d);
+            if (lane >= d) at += v;
+        }
+        __syncthreads();  // (what the last round left has been read)
+        if (lane == 63) o.cpart[wave] = at;
+        if (threadIdx.x == 0) o.low = ~0ull, o.high = 0, o.best = 0, o.first = BUCKETS, o.last = 0;
         __syncthreads();
-        return room;
-    }
-    int m = 2048;
-    while (m < n) m *= 2;
-    for (int i = n + threadIdx.x; i < m; i += THREADS) e[i] = 0;
-    for (int k = 2; k <= m; k *= 2)
-        for (int d = k / 2; d >= 1; d /= 2) {
-            __syncthreads();
-            for (int t = threadIdx.x; t < m / 2; t += THREADS) {
-                const int i = (t / d) * 2 * d + t % d;
-                const unsigned long long p = e[i], q = e[i + d];
-                if ((p < q) == ((i & k) == 0)) e[i] = q, e[i + d] = p;
+        uint32_t off = at - here;
+        n = 0;
+#pragma unroll
+        for (int w = 0; w < NW; w++) {
+            off += w < wave ? o.cpart[w] : 0;
+            n += (int)o.cpart[w];
+        }
+        if (n <= FEW) {
+#pragma unroll
+            for (int i = 0; i < MINE; i++)
+                if (i * THREADS < most && c[i] >= low && c[i] <= high) o.few[off] = c[i], o.few_mass[off++] = mode == BY_COUNT ? 1ull : m[i];
+            break;
+        }
+        if (__any(here)) {
+            hi = wave_max(hi), lo = ~wave_max(~lo);
+            if (lane == 0) {
+                atomicMin(&o.low, lo);
+                atomicMax(&o.high, hi);
             }
         }
+        o.mass[threadIdx.x] = 0, o.count[threadIdx.x] = 0;
+        __syncthreads();
+        low = o.low, high = o.high;
+        const unsigned long long span = high - low;
+        const int bits = 64 - __clzll((long long)span), shift = bits > 10 ? bits - 10 : 0;
+#pragma unroll
+        for (int i = 0; i < MINE; i++)
+            if (i * THREADS < most && c[i] >= low && c[i] <= high) {
+                atomicAdd(&o.count[(high - c[i]) >> shift], 1u);
+                if (mode != BY_COUNT) atomicAdd(&o.mass[(high - c[i]) >> shift], m[i]);
+            }
+        __syncthreads();
+        const bool some = o.count[threadIdx.x] > 0;
+        const unsigned long long mine = mode == BY_COUNT ? o.count[threadIdx.x] : o.mass[threadIdx.x];
+        unsigned long long run = mine;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const unsigned long long v = __shfl_up(run, d);
+            if (lane >= d) run += v;
+        }
+        if (lane == 63) o.part[wave] = run;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < NW; w++) run += w < wave ? o.part[w] : 0ull;
+        run += before;
+        first_of(some && (mode == BY_MASS_STRICT ? run > want : run >= want), &o.first);
+        last_of(some, &o.last);
+        __syncthreads();
+        const int b = o.first < BUCKETS ? (int)o.first : (int)o.last;
+        if ((int)threadIdx.x == b) o.before_mass = run - mine;
+        __syncthreads();
+        before = o.before_mass;
+        const unsigned long long up = high - ((unsigned long long)b << shift), room = (1ull << shift) - 1;
+        low = up - low > room ? up - room : low;
+        high = up;
+    }
     __syncthreads();
-    return e;
+    // eight neighbouring threads an entry, each against every eighth of them
+    unsigned long long got = 0, least = ~0ull;
+    if ((int)(threadIdx.x & ~63u) < n * 8) {
+        const int i = threadIdx.x >> 3;
+        const unsigned long long mine = o.few[i < n ? i : 0];
+        unsigned long long run = 0;
+        for (int j = threadIdx.x & 7; j < n; j += 8) run += o.few[j] >= mine ? o.few_mass[j] : 0ull;
+#pragma unroll
+        for (int d = 1; d < 8; d *= 2) run += __shfl_xor(run, d);
+        run += before;
+        if (i < n) {
+            if (mode == BY_MASS_STRICT ? run > want : run >= want) got = mine;
+            least = mine;
+        }
+        got = wave_max(got), least = ~wave_max(~least);
+        if (lane == 0) {
+            atomicMax(&o.best, got);
+            atomicMin(&o.low, least);
+        }
+    }
+    __syncthreads();
+    return o.best ? o.best : o.low;
+}
+__device__ unsigned long long sum_of(unsigned long long v, Room& o) {
+    v = wave_sum(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) o.part[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0;
+#pragma unroll
+    for (int w = 0; w < NW; w++) v += o.part[w];
+    return v;
 }
 
 template <typename TL>
 __global__ __launch_bounds__(THREADS) void sample_draw_kernel(const SampleArgs a) {
     __shared__ Shared s;
-    __shared__ unsigned long long list[LIST], room[THREADS];
+    __shared__ Room o;
+    __shared__ unsigned long long more[MOST_SUMS];
     const int row_at = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int V = a.V;
     const TL* const row = reinterpret_cast<const TL*>(a.logits + (int64_t)row_at * a.ld);
     const Scratch sc = scratch_of(a, row_at);
     const int segs = sc.segs;
     const RowAsks r = asks_of(a, row_at);
-    const float top = row_top(sc, s.fpart);
+    // (what the next steps want, asked for with the first)
+    const State state = *sc.state;
+    const double first_sum = (int)threadIdx.x < segs ? sc.sums[threadIdx.x] : 0.0;
+    const float first_top = (int)threadIdx.x < segs ? sc.seg_top[threadIdx.x] : NEVER;
+    const double u = (double)a.u[row_at];
+    unsigned long long c[MINE], m[MINE];
+#pragma unroll
+    for (int i = 0; i < MINE; i++) {  // (asked for before anything is known of it; sorted out below)
+        c[i] = r.filtered() && i == 0 ? sc.list[threadIdx.x] : 0;
+    }
+    const float top = row_top<NW>(sc, first_top, s.fpart);
     if (top == NEVER) {
         if (threadIdx.x == 0) a.ids[row_at] = -1;
         return;
     }
-    const double u = (double)a.u[row_at];
     if (r.greedy) {  // the first segment that holds it, its first place in it
-        if (threadIdx.x == 0) s.pick = V;
+        if (threadIdx.x == 0) s.pick = V, s.found = 0xffffffffu;
         __syncthreads();
         for (int g = threadIdx.x; g < segs; g += THREADS)
-            if (sc.seg_top[g] == top) atomicMin(&s.pick, g);
+            if ((g < THREADS ? first_top : sc.seg_top[g]) == top) atomicMin(&s.pick, g);
         __syncthreads();
         const int i = s.pick * SEG + threadIdx.x;
-        if (threadIdx.x == 0) s.found = 0xffffffffu;
+        first_of(i < V && value_at(row, i) == top, &s.found);
         __syncthreads();
-        if (i < V && value_at(row, i) == top) atomicMin(&s.found, (uint32_t)i);
-        __syncthreads();
-        if (threadIdx.x == 0) a.ids[row_at] = (int)s.found;
+        if (threadIdx.x == 0) a.ids[row_at] = s.pick * SEG + (int)s.found;
         return;
     }
-    const uint32_t path = r.filtered() ? sc.state->path : BY_SUMS;
+    const uint32_t path = r.filtered() ? state.path : BY_SUMS;
     const double scale = (double)(1ull << a.shift);
     Cut cut = {key_of(NEVER), V};
-    double* const sums = sc.sums;
     auto stays = [&](float l, int i) __attribute__((always_inline)) {
-        if (l == NEVER || !cut.holds(key_of(l), i)) return 0.0;
-        const double w = weight_of(l, top, r.T);
-        return w < r.min_p && l != top ? 0.0 : w;
+        const double w = weight_of(l, top, r.per);
+        return l == NEVER || !cut.holds(key_of(l), i) || (w < r.min_p && l != top) ? 0.0 : w;
     };
     if (r.filtered() && path != ALONE) {
-        const int n = (int)sc.state->entries;
-        for (int i = threadIdx.x; i < n; i += THREADS) list[i] = sc.list[i];
-        __syncthreads();
-        unsigned long long* const e = sorted(list, room, n);
-        // how many of the list stay: four neighbours a thread, their weights and the weight in front of them
-        double w[LIST / THREADS], mine = 0, total;
-        const int i0 = threadIdx.x * (LIST / THREADS);
+        const int n = (int)state.entries < LIST ? (int)state.entries : LIST;
+        unsigned long long last = 1;
+        uint32_t low_weight = 0;
 #pragma unroll
-        for (int c = 0; c < LIST / THREADS; c++) {
-            const int i = i0 + c;
-            // (above the bin are, by sums, before_count more)
-            const bool in = i < n && (!r.top_k || i + (path == BY_SUMS ? (int)sc.state->before_count : 0) < r.k);
-            w[c] = in ? weight_of(of_key((uint32_t)(e[i] >> 32)), top, r.T) : -1.0;
-            mine += in ? w[c] : 0.0;
+        for (int i = 0; i < MINE; i++) {
+            const int at = threadIdx.x + i * THREADS;
+            m[i] = 0;
+            if (i * THREADS >= n) {
+                c[i] = 0;
+                continue;
+            }
+            if (i > 0) c[i] = at < n ? sc.list[at] : 0;
+            if (at >= n) c[i] = 0;
+            const float l = of_key((uint32_t)(c[i] >> 32));
+            const double w = c[i] ? weight_of(l, top, r.per) : 0.0;
+            m[i] = whole(w, scale);
+            low_weight |= w < r.min_p && l != top ? 1u << i : 0;
         }
-        double before = scan_before(mine, s.part, &total);
-        if (path == BY_SUMS) before += sc.state->before_mass;
-        const double want = r.p * (r.top_k ? total : sc.state->mass);
-        uint32_t kept = 0;
+        const uint32_t above = path == BY_SUMS ? state.before_count : 0;
+        for (int step = 0; step < 3; step++) {  // top_k, top_p, the token
+            int mode = BY_COUNT;
+            unsigned long long want = 0;
+            if (step == 0) {
+                if (!r.top_k || above + (uint32_t)n <= (uint32_t)r.k) continue;
+                want = (uint32_t)r.k - above;
+            } else if (step == 1) {  // (not BY_SUMS and top_k both)
+                if (!r.top_p) continue;
+                unsigned long long of = 0;
 #pragma unroll
-        for (int c = 0; c < LIST / THREADS; c++) {
-            // (of a run by mass the one that reaches it is the last; one token at least)
-            const bool in = w[c] >= 0.0 && (!r.top_p || before < want || i0 + c == 0);
-            if (w[c] >= 0.0) before += w[c];
-            if (in) kept = i0 + c + 1;
+                for (int i = 0; i < MINE; i++) of += c[i] ? m[i] : 0ull;
+                if (r.top_k) of = sum_of(of, o);
+                const double goal = ceil(r.p * (r.top_k ? (double)of : state.mass * scale)) - (path == BY_SUMS ? state.before_mass * scale : 0.0);
+                mode = BY_MASS, want = goal > 1.0 ? (unsigned long long)goal : 1ull;
+            } else {
+                unsigned long long all = 0;
+#pragma unroll
+                for (int i = 0; i < MINE; i++) {
+                    if (low_weight >> i & 1) c[i] = 0;
+                    m[i] = c[i] ? m[i] : 0ull;
+                    all += m[i];
+                    c[i] = (uint32_t)c[i];  // (the order of the vocabulary is that of falling complements of the index)
+                }
+                if (path == BY_SUMS) break;
+                all = sum_of(all, o);
+                const double goal = u > 0.0 ? u * (double)all : 0.0;
+                const bool inside = goal < (double)all;  // (else the last one that has weight)
+                mode = inside ? BY_MASS_STRICT : BY_MASS, want = inside ? (unsigned long long)goal : all;
+            }
+            last = pick(c, m, n, mode, want, o);
+            if (step < 2) {
+#pragma unroll
+                for (int i = 0; i < MINE; i++) c[i] = c[i] < last ? 0 : c[i];
+            }
         }
-        if (threadIdx.x == 0) s.found = 0;
-        __syncthreads();
-        atomicMax(&s.found, kept);
-        __syncthreads();
-        kept = s.found;
-        const unsigned long long last = e[kept - 1];
-        cut = Cut{(uint32_t)(last >> 32), (int)(0xffffffffu - (uint32_t)last)};
         if (path == BY_LIST) {
-            // in the order of the vocabulary: the same once more by index (the order is that of falling complements)
-            __syncthreads();
-            for (int i = threadIdx.x; i < (int)kept; i += THREADS) e[i] = e[i] << 32 | e[i] >> 32;
-            __syncthreads();
-            unsigned long long* const o = sorted(e, e == list ? room : list, (int)kept);
-            double run = 0;
-#pragma unroll
-            for (int c = 0; c < LIST / THREADS; c++) {
-                const int i = i0 + c;
-                w[c] = i < (int)kept ? stays(of_key((uint32_t)o[i]), -1) : 0.0;
-                run += w[c];
-            }
-            double all, at = scan_before(run, s.part, &all);
-            const double goal = u > 0.0 ? u * all : 0.0;
-            if (threadIdx.x == 0) s.found = 0xffffffffu, s.bin = 0;
-            __syncthreads();
-#pragma unroll
-            for (int c = 0; c < LIST / THREADS; c++) {
-                if (w[c] <= 0.0) continue;
-                at += w[c];
-                if (at > goal) atomicMin(&s.found, (uint32_t)(i0 + c));
-                atomicMax(&s.bin, (uint32_t)(i0 + c));
-            }
-            __syncthreads();
-            if (threadIdx.x == 0) a.ids[row_at] = (int)(0xffffffffu - (uint32_t)(o[s.found != 0xffffffffu ? s.found : s.bin] >> 32));
+            if (threadIdx.x == 0) a.ids[row_at] = (int)(0xffffffffu - (uint32_t)last);
             return;
         }
         // what stays of the bin, to its segments' sums
-        unsigned long long* const more = e == list ? room : list;
         for (int g = threadIdx.x; g < segs; g += THREADS) more[g] = 0;
         __syncthreads();
-        for (int i = threadIdx.x; i < (int)kept; i += THREADS) {
-            const double v = weight_of(of_key((uint32_t)(e[i] >> 32)), top, r.T);
-            if (!(v < r.min_p)) atomicAdd(&more[(0xffffffffu - (uint32_t)e[i]) / SEG], whole(v, scale));
-        }
+#pragma unroll
+        for (int i = 0; i < MINE; i++)
+            if (c[i]) atomicAdd(&more[(0xffffffffu - (uint32_t)c[i]) / SEG], m[i]);
+        cut = Cut{(uint32_t)(last >> 32), (int)(0xffffffffu - (uint32_t)last)};
         __syncthreads();
-        for (int g = threadIdx.x; g < segs; g += THREADS) sums[g] += (double)more[g] / scale;
     } else if (path == ALONE) {
-        if (r.top_k) cut = select(row, V, top, r.T, scale, cut, false, (uint32_t)r.k, 0ull, s);
+        if (r.top_k) cut = select(row, V, top, r.per, scale, cut, false, (uint32_t)r.k, 0ull, s);
         if (r.top_p) {
             unsigned long long m = 0;
             for (int g = wave; g < segs; g += NW) {
@@ -607,7 +876,7 @@ __global__ __launch_bounds__(THREADS) void sample_draw_kernel(const SampleArgs a
                 x.load(row, V, g);
 #pragma unroll
                 for (int e = 0; e < 16; e++)
-                    if (cut.holds(key_of(x.v[e]), g * SEG + x.at(e))) m += whole(weight_of(x.v[e], top, r.T), scale);
+                    if (cut.holds(key_of(x.v[e]), g * SEG + x.at(e))) m += whole(weight_of(x.v[e], top, r.per), scale);
             }
             m = wave_sum(m);
             __syncthreads();
@@ -615,7 +884,7 @@ __global__ __launch_bounds__(THREADS) void sample_draw_kernel(const SampleArgs a
             __syncthreads();
             m = 0;
             for (int w = 0; w < NW; w++) m += s.mass[w];
-            cut = select(row, V, top, r.T, scale, cut, true, 0u, (unsigned long long)ceil(r.p * (double)m), s);
+            cut = select(row, V, top, r.per, scale, cut, true, 0u, (unsigned long long)ceil(r.p * (double)m), s);
         }
         for (int g = wave; g < segs; g += NW) {
             Lane16<TL> x;
@@ -624,21 +893,25 @@ __global__ __launch_bounds__(THREADS) void sample_draw_kernel(const SampleArgs a
 #pragma unroll
             for (int e = 0; e < 16; e++) w += stays(x.v[e], g * SEG + x.at(e));
             w = wave_sum(w);
-            if (lane == 0) sums[g] = w;
+            if (lane == 0) sc.sums[g] = w;
         }
-    } else if (!r.min) {  // (relative to its own maximum each)
-        for (int g = threadIdx.x; g < segs; g += THREADS) sums[g] = sums[g] * weight_of(sc.seg_top[g], top, r.T);
+        __syncthreads();
     }
-    __syncthreads();
-    // the segment: up to 1024 of them at a time
+    // a segment's sum: without filters it is relative to its own maximum, with a list there may be more to it
+    const bool own = !r.filtered() && !r.min, added = r.filtered() && path == BY_SUMS;
+    auto sum_at = [&](int g) __attribute__((always_inline)) {
+        if (g >= segs) return 0.0;
+        const bool ready = g < THREADS && path != ALONE;
+        const double w = ready ? first_sum : sc.sums[g];
+        return own ? w * weight_of(ready ? first_top : sc.seg_top[g], top, r.per) : added ? w + (double)more[g] / scale : w;
+    };
     double total = 0;
     for (int g0 = 0; g0 < segs; g0 += THREADS) {
         double all;
-        scan_before(g0 + (int)threadIdx.x < segs ? sums[g0 + threadIdx.x] : 0.0, s.part, &all);
+        scan_before(sum_at(g0 + threadIdx.x), s.part, &all);
         total += all;
     }
     const double want = u > 0.0 ? u * total : 0.0;
-    __syncthreads();
     if (threadIdx.x == 0) s.pick = segs;
     __syncthreads();
     double run = 0;
@@ -646,10 +919,13 @@ __global__ __launch_bounds__(THREADS) void sample_draw_kernel(const SampleArgs a
     for (int g0 = 0; g0 < segs && s.pick == segs; g0 += THREADS) {  // (the same in all threads: a barrier lies between)
         double all;
         const int g = g0 + threadIdx.x;
-        const double w = g < segs ? sums[g] : 0.0, before = run + scan_before(w, s.part, &all);
+        const double w = sum_at(g), before = run + scan_before(w, s.part, &all);
         run += all;
         if (w > 0.0) last = g;
-        if (w > 0.0 && before + w > want) atomicMin(&s.pick, g);
+        {
+            const uint64_t m = __ballot(w > 0.0 && before + w > want);
+            if (m && lane == 0) atomicMin(&s.pick, g + (int)__builtin_ctzll(m));
+        }
         __syncthreads();
         if (g == s.pick) s.rest = want - before;
         __syncthreads();
@@ -660,38 +936,43 @@ __global__ __launch_bounds__(THREADS) void sample_draw_kernel(const SampleArgs a
         if (threadIdx.x == 0) s.pick = -1;
         s.rest = 1e300;
         __syncthreads();
-        atomicMax(&s.pick, last);
+        last = wave_max(last);
+        if (lane == 0) atomicMax(&s.pick, last);
         __syncthreads();
     }
-    const int seg = s.pick;
+    const int i = s.pick * SEG + threadIdx.x;
     const double rest = s.rest;
-    const int i = seg * SEG + threadIdx.x;
+    if (threadIdx.x == 0) s.found = 0xffffffffu, s.bin = 0;
     double all;
     const double w = i < V ? stays(value_at(row, i), i) : 0.0, before = scan_before(w, s.part, &all);
+    first_of(w > 0.0 && before + w > rest, &s.found);
+    last_of(w > 0.0, &s.bin);
     __syncthreads();
-    if (threadIdx.x == 0) s.found = 0xffffffffu, s.bin = 0;
-    __syncthreads();
-    if (w > 0.0) {
-        if (before + w > rest) atomicMin(&s.found, (uint32_t)i);
-        atomicMax(&s.bin, (uint32_t)i);
-    }
-    __syncthreads();
-    if (threadIdx.x == 0) a.ids[row_at] = (int)(s.found != 0xffffffffu ? s.found : s.bin);
+    if (threadIdx.x == 0) a.ids[row_at] = s.pick * SEG + (int)(s.found != 0xffffffffu ? s.found : s.bin);
 }
 
-size_t sample_scratch_bytes(int B, int V) { return (size_t)B * row_bytes(V); }
+// Segments of a slice: 4 where 16 would leave most of the chip idle
+int sample_slice(int B, int V) {
+    const int64_t segs = ((int64_t)V + SEG - 1) / SEG;
+    return B * ((segs + 15) / 16) < 256 && segs <= 4 * MOST_SLICES ? 4 : 16;
+}
+size_t sample_scratch_bytes(int B, int V) { return (size_t)B * row_bytes(V, sample_slice(B, V)); }
 
-template <typename TL>
+template <typename TL, int SLICE>
 static int launch(const SampleArgs& a, int B, hipStream_t st) {
     const int segs = (a.V + SEG - 1) / SEG, slices = (segs + SLICE - 1) / SLICE;
     // (what a number for all rows rules out is not launched)
     const bool greedy = (!a.temperature && !(a.temperature_all > 0.0)) || (!a.top_k && a.top_k_all == 1) || (!a.top_p && a.top_p_all <= 0.0);
     const bool open = !a.top_k && (a.top_k_all <= 0 || a.top_k_all >= a.V) && !a.top_p && a.top_p_all >= 1.0 && !a.min_p && a.min_p_all <= 0.0;
-    hipLaunchKernelGGL(sample_slices_kernel<TL>, dim3((unsigned)slices, (unsigned)B), dim3(THREADS), 0, st, a);
-    if (!greedy && !open) hipLaunchKernelGGL(sample_filter_kernel<TL>, dim3((unsigned)slices, (unsigned)B), dim3(THREADS), 0, st, a);
+    hipLaunchKernelGGL((sample_slices_kernel<TL, SLICE>), dim3((unsigned)slices, (unsigned)B), dim3(SLICE * 64), 0, st, a);
+    if (!greedy && !open) hipLaunchKernelGGL(sample_filter_kernel<TL>, dim3((unsigned)((segs + 3) / 4), (unsigned)B), dim3(256), 0, st, a);
     hipLaunchKernelGGL(sample_draw_kernel<TL>, dim3((unsigned)B), dim3(THREADS), 0, st, a);
     return check_hip(hipGetLastError(), "sample_draw_kernel launch");
 }
-int launch_sample(const SampleArgs& a, int B, bool f32, hipStream_t st) { return f32 ? launch<float>(a, B, st) : launch<uint16_t>(a, B, st); }
+int launch_sample(SampleArgs a, int B, bool f32, hipStream_t st) {
+    a.slice = sample_slice(B, a.V);
+    if (a.slice == 4) return f32 ? launch<float, 4>(a, B, st) : launch<uint16_t, 4>(a, B, st);
+    return f32 ? launch<float, 16>(a, B, st) : launch<uint16_t, 16>(a, B, st);
+}
 
 }  // namespace mmx

@@ -15,6 +15,7 @@ struct SampleArgs {
     int top_k_all;
     int V;
     int shift;  // masses as whole numbers are multiples of 2^-shift: V of them stay below 2^62
+    int slice;  // segments of a slice
     int32_t* ids;
     char* scratch;
 };

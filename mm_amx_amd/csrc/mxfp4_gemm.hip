@@ -208,21 +208,68 @@ __global__ __launch_bounds__(512) void mxfp4_rows_kernel(const Mxfp4Gemm g) {
 // then their 256 bytes of scales, straight from memory into one of R slots of LDS; with the operands in the instruction's own order every LDS read is a KiB in a row.  A stage has four steps of 64 k;
 // the operands of a step are read during the one before.  The one barrier per stage stands in front of its last step: all of it has been read into registers then, so its slot is free for
 // stage t + R, whose loads are spread over the last step and the next stage's first two, and stage t + 1 has landed.
-template <int PM, int PN, int WGM, int WGN, int R>
+// KG groups of wavefronts, each with a ring of its own, take the chunks in turn where there are fewer tiles than CUs; their sums are added in LDS, in order.
+template <int PM, int PN, int WGM, int WGN, int R, int KG>
 struct Mxfp4Tile {
     static constexpr int NW = WGM * WGN, BM = 32 * PM * WGM, BN = 32 * PN * WGN;
     static constexpr int PANELS = PM * WGM + PN * WGN;
     static constexpr int SCALES = PANELS * 4096;          // their place in a stage
     static constexpr int STAGE = SCALES + (PANELS + 3) / 4 * 1024;
-    static constexpr int BYTES = R * STAGE;
+    static constexpr int RING = R * STAGE, BYTES = KG * RING;
+    static_assert((KG - 1) * BM * BN * 4 <= BYTES, "the groups' sums fit where the stages were");
     static constexpr int PIECES = PANELS * 4;             // KiB of values
     static constexpr int DATA_LOADS = PIECES / NW, SCALE_LOADS = ((PANELS + 3) / 4 + NW - 1) / NW, LOADS = DATA_LOADS + SCALE_LOADS;
     static_assert(PIECES % NW == 0 && BYTES <= 160 * 1024 && (R - 1) * LOADS < 64, "every wavefront issues the same number of loads, which a wait can count");
 };
 
-template <int PM, int PN, int WGM, int WGN, int R>
-__global__ __launch_bounds__(WGM * WGN * 64) void mxfp4_tile_kernel(const Mxfp4Gemm g, int tiles_m, int tiles_n, int total, int per_xcd) {
-    using T = Mxfp4Tile<PM, PN, WGM, WGN, R>;
+// A panel's 32 columns from n of row m, of which the lane holds 8 q + 4 half + 0..3: it takes its partner's (that of the same row) in exchange, so that each of the two has eight neighbours
+// at a time, 16 or 32 bytes to store.
+__device__ __forceinline__ void store16(const Epilogue& ep, int m, int M, int n, int n1, int half, const float (&r)[16]) {
+    char* const row = ep.C + (int64_t)m * ep.ldc;
+#pragma unroll
+    for (int p = 0; p < 2; p++) {
+        const int at = n + 16 * p + 8 * half;
+        if (ep.out_dtype == MMX_F32) {
+            uint32_t w[8];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const auto v = __builtin_amdgcn_permlane32_swap(f2u(r[8 * p + e]), f2u(r[8 * p + 4 + e]), false, false);
+                w[e] = v[0], w[4 + e] = v[1];
+            }
+            float* const to = reinterpret_cast<float*>(row) + at;
+            if (m >= M) continue;
+            if (at + 8 <= n1) {
+                __builtin_memcpy(__builtin_assume_aligned(to, 4), w, 32);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (at + e < n1) to[e] = u2f(w[e]);
+            }
+        } else {
+            uint32_t w[4];
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const auto v = __builtin_amdgcn_permlane32_swap((uint32_t)to_bf16(r[8 * p + 2 * e]) | (uint32_t)to_bf16(r[8 * p + 2 * e + 1]) << 16,
+                                                                (uint32_t)to_bf16(r[8 * p + 4 + 2 * e]) | (uint32_t)to_bf16(r[8 * p + 5 + 2 * e]) << 16, false, false);
+                w[e] = v[0], w[2 + e] = v[1];
+            }
+            uint16_t* const to = reinterpret_cast<uint16_t*>(row) + at;
+            if (m >= M) continue;
+            if (at + 8 <= n1) {
+                __builtin_memcpy(__builtin_assume_aligned(to, 2), w, 16);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (at + e < n1) to[e] = (uint16_t)(w[e >> 1] >> 16 * (e & 1));
+            }
+        }
+    }
+}
+
+template <int PM, int PN, int WGM, int WGN, int R, int KG>
+__global__ __launch_bounds__(WGM * WGN * KG * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void mxfp4_tile_kernel(const Mxfp4Gemm g, int tiles_m, int tiles_n, int total, int per_xcd) {
+    using T = Mxfp4Tile<PM, PN, WGM, WGN, R, KG>;
+    static_assert(PM * PN <= 8, "sums of 128 registers at most");
     constexpr int NW = T::NW, STAGE = T::STAGE, LOADS = T::LOADS, DATA = T::DATA_LOADS;
     using lds_u32x4 = __attribute__((address_space(3))) const u32x4;
     using lds_u32 = __attribute__((address_space(3))) const uint32_t;
@@ -232,14 +279,14 @@ __global__ __launch_bounds__(WGM * WGN * 64) void mxfp4_tile_kernel(const Mxfp4G
     if (L >= total) return;
     const int band = L / (8 * tiles_n), in_band = L - band * (8 * tiles_n), high = tiles_m - band * 8 < 8 ? tiles_m - band * 8 : 8;
     const int tn = in_band / high, tm = band * 8 + in_band - tn * high;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, all_waves = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = all_waves % NW, group = all_waves / NW;
     const int wm = wave / WGN, wn = wave % WGN;
     const int half = lane >> 5, c = lane & 31;
     const int panel_m0 = tm * (PM * WGM), panel_n0 = tn * (PN * WGN), panels_m = (g.M + 31) >> 5;
-    const int steps = g.chunks;
+    const int steps = (g.chunks - group + KG - 1) / KG, most = (g.chunks + KG - 1) / KG;  // of this group, of any: chunks group, group + KG, ...
 
     // ---- loads: this wavefront's KiB of a stage.  A tile may reach past the last panel: that one again, never stored.
-    const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem);
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)smem) + group * T::RING;
     auto panel_at = [&](int p) __attribute__((always_inline)) {
         if (p < PM * WGM) {
             const int panel = panel_m0 + p < panels_m ? panel_m0 + p : panels_m - 1;
@@ -271,10 +318,10 @@ __global__ __launch_bounds__(WGM * WGN * 64) void mxfp4_tile_kernel(const Mxfp4G
         constexpr int i = decltype(ic)::value;
         const uint32_t dst = __builtin_amdgcn_readfirstlane(to[i] + slot * STAGE);
         if constexpr (i < DATA) {
-            const char* const src = from[i] + (int64_t)t * MX_CHUNK_BYTES;
+            const char* const src = from[i] + (int64_t)(group + KG * t) * MX_CHUNK_BYTES;
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(dst), "v"(lane16), "s"(src) : "memory");
         } else {
-            const char* const src = from[i] + (int64_t)t * MX_CHUNK_BYTES;
+            const char* const src = from[i] + (int64_t)(group + KG * t) * MX_CHUNK_BYTES;
             asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(dst), "v"(src) : "memory");
         }
     };
@@ -341,7 +388,8 @@ __global__ __launch_bounds__(WGM * WGN * 64) void mxfp4_tile_kernel(const Mxfp4G
                 places(next);
             }
             acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand(fb[u & 1][j]), mx_operand(fa[u & 1][i]), acc[i][j], 4, 4, u, (int)sb[S][j], u, (int)sa[S][i]);
-            asm volatile("" : "+v"(acc[i][j]));  // (else the compiler gathers the products behind the branches of the loads)
+            // (else the compiler gathers the products behind the branches of the loads)
+            asm volatile("" : "+v"(acc[i][j]));
             // the next step's operands (past the last stage what an earlier one left there: never used)
             unrolled<0, READS>([&](auto rc) __attribute__((always_inline)) {
                 constexpr int r = decltype(rc)::value;
@@ -379,28 +427,50 @@ __global__ __launch_bounds__(WGM * WGN * 64) void mxfp4_tile_kernel(const Mxfp4G
     }
     if (t < steps) stage(std::integral_constant<int, 0>(), t);
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    if constexpr (KG > 1) {
+        if (steps < most) __builtin_amdgcn_s_barrier();  // (the others have one stage more)
+        __syncthreads();
+        f32x4* const sums = reinterpret_cast<f32x4*>(smem) + threadIdx.x % (NW * 64);
+        if (group > 0) {
+#pragma unroll
+            for (int i = 0; i < PM; i++)
+#pragma unroll
+                for (int j = 0; j < PN; j++)
+#pragma unroll
+                    for (int q = 0; q < 4; q++)
+                        sums[((((group - 1) * PM + i) * PN + j) * 4 + q) * (NW * 64)] = f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+        }
+        __syncthreads();
+        if (group > 0) return;
+#pragma unroll
+        for (int o = 0; o < KG - 1; o++)
+#pragma unroll
+            for (int i = 0; i < PM; i++)
+#pragma unroll
+                for (int j = 0; j < PN; j++)
+#pragma unroll
+                    for (int q = 0; q < 4; q++) {
+                        const f32x4 v = sums[(((o * PM + i) * PN + j) * 4 + q) * (NW * 64)];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) acc[i][j][4 * q + e] += v[e];
+                    }
+    }
 
     // ---- post-op: a lane holds columns 8 q + 4 half + 0..3, q = 0..3, of row c of each panel of 32 columns
+    if (g.pair) {
+        if constexpr (PN % 2 == 0) {
 #pragma unroll
-    for (int i = 0; i < PM; i++) {
-        const int m = (panel_m0 + wm * PM + i) * 32 + c;
-        if (g.pair) {
-            if constexpr (PN % 2 == 0) {
+            for (int j = 0; j < PN / 2; j++) {
+                const int block = (panel_n0 + wn * PN) / 2 + j;  // of 32 columns of the result
+                if (block * 64 >= g.N) continue;
 #pragma unroll
-                for (int j = 0; j < PN / 2; j++) {
-                    const int block = (panel_n0 + wn * PN) / 2 + j;  // of 32 columns of the result
+                for (int i = 0; i < PM; i++) {
+                    const int m = (panel_m0 + wm * PM + i) * 32 + c;
                     float r[16];
 #pragma unroll
                     for (int e = 0; e < 16; e++) r[e] = silu32(acc[i][2 * j][e]) * acc[i][2 * j + 1][e];
-                    if (block * 64 >= g.N) continue;
                     if (!g.packed_out) {
-                        if (m < g.M) {
-#pragma unroll
-                            for (int q = 0; q < 4; q++) {
-                                const float r4[4] = {r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]};
-                                store4(g.ep, m, block * 32 + q * 8 + half * 4, g.N / 2, r4);
-                            }
-                        }
+                        store16(g.ep, m, g.M, block * 32, g.N / 2, half, r);
                         continue;
                     }
                     uint32_t top = 0;
@@ -429,33 +499,50 @@ __global__ __launch_bounds__(WGM * WGN * 64) void mxfp4_tile_kernel(const Mxfp4G
                     }
                 }
             }
-        } else if (m < g.M) {
+        }
+        return;
+    }
 #pragma unroll
-            for (int j = 0; j < PN; j++) {
+    for (int j = 0; j < PN; j++) {
+        const int n = (panel_n0 + wn * PN + j) * 32;
+        if (n >= g.N) continue;
+        float bias[16];
+        if (g.ep.steps & MMX_PP_BIAS) {
 #pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    const int n = (panel_n0 + wn * PN + j) * 32 + q * 8 + half * 4;
-                    if (n >= g.N) continue;
-                    float r[4] = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-                    post4(g.ep, n, g.N, r);
-                    store4(g.ep, m, n, g.N, r);
-                }
+            for (int e = 0; e < 16; e++) {
+                const int at = n + (e >> 2) * 8 + half * 4 + (e & 3);
+                bias[e] = g.ep.bias[at < g.N ? at : g.N - 1];
             }
+        }
+#pragma unroll
+        for (int i = 0; i < PM; i++) {
+            float r[16];
+#pragma unroll
+            for (int e = 0; e < 16; e++) r[e] = acc[i][j][e];
+            if (g.ep.steps & MMX_PP_BIAS) {
+#pragma unroll
+                for (int e = 0; e < 16; e++) r[e] = r[e] + bias[e];
+            }
+            if (g.ep.steps & MMX_PP_GELU) {
+#pragma unroll
+                for (int e = 0; e < 16; e++) r[e] = gelu_erf_minimax(r[e]);
+            }
+            store16(g.ep, (panel_m0 + wm * PM + i) * 32 + c, g.M, n, g.N, half, r);
         }
     }
 }
 
-template <int PM, int PN, int WGM, int WGN, int R>
+template <int PM, int PN, int WGM, int WGN, int R, int KG = 1>
 static int launch_tile(const Mxfp4Gemm& g, hipStream_t st, const char* name) {
-    using T = Mxfp4Tile<PM, PN, WGM, WGN, R>;
+    using T = Mxfp4Tile<PM, PN, WGM, WGN, R, KG>;
     static std::atomic<uint64_t> done{0};
-    const auto kernel = mxfp4_tile_kernel<PM, PN, WGM, WGN, R>;
+    const auto kernel = mxfp4_tile_kernel<PM, PN, WGM, WGN, R, KG>;
     const int rc = ensure_dynamic_lds(reinterpret_cast<const void*>(kernel), T::BYTES, done);
     if (rc) return rc;
     const int64_t tiles_m = (g.M + T::BM - 1) / T::BM, tiles_n = ((int64_t)g.npanels * 32 + T::BN - 1) / T::BN, total = tiles_m * tiles_n, per_xcd = (total + 7) / 8;
-    if (per_xcd * 8 * (T::NW * 64) > 0xffffffffll) return set_error(MMX_E_INVALID, "mmx_gemm_mxfp4: too many tiles for one launch");
+    if (per_xcd * 8 * (T::NW * KG * 64) > 0xffffffffll) return set_error(MMX_E_INVALID, "mmx_gemm_mxfp4: too many tiles for one launch");
     note_kernel(name);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(per_xcd * 8)), dim3(T::NW * 64), T::BYTES, st, g, (int)tiles_m, (int)tiles_n, (int)total, (int)per_xcd);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(per_xcd * 8)), dim3(T::NW * KG * 64), T::BYTES, st, g, (int)tiles_m, (int)tiles_n, (int)total, (int)per_xcd);
     return check_hip(hipGetLastError(), "mxfp4_tile_kernel launch");
 }
 
@@ -474,11 +561,56 @@ static int launch_rows(const Mxfp4Gemm& g, hipStream_t st, const char* name) {
 // Whether the kernel for few rows quantises bf16 rows on the way
 bool mx_takes_bf16(int M, int K) { return M <= 8 && (int64_t)M * K <= 16384; }
 
+// Which tile: the least of rounds * (fixed + chunks of 256 k * stage), a round being as many tiles as fit on the chip; one that is not full leaves each of its tiles more of the chip, down to `least` of
+// the time.  The constants are fitted to 52 products of 33 to 4096 rows, 256 to 11008 k and 256 to 22016 columns in every tile, each by how near it comes to the fastest; the tile chosen was 0.8 % behind
+// that on average (of those that a pair can have 1 %), 11 % at most.  us at 2048 x 4096 x 11008 / 4096 x 4096 x 4096 / 1024 x 11008 x 4096 / 256 x 4096 x 4096 / 64 x 11008 x 4096:
+//     256 x 256            62 / 39 / 56 / 25 / 51
+//     256 x 192            54 / 47 / 45 / 20 / 43
+//     192 x 256            54 / 47 / 44 / 20 / 43
+//     128 x 256            57 / 44 / 33 / 15 / 29
+//     128 x 128            59 / 43 / 34 / 14 / 30
+//      64 x 128            68 / 51 / 32 / 9.1 / 17
+//      64 x 64             88 / 67 / 39 / 7.4 / 13
+//      64 x 64, K shared    - / 83 / 46 / 7.1 / 11
+struct TileCost {
+    int bm, bn, per_cu;
+    float fixed_us, stage_us, least;
+};
+enum { T_256_256, T_256_192, T_192_256, T_128_256, T_128_128, T_64_128, T_64_64, T_64_64_SHARED, TILES };
+static constexpr TileCost COSTS[TILES] = {{256, 256, 1, 9.9f, 1.72f, 0.59f}, {256, 192, 1, 7.8f, 1.36f, 0.63f}, {192, 256, 1, 8.2f, 1.31f, 0.61f}, {128, 256, 1, 7.1f, 0.90f, 0.65f},
+                                          {128, 128, 2, 5.7f, 1.02f, 0.58f}, {64, 128, 2, 4.5f, 0.48f, 0.72f}, {64, 64, 2, 3.8f, 0.34f, 0.74f}, {64, 64, 1, 3.6f, 0.19f, 0.92f}};
+
+static int choose_tile(const Mxfp4Gemm& g) {
+    int best = -1;
+    double fastest = 0;
+    for (int i = 0; i < TILES; i++) {
+        if (i == (g.pair ? T_256_192 : T_192_256)) continue;  // (a wavefront of a pair has as many gate panels as up panels)
+        const TileCost& t = COSTS[i];
+        const int64_t tiles = (int64_t)((g.M + t.bm - 1) / t.bm) * (((int64_t)g.npanels * 32 + t.bn - 1) / t.bn), at_once = (int64_t)num_cus() * t.per_cu;
+        const double full = (double)(tiles / at_once), rest = (double)(tiles % at_once) / at_once;
+        const double us = (full + (rest > 0 ? t.least + (1 - t.least) * rest : 0)) * (t.fixed_us + g.chunks * t.stage_us);
+        if (best < 0 || us < fastest) {
+            best = i;
+            fastest = us;
+        }
+    }
+    return best;
+}
+
 int launch_gemm_mxfp4(const Mxfp4Gemm& g, hipStream_t st) {
     if (g.a_bf16) return g.pair ? launch_rows<1, 4, true, true>(g, st, "mxfp4_rows_16_pair_bf16") : launch_rows<1, 1, false, true>(g, st, "mxfp4_rows_16_bf16");
     if (g.M <= 16) return g.pair ? launch_rows<1, 4, true>(g, st, "mxfp4_rows_16_pair") : launch_rows<1, 1, false>(g, st, "mxfp4_rows_16");
     if (g.M <= 32) return g.pair ? launch_rows<2, 4, true>(g, st, "mxfp4_rows_32_pair") : launch_rows<2, 1, false>(g, st, "mxfp4_rows_32");
-    return launch_tile<4, 2, 2, 4, 2>(g, st, "mxfp4_256x256");
+    switch (choose_tile(g)) {
+    case T_256_256: return launch_tile<4, 2, 2, 4, 2>(g, st, "mxfp4_256x256");
+    case T_256_192: return launch_tile<2, 3, 4, 2, 2>(g, st, "mxfp4_256x192");
+    case T_192_256: return launch_tile<3, 2, 2, 4, 2>(g, st, "mxfp4_192x256");
+    case T_128_256: return launch_tile<2, 2, 2, 4, 3>(g, st, "mxfp4_128x256");
+    case T_128_128: return launch_tile<2, 2, 2, 2, 2>(g, st, "mxfp4_128x128");
+    case T_64_128: return launch_tile<1, 2, 2, 2, 3>(g, st, "mxfp4_64x128");
+    case T_64_64: return g.pair ? launch_tile<1, 2, 2, 1, 4>(g, st, "mxfp4_64x64_pair") : launch_tile<1, 1, 2, 2, 4>(g, st, "mxfp4_64x64");
+    default: return g.pair ? launch_tile<1, 2, 2, 1, 3, 2>(g, st, "mxfp4_64x64_shared_k_pair") : launch_tile<1, 1, 2, 2, 3, 2>(g, st, "mxfp4_64x64_shared_k");
+    }
 }
 
 }  // namespace mmx

@@ -11,7 +11,7 @@
 // Three kernels.  A workgroup for each slice of a row reads the logits: segments' maxima; without filters their sums too; with top_k or top_p a histogram of the slice, counts and weights by
 // l / T in steps of 1 / 16, on one grid for the row.  With filters workgroups of four segments add the row's histograms up, which shows the bin in which the run ends, and collect what lies in it and above; or,
 // where that is more than a list holds, what lies in it, and the segments' sums of what lies above.  A workgroup a row sorts out from the list where the run ends, and draws.
-// Rows that this does not suit (more than a list of equal or nearly equal logits in the last bin, 2^50 bins and more) are worked on by that one workgroup alone, a pass over the row for every eight bits of the key.
+// Rows that this does not suit (more than a list of equal or nearly equal logits in the last bin, 2^26 bins and more) are worked on by that one workgroup alone, a pass over the row for every eight bits of the key.
 #include "sample.hpp"
 
 #include "ffn.hpp"
@@ -24,7 +24,7 @@ constexpr double PER_UNIT = 16;           // bins of a unit of l / T
 constexpr int LIST = 4096;                // entries
 constexpr int MOST_SLICES = 256;          // of a row
 constexpr int MOST_SUMS = 1024;           // segments of a row whose sums fit beside a list
-constexpr double GRID = 1125899906842624.0;  // 2^50: up to here bins are exact
+constexpr double GRID = 67108864.0;        // 2^26: up to here what lies behind a bin's point is good to 2^-27
 constexpr float NEVER = -__builtin_huge_valf();
 
 // What a row asks for
@@ -56,29 +56,35 @@ __device__ __forceinline__ uint32_t key_of(float x) {
 __device__ __forceinline__ float of_key(uint32_t k) { return u2f(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 __device__ __forceinline__ float settled(float x) { return x != x ? NEVER : x + 0.0f; }
 
-// e^x for x <= 0: 2^n times the series of e^r to its eleventh power, |r| <= ln 2 / 2, whose rest is r^12 / 12! = 6e-15.  (The library's exp, with a division by the temperature, took most of
-// the time: 256 rows of 131072 62 us, so 26; 1 row of 32000 12.8, so 5.)
-__device__ __forceinline__ double exp_of(double x) {
-    x = fmax(x, -1000.0);  // (NaN, which +inf beside +inf makes, too: it has no weight)
-    const double n = rint(x * 1.4426950408889634);
-    const double r = __builtin_fma(n, -0.6931471805599453, x);
-    double p = 1.0 / 39916800;
-    p = __builtin_fma(p, r, 1.0 / 3628800);
-    p = __builtin_fma(p, r, 1.0 / 362880);
-    p = __builtin_fma(p, r, 1.0 / 40320);
-    p = __builtin_fma(p, r, 1.0 / 5040);
-    p = __builtin_fma(p, r, 1.0 / 720);
-    p = __builtin_fma(p, r, 1.0 / 120);
-    p = __builtin_fma(p, r, 1.0 / 24);
-    p = __builtin_fma(p, r, 1.0 / 6);
-    p = __builtin_fma(p, r, 0.5);
-    p = __builtin_fma(p, r, 1.0);
-    p = __builtin_fma(p, r, 1.0);
-    return ldexp(p, (int)n);
+// 2^y for y <= 0: 2^n times the series of 2^f = e^(f ln 2) to its tenth power, |f| <= 1 / 2, whose rest is (ln 2 / 2)^11 / 11! = 2e-13.  n comes out of adding a number so large that
+// nothing is left behind the point.  (The library's exp, with a division by the temperature, took most of the time: 256 rows of 131072 62 us in the first kernel.)
+__device__ __forceinline__ double exp2_of(double y) {
+    y = fmax(y, -2000.0);  // (NaN too)
+    const double big = 6755399441055744.0;  // 1.5 * 2^52
+    const double t = y + big, f = y - (t - big);
+    constexpr double L = 0.6931471805599453094;
+    constexpr double L2 = L * L, L4 = L2 * L2, L8 = L4 * L4;
+    double p = L8 * L2 / 3628800;
+    p = __builtin_fma(p, f, L8 * L / 362880);
+    p = __builtin_fma(p, f, L8 / 40320);
+    p = __builtin_fma(p, f, L4 * L2 * L / 5040);
+    p = __builtin_fma(p, f, L4 * L2 / 720);
+    p = __builtin_fma(p, f, L4 * L / 120);
+    p = __builtin_fma(p, f, L4 / 24);
+    p = __builtin_fma(p, f, L2 * L / 6);
+    p = __builtin_fma(p, f, L2 / 2);
+    p = __builtin_fma(p, f, L);
+    p = __builtin_fma(p, f, 1.0);
+    return ldexp(p, (int)(uint32_t)__builtin_bit_cast(uint64_t, t));
 }
+constexpr double LOG2_E = 1.4426950408889634074;
+__device__ __forceinline__ double exp_of(double x) { return exp2_of(x * LOG2_E); }
 // per: 1 / temperature
+__device__ __forceinline__ double weight_below(float l, float top, double per) {  // (of a top that is finite; -inf comes out as zero)
+    return exp2_of(((double)l - (double)top) * (per * LOG2_E));  // (the difference first: of products it would be off by what is left of theirs, without bound for large logits)
+}
 __device__ __forceinline__ double weight_of(float l, float top, double per) {
-    const double w = exp_of(((double)l - (double)top) * per);
+    const double w = weight_below(l, top, per);
     return l == top ? 1.0 : l == NEVER ? 0.0 : w;  // (an infinite one too: the others have no weight beside it)
 }
 
@@ -336,7 +342,7 @@ __device__ __forceinline__ void last_of(bool holds, uint32_t* last) {
 
 // SLICE wavefronts, a segment each
 template <typename TL, int SLICE>
-__global__ __launch_bounds__(SLICE * 64) void sample_slices_kernel(const SampleArgs a) {
+__global__ __launch_bounds__(SLICE * 64) __attribute__((amdgpu_waves_per_eu(8, 8))) void sample_slices_kernel(const SampleArgs a) {
     constexpr int WG = SLICE * 64;
     __shared__ unsigned long long bins[BINS];
     __shared__ uint32_t last;
@@ -360,8 +366,13 @@ __global__ __launch_bounds__(SLICE * 64) void sample_slices_kernel(const SampleA
     if (!r.filtered()) {
         if (!here || r.greedy || r.min) return;
         double w = 0;
+        if (top < __builtin_huge_valf()) {
 #pragma unroll
-        for (int e = 0; e < 16; e++) w += weight_of(x.v[e], top, r.per);
+            for (int e = 0; e < 16; e++) w += weight_below(x.v[e], top, r.per);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 16; e++) w += x.v[e] == top ? 1.0 : 0.0;
+        }
         w = wave_sum(top == NEVER ? 0.0 : w);
         if (lane == 0) sc.sums[g] = w;
         return;
@@ -643,8 +654,13 @@ enum { BY_COUNT, BY_MASS, BY_MASS_STRICT };
 __device__ __forceinline__ unsigned long long pick(const unsigned long long (&c)[MINE], const unsigned long long (&m)[MINE], int most, int mode, unsigned long long want, Room& o) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     unsigned long long low = 1, high = ~0ull, before = 0;  // of the entries from low to high; what lies above them
-    int n;
-    for (;;) {
+    int n = most;
+    __syncthreads();  // (what an earlier call left has been read)
+    if (most <= FEW) {
+        if ((int)threadIdx.x < most) o.few[threadIdx.x] = c[0], o.few_mass[threadIdx.x] = c[0] == 0 ? 0ull : mode == BY_COUNT ? 1ull : m[0];
+        if (threadIdx.x == 0) o.best = 0, o.low = 0;
+    }
+    while (most > FEW) {
         unsigned long long lo = ~0ull, hi = 0;
         uint32_t here = 0;
 #pragma unroll
@@ -721,24 +737,24 @@ __device__ __forceinline__ unsigned long long pick(const unsigned long long (&c)
         high = up;
     }
     __syncthreads();
-    // eight neighbouring threads an entry, each against every eighth of them
-    unsigned long long got = 0, least = ~0ull;
+    // Eight neighbouring threads an entry, each against every eighth of them.  The one that is sought is the only one that reaches the goal and does not without its own mass.
     if ((int)(threadIdx.x & ~63u) < n * 8) {
         const int i = threadIdx.x >> 3;
-        const unsigned long long mine = o.few[i < n ? i : 0];
+        const unsigned long long mine = i < n ? o.few[i] : 0ull;
         unsigned long long run = 0;
-        for (int j = threadIdx.x & 7; j < n; j += 8) run += o.few[j] >= mine ? o.few_mass[j] : 0ull;
-#pragma unroll
-        for (int d = 1; d < 8; d *= 2) run += __shfl_xor(run, d);
-        run += before;
-        if (i < n) {
-            if (mode == BY_MASS_STRICT ? run > want : run >= want) got = mine;
-            least = mine;
+        uint32_t after = 0;  // entries behind it
+        for (int j = threadIdx.x & 7; j < n; j += 8) {
+            const unsigned long long other = o.few[j];
+            run += other >= mine ? o.few_mass[j] : 0ull;
+            after += other < mine && other != 0 ? 1 : 0;
         }
-        got = wave_max(got), least = ~wave_max(~least);
-        if (lane == 0) {
-            atomicMax(&o.best, got);
-            atomicMin(&o.low, least);
+#pragma unroll
+        for (int d = 1; d < 8; d *= 2) run += __shfl_xor(run, d), after += __shfl_xor(after, d);
+        run += before;
+        if (mine && (threadIdx.x & 7) == 0) {
+            const unsigned long long less = run - o.few_mass[i];
+            if (mode == BY_MASS_STRICT ? run > want && less <= want : run >= want && less < want) o.best = mine;
+            if (after == 0) o.low = mine;
         }
     }
     __syncthreads();
@@ -787,10 +803,10 @@ __global__ __launch_bounds__(THREADS) void sample_draw_kernel(const SampleArgs a
         for (int g = threadIdx.x; g < segs; g += THREADS)
             if ((g < THREADS ? first_top : sc.seg_top[g]) == top) atomicMin(&s.pick, g);
         __syncthreads();
-        const int i = s.pick * SEG + threadIdx.x;
+        const int seg = s.pick < segs ? s.pick : 0, i = seg * SEG + threadIdx.x;
         first_of(i < V && value_at(row, i) == top, &s.found);
         __syncthreads();
-        if (threadIdx.x == 0) a.ids[row_at] = s.pick * SEG + (int)s.found;
+        if (threadIdx.x == 0) a.ids[row_at] = seg * SEG + (int)s.found;
         return;
     }
     const uint32_t path = r.filtered() ? state.path : BY_SUMS;
@@ -815,6 +831,7 @@ __global__ __launch_bounds__(THREADS) void sample_draw_kernel(const SampleArgs a
             if (i > 0) c[i] = at < n ? sc.list[at] : 0;
             if (at >= n) c[i] = 0;
             const float l = of_key((uint32_t)(c[i] >> 32));
+            if (!__any(c[i] != 0)) continue;
             const double w = c[i] ? weight_of(l, top, r.per) : 0.0;
             m[i] = whole(w, scale);
             low_weight |= w < r.min_p && l != top ? 1u << i : 0;
@@ -940,7 +957,8 @@ __global__ __launch_bounds__(THREADS) void sample_draw_kernel(const SampleArgs a
         if (lane == 0) atomicMax(&s.pick, last);
         __syncthreads();
     }
-    const int i = s.pick * SEG + threadIdx.x;
+    const int seg = s.pick < 0 ? 0 : s.pick;  // (a row that gets here has a token of weight 1: some segment was found)
+    const int i = seg * SEG + threadIdx.x;
     const double rest = s.rest;
     if (threadIdx.x == 0) s.found = 0xffffffffu, s.bin = 0;
     double all;
@@ -948,13 +966,13 @@ __global__ __launch_bounds__(THREADS) void sample_draw_kernel(const SampleArgs a
     first_of(w > 0.0 && before + w > rest, &s.found);
     last_of(w > 0.0, &s.bin);
     __syncthreads();
-    if (threadIdx.x == 0) a.ids[row_at] = s.pick * SEG + (int)(s.found != 0xffffffffu ? s.found : s.bin);
+    if (threadIdx.x == 0) a.ids[row_at] = seg * SEG + (int)(s.found != 0xffffffffu ? s.found : s.bin);
 }
 
 // Segments of a slice: 4 where 16 would leave most of the chip idle
 int sample_slice(int B, int V) {
     const int64_t segs = ((int64_t)V + SEG - 1) / SEG;
-    return B * ((segs + 15) / 16) < 256 && segs <= 4 * MOST_SLICES ? 4 : 16;
+    return B * ((segs + 15) / 16) < 64 && segs <= 4 * MOST_SLICES ? 4 : 16;
 }
 size_t sample_scratch_bytes(int B, int V) { return (size_t)B * row_bytes(V, sample_slice(B, V)); }
 
@@ -964,7 +982,11 @@ static int launch(const SampleArgs& a, int B, hipStream_t st) {
     // (what a number for all rows rules out is not launched)
     const bool greedy = (!a.temperature && !(a.temperature_all > 0.0)) || (!a.top_k && a.top_k_all == 1) || (!a.top_p && a.top_p_all <= 0.0);
     const bool open = !a.top_k && (a.top_k_all <= 0 || a.top_k_all >= a.V) && !a.top_p && a.top_p_all >= 1.0 && !a.min_p && a.min_p_all <= 0.0;
-    hipLaunchKernelGGL((sample_slices_kernel<TL, SLICE>), dim3((unsigned)slices, (unsigned)B), dim3(SLICE * 64), 0, st, a);
+    const bool filters = a.top_k || (a.top_k_all > 0 && a.top_k_all < a.V) || a.top_p || a.top_p_all < 1.0;
+    if (greedy || !filters)  // (no histograms: small workgroups, of which more overlap)
+        hipLaunchKernelGGL((sample_slices_kernel<TL, 4>), dim3((unsigned)((segs + 3) / 4), (unsigned)B), dim3(256), 0, st, a);
+    else
+        hipLaunchKernelGGL((sample_slices_kernel<TL, SLICE>), dim3((unsigned)slices, (unsigned)B), dim3(SLICE * 64), 0, st, a);
     if (!greedy && !open) hipLaunchKernelGGL(sample_filter_kernel<TL>, dim3((unsigned)((segs + 3) / 4), (unsigned)B), dim3(256), 0, st, a);
     hipLaunchKernelGGL(sample_draw_kernel<TL>, dim3((unsigned)B), dim3(THREADS), 0, st, a);
     return check_hip(hipGetLastError(), "sample_draw_kernel launch");

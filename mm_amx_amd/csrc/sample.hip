@@ -8,9 +8,9 @@
 // What stays is a run of the order whatever the filters are, so it is held as its last element: a key (the bits of l, made to order like l) and, among equal keys, an index.
 // A row is cut into segments of 1024 neighbours, one wavefront's 16 values a lane, whose maxima and sums are what the draw goes by: it finds its segment, then its token in it.
 //
-// Three kernels.  A workgroup for each slice of a row reads the logits: segments' maxima; without filters their sums too; with top_k or top_p a histogram of the slice, counts and weights by
-// l / T in steps of 1 / 16, on one grid for the row.  With filters workgroups of four segments add the row's histograms up, which shows the bin in which the run ends, and collect what lies in it and above; or,
-// where that is more than a list holds, what lies in it, and the segments' sums of what lies above.  A workgroup a row sorts out from the list where the run ends, and draws.
+// Four kernels.  A workgroup for each slice of a row reads the logits: segments' maxima; without filters their sums too; with top_k or top_p a histogram of the slice, counts and weights by
+// l / T in steps of 1 / 16, on one grid for the row.  With filters a workgroup a row adds the histograms up, which shows the bin in which the run ends.  Workgroups of four segments collect what lies in it
+// and above; or, where that is more than a list holds, what lies in it, and the segments' sums of what lies above.  A workgroup a row sorts out from the list where the run ends, and draws.
 // Rows that this does not suit (more than a list of equal or nearly equal logits in the last bin, 2^26 bins and more) are worked on by that one workgroup alone, a pass over the row for every eight bits of the key.
 #include "sample.hpp"
 
@@ -23,6 +23,7 @@ constexpr int BINS = 512;                 // the last one: everything below, e^-
 constexpr double PER_UNIT = 16;           // bins of a unit of l / T
 constexpr int LIST = 4096;                // entries
 constexpr int MOST_SLICES = 256;          // of a row
+static_assert(MOST_SLICES * 16 * SEG == 1 << 22, "the longest row, in slices of sixteen segments");
 constexpr int MOST_SUMS = 1024;           // segments of a row whose sums fit beside a list
 constexpr double GRID = 67108864.0;        // 2^26: up to here what lies behind a bin's point is good to 2^-27
 constexpr float NEVER = -__builtin_huge_valf();
@@ -174,7 +175,8 @@ __device__ __forceinline__ double factor_less_1(double f) {
 }
 enum { BY_LIST, BY_SUMS, ALONE };
 struct State {
-    uint32_t entries, path, before_count, pad;
+    uint32_t entries, path, before_count;
+    float top, from, to;       // logits from `from` on go into the list, those from `to` on into the sums
     double before_mass, mass;  // of what lies above the last bin, and of everything
 };
 // A row's scratch
@@ -205,7 +207,7 @@ __device__ __forceinline__ Scratch scratch_of(const SampleArgs& a, int row) {
     r.seg_top = reinterpret_cast<float*>(p);
     return r;
 }
-static_assert(sizeof(Slice) % 8 == 0 && sizeof(State) % 8 == 0, "what lies behind them stays aligned");
+static_assert(sizeof(Slice) % 8 == 0 && sizeof(State) % 8 == 0 && MOST_SLICES <= BINS, "what lies behind them stays aligned; a slice a thread");
 
 __device__ __forceinline__ unsigned long long whole(double w, double scale) { return (unsigned long long)(w * scale + 0.5); }
 
@@ -440,11 +442,10 @@ __global__ __launch_bounds__(SLICE * 64) __attribute__((amdgpu_waves_per_eu(8, 8
 #pragma unroll
         for (int w = 0; w < SLICE; w++) all += counts[w];
         sc.slices[blockIdx.x] = Slice{bin, all, 0};
-        if (blockIdx.x == 0) sc.state->entries = 0;
     }
 }
 
-// ---- what the filters leave: workgroups of four segments ---------------------------------------------------------------------------
+// ---- what the filters leave ---------------------------------------------------------------------------
 // the largest of all (first: this thread's own of the row's segments' maxima)
 template <int WAVES>
 __device__ __forceinline__ float row_top(const Scratch& sc, float first, float* part) {
@@ -466,36 +467,118 @@ __device__ __forceinline__ float least_of(double at, double per) {
     return settled(of_key(k));
 }
 
-template <typename TL>
-__global__ __launch_bounds__(256) void sample_filter_kernel(const SampleArgs a) {
-    constexpr int WAVES = 4, HALF = 256;
-    static_assert(BINS == 2 * HALF, "two bins a thread");
-    __shared__ double part[WAVES][4], before_mass, before_count;
+// the row's histogram, a bin a thread, and the bin in which the run ends
+__global__ __launch_bounds__(BINS) void sample_cut_kernel(const SampleArgs a) {
+    constexpr int WAVES = BINS / 64, AHEAD = 8;
+    __shared__ double part[2][WAVES];
     __shared__ int slice_ahead[MOST_SLICES];
     __shared__ float fpart[WAVES];
-    __shared__ uint32_t found, last_bin, base, n_last, n_run, taken[WAVES], all_count;
+    __shared__ uint32_t found, last_bin, all_count;
+    const int row_at = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, b = threadIdx.x;
+    const Scratch sc = scratch_of(a, row_at);
+    const float first_top = b < sc.segs ? sc.seg_top[b] : NEVER;
+    const RowAsks r = asks_of(a, row_at);
+    if (!r.filtered()) return;
+    Slice own = {0.0, 0, 0};
+    if (b < sc.n_slices) own = sc.slices[b];
+    if (b == 0) found = BINS, last_bin = 0, all_count = 0;
+    const float top = row_top<WAVES>(sc, first_top, fpart);
+    if (top == NEVER) {
+        if (b == 0) sc.state->path = ALONE;
+        return;
+    }
+    const double per = PER_UNIT * r.per, at0 = (double)top * per, bin = floor(at0);
+    const bool odd = !(fabs(bin) <= GRID) || !(per <= 1e300) || per < 1e-30;
+    if (b < sc.n_slices) {
+        // (a slice that lies below the grid, or holds nothing, has nothing in the row's other bins)
+        const double ahead = bin - own.bin;
+        slice_ahead[b] = ahead < BINS ? (int)ahead : BINS;
+    }
+    const uint32_t held = wave_sum(own.count);
+    if (lane == 0 && held) atomicAdd(&all_count, held);
+    __syncthreads();
+    unsigned long long masses = 0;
+    uint32_t count = 0;
+    if (!odd) {
+        for (int i0 = 0; i0 < sc.n_slices; i0 += AHEAD) {  // (AHEAD slices' bins on their way together)
+            unsigned long long v[AHEAD];
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++) {
+                const int at = i0 + i < sc.n_slices && b < BINS - 1 ? b - slice_ahead[i0 + i] : -1;
+                v[i] = at >= 0 ? sc.bins[(int64_t)(i0 + i) * BINS + at] : 0ull;
+            }
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++) {
+                masses += v[i] & ((1ull << MASS_BITS) - 1);
+                count += (uint32_t)(v[i] >> MASS_BITS);
+            }
+        }
+    }
+    const double mass = r.top_k ? 0.0 : (double)masses / FACTOR_SCALE * exp_of((bin - b - at0) * (1.0 / PER_UNIT));
+    double run_mass = mass;
+    uint32_t run_count = count;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const double o = __shfl_up(run_mass, d);
+        const uint32_t c = __shfl_up(run_count, d);
+        if (lane >= d) run_mass += o, run_count += c;
+    }
+    if (lane == 63) part[0][wave] = run_mass, part[1][wave] = run_count;
+    __syncthreads();
+    double all_mass = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) {
+        run_mass += w < wave ? part[0][w] : 0.0;
+        run_count += w < wave ? (uint32_t)part[1][w] : 0u;
+        all_mass += part[0][w];
+    }
+    if (b == BINS - 1) count = all_count - run_count, run_count = all_count;
+    // of top_k the first whose count is enough, of top_p alone the first whose mass is (of both: top_p's share is of what top_k leaves, which only the list tells)
+    first_of(r.top_k ? run_count >= (uint32_t)r.k : run_mass >= r.p * all_mass, &found);
+    last_of(count > 0, &last_bin);
+    __syncthreads();
+    const int cut = found < BINS ? (int)found : (int)last_bin;  // (none: fewer tokens than top_k, or sums that were rounded)
+    if (b != cut) return;
+    State s;
+    s.entries = 0, s.before_count = run_count - count, s.top = top, s.before_mass = run_mass - mass, s.mass = all_mass;
+    s.path = odd ? ALONE : run_count <= LIST ? BY_LIST : (r.top_k && r.top_p) || count > LIST || sc.segs > MOST_SUMS ? ALONE : BY_SUMS;
+    s.from = s.to = __builtin_huge_valf();
+    if (s.path != ALONE) {
+        s.from = cut == BINS - 1 ? of_key(key_of(NEVER) + 1) : least_of(bin - cut, per);
+        if (s.path == BY_SUMS && cut > 0) s.to = least_of(bin - cut + 1, per);
+    }
+    *sc.state = s;
+}
+
+template <typename TL>
+__global__ __launch_bounds__(256) void sample_filter_kernel(const SampleArgs a) {
+    constexpr int WAVES = 4;
+    __shared__ float fpart[WAVES];
+    __shared__ uint32_t base, taken[WAVES];
     const int row_at = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const Scratch sc = scratch_of(a, row_at);
     const int g = blockIdx.x * WAVES + wave;
     const TL* const row = reinterpret_cast<const TL*>(a.logits + (int64_t)row_at * a.ld);
     const bool here = g < sc.segs;
     // (everything that does not wait for something else first)
-    const float first_top = (int)threadIdx.x < sc.segs ? sc.seg_top[threadIdx.x] : NEVER;
+    const State state = *sc.state;
     const float seg_top = here ? sc.seg_top[g] : NEVER;
     const RowAsks r = asks_of(a, row_at);
     if (r.greedy || !(r.filtered() || r.min)) return;
-    Slice own = {0.0, 0, 0};
-    if (r.filtered() && (int)threadIdx.x < sc.n_slices) own = sc.slices[threadIdx.x];
+    float top = state.top;
     Lane16<TL> x;
-    if (here) x.ask(row, a.V, g);
-    const float top = row_top<WAVES>(sc, first_top, fpart);
-    if (top == NEVER) return;
+    if (!r.filtered()) {
+        if (here) x.ask(row, a.V, g);
+        top = row_top<WAVES>(sc, (int)threadIdx.x < sc.segs ? sc.seg_top[threadIdx.x] : NEVER, fpart);
+        if (top == NEVER || !here) return;
+    } else if (state.path == ALONE) {
+        return;
+    }
     auto weight = [&](float l) __attribute__((always_inline)) {
         const double v = weight_of(l, top, r.per);
         return v < r.min_p && l != top ? 0.0 : v;
     };
     if (!r.filtered()) {
-        if (!here) return;
         double w = 0;
         if (seg_top != NEVER) {
             x.get(row, a.V, g);
@@ -506,108 +589,25 @@ __global__ __launch_bounds__(256) void sample_filter_kernel(const SampleArgs a) 
         if (lane == 0) sc.sums[g] = w;
         return;
     }
-    const double per = PER_UNIT * r.per, bin = floor((double)top * per);
-    const bool odd = !(fabs(bin) <= GRID) || !(per <= 1e300) || per < 1e-30;
-    if (threadIdx.x == 0) found = BINS, last_bin = 0, all_count = 0;
-    __syncthreads();
-    if ((int)threadIdx.x < sc.n_slices) {
-        // (a slice that lies below the grid, or holds nothing, has nothing in the row's other bins)
-        const double ahead = bin - own.bin;
-        slice_ahead[threadIdx.x] = ahead < BINS ? (int)ahead : BINS;
-    }
-    const uint32_t held = wave_sum(own.count);
-    if (lane == 0 && held) atomicAdd(&all_count, held);
-    __syncthreads();
-    // The row's histogram, bins b and b + 256 a thread; four slices at a time, so that nothing waits for one load after the other.
-    const int b = threadIdx.x;
-    unsigned long long mass[2] = {0, 0};
-    uint32_t count[2] = {0, 0};
-    if (!odd) {
-        for (int i0 = 0; i0 < sc.n_slices; i0 += 8) {
-            unsigned long long v[8][2];
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                const int at = i0 + i < sc.n_slices ? b - slice_ahead[i0 + i] : -BINS;
-                const unsigned long long* const p = sc.bins + (int64_t)(i0 + i) * BINS + at;
-                v[i][0] = at >= 0 ? p[0] : 0ull;
-                v[i][1] = at + HALF >= 0 && b + HALF < BINS - 1 ? p[HALF] : 0ull;
-            }
-#pragma unroll
-            for (int i = 0; i < 8; i++)
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    mass[h] += v[i][h] & ((1ull << MASS_BITS) - 1);
-                    count[h] += (uint32_t)(v[i][h] >> MASS_BITS);
-                }
-        }
-    }
-    double m[2], v[4], run[4], all[4];
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-        m[h] = r.top_k ? 0.0 : (double)mass[h] / FACTOR_SCALE * exp_of((bin - (b + h * HALF) - (double)top * per) * (1.0 / PER_UNIT));
-        v[h] = m[h], v[2 + h] = count[h];
-    }
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-        run[k] = v[k];
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const double o = __shfl_up(run[k], d);
-            if (lane >= d) run[k] += o;
-        }
-        if (lane == 63) part[wave][k] = run[k];
-    }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-        double before = 0;
-        all[k] = 0;
-#pragma unroll
-        for (int w = 0; w < WAVES; w++) {
-            before += w < wave ? part[w][k] : 0.0;
-            all[k] += part[w][k];
-        }
-        run[k] += before;  // (up to this bin and with it)
-    }
-    run[1] += all[0], run[3] += all[2];
-    const double all_mass = all[0] + all[1];
-    if (b + HALF == BINS - 1) run[3] = all_count, v[3] = run[3] - all[2] - all[3], count[1] = (uint32_t)v[3];
-    // the bin in which the run ends: of top_k the first whose count is enough, of top_p alone the first whose mass is (of both: top_p's share is of what top_k leaves, which only the list tells)
-#pragma unroll
-    for (int h = 1; h >= 0; h--) {
-        const uint64_t e = __ballot(r.top_k ? run[2 + h] >= (double)r.k : run[h] >= r.p * all_mass), o = __ballot(count[h] > 0);
-        if (lane == 0) {
-            if (e) atomicMin(&found, (uint32_t)(b + h * HALF + __builtin_ctzll(e)));
-            if (o) atomicMax(&last_bin, (uint32_t)(b + h * HALF + 63 - __builtin_clzll(o)));
-        }
-    }
-    __syncthreads();
-    const int cut = found < BINS ? (int)found : (int)last_bin;  // (none: fewer tokens than top_k, or sums that were rounded)
-#pragma unroll
-    for (int h = 0; h < 2; h++)
-        if (b + h * HALF == cut) before_mass = run[h] - m[h], before_count = run[2 + h] - v[2 + h], n_last = count[h], n_run = (uint32_t)run[2 + h];
-    __syncthreads();
-    const uint32_t path = odd ? ALONE : n_run <= LIST ? BY_LIST : (r.top_k && r.top_p) || n_last > LIST || sc.segs > MOST_SUMS ? ALONE : BY_SUMS;
-    if (blockIdx.x == 0 && threadIdx.x == 0) {
-        State* const s = sc.state;
-        s->path = path, s->before_count = (uint32_t)before_count, s->before_mass = before_mass, s->mass = all_mass;
-    }
-    if (path == ALONE) return;
-    // into the list what lies in the bin, or in it and above
-    const float from = cut == BINS - 1 ? of_key(key_of(NEVER) + 1) : least_of(bin - cut, per), to = path == BY_SUMS && cut > 0 ? least_of(bin - cut + 1, per) : __builtin_huge_valf();
     uint32_t takes = 0;
-    double w = 0;
-    if (here && seg_top >= from) {
+    const bool some = here && seg_top >= state.from;
+    if (some) {
+        x.ask(row, a.V, g);
         x.get(row, a.V, g);
-#pragma unroll
-        for (int e = 0; e < 16; e++) {
-            takes |= x.v[e] >= from && x.v[e] < to ? 1u << e : 0;
-            if (path == BY_SUMS && __any(x.v[e] >= to)) w += x.v[e] >= to ? weight(x.v[e]) : 0.0;
-        }
     }
-    if (path == BY_SUMS && here) {
-        w = wave_sum(w);
+    if (state.path == BY_SUMS && here) {
+        double w = 0;
+        if (some && seg_top >= state.to) {
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                if (__any(x.v[e] >= state.to)) w += x.v[e] >= state.to ? weight(x.v[e]) : 0.0;
+            w = wave_sum(w);
+        }
         if (lane == 0) sc.sums[g] = w;
+    }
+    if (some) {
+#pragma unroll
+        for (int e = 0; e < 16; e++) takes |= x.v[e] >= state.from && x.v[e] < state.to ? 1u << e : 0;
     }
     uint32_t at = __popc(takes);
     const uint32_t mine = at;
@@ -792,7 +792,8 @@ __global__ __launch_bounds__(THREADS) void sample_draw_kernel(const SampleArgs a
     for (int i = 0; i < MINE; i++) {  // (asked for before anything is known of it; sorted out below)
         c[i] = r.filtered() && i == 0 ? sc.list[threadIdx.x] : 0;
     }
-    const float top = row_top<NW>(sc, first_top, s.fpart);
+    const bool known = r.filtered() && state.path != ALONE;  // (its largest logit)
+    const float top = known ? state.top : row_top<NW>(sc, first_top, s.fpart);
     if (top == NEVER) {
         if (threadIdx.x == 0) a.ids[row_at] = -1;
         return;
@@ -914,55 +915,54 @@ __global__ __launch_bounds__(THREADS) void sample_draw_kernel(const SampleArgs a
         }
         __syncthreads();
     }
-    // a segment's sum: without filters it is relative to its own maximum, with a list there may be more to it
+    // A segment's sum: without filters it is relative to its own maximum, with a list there may be more to it.  A thread has up to four neighbouring segments (of 2^22 logits).
+    constexpr int MOST = 4;
     const bool own = !r.filtered() && !r.min, added = r.filtered() && path == BY_SUMS;
-    auto sum_at = [&](int g) __attribute__((always_inline)) {
-        if (g >= segs) return 0.0;
-        const bool ready = g < THREADS && path != ALONE;
+    const int each = (segs + THREADS - 1) / THREADS, g0 = threadIdx.x * each;
+    double sums[MOST], mine = 0, total;
+#pragma unroll
+    for (int k = 0; k < MOST; k++) {
+        const int g = g0 + k;
+        sums[k] = 0;
+        if (k >= each || g >= segs) continue;
+        const bool ready = each == 1 && path != ALONE;
         const double w = ready ? first_sum : sc.sums[g];
-        return own ? w * weight_of(ready ? first_top : sc.seg_top[g], top, r.per) : added ? w + (double)more[g] / scale : w;
-    };
-    double total = 0;
-    for (int g0 = 0; g0 < segs; g0 += THREADS) {
-        double all;
-        scan_before(sum_at(g0 + threadIdx.x), s.part, &all);
-        total += all;
+        sums[k] = own ? w * weight_of(ready ? first_top : sc.seg_top[g], top, r.per) : added ? w + (double)more[g] / scale : w;
+        mine += sums[k];
     }
+    if (threadIdx.x == 0) s.pick = segs, s.bin = 0;
+    double run = scan_before(mine, s.part, &total);
     const double want = u > 0.0 ? u * total : 0.0;
-    if (threadIdx.x == 0) s.pick = segs;
-    __syncthreads();
-    double run = 0;
-    int last = -1;
-    for (int g0 = 0; g0 < segs && s.pick == segs; g0 += THREADS) {  // (the same in all threads: a barrier lies between)
-        double all;
-        const int g = g0 + threadIdx.x;
-        const double w = sum_at(g), before = run + scan_before(w, s.part, &all);
-        run += all;
-        if (w > 0.0) last = g;
-        {
-            const uint64_t m = __ballot(w > 0.0 && before + w > want);
-            if (m && lane == 0) atomicMin(&s.pick, g + (int)__builtin_ctzll(m));
+    int here = -1, last = -1;
+    double rest = 0;
+#pragma unroll
+    for (int k = 0; k < MOST; k++) {
+        if (sums[k] > 0.0) {
+            if (here < 0 && run + sums[k] > want) here = g0 + k, rest = want - run;
+            last = g0 + k;
         }
-        __syncthreads();
-        if (g == s.pick) s.rest = want - before;
-        __syncthreads();
+        run += sums[k];
     }
+    {
+        const uint64_t m = __ballot(here >= 0), any = __ballot(last >= 0);
+        const int first = __shfl(here, m ? __builtin_ctzll(m) : 0), end = __shfl(last, any ? 63 - __builtin_clzll(any) : 0);
+        if (lane == 0) {
+            if (m) atomicMin(&s.pick, first);
+            if (any) atomicMax(&s.bin, (uint32_t)end);
+        }
+    }
+    __syncthreads();
     // (nothing found: u is 1 or more, or the sums were rounded: the last token that stays)
-    if (s.pick == segs) {
-        __syncthreads();
-        if (threadIdx.x == 0) s.pick = -1;
-        s.rest = 1e300;
-        __syncthreads();
-        last = wave_max(last);
-        if (lane == 0) atomicMax(&s.pick, last);
-        __syncthreads();
-    }
-    const int seg = s.pick < 0 ? 0 : s.pick;  // (a row that gets here has a token of weight 1: some segment was found)
+    const int seg = s.pick < segs ? s.pick : (int)s.bin;
+    if (here == seg) s.rest = rest;
+    else if (s.pick == segs && threadIdx.x == 0) s.rest = 1e300;
     const int i = seg * SEG + threadIdx.x;
-    const double rest = s.rest;
+    const double w = i < V ? stays(value_at(row, i), i) : 0.0;
+    __syncthreads();
+    rest = s.rest;
     if (threadIdx.x == 0) s.found = 0xffffffffu, s.bin = 0;
     double all;
-    const double w = i < V ? stays(value_at(row, i), i) : 0.0, before = scan_before(w, s.part, &all);
+    const double before = scan_before(w, s.part, &all);
     first_of(w > 0.0 && before + w > rest, &s.found);
     last_of(w > 0.0, &s.bin);
     __syncthreads();
@@ -987,6 +987,7 @@ static int launch(const SampleArgs& a, int B, hipStream_t st) {
         hipLaunchKernelGGL((sample_slices_kernel<TL, 4>), dim3((unsigned)((segs + 3) / 4), (unsigned)B), dim3(256), 0, st, a);
     else
         hipLaunchKernelGGL((sample_slices_kernel<TL, SLICE>), dim3((unsigned)slices, (unsigned)B), dim3(SLICE * 64), 0, st, a);
+    if (!greedy && filters) hipLaunchKernelGGL(sample_cut_kernel, dim3((unsigned)B), dim3(BINS), 0, st, a);
     if (!greedy && !open) hipLaunchKernelGGL(sample_filter_kernel<TL>, dim3((unsigned)((segs + 3) / 4), (unsigned)B), dim3(256), 0, st, a);
     hipLaunchKernelGGL(sample_draw_kernel<TL>, dim3((unsigned)B), dim3(THREADS), 0, st, a);
     return check_hip(hipGetLastError(), "sample_draw_kernel launch");

@@ -83,7 +83,7 @@ def _host_module(l):
         l.mmx_packed_b_bytes, l.mmx_repack_b, l.mmx_quantize_weights_scratch, l.mmx_quantize_weights_scaled, l.mmx_quantize_pack_int4,
         l.mmx_quantize_pack_scaled, l.mmx_quantize_rows_fp8, l.mmx_gemm_fp8_scratch_bytes, l.mmx_gemm_fp8, l.mmx_mlp_fp8_scratch_bytes, l.mmx_mlp_fp8,
         l.mmx_moe_route, l.mmx_moe_experts_scratch_bytes, l.mmx_moe_experts, l.mmx_block_norm,
-        l.mmx_mxfp4_bytes, l.mmx_quantize_mxfp4, l.mmx_gemm_mxfp4_scratch_bytes, l.mmx_gemm_mxfp4, l.mmx_mlp_mxfp4_scratch_bytes, l.mmx_mlp_mxfp4,
+        l.mmx_mxfp4_bytes, l.mmx_quantize_mxfp4, l.mmx_dequantize_mxfp4, l.mmx_gemm_mxfp4_scratch_bytes, l.mmx_gemm_mxfp4, l.mmx_mlp_mxfp4_scratch_bytes, l.mmx_mlp_mxfp4,
         l.mmx_sample_scratch_bytes, l.mmx_sample)))
     return _host_call
 

@@ -402,6 +402,7 @@ decltype(&mmx_moe_experts) call_moe_experts = nullptr;
 decltype(&mmx_block_norm) call_block_norm = nullptr;
 decltype(&mmx_mxfp4_bytes) call_mxfp4_bytes = nullptr;
 decltype(&mmx_quantize_mxfp4) call_quantize_mxfp4 = nullptr;
+decltype(&mmx_dequantize_mxfp4) call_dequantize_mxfp4 = nullptr;
 decltype(&mmx_gemm_mxfp4_scratch_bytes) call_gemm_mxfp4_need = nullptr;
 decltype(&mmx_gemm_mxfp4) call_gemm_mxfp4 = nullptr;
 decltype(&mmx_mlp_mxfp4_scratch_bytes) call_mlp_mxfp4_need = nullptr;
@@ -619,6 +620,26 @@ PyObject* quantize_mxfp4(PyObject*, PyObject* const* a, Py_ssize_t count) {
     }
 }
 
+// dequantize_mxfp4(packed rows, M, K, whether fp32, device, stream) -> their values
+PyObject* dequantize_mxfp4(PyObject*, PyObject* const* a, Py_ssize_t count) {
+    if (count != 6 || !call_dequantize_mxfp4) Py_RETURN_NONE;
+    try {
+        int device, rc = 0;
+        if (!whole_number(a[4], 0, 1 << 20, device) || a[1] == Py_None || !PyBool_Check(a[3])) throw Leave();
+        const Rows4 x = rows4(a, device);
+        const bool wide = a[3] == Py_True;
+        void* const stream = stream_of(a[5]);
+        at::Tensor y;
+        if (!unlocked([&] {
+                y = make({x.M, x.K}, wide ? at::kFloat : at::kBFloat16, *x.t);
+                rc = call_dequantize_mxfp4(x.data, x.M, x.K, wide ? MMX_F32 : MMX_BF16, y.mutable_data_ptr(), (int64_t)x.K * (wide ? 4 : 2), stream);
+            })) throw Leave();
+        return rc ? PyLong_FromLong(rc) : THPVariable_Wrap(y);
+    } catch (...) {
+        Py_RETURN_NONE;
+    }
+}
+
 // gemm_mxfp4(x, M, K, packed, N, device, stream, C, steps, bias, deq, deq_per_oc, q, q_per_oc)
 PyObject* gemm_mxfp4(PyObject*, PyObject* const* a, Py_ssize_t count) {
     if (count != 14 || !call_gemm_mxfp4) Py_RETURN_NONE;
@@ -800,7 +821,7 @@ PyObject* sample(PyObject*, PyObject* const* a, Py_ssize_t count) {
 
 // bind(addresses of the entry points, in the order below)
 PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t count) {
-    constexpr int ENTRIES = 28;
+    constexpr int ENTRIES = 29;
     if (count != ENTRIES) {
         PyErr_SetString(PyExc_TypeError, "bind takes an address for each entry point");
         return nullptr;
@@ -832,6 +853,7 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t count) {
     set(call_block_norm);
     set(call_mxfp4_bytes);
     set(call_quantize_mxfp4);
+    set(call_dequantize_mxfp4);
     set(call_gemm_mxfp4_need);
     set(call_gemm_mxfp4);
     set(call_mlp_mxfp4_need);
@@ -845,7 +867,7 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t count) {
 PyMethodDef methods[] = {METHOD(gemm), METHOD(gemm_unpacked), METHOD(gemm_packing), METHOD(matvec), METHOD(repack), METHOD(quantize), METHOD(quantize_scaled),
                          METHOD(quantize_pack_int4), METHOD(quantize_pack_scaled), METHOD(quantize_fp8),
                          METHOD(gemm_fp8), METHOD(mlp_fp8), METHOD(moe), METHOD(block_norm),
-                         METHOD(quantize_mxfp4), METHOD(gemm_mxfp4), METHOD(mlp_mxfp4), METHOD(sample), METHOD(bind), {nullptr, nullptr, 0, nullptr}};
+                         METHOD(quantize_mxfp4), METHOD(dequantize_mxfp4), METHOD(gemm_mxfp4), METHOD(mlp_mxfp4), METHOD(sample), METHOD(bind), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host_call", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

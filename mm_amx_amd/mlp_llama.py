@@ -5,17 +5,18 @@ Follows torch-ext/test.py:176-218 (``perf_llama7b_MLP``: 32 layers, per-layer ti
 closeness of the two results) and torch-ext/mlp_llama.py:6-19 (the module).  Every layer has its own
 weights (32 x 270 MB stay resident in HBM), as in the reference's deep-copied stack.
 
-With ``fp8`` the same stack runs a third time over e4m3 weights, its norms and quantisation in one kernel in front of each MLP
-(no counterpart in the reference).
+With ``fp8`` the same stack runs a third time over e4m3 weights, its norms and quantisation in one kernel in front of each MLP, and with ``mxfp4`` once more
+over weights in microscaled 4-bit floating point; with a ``vocab`` that stack has a head behind it, of such weights too, and a token is drawn for each row from
+its logits (no counterpart in the reference).
 
-    python -m mm_amx_amd.mlp_llama --M 256 --layers 32 --rounds 10 --fp8
+    python -m mm_amx_amd.mlp_llama --M 256 --layers 32 --rounds 10 --fp8 --mxfp4 --vocab 32000
 """
 import argparse
 import time
 
 import torch
 
-from . import ffn, ops
+from . import ffn, ops, sampling
 
 
 class LlamaRMSNorm(torch.nn.Module):
@@ -54,14 +55,15 @@ class LlamaMLP(torch.nn.Module):
     def numel(self, M):
         return 3 * self.hidden_size * self.intermediate_size
 
-    def compress(self):
-        """Adds the MLP over e4m3 weights."""
-        self.fp8 = ops.MLP()
-        self.fp8.setup(self.w_gate, self.w_up, self.w_down, compress="fp8")
+    def compress(self, kind="fp8"):
+        """Adds the MLP over e4m3 weights, or over such in microscaled 4-bit floating point ("mxfp4")."""
+        mlp = ops.MLP()
+        mlp.setup(self.w_gate, self.w_up, self.w_down, compress=kind)
+        setattr(self, kind, mlp)
 
-    def forward_fp8(self, x):
+    def forward_fp8(self, x, kind="fp8"):
         """LlamaRMSNorm and the MLP: the normed rows go quantised from the one to the other."""
-        return self.fp8.run(ffn.block_norm(x, eps=1e-6, quantize=True, r=False)[1])
+        return getattr(self, kind).run(ffn.block_norm(x, eps=1e-6, quantize=kind, r=False)[1])
 
     def forward(self, x):
         if self.opt:
@@ -70,7 +72,8 @@ class LlamaMLP(torch.nn.Module):
         return F.linear(F.silu(F.linear(x, self.w_gate)) * F.linear(x, self.w_up), self.w_down)
 
 
-def perf_llama7b_MLP(M=256, num_layers=32, rounds=10, hidden_size=4096, intermediate_size=11008, verbose=True, graph=False, fp8=False):
+def perf_llama7b_MLP(M=256, num_layers=32, rounds=10, hidden_size=4096, intermediate_size=11008, verbose=True, graph=False, fp8=False, mxfp4=False,
+                     vocab=0):
     layers = []
     for i in range(num_layers):
         layers += [LlamaRMSNorm(), LlamaMLP(hidden_size, intermediate_size, seed=i)]
@@ -121,13 +124,13 @@ def perf_llama7b_MLP(M=256, num_layers=32, rounds=10, hidden_size=4096, intermed
                 print(f"{'graph':>11}: per-layer dt {dt * 1e6:9.1f} us   GFlops {out['mm_amx_amd_graph']['GFlops']:10.0f}   "
                       f"GB/s {out['mm_amx_amd_graph']['GBps']:8.0f}")
             del gr
-        if fp8:
+        for kind, size in [("fp8", 1.0)] * fp8 + [("mxfp4", 17 / 32)] * (mxfp4 or vocab > 0):  # bytes a weight
             def stack(y):
                 for m in mlps:
-                    y = m.forward_fp8(y)
+                    y = m.forward_fp8(y, kind)
                 return y
             for m in mlps:
-                m.compress()
+                m.compress(kind)
             stack(x)  # warm-up
             torch.cuda.synchronize()
             t0 = time.time()
@@ -135,13 +138,32 @@ def perf_llama7b_MLP(M=256, num_layers=32, rounds=10, hidden_size=4096, intermed
                 stack(x)
             torch.cuda.synchronize()
             dt = (time.time() - t0) / rounds / num_layers
-            out["fp8"] = {"per_layer_us": dt * 1e6, "GFlops": mlps[0].flops(M) * 1e-9 / dt, "GBps": mlps[0].numel(M) * 1e-9 / dt}
+            out[kind] = {"per_layer_us": dt * 1e6, "GFlops": mlps[0].flops(M) * 1e-9 / dt, "GBps": mlps[0].numel(M) * size * 1e-9 / dt}
             mlps[0].opt = False
             want = mlps[0](layers[0](x)).float()
-            out["rel_err_fp8_one_layer"] = (torch.linalg.norm(mlps[0].forward_fp8(x).float() - want) / torch.linalg.norm(want)).item()
+            out[f"rel_err_{kind}_one_layer"] = (torch.linalg.norm(mlps[0].forward_fp8(x, kind).float() - want) / torch.linalg.norm(want)).item()
             if verbose:
-                print(f"{'fp8':>11}: per-layer dt {dt * 1e6:9.1f} us   GFlops {out['fp8']['GFlops']:10.0f}   "
-                      f"GB/s {out['fp8']['GBps']:8.0f}   relative difference to torch's bf16, one layer {out['rel_err_fp8_one_layer']:.2e}")
+                print(f"{kind:>11}: per-layer dt {dt * 1e6:9.1f} us   GFlops {out[kind]['GFlops']:10.0f}   "
+                      f"GB/s {out[kind]['GBps']:8.0f}   relative difference to torch's bf16, one layer {out[f'rel_err_{kind}_one_layer']:.2e}")
+        if vocab:
+            # a decode step of what there is of a model here: the stack, the head and a token for each row
+            g = torch.Generator(device="cuda").manual_seed(num_layers)
+            head, logits = ops.LinearMxfp4(), torch.empty((M, vocab), device="cuda")
+            head.set_weight((torch.randn((vocab, hidden_size), device="cuda", generator=g) * 0.05).to(torch.bfloat16))
+            u = torch.rand(M, device="cuda", generator=g)
+
+            def step(y):
+                head.forward(ffn.block_norm(stack(y), eps=1e-6, quantize="mxfp4", r=False)[1], logits)
+                return sampling.sample(logits, u, temperature=0.8, top_k=50, top_p=0.95)
+            out["tokens"] = step(x)
+            torch.cuda.synchronize()
+            t0 = time.time()
+            for _ in range(rounds):
+                step(x)
+            torch.cuda.synchronize()
+            out["step_us"] = (time.time() - t0) / rounds * 1e6
+            if verbose:
+                print(f"{'step':>11}: {out['step_us']:9.1f} us with a head of {vocab} columns and the draw, first tokens {out['tokens'][:8].tolist()}")
     y0, y1 = out.pop("y_torch"), out.pop("y_mm_amx_amd")
     out["rel_err"] = (torch.linalg.norm(y1 - y0) / torch.linalg.norm(y0)).item()
     # one layer on the same input: the stack has no residual connections, so rounding differences of
@@ -166,6 +188,8 @@ if __name__ == "__main__":
     ap.add_argument("--rounds", type=int, default=10)
     ap.add_argument("--graph", action="store_true", help="also replay the stack from a HIP graph")
     ap.add_argument("--fp8", action="store_true", help="also run the stack over e4m3 weights, norms fused with the quantisation")
+    ap.add_argument("--mxfp4", action="store_true", help="also run it over weights in microscaled 4-bit floating point")
+    ap.add_argument("--vocab", type=int, default=0, help="with mxfp4 weights, a head of this many columns and a token drawn for each row")
     a = ap.parse_args()
     ops.L.init(0)
-    perf_llama7b_MLP(a.M, a.layers, a.rounds, graph=a.graph, fp8=a.fp8)
+    perf_llama7b_MLP(a.M, a.layers, a.rounds, graph=a.graph, fp8=a.fp8, mxfp4=a.mxfp4, vocab=a.vocab)

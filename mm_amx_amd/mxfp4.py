@@ -120,6 +120,10 @@ def dequantize_mxfp4(rows, dtype=torch.bfloat16):
         raise MmxError("rows must be Mxfp4Rows")
     if dtype not in (torch.bfloat16, torch.float32):
         raise MmxError("values come in torch.bfloat16 or torch.float32")
+    if L._native is not None and L._initialised:
+        made = L._made(L._native.dequantize_mxfp4, rows.packed, rows.M, rows.K, dtype == torch.float32)
+        if made is not None:
+            return made
     p = rows._args("rows")
     y = torch.empty((rows.M, rows.K), dtype=dtype, device=rows.device)
     if rows.M:

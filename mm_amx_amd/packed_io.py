@@ -14,21 +14,28 @@ from safetensors import safe_open
 from safetensors.torch import save_file
 
 from . import _lib as L
+from . import mxfp4
 
 FORMAT = "mm_amx_amd.packed_b/1"
-_DT = {"bf16": L.BF16, "int8": L.I8, "int4": L.I4, "fp8": L.F8}
+_DT = {"bf16": L.BF16, "int8": L.I8, "int4": L.I4, "fp8": L.F8, "mxfp4": L.F4}
+
+
+def _bytes(dtype, K, N):
+    return mxfp4.packed_bytes(N, K) if dtype == "mxfp4" else L.packed_b_bytes(_DT[dtype], K, N)
 
 
 def save_packed(path, packed, dtype, K, N, scales=None, layout="b", extra=None):
-    """packed: uint8 tensor from repack_b / repack_gate_up / quantize_pack_int4 / quantize_pack_fp8 / pack_fp8 / pack_gate_up_fp8; dtype 'bf16', 'int8', 'int4'
-    or 'fp8'; K, N: the logical [K, N] of the packed matrix (for a gate/up pair N is 2 x the projection width, layout='gate_up');
+    """packed: uint8 tensor from repack_b / repack_gate_up / quantize_pack_int4 / quantize_pack_fp8 / pack_fp8 / pack_gate_up_fp8 / pack_mxfp4 / pack_gate_up_mxfp4; dtype 'bf16', 'int8', 'int4',
+    'fp8' or 'mxfp4' (whose scales are among the packed bytes); K, N: the logical [K, N] of the packed matrix (for a gate/up pair N is 2 x the projection width, layout='gate_up');
     scales: optional fp32 [N] per-output-channel dequantisation scales; of 'fp8' weights the scales of their blocks [rows, ceil(K / 128)]."""
     if dtype not in _DT:
-        raise L.MmxError("dtype must be 'bf16', 'int8', 'int4' or 'fp8'")
-    if packed.dtype != torch.uint8 or packed.numel() != L.packed_b_bytes(_DT[dtype], K, N):
+        raise L.MmxError("dtype must be 'bf16', 'int8', 'int4', 'fp8' or 'mxfp4'")
+    if packed.dtype != torch.uint8 or packed.numel() != _bytes(dtype, K, N):
         raise L.MmxError("packed does not have the size of a packed [K, N] matrix of this dtype")
     if dtype == "fp8" and scales is None:
         raise L.MmxError("e4m3 weights come with scales")
+    if dtype == "mxfp4" and scales is not None:
+        raise L.MmxError("weights in microscaled 4-bit floating point have their scales among the packed bytes")
     tensors = {"packed": packed.detach().cpu().contiguous()}
     if scales is not None:
         if dtype == "fp8":
@@ -52,7 +59,7 @@ def load_packed(path, device="cuda"):
         dtype, K, N = meta["dtype"], int(meta["K"]), int(meta["N"])
         packed = f.get_tensor("packed")
         scales = f.get_tensor("scales") if "scales" in f.keys() else None
-    if dtype not in _DT or packed.dtype != torch.uint8 or packed.numel() != L.packed_b_bytes(_DT[dtype], K, N):
+    if dtype not in _DT or packed.dtype != torch.uint8 or packed.numel() != _bytes(dtype, K, N):
         raise L.MmxError(f"{path}: geometry and byte count disagree")
     return {"packed": packed.to(device), "scales": None if scales is None else scales.to(device), "dtype": dtype, "K": K,
             "N": N, "layout": meta.get("layout", "b"), "extra": json.loads(meta.get("extra", "{}"))}

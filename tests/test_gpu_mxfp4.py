@@ -440,3 +440,108 @@ def test_refusals_on_the_gpu():
                  lambda: mx.MLP().setup(q, q, q, scales=(s, s, s)), lambda: mx.MLP().setup(x, x, x.t(), compress="mxfp8")):
         with pytest.raises(mx.MmxError):
             call()
+
+
+@pytest.mark.parametrize("M,K,N,pair,kernel", [
+    (4096, 300, 4090, False, "256x256"), (582, 110, 19008, True, "256x256"), (2048, 4096, 5900, False, "256x192"), (700, 520, 21952, True, "192x256"), (1030, 10900, 4090, False, "128x256"),
+    (264, 4159, 14528, True, "128x256"), (223, 103, 17257, False, "128x128"), (900, 400, 8192, True, "128x128"), (700, 1000, 4001, False, "64x128"), (513, 1000, 4032, True, "64x128"),
+    (391, 1001, 3001, False, "64x64"), (300, 260, 3008, True, "64x64_pair"), (65, 3100, 705, False, "64x64_shared_k"), (33, 2950, 130, False, "64x64_shared_k"),
+    (33, 3100, 704, True, "64x64_shared_k_pair"), (70, 2950, 128, True, "64x64_shared_k_pair"), (33, 100, 70, False, "64x64"), (20, 300, 9000, False, "rows_32"), (31, 515, 70, False, "rows_32"),
+    (17, 300, 640, True, "rows_32_pair"), (16, 1000, 65, False, "rows_16"), (9, 5000, 192, True, "rows_16_pair"), (3, 1000, 190, False, "rows_16"), (3, 1000, 192, True, "rows_16_pair")])
+def test_every_kernel_that_products_choose(M, K, N, pair, kernel):
+    """Sizes with rows, k and columns left over, an even and an odd number of chunks of k, one band of eight rows of tiles and more.  N: packed columns."""
+    rows = mx.quantize_mxfp4(normal((M, K), 1))
+    a = torch.from_numpy(m4.values(*m4.unpack(bits(rows.packed), M, K)[:2])).cuda()
+    wb = normal((N, K), 2, 0.05)
+    codes = [mx.quantize_mxfp4(w) for w in ((wb[:N // 2], wb[N // 2:]) if pair else (wb,))]
+    w = [mx.dequantize_mxfp4(c, torch.float32).double() for c in codes]
+    packed = mx.pack_gate_up_mxfp4(wb[:N // 2].contiguous(), wb[N // 2:].contiguous()) if pair else mx.pack_mxfp4(wb)
+    product = lambda b: (a @ b.T, (m4.blocks(K) + 4) * u.U * (a.abs() @ b.abs().T))  # noqa: E731 (m4.product, on the GPU in 64 bits)
+    n = N // 2 if pair else N
+    for dtype in (torch.float32, torch.bfloat16):
+        y, wide = in_wide(torch.empty((M, n), dtype=dtype, device="cuda"), 3, 9.0)
+        mx.gemm_mxfp4(rows, packed, N, mx.Epilogue(y, mx.PP_SILU_GATE if pair else mx.PP_NONE))
+        assert mx.last_kernel() == f"mxfp4_{kernel}"
+        if pair:
+            (g, eg), (v, ev) = product(w[0]), product(w[1])
+            want, bound = u.gated(*(t.cpu().numpy() for t in (g, eg, v, ev)))
+        else:
+            want, bound = (t.cpu().numpy() for t in product(w[0]))
+        u.close(y, want, bound, dtype, kernel)
+        assert (wide[:, n:] == 9.0).all()
+
+
+@pytest.mark.parametrize("M,K,N", [(40, 640, 288), (300, 512, 1056), (700, 520, 10976), (1030, 5000, 4000), (900, 400, 4096)])
+def test_the_intermediate_of_every_tile_is_quantised_as_by_the_quantiser(M, K, N):
+    """The MLP's own quantisation in the tiles that a pair can have, against its two products through the public calls, bit for bit."""
+    x = mx.quantize_mxfp4(normal((M, K), 1))
+    g, v, d = normal((N, K), 2, 0.05), normal((N, K), 3, 0.05), normal((K, N), 4, 0.05)
+    mlp = mx.MLP()
+    mlp.setup(g, v, d, compress="mxfp4")
+    h, want = torch.empty((M, N), device="cuda"), torch.empty((M, K), device="cuda")
+    mx.gemm_mxfp4(x, mx.pack_gate_up_mxfp4(g, v), 2 * N, mx.Epilogue(h, mx.PP_SILU_GATE))
+    mx.gemm_mxfp4(mx.quantize_mxfp4(h), mx.pack_mxfp4(d), K, mx.Epilogue(want, mx.PP_NONE))
+    assert torch.equal(mlp.run(x, torch.empty((M, K), device="cuda")), want)
+
+
+def test_weights_of_more_than_4_gib():
+    """Panels past 2^32 bytes: columns at the far end of [600000, 14336] weights, of which the others are zero."""
+    N, K, M = 600000, 14336, 3
+    packed = torch.zeros(-(-N // 32) * -(-K // 256) * 4352, dtype=torch.uint8, device="cuda")
+    assert packed.numel() > 2 ** 32
+    w = normal((64, K), 2, 0.05)
+    part = mx.pack_mxfp4(w)
+    packed[packed.numel() - part.numel():] = part
+    x = normal((40, K), 1)
+    a, b = m4.values(*m4.quantize(u.f64(x))), m4.values(*m4.quantize(u.f64(w)))
+    want, bound = m4.product(a, b)
+    for M in (3, 40):
+        y = torch.full((M, N), 5.0, dtype=torch.bfloat16, device="cuda")
+        mx.gemm_mxfp4(x[:M], packed, N, mx.Epilogue(y, mx.PP_NONE))
+        u.close(y[:, N - 64:], want[:M], bound[:M], torch.bfloat16, mx.last_kernel())
+        assert (y[:, :N - 64] == 0).all()
+        del y
+
+
+def test_native_and_python_calls_agree(monkeypatch):
+    from mm_amx_amd import _lib as L
+    K, N = 300, 96
+    x, w = normal((20, K), 1), normal((N, K), 2, 0.05)
+    d = normal((K, N), 3, 0.05)
+    packed, bias = mx.pack_mxfp4(w), normal((N,), 4, 1.0, torch.float32)
+    gu, down = mx.pack_gate_up_mxfp4(w, w), mx.pack_mxfp4(d)
+
+    def calls():
+        y = torch.empty((20, N), device="cuda")
+        mx.gemm_mxfp4(x, packed, N, mx.Epilogue(y, mx.PP_BIAS, bias=bias))
+        rows = mx.quantize_mxfp4(x)
+        r, z = mx.block_norm(x, x, quantize="mxfp4")
+        return [y, mx.dequantize_mxfp4(rows), mx.dequantize_mxfp4(rows, torch.float32), mx.mlp_mxfp4(rows, gu, down, N), mx.mlp_mxfp4(x, gu, down, N, y=torch.empty((20, K), device="cuda")), r,
+                mx.dequantize_mxfp4(z)]
+
+    native = calls()
+    assert L._native is not None
+    monkeypatch.setattr(L, "_native", None)
+    for a, b in zip(native, calls()):
+        assert a.dtype == b.dtype and torch.equal(a, b)
+
+
+def test_packed_weights_on_disk(tmp_path):
+    from mm_amx_amd import packed_io
+    N, K = 160, 300
+    packed = mx.pack_mxfp4(normal((N, K), 1))
+    path = str(tmp_path / "w.safetensors")
+    packed_io.save_packed(path, packed, "mxfp4", K, N)
+    w = packed_io.load_packed(path)
+    assert torch.equal(w["packed"], packed) and w["scales"] is None and (w["dtype"], w["K"], w["N"]) == ("mxfp4", K, N)
+    for bad in (dict(packed=packed[:-1]), dict(scales=torch.ones(N)), dict(K=2 * K)):
+        with pytest.raises(mx.MmxError):
+            packed_io.save_packed(path, **{**dict(packed=packed, dtype="mxfp4", K=K, N=N), **bad})
+
+
+def test_the_stack_over_4_bit_weights_with_a_head_and_tokens():
+    from mm_amx_amd import mlp_llama
+    out = mlp_llama.perf_llama7b_MLP(M=5, num_layers=2, rounds=1, hidden_size=256, intermediate_size=704, verbose=False, vocab=1000)
+    assert out["tokens"].shape == (5,) and bool(((out["tokens"] >= 0) & (out["tokens"] < 1000)).all())
+    # three quantisations to 3 significant bits, 2^-2 of a value at most, against none
+    assert out["rel_err_mxfp4_one_layer"] < 3 * 2.0 ** -2

@@ -219,3 +219,51 @@ def test_nothing_to_do_and_refusals():
                 dict(out=torch.empty(4, device="cuda")), dict(u=torch.stack((u, u), 1)[:, 0])):
         with pytest.raises(mx.MmxError):
             mx.sample(**{**dict(logits=l, u=u), **bad})
+
+
+def test_logits_of_more_than_4_gib():
+    """Rows past 2^32 bytes, some of them against the definition."""
+    B, V = 1100, 1 << 21
+    l = torch.empty((B, V), dtype=torch.bfloat16, device="cuda")
+    for b in range(0, B, 100):
+        l[b:b + 100] = torch.randn((100, V), device="cuda", generator=torch.Generator(device="cuda").manual_seed(b)).to(torch.bfloat16)
+    assert l.numel() * 2 > 2 ** 32
+    u = torch.rand(B, generator=torch.Generator().manual_seed(1))
+    for f in ((1.0, 0, 1.0, 0.0), (1.0, 50, 0.9, 0.0)):
+        got = mx.sample(l, u.cuda(), *f).tolist()
+        for b in (0, 700, 1098, 1099):
+            assert got[b] == su.token(l[b].double().cpu().numpy(), float(u[b]), *f)
+
+
+def test_large_logits_and_small_temperatures():
+    """l / T far outside what a grid of bins holds, and logits whose differences are all that counts."""
+    g = torch.Generator().manual_seed(3)
+    u = torch.rand(6, generator=g)
+    for scale, T in ((1e30, 1e30), (1e6, 1.0), (1e4, 1e4), (1.0, 1e-6), (1e-20, 1e-20), (3e37, 1.0)):
+        for at in (0.0, 5.0, -7.0):  # (in units of the scale)
+            l = (torch.randn((6, 3000), generator=g) * 2 + at) * scale
+            for k, p, m in ((0, 1.0, 0.0), (40, 1.0, 0.0), (0, 0.9, 0.0), (40, 0.9, 0.0), (0, 1.0, 0.05), (2000, 0.5, 0.0)):
+                check(l, u, T, k, p, m)
+
+
+def test_the_same_every_time():
+    """Nothing depends on the order in which workgroups come: lists, sums and tokens of many replays."""
+    l, u = logits(40, 50001, 9, dtype=torch.bfloat16)
+    l, u = l.cuda(), u.cuda()
+    for f in ((1.0, 0, 0.95, 0.0), (1.0, 300, 0.9, 0.01), (1.0, 0, 1.0, 0.0), (20.0, 0, 0.9, 0.0)):
+        first = mx.sample(l, u, *f)
+        for _ in range(20):
+            assert torch.equal(mx.sample(l, u, *f), first)
+
+
+def test_native_and_python_calls_agree(monkeypatch):
+    from mm_amx_amd import _lib as L
+    l, u = logits(9, 5000, 4)
+    l, u = l.cuda(), u.cuda()
+    rows = dict(temperature=torch.full((9,), 0.7, device="cuda"), top_k=torch.arange(9, dtype=torch.int32, device="cuda"), top_p=torch.full((9,), 0.9, device="cuda"),
+                min_p=torch.full((9,), 0.01, device="cuda"))
+    calls = lambda: [mx.sample(l, u), mx.sample(l, u, 0.7, 40, 0.9, 0.01), mx.sample(l, u, temperature=2, top_k=40), mx.sample(l, u, **rows)]  # noqa: E731
+    native = calls()
+    assert L._native is not None
+    monkeypatch.setattr(L, "_native", None)
+    assert all(torch.equal(a, b) for a, b in zip(native, calls()))

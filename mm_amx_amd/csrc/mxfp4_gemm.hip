@@ -215,8 +215,8 @@ struct Mxfp4Tile {
     static constexpr int PANELS = PM * WGM + PN * WGN;
     static constexpr int SCALES = PANELS * 4096;          // their place in a stage
     static constexpr int STAGE = SCALES + (PANELS + 3) / 4 * 1024;
-    static constexpr int RING = R * STAGE, BYTES = KG * RING;
-    static_assert((KG - 1) * BM * BN * 4 <= BYTES, "the groups' sums fit where the stages were");
+    static constexpr int RING = R * STAGE, BIAS = KG * RING, BYTES = BIAS + 2 * BN * 4;  // (the columns' biases behind the rings, of this tile and the next)
+    static_assert((KG - 1) * BM * BN * 4 <= BIAS, "the groups' sums fit where the stages were");
     static constexpr int PIECES = PANELS * 4;             // KiB of values
     static constexpr int DATA_LOADS = PIECES / NW, SCALE_LOADS = ((PANELS + 3) / 4 + NW - 1) / NW, LOADS = DATA_LOADS + SCALE_LOADS;
     static_assert(PIECES % NW == 0 && BYTES <= 160 * 1024 && (R - 1) * LOADS < 64, "every wavefront issues the same number of loads, which a wait can count");
@@ -275,14 +275,15 @@ __global__ __launch_bounds__(WGM * WGN * KG * 64) __attribute__((amdgpu_waves_pe
     using lds_u32 = __attribute__((address_space(3))) const uint32_t;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     // Neighbouring workgroups go to different XCDs: each XCD gets a run of tiles, eight rows of them at a time and those fastest, so that the ones it works on share both operands in its L2.
-    const int L = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
-    if (L >= total) return;
-    const int band = L / (8 * tiles_n), in_band = L - band * (8 * tiles_n), high = tiles_m - band * 8 < 8 ? tiles_m - band * 8 : 8;
-    const int tn = in_band / high, tm = band * 8 + in_band - tn * high;
+    // A workgroup takes every stride-th tile of its XCD's run; the next one's first stages are on their way while its results are stored.
+    const int first = (blockIdx.x & 7) * per_xcd, stride = gridDim.x >> 3;
+    int turn = blockIdx.x >> 3;
+    if (first + turn >= total) return;
     const int lane = threadIdx.x & 63, all_waves = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = all_waves % NW, group = all_waves / NW;
     const int wm = wave / WGN, wn = wave % WGN;
     const int half = lane >> 5, c = lane & 31;
-    const int panel_m0 = tm * (PM * WGM), panel_n0 = tn * (PN * WGN), panels_m = (g.M + 31) >> 5;
+    const int panels_m = (g.M + 31) >> 5;
+    int panel_m0, panel_n0;
     const int steps = (g.chunks - group + KG - 1) / KG, most = (g.chunks + KG - 1) / KG;  // of this group, of any: chunks group, group + KG, ...
 
     // ---- loads: this wavefront's KiB of a stage.  A tile may reach past the last panel: that one again, never stored.
@@ -298,21 +299,26 @@ __global__ __launch_bounds__(WGM * WGN * KG * 64) __attribute__((amdgpu_waves_pe
     };
     const char* from[LOADS];  // (uniform for values, each lane's own for scales)
     uint32_t to[LOADS];
+    auto go_to = [&](int L) __attribute__((always_inline)) {
+        const int band = L / (8 * tiles_n), in_band = L - band * (8 * tiles_n), high = tiles_m - band * 8 < 8 ? tiles_m - band * 8 : 8;
+        const int tn = in_band / high, tm = band * 8 + in_band - tn * high;
+        panel_m0 = tm * (PM * WGM), panel_n0 = tn * (PN * WGN);
 #pragma unroll
-    for (int i = 0; i < LOADS; i++) {
-        if (i < DATA) {
-            const int piece = i * NW + wave;
-            from[i] = panel_at(piece >> 2) + (piece & 3) * 1024;
-            to[i] = lds0 + piece * 1024;
-        } else {
-            // 16 lanes a panel's scales; what is past the last group of four panels again
-            int group = (i - DATA) * NW + wave;
-            group = group < (T::PANELS + 3) / 4 ? group : (T::PANELS + 3) / 4 - 1;
-            const int p = group * 4 + (lane >> 4);
-            from[i] = panel_at(p < T::PANELS ? p : T::PANELS - 1) + MX_SCALES_AT + (lane & 15) * 16;
-            to[i] = lds0 + T::SCALES + group * 1024;
+        for (int i = 0; i < LOADS; i++) {
+            if (i < DATA) {
+                const int piece = i * NW + wave;
+                from[i] = panel_at(piece >> 2) + (piece & 3) * 1024;
+                to[i] = lds0 + piece * 1024;
+            } else {
+                // 16 lanes a panel's scales; what is past the last group of four panels again
+                int four = (i - DATA) * NW + wave;
+                four = four < (T::PANELS + 3) / 4 ? four : (T::PANELS + 3) / 4 - 1;
+                const int p = four * 4 + (lane >> 4);
+                from[i] = panel_at(p < T::PANELS ? p : T::PANELS - 1) + MX_SCALES_AT + (lane & 15) * 16;
+                to[i] = lds0 + T::SCALES + four * 1024;
+            }
         }
-    }
+    };
     const uint32_t lane16 = lane * 16;
     auto load = [&](auto ic, int t, int slot) __attribute__((always_inline)) {
         constexpr int i = decltype(ic)::value;
@@ -327,12 +333,6 @@ __global__ __launch_bounds__(WGM * WGN * KG * 64) __attribute__((amdgpu_waves_pe
     };
 
     f32x16 acc[PM][PN];
-#pragma unroll
-    for (int i = 0; i < PM; i++)
-#pragma unroll
-        for (int j = 0; j < PN; j++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) acc[i][j][e] = 0.0f;
     u32x4 fa[2][PM], fb[2][PN];  // a step's operands, now and next
     uint32_t sa[2][PM], sb[2][PN];
     const uint32_t a_lane = wm * PM * 4096 + lane * 16, b_lane = (PM * WGM + wn * PN) * 4096 + lane * 16;
@@ -348,187 +348,227 @@ __global__ __launch_bounds__(WGM * WGN * KG * 64) __attribute__((amdgpu_waves_pe
     auto read_sa = [&](int i) __attribute__((always_inline)) { return *reinterpret_cast<lds_u32*>(at_sa + i * 256); };
     auto read_sb = [&](int j) __attribute__((always_inline)) { return *reinterpret_cast<lds_u32*>(at_sb + j * 256); };
 
-    unrolled<0, R>([&](auto rc) __attribute__((always_inline)) {
-        constexpr int r = decltype(rc)::value;
-        unrolled<0, LOADS>([&](auto ic) __attribute__((always_inline)) { if (r < steps) load(ic, r, r); });
-    });
-    if (steps >= R) asm volatile("s_waitcnt vmcnt(%0)" : : "n"((R - 1) * LOADS) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    places(0);
+    // a tile's biases, 64 columns a wavefront, and its first stages
+    const bool biased = g.ep.steps & MMX_PP_BIAS;
+    auto start = [&](int parity) __attribute__((always_inline)) {
+        if (biased && group == 0) {
 #pragma unroll
-    for (int i = 0; i < PM; i++) {
-        fa[0][i] = read_a(i, 0);
-        sa[0][i] = read_sa(i);
-    }
-#pragma unroll
-    for (int j = 0; j < PN; j++) {
-        fb[0][j] = read_b(j, 0);
-        sb[0][j] = read_sb(j);
-    }
-    __builtin_amdgcn_sched_barrier(0);
-
-    // One slot per MFMA, in this order and no other: the MFMA, an LDS read for the next step, a load.
-    constexpr int PER = PM * PN, READS = PM + PN;
-    int slot = 0;
-    // ODD: which set of scales the stage has
-    auto stage = [&](auto odd_c, int t) __attribute__((always_inline)) {
-        constexpr int S = decltype(odd_c)::value;
-        const int next = slot + 1 < R ? slot + 1 : 0, before = slot > 0 ? slot - 1 : R - 1;
-        const bool more_before = t > 0 && t - 1 + R < steps, more = t + R < steps;
-        unrolled<0, 4 * PER>([&](auto xc) __attribute__((always_inline)) {
-            constexpr int x = decltype(xc)::value, u = x / PER, y = x % PER, i = y / PN, j = y % PN;
-            if constexpr (x == 3 * PER) {
-                // all of this stage is in registers (its last step's operands arrive now); the next one has landed, R - 2 younger ones may be on their way
-                if (R > 2 && t + R - 1 < steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"((R - 2) * LOADS) : "memory");
-                else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-                __builtin_amdgcn_s_barrier();
-                asm volatile("" ::: "memory");
-                places(next);
+            for (int b = 0; b < (T::BN / 64 + NW - 1) / NW; b++) {
+                const int part = b * NW + wave;
+                if (part * 64 < T::BN) {
+                    const int n = panel_n0 * 32 + part * 64 + lane;
+                    const float* const src = g.ep.bias + (n < g.N ? n : g.N - 1);
+                    const uint32_t dst = __builtin_amdgcn_readfirstlane(lds0 + T::BIAS + parity * (T::BN * 4) + part * 256);
+                    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" : : "s"(dst), "v"(src) : "memory");
+                }
             }
-            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand(fb[u & 1][j]), mx_operand(fa[u & 1][i]), acc[i][j], 4, 4, u, (int)sb[S][j], u, (int)sa[S][i]);
-            // (else the compiler gathers the products behind the branches of the loads)
-            asm volatile("" : "+v"(acc[i][j]));
-            // the next step's operands (past the last stage what an earlier one left there: never used)
-            unrolled<0, READS>([&](auto rc) __attribute__((always_inline)) {
-                constexpr int r = decltype(rc)::value;
-                if constexpr (r * PER / READS == y) {
-                    // in the order in which the step uses them
-                    if constexpr (r == 0) fa[(u + 1) & 1][0] = read_a(0, (u + 1) & 3);
-                    else if constexpr (r <= PN) fb[(u + 1) & 1][r - 1] = read_b(r - 1, (u + 1) & 3);
-                    else fa[(u + 1) & 1][r - PN] = read_a(r - PN, (u + 1) & 3);
-                    if constexpr (u == 3) {
-                        if constexpr (r == 0) sa[S ^ 1][0] = read_sa(0);
-                        else if constexpr (r <= PN) sb[S ^ 1][r - 1] = read_sb(r - 1);
-                        else sa[S ^ 1][r - PN] = read_sa(r - PN);
-                    }
-                }
-            });
-            // stage t + R from the last step on; the rest of t - 1 + R before
-            unrolled<0, LOADS>([&](auto lc) __attribute__((always_inline)) {
-                constexpr int l = decltype(lc)::value, when = l * 3 * PER / LOADS;  // of three steps, the first of which is a stage's last
-                if constexpr (when < PER) {
-                    if constexpr (x == 3 * PER + when) {
-                        if (more) load(lc, t + R, slot);
-                    }
-                } else if constexpr (x == when - PER) {
-                    if (more_before) load(lc, t - 1 + R, before);
-                }
-            });
-            __builtin_amdgcn_sched_barrier(0);
-        });
-        slot = next;
-    };
-    int t = 0;
-    for (; t + 2 <= steps; t += 2) {
-        stage(std::integral_constant<int, 0>(), t);
-        stage(std::integral_constant<int, 1>(), t + 1);
-    }
-    if (t < steps) stage(std::integral_constant<int, 0>(), t);
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    if constexpr (KG > 1) {
-        if (steps < most) __builtin_amdgcn_s_barrier();  // (the others have one stage more)
-        __syncthreads();
-        f32x4* const sums = reinterpret_cast<f32x4*>(smem) + threadIdx.x % (NW * 64);
-        if (group > 0) {
-#pragma unroll
-            for (int i = 0; i < PM; i++)
-#pragma unroll
-                for (int j = 0; j < PN; j++)
-#pragma unroll
-                    for (int q = 0; q < 4; q++)
-                        sums[((((group - 1) * PM + i) * PN + j) * 4 + q) * (NW * 64)] = f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
         }
-        __syncthreads();
-        if (group > 0) return;
+        unrolled<0, R>([&](auto rc) __attribute__((always_inline)) {
+            constexpr int r = decltype(rc)::value;
+            unrolled<0, LOADS>([&](auto ic) __attribute__((always_inline)) { if (r < steps) load(ic, r, r); });
+        });
+    };
+    go_to(first + turn);
+    start(0);
+    for (int parity = 0;; parity ^= 1) {
+        // (behind the first tile its stores are among what is on its way, in an order of their own: all of it is waited for)
+        if (parity == 0 && turn < stride && steps >= R) asm volatile("s_waitcnt vmcnt(%0)" : : "n"((R - 1) * LOADS) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        places(0);
 #pragma unroll
-        for (int o = 0; o < KG - 1; o++)
+        for (int i = 0; i < PM; i++)
 #pragma unroll
-            for (int i = 0; i < PM; i++)
+            for (int j = 0; j < PN; j++)
 #pragma unroll
-                for (int j = 0; j < PN; j++)
+                for (int e = 0; e < 16; e++) acc[i][j][e] = 0.0f;
 #pragma unroll
-                    for (int q = 0; q < 4; q++) {
-                        const f32x4 v = sums[(((o * PM + i) * PN + j) * 4 + q) * (NW * 64)];
+        for (int i = 0; i < PM; i++) {
+            fa[0][i] = read_a(i, 0);
+            sa[0][i] = read_sa(i);
+        }
 #pragma unroll
-                        for (int e = 0; e < 4; e++) acc[i][j][4 * q + e] += v[e];
-                    }
-    }
+        for (int j = 0; j < PN; j++) {
+            fb[0][j] = read_b(j, 0);
+            sb[0][j] = read_sb(j);
+        }
+        __builtin_amdgcn_sched_barrier(0);
 
-    // ---- post-op: a lane holds columns 8 q + 4 half + 0..3, q = 0..3, of row c of each panel of 32 columns
-    if (g.pair) {
-        if constexpr (PN % 2 == 0) {
-#pragma unroll
-            for (int j = 0; j < PN / 2; j++) {
-                const int block = (panel_n0 + wn * PN) / 2 + j;  // of 32 columns of the result
-                if (block * 64 >= g.N) continue;
-#pragma unroll
-                for (int i = 0; i < PM; i++) {
-                    const int m = (panel_m0 + wm * PM + i) * 32 + c;
-                    float r[16];
-#pragma unroll
-                    for (int e = 0; e < 16; e++) r[e] = silu32(acc[i][2 * j][e]) * acc[i][2 * j + 1][e];
-                    if (!g.packed_out) {
-                        store16(g.ep, m, g.M, block * 32, g.N / 2, half, r);
-                        continue;
+        // One slot per MFMA, in this order and no other: the MFMA, an LDS read for the next step, a load.
+        constexpr int PER = PM * PN, READS = PM + PN;
+        int slot = 0;
+        // ODD: which set of scales the stage has
+        auto stage = [&](auto odd_c, int t) __attribute__((always_inline)) {
+            constexpr int S = decltype(odd_c)::value;
+            const int next = slot + 1 < R ? slot + 1 : 0, before = slot > 0 ? slot - 1 : R - 1;
+            const bool more_before = t > 0 && t - 1 + R < steps, more = t + R < steps;
+            unrolled<0, 4 * PER>([&](auto xc) __attribute__((always_inline)) {
+                constexpr int x = decltype(xc)::value, u = x / PER, y = x % PER, i = y / PN, j = y % PN;
+                if constexpr (x == 3 * PER) {
+                    // all of this stage is in registers (its last step's operands arrive now); the next one has landed, R - 2 younger ones may be on their way
+                    if (R > 2 && t + R - 1 < steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"((R - 2) * LOADS) : "memory");
+                    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                    __builtin_amdgcn_s_barrier();
+                    asm volatile("" ::: "memory");
+                    places(next);
+                }
+                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand(fb[u & 1][j]), mx_operand(fa[u & 1][i]), acc[i][j], 4, 4, u, (int)sb[S][j], u, (int)sa[S][i]);
+                // (else the compiler gathers the products behind the branches of the loads)
+                asm volatile("" : "+v"(acc[i][j]));
+                // the next step's operands (past the last stage what an earlier one left there: never used)
+                unrolled<0, READS>([&](auto rc) __attribute__((always_inline)) {
+                    constexpr int r = decltype(rc)::value;
+                    if constexpr (r * PER / READS == y) {
+                        // in the order in which the step uses them
+                        if constexpr (r == 0) fa[(u + 1) & 1][0] = read_a(0, (u + 1) & 3);
+                        else if constexpr (r <= PN) fb[(u + 1) & 1][r - 1] = read_b(r - 1, (u + 1) & 3);
+                        else fa[(u + 1) & 1][r - PN] = read_a(r - PN, (u + 1) & 3);
+                        if constexpr (u == 3) {
+                            if constexpr (r == 0) sa[S ^ 1][0] = read_sa(0);
+                            else if constexpr (r <= PN) sb[S ^ 1][r - 1] = read_sb(r - 1);
+                            else sa[S ^ 1][r - PN] = read_sa(r - PN);
+                        }
                     }
-                    uint32_t top = 0;
+                });
+                // stage t + R from the last step on; the rest of t - 1 + R before
+                unrolled<0, LOADS>([&](auto lc) __attribute__((always_inline)) {
+                    constexpr int l = decltype(lc)::value, when = l * 3 * PER / LOADS;  // of three steps, the first of which is a stage's last
+                    if constexpr (when < PER) {
+                        if constexpr (x == 3 * PER + when) {
+                            if (more) load(lc, t + R, slot);
+                        }
+                    } else if constexpr (x == when - PER) {
+                        if (more_before) load(lc, t - 1 + R, before);
+                    }
+                });
+                __builtin_amdgcn_sched_barrier(0);
+            });
+            slot = next;
+        };
+        int t = 0;
+        for (; t + 2 <= steps; t += 2) {
+            stage(std::integral_constant<int, 0>(), t);
+            stage(std::integral_constant<int, 1>(), t + 1);
+        }
+        if (t < steps) stage(std::integral_constant<int, 0>(), t);
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+        if constexpr (KG > 1) {
+            if (steps < most) __builtin_amdgcn_s_barrier();  // (the others have one stage more)
+            __syncthreads();
+            f32x4* const sums = reinterpret_cast<f32x4*>(smem) + threadIdx.x % (NW * 64);
+            if (group > 0) {
 #pragma unroll
-                    for (int e = 0; e < 16; e++) top = umax(top, abs_bits(r[e]));
-                    top = umax(top, (uint32_t)__shfl_xor((int)top, 32));
-                    const uint32_t b = mx_scale_of(top);
-                    const float s = mx_value_of(b);
-                    uint32_t mine[2], other[2];
+                for (int i = 0; i < PM; i++)
 #pragma unroll
-                    for (int q = 0; q < 2; q++)
-                        mine[q] = to_fp4x4(r[8 * q], r[8 * q + 1], r[8 * q + 2], r[8 * q + 3], s) | to_fp4x4(r[8 * q + 4], r[8 * q + 5], r[8 * q + 6], r[8 * q + 7], s) << 16;
+                    for (int j = 0; j < PN; j++)
 #pragma unroll
-                    for (int q = 0; q < 2; q++) other[q] = (uint32_t)__shfl_xor((int)mine[q], 32);
-                    if (half == 0 && m < g.M) {
-                        char* const panel = g.packed_out + (int64_t)(m >> 5) * g.ld_out;
-                        *reinterpret_cast<u32x4*>(panel + mx_piece(m, block)) =
-                            u32x4{(mine[0] & 0xffffu) | other[0] << 16, mine[0] >> 16 | (other[0] & 0xffff0000u), (mine[1] & 0xffffu) | other[1] << 16, mine[1] >> 16 | (other[1] & 0xffff0000u)};
-                        panel[mx_scale_at(m, block)] = (char)b;
-                        if ((block + 1) * 64 == g.N) {  // what is left of the last chunk
-                            for (int kb = block + 1; kb & 7; kb++) {
-                                *reinterpret_cast<u32x4*>(panel + mx_piece(m, kb)) = u32x4{0, 0, 0, 0};
-                                panel[mx_scale_at(m, kb)] = 127;
+                        for (int q = 0; q < 4; q++)
+                            sums[((((group - 1) * PM + i) * PN + j) * 4 + q) * (NW * 64)] = f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+            }
+            __syncthreads();
+            if (group > 0) return;
+#pragma unroll
+            for (int o = 0; o < KG - 1; o++)
+#pragma unroll
+                for (int i = 0; i < PM; i++)
+#pragma unroll
+                    for (int j = 0; j < PN; j++)
+#pragma unroll
+                        for (int q = 0; q < 4; q++) {
+                            const f32x4 v = sums[(((o * PM + i) * PN + j) * 4 + q) * (NW * 64)];
+#pragma unroll
+                            for (int e = 0; e < 4; e++) acc[i][j][4 * q + e] += v[e];
+                        }
+        }
+
+        const int done_m0 = panel_m0, done_n0 = panel_n0;
+        bool more = false;
+        if constexpr (KG == 1) {
+            turn += stride;
+            more = turn < per_xcd && first + turn < total;
+            if (more) {
+                go_to(first + turn);
+                start(parity ^ 1);
+            }
+        }
+
+        // ---- post-op: a lane holds columns 8 q + 4 half + 0..3, q = 0..3, of row c of each panel of 32 columns
+        if (g.pair) {
+            if constexpr (PN % 2 == 0) {
+#pragma unroll
+                for (int j = 0; j < PN / 2; j++) {
+                    const int block = (done_n0 + wn * PN) / 2 + j;  // of 32 columns of the result
+                    if (block * 64 >= g.N) continue;
+#pragma unroll
+                    for (int i = 0; i < PM; i++) {
+                        const int m = (done_m0 + wm * PM + i) * 32 + c;
+                        float r[16];
+#pragma unroll
+                        for (int e = 0; e < 16; e++) r[e] = silu32(acc[i][2 * j][e]) * acc[i][2 * j + 1][e];
+                        if (!g.packed_out) {
+                            store16(g.ep, m, g.M, block * 32, g.N / 2, half, r);
+                            continue;
+                        }
+                        uint32_t top = 0;
+#pragma unroll
+                        for (int e = 0; e < 16; e++) top = umax(top, abs_bits(r[e]));
+                        top = umax(top, (uint32_t)__shfl_xor((int)top, 32));
+                        const uint32_t b = mx_scale_of(top);
+                        const float s = mx_value_of(b);
+                        uint32_t mine[2], other[2];
+#pragma unroll
+                        for (int q = 0; q < 2; q++)
+                            mine[q] = to_fp4x4(r[8 * q], r[8 * q + 1], r[8 * q + 2], r[8 * q + 3], s) | to_fp4x4(r[8 * q + 4], r[8 * q + 5], r[8 * q + 6], r[8 * q + 7], s) << 16;
+#pragma unroll
+                        for (int q = 0; q < 2; q++) other[q] = (uint32_t)__shfl_xor((int)mine[q], 32);
+                        if (half == 0 && m < g.M) {
+                            char* const panel = g.packed_out + (int64_t)(m >> 5) * g.ld_out;
+                            *reinterpret_cast<u32x4*>(panel + mx_piece(m, block)) =
+                                u32x4{(mine[0] & 0xffffu) | other[0] << 16, mine[0] >> 16 | (other[0] & 0xffff0000u), (mine[1] & 0xffffu) | other[1] << 16, mine[1] >> 16 | (other[1] & 0xffff0000u)};
+                            panel[mx_scale_at(m, block)] = (char)b;
+                            if ((block + 1) * 64 == g.N) {  // what is left of the last chunk
+                                for (int kb = block + 1; kb & 7; kb++) {
+                                    *reinterpret_cast<u32x4*>(panel + mx_piece(m, kb)) = u32x4{0, 0, 0, 0};
+                                    panel[mx_scale_at(m, kb)] = 127;
+                                }
                             }
                         }
                     }
                 }
             }
-        }
-        return;
-    }
+        } else {
 #pragma unroll
-    for (int j = 0; j < PN; j++) {
-        const int n = (panel_n0 + wn * PN + j) * 32;
-        if (n >= g.N) continue;
-        float bias[16];
-        if (g.ep.steps & MMX_PP_BIAS) {
+            for (int j = 0; j < PN; j++) {
+                const int n = (done_n0 + wn * PN + j) * 32;
+                if (n >= g.N) continue;
+                float bias[16];
+                if (biased) {
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const int at = n + (e >> 2) * 8 + half * 4 + (e & 3);
-                bias[e] = g.ep.bias[at < g.N ? at : g.N - 1];
+                    for (int q = 0; q < 4; q++) {
+                        const f32x4 v = *reinterpret_cast<const f32x4*>(smem + T::BIAS + parity * (T::BN * 4) + ((wn * PN + j) * 32 + q * 8 + half * 4) * 4);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) bias[4 * q + e] = v[e];
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < PM; i++) {
+                    float r[16];
+#pragma unroll
+                    for (int e = 0; e < 16; e++) r[e] = acc[i][j][e];
+                    if (biased) {
+#pragma unroll
+                        for (int e = 0; e < 16; e++) r[e] = r[e] + bias[e];
+                    }
+                    if (g.ep.steps & MMX_PP_GELU) {
+#pragma unroll
+                        for (int e = 0; e < 16; e++) r[e] = gelu_erf_minimax(r[e]);
+                    }
+                    store16(g.ep, (done_m0 + wm * PM + i) * 32 + c, g.M, n, g.N, half, r);
+                }
             }
         }
-#pragma unroll
-        for (int i = 0; i < PM; i++) {
-            float r[16];
-#pragma unroll
-            for (int e = 0; e < 16; e++) r[e] = acc[i][j][e];
-            if (g.ep.steps & MMX_PP_BIAS) {
-#pragma unroll
-                for (int e = 0; e < 16; e++) r[e] = r[e] + bias[e];
-            }
-            if (g.ep.steps & MMX_PP_GELU) {
-#pragma unroll
-                for (int e = 0; e < 16; e++) r[e] = gelu_erf_minimax(r[e]);
-            }
-            store16(g.ep, (panel_m0 + wm * PM + i) * 32 + c, g.M, n, g.N, half, r);
-        }
+        if (!more) return;
     }
 }
 
@@ -542,7 +582,10 @@ static int launch_tile(const Mxfp4Gemm& g, hipStream_t st, const char* name) {
     const int64_t tiles_m = (g.M + T::BM - 1) / T::BM, tiles_n = ((int64_t)g.npanels * 32 + T::BN - 1) / T::BN, total = tiles_m * tiles_n, per_xcd = (total + 7) / 8;
     if (per_xcd * 8 * (T::NW * KG * 64) > 0xffffffffll) return set_error(MMX_E_INVALID, "mmx_gemm_mxfp4: too many tiles for one launch");
     note_kernel(name);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(per_xcd * 8)), dim3(T::NW * KG * 64), T::BYTES, st, g, (int)tiles_m, (int)tiles_n, (int)total, (int)per_xcd);
+    constexpr int by_lds = 160 * 1024 / T::BYTES, by_waves = 8 / (T::NW * KG);  // (of a CU: two wavefronts a SIMD)
+    const int64_t at_once = (int64_t)num_cus() * (by_lds < by_waves ? by_lds : by_waves) / 8 * 8;
+    const int64_t grid = KG > 1 || per_xcd * 8 < at_once ? per_xcd * 8 : at_once;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(T::NW * KG * 64), T::BYTES, st, g, (int)tiles_m, (int)tiles_n, (int)total, (int)per_xcd);
     return check_hip(hipGetLastError(), "mxfp4_tile_kernel launch");
 }
 

@@ -8,7 +8,6 @@ namespace mmx {
 
 int num_cus();
 
-typedef int i32x2 __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ i32x8 mx_operand(u32x4 a) { return i32x8{(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0}; }
 

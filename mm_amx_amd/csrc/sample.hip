@@ -38,7 +38,7 @@ struct RowAsks {
 __device__ __forceinline__ RowAsks asks_of(const SampleArgs& a, int row) {
     RowAsks r;
     r.T = a.temperature ? (double)a.temperature[row] : a.temperature_all;
-    r.per = 1.0 / r.T;
+    r.per = 1.0 / fmax(r.T, 1e-300);  // (that and less: any two logits that differ are too far apart for a weight; 1 / T must stay a number)
     r.k = a.top_k ? a.top_k[row] : a.top_k_all;
     r.p = a.top_p ? (double)a.top_p[row] : a.top_p_all;
     r.min_p = a.min_p ? (double)a.min_p[row] : a.min_p_all;

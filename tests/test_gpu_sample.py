@@ -246,6 +246,16 @@ def test_large_logits_and_small_temperatures():
                 check(l, u, T, k, p, m)
 
 
+@pytest.mark.parametrize("T", [5e-324, 1e-310, 6e-309, 1e-300, 1e-45, 1e30, float("inf")])
+def test_temperatures_at_the_ends(T):
+    l, u = logits(3, 5000, 11)
+    l[0, 4321] = l[0, 4322] = 60.0
+    l[1, :] = -1e-45
+    l[1, 4000:4500] = 0.0
+    for f in ((0, 1.0, 0.0), (40, 1.0, 0.0), (0, 0.9, 0.0), (40, 0.9, 0.0), (0, 1.0, 0.5)):
+        check(l, u, T, *f)
+
+
 def test_the_same_every_time():
     """Nothing depends on the order in which workgroups come: lists, sums and tokens of many replays."""
     l, u = logits(40, 50001, 9, dtype=torch.bfloat16)

@@ -604,29 +604,30 @@ static int launch_rows(const Mxfp4Gemm& g, hipStream_t st, const char* name) {
 bool mx_takes_bf16(int M, int K) { return M <= 8 && (int64_t)M * K <= 16384; }
 
 // Which tile: the least of rounds * (fixed + chunks of 256 k * stage), a round being as many tiles as fit on the chip; one that is not full leaves each of its tiles more of the chip, down to `least` of
-// the time.  The constants are fitted to 52 products of 33 to 4096 rows, 256 to 11008 k and 256 to 22016 columns in every tile, each by how near it comes to the fastest; the tile chosen was 0.8 % behind
-// that on average (of those that a pair can have 1 %), 11 % at most.  us at 2048 x 4096 x 11008 / 4096 x 4096 x 4096 / 1024 x 11008 x 4096 / 256 x 4096 x 4096 / 64 x 11008 x 4096:
-//     256 x 256            62 / 39 / 56 / 25 / 51
-//     256 x 192            54 / 47 / 45 / 20 / 43
-//     192 x 256            54 / 47 / 44 / 20 / 43
-//     128 x 256            57 / 44 / 33 / 15 / 29
-//     128 x 128            59 / 43 / 34 / 14 / 30
-//      64 x 128            68 / 51 / 32 / 9.1 / 17
-//      64 x 64             88 / 67 / 39 / 7.4 / 13
-//      64 x 64, K shared    - / 83 / 46 / 7.1 / 11
+// the time.  The constants are fitted to 65 products of 33 to 4096 rows, 256 to 11008 k and 256 to 22016 columns in every tile, each by how near it comes to the fastest; the tile chosen was 0.5 % behind
+// that on average (of those that a pair has 0.2 %), 10 % at most.  us at 2048 x 4096 x 11008 / 4096 x 4096 x 4096 / 1024 x 11008 x 4096 / 256 x 4096 x 4096 / 64 x 11008 x 4096:
+//     256 x 256            64 / 39 / 57 / 25 / 52
+//     256 x 192            57 / 55 / 46 / 21 / 42
+//     128 x 256            61 / 45 / 36 / 16 / 30
+//     128 x 128            63 / 47 / 36 / 15 / 33
+//     128 x 128, K shared  @1
+//      64 x 128, K shared  @2
+//      64 x 64             93 / 70 / 44 / 8.1 / 14
+//      64 x 64, K shared  115 / 85 / 46 / 7.3 / 12
+// (64 x 128 without sharing, 73 / 54 / 33 / 10 / 19, a 192 x 256 for pairs and a 64 x 64 of their own came out first too rarely to be kept.)
 struct TileCost {
     int bm, bn, per_cu;
     float fixed_us, stage_us, least;
 };
-enum { T_256_256, T_256_192, T_192_256, T_128_256, T_128_128, T_64_128, T_64_64, T_64_64_SHARED, TILES };
-static constexpr TileCost COSTS[TILES] = {{256, 256, 1, 9.9f, 1.72f, 0.59f}, {256, 192, 1, 7.8f, 1.36f, 0.63f}, {192, 256, 1, 8.2f, 1.31f, 0.61f}, {128, 256, 1, 7.1f, 0.90f, 0.65f},
-                                          {128, 128, 2, 5.7f, 1.02f, 0.58f}, {64, 128, 2, 4.5f, 0.48f, 0.72f}, {64, 64, 2, 3.8f, 0.34f, 0.74f}, {64, 64, 1, 3.6f, 0.19f, 0.92f}};
+enum { T_256_256, T_256_192, T_128_256, T_128_128, T_128_128_SHARED, T_64_128_SHARED, T_64_64, T_64_64_SHARED, TILES };
+static constexpr TileCost COSTS[TILES] = {{256, 256, 1, 10.5f, 1.69f, 0.62f}, {256, 192, 1, 8.4f, 1.34f, 0.63f}, {128, 256, 1, 7.5f, 0.88f, 0.68f}, {128, 128, 2, 6.3f, 1.0f, 0.62f},
+                                          {128, 128, 1, 5.9f, 0.53f, 0.81f},  {64, 128, 1, 4.7f, 0.294f, 0.88f}, {64, 64, 2, 4.0f, 0.336f, 0.8f}, {64, 64, 1, 3.8f, 0.189f, 0.95f}};
 
 static int choose_tile(const Mxfp4Gemm& g) {
     int best = -1;
     double fastest = 0;
     for (int i = 0; i < TILES; i++) {
-        if (i == (g.pair ? T_256_192 : T_192_256)) continue;  // (a wavefront of a pair has as many gate panels as up panels)
+        if (g.pair && (i == T_256_192 || i == T_64_64)) continue;  // (a wavefront of a pair has as many gate panels as up panels)
         const TileCost& t = COSTS[i];
         const int64_t tiles = (int64_t)((g.M + t.bm - 1) / t.bm) * (((int64_t)g.npanels * 32 + t.bn - 1) / t.bn), at_once = (int64_t)num_cus() * t.per_cu;
         const double full = (double)(tiles / at_once), rest = (double)(tiles % at_once) / at_once;
@@ -646,11 +647,11 @@ int launch_gemm_mxfp4(const Mxfp4Gemm& g, hipStream_t st) {
     switch (choose_tile(g)) {
     case T_256_256: return launch_tile<4, 2, 2, 4, 2>(g, st, "mxfp4_256x256");
     case T_256_192: return launch_tile<2, 3, 4, 2, 2>(g, st, "mxfp4_256x192");
-    case T_192_256: return launch_tile<3, 2, 2, 4, 2>(g, st, "mxfp4_192x256");
     case T_128_256: return launch_tile<2, 2, 2, 4, 3>(g, st, "mxfp4_128x256");
     case T_128_128: return launch_tile<2, 2, 2, 2, 2>(g, st, "mxfp4_128x128");
-    case T_64_128: return launch_tile<1, 2, 2, 2, 3>(g, st, "mxfp4_64x128");
-    case T_64_64: return g.pair ? launch_tile<1, 2, 2, 1, 4>(g, st, "mxfp4_64x64_pair") : launch_tile<1, 1, 2, 2, 4>(g, st, "mxfp4_64x64");
+    case T_128_128_SHARED: return launch_tile<2, 2, 2, 2, 2, 2>(g, st, "mxfp4_128x128_shared_k");
+    case T_64_128_SHARED: return launch_tile<1, 2, 2, 2, 3, 2>(g, st, "mxfp4_64x128_shared_k");
+    case T_64_64: return launch_tile<1, 1, 2, 2, 4>(g, st, "mxfp4_64x64");
     default: return g.pair ? launch_tile<1, 2, 2, 1, 3, 2>(g, st, "mxfp4_64x64_shared_k_pair") : launch_tile<1, 1, 2, 2, 3, 2>(g, st, "mxfp4_64x64_shared_k");
     }
 }

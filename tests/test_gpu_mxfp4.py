@@ -443,9 +443,10 @@ def test_refusals_on_the_gpu():
 
 
 @pytest.mark.parametrize("M,K,N,pair,kernel", [
-    (4096, 300, 4090, False, "256x256"), (582, 110, 19008, True, "256x256"), (2048, 4096, 5900, False, "256x192"), (700, 520, 21952, True, "192x256"), (1030, 10900, 4090, False, "128x256"),
-    (264, 4159, 14528, True, "128x256"), (223, 103, 17257, False, "128x128"), (900, 400, 8192, True, "128x128"), (700, 1000, 4001, False, "64x128"), (513, 1000, 4032, True, "64x128"),
-    (391, 1001, 3001, False, "64x64"), (300, 260, 3008, True, "64x64_pair"), (65, 3100, 705, False, "64x64_shared_k"), (33, 2950, 130, False, "64x64_shared_k"),
+    (4096, 300, 4090, False, "256x256"), (582, 110, 19008, True, "256x256"), (2048, 4096, 5900, False, "256x192"), (700, 520, 21952, True, "128x128"), (1030, 10900, 4090, False, "128x256"),
+    (264, 4159, 14528, True, "128x256"), (223, 103, 17257, False, "128x128"), (900, 400, 8192, True, "128x128"), (700, 1000, 4001, False, "128x128_shared_k"),
+    (513, 1000, 4032, True, "128x128_shared_k"), (68, 5225, 15139, False, "64x128_shared_k"), (73, 127, 9216, True, "64x128_shared_k"), (300, 2950, 5056, True, "64x128_shared_k"),
+    (391, 1001, 3001, False, "64x64"), (300, 260, 3008, True, "64x64_shared_k_pair"), (65, 3100, 705, False, "64x64_shared_k"), (33, 2950, 130, False, "64x64_shared_k"),
     (33, 3100, 704, True, "64x64_shared_k_pair"), (70, 2950, 128, True, "64x64_shared_k_pair"), (33, 100, 70, False, "64x64"), (20, 300, 9000, False, "rows_32"), (31, 515, 70, False, "rows_32"),
     (17, 300, 640, True, "rows_32_pair"), (16, 1000, 65, False, "rows_16"), (9, 5000, 192, True, "rows_16_pair"), (3, 1000, 190, False, "rows_16"), (3, 1000, 192, True, "rows_16_pair")])
 def test_every_kernel_that_products_choose(M, K, N, pair, kernel):
@@ -471,7 +472,7 @@ def test_every_kernel_that_products_choose(M, K, N, pair, kernel):
         assert (wide[:, n:] == 9.0).all()
 
 
-@pytest.mark.parametrize("M,K,N", [(40, 640, 288), (300, 512, 1056), (700, 520, 10976), (1030, 5000, 4000), (900, 400, 4096)])
+@pytest.mark.parametrize("M,K,N", [(40, 640, 288), (300, 512, 1056), (700, 520, 10976), (1030, 5000, 4000), (900, 400, 4096), (264, 4159, 7264), (700, 1000, 2016), (130, 1000, 4096)])
 def test_the_intermediate_of_every_tile_is_quantised_as_by_the_quantiser(M, K, N):
     """The MLP's own quantisation in the tiles that a pair can have, against its two products through the public calls, bit for bit."""
     x = mx.quantize_mxfp4(normal((M, K), 1))

@@ -215,6 +215,7 @@ struct Mxfp4Tile {
     static constexpr int SCALES = PANELS * 4096;          // their place in a stage
     static constexpr int STAGE = SCALES + (PANELS + 3) / 4 * 1024;
     static constexpr int RING = R * STAGE, BIAS = KG * RING, BYTES = BIAS + 2 * BN * 4;  // (the columns' biases behind the rings, of this tile and the next)
+    static_assert(BN % 64 == 0 || KG > 1, "64 biases at a time: those of 32 columns take the next tile's place, of which there is none where K is shared");
     static_assert((KG - 1) * BM * BN * 4 <= BIAS, "the groups' sums fit where the stages were");
     static constexpr int PIECES = PANELS * 4;             // KiB of values
     static constexpr int DATA_LOADS = PIECES / NW, SCALE_LOADS = ((PANELS + 3) / 4 + NW - 1) / NW, LOADS = DATA_LOADS + SCALE_LOADS;
@@ -352,7 +353,7 @@ __global__ __launch_bounds__(WGM * WGN * KG * 64) __attribute__((amdgpu_waves_pe
     auto start = [&](int parity) __attribute__((always_inline)) {
         if (biased && group == 0) {
 #pragma unroll
-            for (int b = 0; b < (T::BN / 64 + NW - 1) / NW; b++) {
+            for (int b = 0; b < ((T::BN + 63) / 64 + NW - 1) / NW; b++) {
                 const int part = b * NW + wave;
                 if (part * 64 < T::BN) {
                     const int n = panel_n0 * 32 + part * 64 + lane;
@@ -604,30 +605,34 @@ static int launch_rows(const Mxfp4Gemm& g, hipStream_t st, const char* name) {
 bool mx_takes_bf16(int M, int K) { return M <= 8 && (int64_t)M * K <= 16384; }
 
 // Which tile: the least of rounds * (fixed + chunks of 256 k * stage), a round being as many tiles as fit on the chip; one that is not full leaves each of its tiles more of the chip, down to `least` of
-// the time.  The constants are fitted to 65 products of 33 to 4096 rows, 256 to 11008 k and 256 to 22016 columns in every tile, each by how near it comes to the fastest; the tile chosen was 0.5 % behind
-// that on average (of those that a pair has 0.2 %), 10 % at most.  us at 2048 x 4096 x 11008 / 4096 x 4096 x 4096 / 1024 x 11008 x 4096 / 256 x 4096 x 4096 / 64 x 11008 x 4096:
+// the time.  The constants are fitted to 86 products of 33 to 4096 rows, 256 to 11008 k and 256 to 32000 columns in every tile, each by how near it comes to the fastest; the tile chosen was 0.5 % behind
+// that on average, 10 % at most.  us at 2048 x 4096 x 11008 / 4096 x 4096 x 4096 / 1024 x 11008 x 4096 / 256 x 4096 x 4096 / 64 x 11008 x 4096:
 //     256 x 256            64 / 39 / 57 / 25 / 52
 //     256 x 192            57 / 55 / 46 / 21 / 42
 //     128 x 256            61 / 45 / 36 / 16 / 30
 //     128 x 128            63 / 47 / 36 / 15 / 33
-//     128 x 128, K shared  @1
-//      64 x 128, K shared  @2
+//     128 x 128, K by two  77 / 53 / 31 / 13 / 24
+//      64 x 128, K by two  87 / 67 / 39 / 9.2 / 15
 //      64 x 64             93 / 70 / 44 / 8.1 / 14
-//      64 x 64, K shared  115 / 85 / 46 / 7.3 / 12
-// (64 x 128 without sharing, 73 / 54 / 33 / 10 / 19, a 192 x 256 for pairs and a 64 x 64 of their own came out first too rarely to be kept.)
+//      64 x 64, K by two  115 / 85 / 46 / 7.4 / 12
+//      32 x 64, K by four   - / - / - / 10.5 / 9.3
+//      32 x 32, K by eight  - / - / - / 15.4 / 9.0
+// (64 x 128 with K whole, 73 / 54 / 33 / 10 / 19, a 192 x 256 for pairs and a 64 x 64 of their own came out first too rarely to be kept; without the last two here the mean was 4 % behind.)
 struct TileCost {
     int bm, bn, per_cu;
     float fixed_us, stage_us, least;
+    bool pair;  // (a wavefront of a pair has as many gate panels as up panels)
 };
-enum { T_256_256, T_256_192, T_128_256, T_128_128, T_128_128_SHARED, T_64_128_SHARED, T_64_64, T_64_64_SHARED, TILES };
-static constexpr TileCost COSTS[TILES] = {{256, 256, 1, 10.5f, 1.69f, 0.62f}, {256, 192, 1, 8.4f, 1.34f, 0.63f}, {128, 256, 1, 7.5f, 0.88f, 0.68f}, {128, 128, 2, 6.3f, 1.0f, 0.62f},
-                                          {128, 128, 1, 5.9f, 0.53f, 0.81f},  {64, 128, 1, 4.7f, 0.294f, 0.88f}, {64, 64, 2, 4.0f, 0.336f, 0.8f}, {64, 64, 1, 3.8f, 0.189f, 0.95f}};
+enum { T_256_256, T_256_192, T_128_256, T_128_128, T_128_128_BY_2, T_64_128_BY_2, T_64_64, T_64_64_BY_2, T_32_64_BY_4, T_32_32_BY_8, TILES };
+static constexpr TileCost COSTS[TILES] = {{256, 256, 1, 10.3f, 1.70f, 0.62f, true}, {256, 192, 1, 8.4f, 1.32f, 0.64f, false}, {128, 256, 1, 7.5f, 0.90f, 0.67f, true},  {128, 128, 2, 6.3f, 1.01f, 0.63f, true},
+                                          {128, 128, 1, 5.9f, 0.546f, 0.81f, true}, {64, 128, 1, 4.9f, 0.30f, 0.85f, true},  {64, 64, 2, 4.04f, 0.347f, 0.79f, false}, {64, 64, 1, 3.8f, 0.192f, 0.95f, true},
+                                          {32, 64, 1, 3.55f, 0.133f, 0.94f, false}, {32, 32, 1, 3.57f, 0.10f, 0.92f, false}};
 
 static int choose_tile(const Mxfp4Gemm& g) {
     int best = -1;
     double fastest = 0;
     for (int i = 0; i < TILES; i++) {
-        if (g.pair && (i == T_256_192 || i == T_64_64)) continue;  // (a wavefront of a pair has as many gate panels as up panels)
+        if (g.pair && !COSTS[i].pair) continue;
         const TileCost& t = COSTS[i];
         const int64_t tiles = (int64_t)((g.M + t.bm - 1) / t.bm) * (((int64_t)g.npanels * 32 + t.bn - 1) / t.bn), at_once = (int64_t)num_cus() * t.per_cu;
         const double full = (double)(tiles / at_once), rest = (double)(tiles % at_once) / at_once;
@@ -649,10 +654,12 @@ int launch_gemm_mxfp4(const Mxfp4Gemm& g, hipStream_t st) {
     case T_256_192: return launch_tile<2, 3, 4, 2, 2>(g, st, "mxfp4_256x192");
     case T_128_256: return launch_tile<2, 2, 2, 4, 3>(g, st, "mxfp4_128x256");
     case T_128_128: return launch_tile<2, 2, 2, 2, 2>(g, st, "mxfp4_128x128");
-    case T_128_128_SHARED: return launch_tile<2, 2, 2, 2, 2, 2>(g, st, "mxfp4_128x128_shared_k");
-    case T_64_128_SHARED: return launch_tile<1, 2, 2, 2, 3, 2>(g, st, "mxfp4_64x128_shared_k");
+    case T_128_128_BY_2: return launch_tile<2, 2, 2, 2, 2, 2>(g, st, "mxfp4_128x128_k_by_2");
+    case T_64_128_BY_2: return launch_tile<1, 2, 2, 2, 3, 2>(g, st, "mxfp4_64x128_k_by_2");
     case T_64_64: return launch_tile<1, 1, 2, 2, 4>(g, st, "mxfp4_64x64");
-    default: return g.pair ? launch_tile<1, 2, 2, 1, 3, 2>(g, st, "mxfp4_64x64_shared_k_pair") : launch_tile<1, 1, 2, 2, 3, 2>(g, st, "mxfp4_64x64_shared_k");
+    case T_64_64_BY_2: return g.pair ? launch_tile<1, 2, 2, 1, 3, 2>(g, st, "mxfp4_64x64_k_by_2_pair") : launch_tile<1, 1, 2, 2, 3, 2>(g, st, "mxfp4_64x64_k_by_2");
+    case T_32_64_BY_4: return launch_tile<1, 1, 1, 2, 3, 4>(g, st, "mxfp4_32x64_k_by_4");
+    default: return launch_tile<1, 1, 1, 1, 2, 8>(g, st, "mxfp4_32x32_k_by_8");
     }
 }
 

@@ -444,10 +444,10 @@ def test_refusals_on_the_gpu():
 
 @pytest.mark.parametrize("M,K,N,pair,kernel", [
     (4096, 300, 4090, False, "256x256"), (582, 110, 19008, True, "256x256"), (2048, 4096, 5900, False, "256x192"), (700, 520, 21952, True, "128x128"), (1030, 10900, 4090, False, "128x256"),
-    (264, 4159, 14528, True, "128x256"), (223, 103, 17257, False, "128x128"), (900, 400, 8192, True, "128x128"), (700, 1000, 4001, False, "128x128_shared_k"),
-    (513, 1000, 4032, True, "128x128_shared_k"), (68, 5225, 15139, False, "64x128_shared_k"), (73, 127, 9216, True, "64x128_shared_k"), (300, 2950, 5056, True, "64x128_shared_k"),
-    (391, 1001, 3001, False, "64x64"), (300, 260, 3008, True, "64x64_shared_k_pair"), (65, 3100, 705, False, "64x64_shared_k"), (33, 2950, 130, False, "64x64_shared_k"),
-    (33, 3100, 704, True, "64x64_shared_k_pair"), (70, 2950, 128, True, "64x64_shared_k_pair"), (33, 100, 70, False, "64x64"), (20, 300, 9000, False, "rows_32"), (31, 515, 70, False, "rows_32"),
+    (264, 4159, 14528, True, "128x256"), (223, 103, 17257, False, "128x128"), (900, 400, 8192, True, "128x128"), (700, 1000, 4001, False, "128x128_k_by_2"),
+    (513, 1000, 4032, True, "128x128_k_by_2"), (68, 5225, 15139, False, "64x128_k_by_2"), (73, 127, 9216, True, "64x128_k_by_2"), (300, 2950, 5056, True, "64x128_k_by_2"),
+    (391, 1001, 3001, False, "64x64"), (300, 260, 3008, True, "64x64_k_by_2_pair"), (65, 3100, 705, False, "32x32_k_by_8"), (33, 2950, 130, False, "32x32_k_by_8"), (35, 349, 13318, False, "64x64_k_by_2"),
+    (33, 3100, 704, True, "64x64_k_by_2_pair"), (70, 2950, 128, True, "64x64_k_by_2_pair"), (33, 100, 70, False, "32x32_k_by_8"), (65, 1300, 2050, False, "32x32_k_by_8"), (65, 128, 1537, False, "32x64_k_by_4"), (100, 2600, 4001, False, "32x64_k_by_4"), (20, 300, 9000, False, "rows_32"), (31, 515, 70, False, "rows_32"),
     (17, 300, 640, True, "rows_32_pair"), (16, 1000, 65, False, "rows_16"), (9, 5000, 192, True, "rows_16_pair"), (3, 1000, 190, False, "rows_16"), (3, 1000, 192, True, "rows_16_pair")])
 def test_every_kernel_that_products_choose(M, K, N, pair, kernel):
     """Sizes with rows, k and columns left over, an even and an odd number of chunks of k, one band of eight rows of tiles and more.  N: packed columns."""
@@ -470,6 +470,11 @@ def test_every_kernel_that_products_choose(M, K, N, pair, kernel):
             want, bound = (t.cpu().numpy() for t in product(w[0]))
         u.close(y, want, bound, dtype, kernel)
         assert (wide[:, n:] == 9.0).all()
+        if dtype == torch.float32 and not pair:  # (one addition more)
+            b = normal((N,), 5, 1.0, torch.float32)
+            biased = torch.empty((M, N), device="cuda")
+            mx.gemm_mxfp4(rows, packed, N, mx.Epilogue(biased, mx.PP_BIAS, bias=b))
+            assert torch.equal(biased, y + b)
 
 
 @pytest.mark.parametrize("M,K,N", [(40, 640, 288), (300, 512, 1056), (700, 520, 10976), (1030, 5000, 4000), (900, 400, 4096), (264, 4159, 7264), (700, 1000, 2016), (130, 1000, 4096)])

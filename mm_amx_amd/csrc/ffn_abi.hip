@@ -148,7 +148,7 @@ static int check_codes(const char* who, const void* q, int64_t ldq, const void* 
 }
 // A packed: as given, or made in scratch; or as bf16 rows that the product quantises itself
 static int packed_rows(int dtype, const void* A, int64_t lda, int M, int K, void* scratch, Mxfp4Gemm* g, hipStream_t st) {
-    g->a_bf16 = dtype == MMX_BF16 && mx_takes_bf16(M, K);
+    g->a_bf16 = dtype == MMX_BF16 && mx_takes_bf16(M, K, g->N, g->pair);
     g->A = static_cast<const char*>(A);
     g->lda = g->a_bf16 ? lda : mx_bytes(32, K);
     if (dtype == MMX_F4 || g->a_bf16) return MMX_OK;
@@ -398,7 +398,7 @@ int mmx_dequantize_mxfp4(const void* packed, int M, int K, int y_dtype, void* y,
 }
 
 size_t mmx_gemm_mxfp4_scratch_bytes(int a_dtype, int M, int K, int N) {
-    if (M <= 0 || K <= 0 || N <= 0 || (a_dtype != MMX_BF16 && a_dtype != MMX_F32) || (a_dtype == MMX_BF16 && mx_takes_bf16(M, K))) return 0;
+    if (M <= 0 || K <= 0 || N <= 0 || (a_dtype != MMX_BF16 && a_dtype != MMX_F32) || (a_dtype == MMX_BF16 && mx_takes_bf16(M, K, N, false))) return 0;  // (then a pair takes them too)
     return round256((size_t)mx_bytes(M, K));
 }
 

@@ -46,7 +46,7 @@ __device__ __forceinline__ int64_t mx_scale_at(int row, int64_t kb) {
     return (kb >> 3) * MX_CHUNK_BYTES + MX_SCALES_AT + (((int)kb & 1) * 32 + (row & 31)) * 4 + (((int)kb & 7) >> 1);
 }
 
-// What a product is made of.  A and B in the layout above; or, where mx_takes_bf16(M, K), A rows of K bf16 that lie anywhere, lda bytes apart.
+// What a product is made of.  A and B in the layout above; or, where mx_takes_bf16(), A rows of K bf16 that lie anywhere, lda bytes apart.
 struct Mxfp4Gemm {
     const char* A;
     int64_t lda;       // bytes of a 32-row panel of A, or of a row of bf16
@@ -61,6 +61,6 @@ struct Mxfp4Gemm {
     Epilogue ep;
 };
 
-bool mx_takes_bf16(int M, int K);
+bool mx_takes_bf16(int M, int K, int N, bool pair);
 
 }  // namespace mmx

@@ -8,7 +8,6 @@ namespace mmx {
 
 int num_cus();
 
-
 __device__ __forceinline__ i32x8 mx_operand(u32x4 a) { return i32x8{(int)a[0], (int)a[1], (int)a[2], (int)a[3], 0, 0, 0, 0}; }
 
 // ---- few rows: every wavefront multiplies its own chunks of k --------------------------------------------------------------
@@ -16,6 +15,8 @@ __device__ __forceinline__ i32x8 mx_operand(u32x4 a) { return i32x8{(int)a[0], (
 // wavefronts.  The 16 x 16 x 128 form of the instruction (half the rate of the other, which does not matter here) lets a workgroup have half a panel.
 // PAIR: the four column tiles are both halves of a gate panel and of its up panel, 32 columns of the result, a whole block of it.
 // QUANTIZE: A is bf16 rows, which every workgroup quantises into LDS while its first weights are on their way.
+// Bound: HBM, at M = 1 the launch too.  1 x 4096 x 11008 6.4 us from bf16 rows (3.8 TB/s of weights; a quantiser of its own in front costs 4 us more), 16 x 4096 x 22016 as a pair 10.3,
+// 24 x 11008 x 4096 6.9 (16 rows a workgroup 7.9, 64 8.0, 32 columns 8.5).
 template <int MT, int NT, bool PAIR, bool QUANTIZE>
 __global__ __launch_bounds__(512) void mxfp4_rows_kernel(const Mxfp4Gemm g) {
     static_assert(!PAIR || NT == 4, "both halves of a gate and an up panel");
@@ -207,6 +208,9 @@ __global__ __launch_bounds__(512) void mxfp4_rows_kernel(const Mxfp4Gemm g) {
 // then their 256 bytes of scales, straight from memory into one of R slots of LDS; with the operands in the instruction's own order every LDS read is a KiB in a row.  A stage has four steps of 64 k;
 // the operands of a step are read during the one before.  The one barrier per stage stands in front of its last step: all of it has been read into registers then, so its slot is free for
 // stage t + R, whose loads are spread over the last step and the next stage's first two, and stage t + 1 has landed.
+// Bound: what a CU gets from L2 into LDS (48 to 65 bytes a nanosecond) and the LDS itself, whose reads and writes a step of the 256 x 192 tile take as long as its MFMAs; 2048 x 4096 x 11008
+// comes to 3250 TFLOP/s, 4096 x 4096 x 4096 to 3500, where the MFMAs alone reach 6670 on random values.  Refilling slots by halves, with loads R - 1 stages ahead, was no faster (57 -> 60 us),
+// nor were 4 x 3 panels a wavefront with a third fewer LDS reads and one wavefront a SIMD (59).
 // KG groups of wavefronts, each with a ring of its own, take the chunks in turn where there are fewer tiles than CUs; their sums are added in LDS, in order.
 template <int PM, int PN, int WGM, int WGN, int R, int KG>
 struct Mxfp4Tile {
@@ -275,7 +279,7 @@ __global__ __launch_bounds__(WGM * WGN * KG * 64) __attribute__((amdgpu_waves_pe
     using lds_u32 = __attribute__((address_space(3))) const uint32_t;
     extern __shared__ __attribute__((aligned(1024))) char smem[];
     // Neighbouring workgroups go to different XCDs: each XCD gets a run of tiles, eight rows of them at a time and those fastest, so that the ones it works on share both operands in its L2.
-    // A workgroup takes every stride-th tile of its XCD's run; the next one's first stages are on their way while its results are stored.
+    // A workgroup takes every stride-th tile of its XCD's run; the next one's first stages are on their way while its results are stored (2048 x 4096 x 11008 with a bias 62.5 -> 55 us).
     const int first = (blockIdx.x & 7) * per_xcd, stride = gridDim.x >> 3;
     int turn = blockIdx.x >> 3;
     if (first + turn >= total) return;
@@ -601,8 +605,10 @@ static int launch_rows(const Mxfp4Gemm& g, hipStream_t st, const char* name) {
     return check_hip(hipGetLastError(), "mxfp4_rows_kernel launch");
 }
 
-// Whether the kernel for few rows quantises bf16 rows on the way
-bool mx_takes_bf16(int M, int K) { return M <= 8 && (int64_t)M * K <= 16384; }
+// Whether the kernel for few rows quantises bf16 rows on the way.  That saves a launch, 2.6 us, and costs (0.3 + workgroups / 1540) us for every 4096 values (a CU's workgroups do it again and again).
+// On the way / by the quantiser, us: M 1, 2, 4, 8 x 4096 x 4096 4.3, 4.8, 5.6, 7.5 / 6.4; x 4096 x 11008 6.5, 7.4, 9.1, 12.9 / 8.6; x 4096 x 32000 13.1, 14.4, 17.5, 25.7 / 15.3.
+// (A pair has fewer workgroups: where the plain product takes the rows, so does the pair.)
+bool mx_takes_bf16(int M, int K, int N, bool pair) { return M <= 8 && (int64_t)M * K * (N / (pair ? 64 : 16) + 460) <= 16400000; }
 
 // Which tile: the least of rounds * (fixed + chunks of 256 k * stage), a round being as many tiles as fit on the chip; one that is not full leaves each of its tiles more of the chip, down to `least` of
 // the time.  The constants are fitted to 86 products of 33 to 4096 rows, 256 to 11008 k and 256 to 32000 columns in every tile, each by how near it comes to the fastest; the tile chosen was 0.5 % behind

@@ -11,6 +11,9 @@
 // Four kernels.  A workgroup for each slice of a row reads the logits: segments' maxima; without filters their sums too; with top_k or top_p a histogram of the slice, counts and weights by
 // l / T in steps of 1 / 16, on one grid for the row.  With filters a workgroup a row adds the histograms up, which shows the bin in which the run ends.  Workgroups of four segments collect what lies in it
 // and above; or, where that is more than a list holds, what lies in it, and the segments' sums of what lies above.  A workgroup a row sorts out from the list where the run ends, and draws.
+// Bound: the launches and the steps that wait for each other in them (barriers, LDS, a dependent read), each kernel 5 us at the least; HBM only for many rows without filters, where the one pass over
+// 256 x 131072 fp32 takes 35 us, 3.8 TB/s, of 41.  us, slices / cut / filter / draw: 1 x 32000 fp32, top_k and top_p 5.4 / 4.0 / 4.4 / 9.4; 33 x 100003 fp32, top_p 9.4 / 4.9 / 12 / 13.7;
+// 64 x 131072 bf16, a mixture 13.0 / 5.1 / 10.2 / 17.4.  (One kernel, a workgroup a row that passes over it again and again: 130, 349 and 589 us for these three.)
 // Rows that this does not suit (more than a list of equal or nearly equal logits in the last bin, 2^26 bins and more) are worked on by that one workgroup alone, a pass over the row for every eight bits of the key.
 #include "sample.hpp"
 
@@ -128,20 +131,61 @@ struct Lane16 {
     }
 };
 
+// Neighbours' values within a wavefront, by the register file's own paths (through LDS, as a general exchange goes, a sum of 64-bit values over a wavefront and its workgroup took 1.7 us in place of 0.9).
+// A lane that has no such neighbour gets `none`.
+template <int CTRL, int ROWS, typename T>
+__device__ __forceinline__ T neighbour(T none, T v) {
+    if constexpr (sizeof(T) == 4) {
+        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, none), __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
+    } else {
+        const uint64_t n = __builtin_bit_cast(uint64_t, none), x = __builtin_bit_cast(uint64_t, v);
+        const uint32_t low = (uint32_t)__builtin_amdgcn_update_dpp((int)(uint32_t)n, (int)(uint32_t)x, CTRL, ROWS, 0xf, false);
+        const uint32_t high = (uint32_t)__builtin_amdgcn_update_dpp((int)(n >> 32), (int)(x >> 32), CTRL, ROWS, 0xf, false);
+        return __builtin_bit_cast(T, (uint64_t)high << 32 | low);
+    }
+}
+constexpr int SHR_1 = 0x111, SHR_2 = 0x112, SHR_4 = 0x114, SHR_8 = 0x118, ROW_TO_NEXT = 0x142, HALF_TO_NEXT = 0x143;  // (rows of 16 lanes; a row's last lane to the next row, lane 31 to the upper half)
+constexpr int XOR_1 = 0xb1, XOR_2 = 0x4e, MIRROR_8 = 0x141;
+// a lane's value, for all
 template <typename T>
-__device__ __forceinline__ T wave_sum(T v) {
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) v += __shfl_xor(v, d);
+__device__ __forceinline__ T of_lane(T v, int lane) {
+    if constexpr (sizeof(T) == 4) {
+        return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+    } else {
+        const uint64_t x = __builtin_bit_cast(uint64_t, v);
+        const uint32_t low = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x, lane), high = (uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), lane);
+        return __builtin_bit_cast(T, (uint64_t)high << 32 | low);
+    }
+}
+// the sum over the lanes up to this one
+template <typename T>
+__device__ __forceinline__ T wave_scan(T v) {
+    const T zero = 0;
+    v += neighbour<SHR_1, 0xf>(zero, v);
+    v += neighbour<SHR_2, 0xf>(zero, v);
+    v += neighbour<SHR_4, 0xf>(zero, v);
+    v += neighbour<SHR_8, 0xf>(zero, v);
+    v += neighbour<ROW_TO_NEXT, 0xa>(zero, v);
+    v += neighbour<HALF_TO_NEXT, 0xc>(zero, v);
     return v;
 }
 template <typename T>
+__device__ __forceinline__ T wave_sum(T v) {
+    return of_lane(wave_scan(v), 63);
+}
+template <typename T>
+__device__ __forceinline__ T larger(T a, T b) {
+    return a > b ? a : b;
+}
+template <typename T>
 __device__ __forceinline__ T wave_max(T v) {
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) {
-        const T o = __shfl_xor(v, d);
-        v = o > v ? o : v;
-    }
-    return v;
+    v = larger(v, neighbour<SHR_1, 0xf>(v, v));
+    v = larger(v, neighbour<SHR_2, 0xf>(v, v));
+    v = larger(v, neighbour<SHR_4, 0xf>(v, v));
+    v = larger(v, neighbour<SHR_8, 0xf>(v, v));
+    v = larger(v, neighbour<ROW_TO_NEXT, 0xa>(v, v));
+    v = larger(v, neighbour<HALF_TO_NEXT, 0xc>(v, v));
+    return of_lane(v, 63);
 }
 
 constexpr int NW = 16, THREADS = NW * 64;
@@ -227,12 +271,7 @@ struct Shared {
 template <int WAVES = NW>
 __device__ __forceinline__ double scan_before(double v, double* part, double* all) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    double run = v;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const double o = __shfl_up(run, d);
-        if (lane >= d) run += o;
-    }
+    const double run = wave_scan(v);
     __syncthreads();
     if (lane == 63) part[wave] = run;
     __syncthreads();
@@ -412,7 +451,7 @@ __global__ __launch_bounds__(SLICE * 64) __attribute__((amdgpu_waves_per_eu(8, 8
             if (!enough && run >= (double)r.k) enough = true, at = threadIdx.x * EACH + i;
         }
         const uint64_t m = __ballot(enough && threadIdx.x * EACH < BINS);
-        const uint32_t first = __shfl(at, m ? __builtin_ctzll(m) : 0);
+        const uint32_t first = of_lane(at, m ? __builtin_ctzll(m) : 0);
         if (m && lane == 0) atomicMin(&last, first);
         __syncthreads();
         until = (int)last + 1;
@@ -515,14 +554,8 @@ __global__ __launch_bounds__(BINS) void sample_cut_kernel(const SampleArgs a) {
         }
     }
     const double mass = r.top_k ? 0.0 : (double)masses / FACTOR_SCALE * exp_of((bin - b - at0) * (1.0 / PER_UNIT));
-    double run_mass = mass;
-    uint32_t run_count = count;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const double o = __shfl_up(run_mass, d);
-        const uint32_t c = __shfl_up(run_count, d);
-        if (lane >= d) run_mass += o, run_count += c;
-    }
+    double run_mass = wave_scan(mass);
+    uint32_t run_count = wave_scan(count);
     if (lane == 63) part[0][wave] = run_mass, part[1][wave] = run_count;
     __syncthreads();
     double all_mass = 0;
@@ -609,13 +642,8 @@ __global__ __launch_bounds__(256) void sample_filter_kernel(const SampleArgs a) 
 #pragma unroll
         for (int e = 0; e < 16; e++) takes |= x.v[e] >= state.from && x.v[e] < state.to ? 1u << e : 0;
     }
-    uint32_t at = __popc(takes);
-    const uint32_t mine = at;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t o = __shfl_up(at, d);
-        if (lane >= d) at += o;
-    }
+    const uint32_t mine = __popc(takes);
+    uint32_t at = wave_scan(mine);
     if (lane == 63) taken[wave] = at;
     __syncthreads();
     uint32_t every = 0, before = 0;
@@ -670,12 +698,7 @@ __device__ __forceinline__ unsigned long long pick(const unsigned long long (&c)
                 lo = c[i] < lo ? c[i] : lo;
                 hi = c[i] > hi ? c[i] : hi;
             }
-        uint32_t at = here;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const uint32_t v = __shfl_up(at, d);
-            if (lane >= d) at += v;
-        }
+        const uint32_t at = wave_scan(here);
         __syncthreads();  // (what the last round left has been read)
         if (lane == 63) o.cpart[wave] = at;
         if (threadIdx.x == 0) o.low = ~0ull, o.high = 0, o.best = 0, o.first = BUCKETS, o.last = 0;
@@ -714,12 +737,7 @@ __device__ __forceinline__ unsigned long long pick(const unsigned long long (&c)
         __syncthreads();
         const bool some = o.count[threadIdx.x] > 0;
         const unsigned long long mine = mode == BY_COUNT ? o.count[threadIdx.x] : o.mass[threadIdx.x];
-        unsigned long long run = mine;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const unsigned long long v = __shfl_up(run, d);
-            if (lane >= d) run += v;
-        }
+        unsigned long long run = wave_scan(mine);
         if (lane == 63) o.part[wave] = run;
         __syncthreads();
 #pragma unroll
@@ -748,8 +766,9 @@ __device__ __forceinline__ unsigned long long pick(const unsigned long long (&c)
             run += other >= mine ? o.few_mass[j] : 0ull;
             after += other < mine && other != 0 ? 1 : 0;
         }
-#pragma unroll
-        for (int d = 1; d < 8; d *= 2) run += __shfl_xor(run, d), after += __shfl_xor(after, d);
+        run += neighbour<XOR_1, 0xf>(0ull, run), after += neighbour<XOR_1, 0xf>(0u, after);
+        run += neighbour<XOR_2, 0xf>(0ull, run), after += neighbour<XOR_2, 0xf>(0u, after);
+        run += neighbour<MIRROR_8, 0xf>(0ull, run), after += neighbour<MIRROR_8, 0xf>(0u, after);  // (fours are alike by now)
         run += before;
         if (mine && (threadIdx.x & 7) == 0) {
             const unsigned long long less = run - o.few_mass[i];
@@ -945,7 +964,7 @@ __global__ __launch_bounds__(THREADS) void sample_draw_kernel(const SampleArgs a
     }
     {
         const uint64_t m = __ballot(here >= 0), any = __ballot(last >= 0);
-        const int first = __shfl(here, m ? __builtin_ctzll(m) : 0), end = __shfl(last, any ? 63 - __builtin_clzll(any) : 0);
+        const int first = of_lane(here, m ? __builtin_ctzll(m) : 0), end = of_lane(last, any ? 63 - __builtin_clzll(any) : 0);
         if (lane == 0) {
             if (m) atomicMin(&s.pick, first);
             if (any) atomicMax(&s.bin, (uint32_t)end);
@@ -969,7 +988,7 @@ __global__ __launch_bounds__(THREADS) void sample_draw_kernel(const SampleArgs a
     if (threadIdx.x == 0) a.ids[row_at] = seg * SEG + (int)(s.found != 0xffffffffu ? s.found : s.bin);
 }
 
-// Segments of a slice: 4 where 16 would leave most of the chip idle
+// Segments of a slice: 4 where 16 would leave most of the chip idle (1 x 32000: 8 workgroups in place of 2); 16 elsewhere, since every slice's histogram is written and read
 int sample_slice(int B, int V) {
     const int64_t segs = ((int64_t)V + SEG - 1) / SEG;
     return B * ((segs + 15) / 16) < 64 && segs <= 4 * MOST_SLICES ? 4 : 16;

@@ -58,6 +58,20 @@ __device__ __forceinline__ uint32_t key_of(float x) {
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 __device__ __forceinline__ float of_key(uint32_t k) { return u2f(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
+// A list's entry: the key, of bf16 without the half that they have in common, above as many bits as V has of the complement of the index.  So entries are ordered like the tokens, none is 0, and equal
+// or neighbouring keys lie as close as their indexes allow, which is what a search by ranges goes by (with the index in 32 bits below 32 of key, bf16's equal logits all fell into one bucket's counter).
+template <typename TL>
+__device__ __forceinline__ unsigned long long entry_of(float x, int i, int V) {
+    const int bits = 32 - __clz(V);
+    return (unsigned long long)(key_of(x) >> (sizeof(TL) == 2 ? 16 : 0)) << bits | ((1u << bits) - 1u - (uint32_t)i);
+}
+__device__ __forceinline__ unsigned long long order_of(unsigned long long c, int V) { return c & ((1u << (32 - __clz(V))) - 1u); }  // (falls where the index rises; 1 at the least)
+__device__ __forceinline__ int index_of(unsigned long long c, int V) { return (int)((1u << (32 - __clz(V))) - 1u - (uint32_t)order_of(c, V)); }
+template <typename TL>
+__device__ __forceinline__ uint32_t key_in(unsigned long long c, int V) {
+    const uint32_t k = (uint32_t)(c >> (32 - __clz(V)));
+    return sizeof(TL) == 2 ? k << 16 | (k & 0x8000u ? 0u : 0xffffu) : k;
+}
 __device__ __forceinline__ float settled(float x) { return x != x ? NEVER : x + 0.0f; }
 
 // 2^y for y <= 0: 2^n times the series of 2^f = e^(f ln 2) to its tenth power, |f| <= 1 / 2, whose rest is (ln 2 / 2)^11 / 11! = 2e-13.  n comes out of adding a number so large that
@@ -188,6 +202,22 @@ __device__ __forceinline__ T wave_max(T v) {
     return of_lane(v, 63);
 }
 
+// Of a number from each of up to sixteen wavefronts: what those before this one come to, and all of them.  (A lane reads one number; every lane reading all sixteen kept the LDS busy for half a
+// microsecond.)
+template <int WAVES, typename T>
+__device__ __forceinline__ T of_waves(const T* part, T* all) {
+    static_assert(WAVES <= 16, "a row of lanes");
+    const int at = threadIdx.x & 15, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const T zero = 0;
+    T v = at < WAVES ? part[at] : zero;
+    v += neighbour<SHR_1, 0xf>(zero, v);
+    v += neighbour<SHR_2, 0xf>(zero, v);
+    v += neighbour<SHR_4, 0xf>(zero, v);
+    v += neighbour<SHR_8, 0xf>(zero, v);
+    *all = of_lane(v, 15);
+    return wave > 0 ? of_lane(v, wave - 1) : zero;
+}
+
 constexpr int NW = 16, THREADS = NW * 64;
 
 struct Cut {       // what stays: keys above, and of the equal ones indexes up to `index`
@@ -275,14 +305,7 @@ __device__ __forceinline__ double scan_before(double v, double* part, double* al
     __syncthreads();
     if (lane == 63) part[wave] = run;
     __syncthreads();
-    double before = 0, total = 0;
-#pragma unroll
-    for (int w = 0; w < WAVES; w++) {
-        before += w < wave ? part[w] : 0.0;
-        total += part[w];
-    }
-    *all = total;
-    return before + run - v;
+    return of_waves<WAVES>(part, all) + run - v;
 }
 
 // The cut that keeps the first `want_count` of what `limit` holds (by_mass: the shortest run of it that holds `want_mass`): its key by eight bits at a time from the top, over the whole row each time,
@@ -558,13 +581,9 @@ __global__ __launch_bounds__(BINS) void sample_cut_kernel(const SampleArgs a) {
     uint32_t run_count = wave_scan(count);
     if (lane == 63) part[0][wave] = run_mass, part[1][wave] = run_count;
     __syncthreads();
-    double all_mass = 0;
-#pragma unroll
-    for (int w = 0; w < WAVES; w++) {
-        run_mass += w < wave ? part[0][w] : 0.0;
-        run_count += w < wave ? (uint32_t)part[1][w] : 0u;
-        all_mass += part[0][w];
-    }
+    double all_mass, counted;
+    run_mass += of_waves<WAVES>(part[0], &all_mass);
+    run_count += (uint32_t)of_waves<WAVES>(part[1], &counted);
     if (b == BINS - 1) count = all_count - run_count, run_count = all_count;
     // of top_k the first whose count is enough, of top_p alone the first whose mass is (of both: top_p's share is of what top_k leaves, which only the list tells)
     first_of(r.top_k ? run_count >= (uint32_t)r.k : run_mass >= r.p * all_mass, &found);
@@ -659,7 +678,7 @@ __global__ __launch_bounds__(256) void sample_filter_kernel(const SampleArgs a) 
 #pragma unroll
     for (int e = 0; e < 16; e++)
         if (takes >> e & 1) {
-            if (at < LIST) sc.list[at] = (unsigned long long)key_of(x.v[e]) << 32 | (0xffffffffu - (uint32_t)(g * SEG + x.at(e)));
+            if (at < LIST) sc.list[at] = entry_of<TL>(x.v[e], g * SEG + x.at(e), a.V);
             at++;
         }
 }
@@ -669,7 +688,7 @@ constexpr int MINE = LIST / THREADS, BUCKETS = 1024, FEW = 128;
 struct Room {
     unsigned long long mass[BUCKETS];
     uint32_t count[BUCKETS];
-    unsigned long long few[FEW], few_mass[FEW];
+    __attribute__((aligned(16))) unsigned long long few[FEW][2];  // (with its mass)
     unsigned long long low, high, best, part[NW], before_mass;
     uint32_t cpart[NW], first, last;
 };
@@ -685,7 +704,7 @@ __device__ __forceinline__ unsigned long long pick(const unsigned long long (&c)
     int n = most;
     __syncthreads();  // (what an earlier call left has been read)
     if (most <= FEW) {
-        if ((int)threadIdx.x < most) o.few[threadIdx.x] = c[0], o.few_mass[threadIdx.x] = c[0] == 0 ? 0ull : mode == BY_COUNT ? 1ull : m[0];
+        if ((int)threadIdx.x < most) o.few[threadIdx.x][0] = c[0], o.few[threadIdx.x][1] = c[0] == 0 ? 0ull : mode == BY_COUNT ? 1ull : m[0];
         if (threadIdx.x == 0) o.best = 0, o.low = 0;
     }
     while (most > FEW) {
@@ -703,17 +722,13 @@ __device__ __forceinline__ unsigned long long pick(const unsigned long long (&c)
         if (lane == 63) o.cpart[wave] = at;
         if (threadIdx.x == 0) o.low = ~0ull, o.high = 0, o.best = 0, o.first = BUCKETS, o.last = 0;
         __syncthreads();
-        uint32_t off = at - here;
-        n = 0;
-#pragma unroll
-        for (int w = 0; w < NW; w++) {
-            off += w < wave ? o.cpart[w] : 0;
-            n += (int)o.cpart[w];
-        }
+        uint32_t every;
+        uint32_t off = of_waves<NW>(o.cpart, &every) + at - here;
+        n = (int)every;
         if (n <= FEW) {
 #pragma unroll
             for (int i = 0; i < MINE; i++)
-                if (i * THREADS < most && c[i] >= low && c[i] <= high) o.few[off] = c[i], o.few_mass[off++] = mode == BY_COUNT ? 1ull : m[i];
+                if (i * THREADS < most && c[i] >= low && c[i] <= high) o.few[off][0] = c[i], o.few[off++][1] = mode == BY_COUNT ? 1ull : m[i];
             break;
         }
         if (__any(here)) {
@@ -740,9 +755,8 @@ __device__ __forceinline__ unsigned long long pick(const unsigned long long (&c)
         unsigned long long run = wave_scan(mine);
         if (lane == 63) o.part[wave] = run;
         __syncthreads();
-#pragma unroll
-        for (int w = 0; w < NW; w++) run += w < wave ? o.part[w] : 0ull;
-        run += before;
+        unsigned long long every_mass;
+        run += of_waves<NW>(o.part, &every_mass) + before;
         first_of(some && (mode == BY_MASS_STRICT ? run > want : run >= want), &o.first);
         last_of(some, &o.last);
         __syncthreads();
@@ -758,12 +772,13 @@ __device__ __forceinline__ unsigned long long pick(const unsigned long long (&c)
     // Eight neighbouring threads an entry, each against every eighth of them.  The one that is sought is the only one that reaches the goal and does not without its own mass.
     if ((int)(threadIdx.x & ~63u) < n * 8) {
         const int i = threadIdx.x >> 3;
-        const unsigned long long mine = i < n ? o.few[i] : 0ull;
+        const unsigned long long mine = i < n ? o.few[i][0] : 0ull;
         unsigned long long run = 0;
         uint32_t after = 0;  // entries behind it
+#pragma unroll 4
         for (int j = threadIdx.x & 7; j < n; j += 8) {
-            const unsigned long long other = o.few[j];
-            run += other >= mine ? o.few_mass[j] : 0ull;
+            const unsigned long long other = o.few[j][0], mass = o.few[j][1];
+            run += other >= mine ? mass : 0ull;
             after += other < mine && other != 0 ? 1 : 0;
         }
         run += neighbour<XOR_1, 0xf>(0ull, run), after += neighbour<XOR_1, 0xf>(0u, after);
@@ -771,7 +786,7 @@ __device__ __forceinline__ unsigned long long pick(const unsigned long long (&c)
         run += neighbour<MIRROR_8, 0xf>(0ull, run), after += neighbour<MIRROR_8, 0xf>(0u, after);  // (fours are alike by now)
         run += before;
         if (mine && (threadIdx.x & 7) == 0) {
-            const unsigned long long less = run - o.few_mass[i];
+            const unsigned long long less = run - o.few[i][1];
             if (mode == BY_MASS_STRICT ? run > want && less <= want : run >= want && less < want) o.best = mine;
             if (after == 0) o.low = mine;
         }
@@ -784,10 +799,9 @@ __device__ unsigned long long sum_of(unsigned long long v, Room& o) {
     __syncthreads();
     if ((threadIdx.x & 63) == 0) o.part[threadIdx.x >> 6] = v;
     __syncthreads();
-    v = 0;
-#pragma unroll
-    for (int w = 0; w < NW; w++) v += o.part[w];
-    return v;
+    unsigned long long all;
+    of_waves<NW>(o.part, &all);
+    return all;
 }
 
 template <typename TL>
@@ -850,7 +864,7 @@ __global__ __launch_bounds__(THREADS) void sample_draw_kernel(const SampleArgs a
             }
             if (i > 0) c[i] = at < n ? sc.list[at] : 0;
             if (at >= n) c[i] = 0;
-            const float l = of_key((uint32_t)(c[i] >> 32));
+            const float l = of_key(key_in<TL>(c[i], V));
             if (!__any(c[i] != 0)) continue;
             const double w = c[i] ? weight_of(l, top, r.per) : 0.0;
             m[i] = whole(w, scale);
@@ -878,7 +892,7 @@ __global__ __launch_bounds__(THREADS) void sample_draw_kernel(const SampleArgs a
                     if (low_weight >> i & 1) c[i] = 0;
                     m[i] = c[i] ? m[i] : 0ull;
                     all += m[i];
-                    c[i] = (uint32_t)c[i];  // (the order of the vocabulary is that of falling complements of the index)
+                    c[i] = order_of(c[i], V);  // (the order of the vocabulary)
                 }
                 if (path == BY_SUMS) break;
                 all = sum_of(all, o);
@@ -893,7 +907,7 @@ __global__ __launch_bounds__(THREADS) void sample_draw_kernel(const SampleArgs a
             }
         }
         if (path == BY_LIST) {
-            if (threadIdx.x == 0) a.ids[row_at] = (int)(0xffffffffu - (uint32_t)last);
+            if (threadIdx.x == 0) a.ids[row_at] = index_of(last, V);
             return;
         }
         // what stays of the bin, to its segments' sums
@@ -901,8 +915,8 @@ __global__ __launch_bounds__(THREADS) void sample_draw_kernel(const SampleArgs a
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < MINE; i++)
-            if (c[i]) atomicAdd(&more[(0xffffffffu - (uint32_t)c[i]) / SEG], m[i]);
-        cut = Cut{(uint32_t)(last >> 32), (int)(0xffffffffu - (uint32_t)last)};
+            if (c[i]) atomicAdd(&more[index_of(c[i], V) / SEG], m[i]);
+        cut = Cut{key_in<TL>(last, V), index_of(last, V)};
         __syncthreads();
     } else if (path == ALONE) {
         if (r.top_k) cut = select(row, V, top, r.per, scale, cut, false, (uint32_t)r.k, 0ull, s);

@@ -14,7 +14,7 @@
 // Bound: the launches and the steps that wait for each other in them (barriers, LDS, a dependent read), each kernel 5 us at the least; HBM only for many rows without filters, where the one pass over
 // 256 x 131072 fp32 takes 35 us, 3.8 TB/s, of 41.  us, slices / cut / filter / draw: 1 x 32000 fp32, top_k and top_p 5.6 / 4.0 / 4.5 / 8.2; 33 x 100003 fp32, top_p 8.6 / 4.6 / 13 / 12;
 // 64 x 131072 bf16, a mixture 13.0 / 4.8 / 11 / 15.8.  (One kernel, a workgroup a row that passes over it again and again: 130, 349 and 589 us for these three.)
-// Rows that this does not suit (more than a list of equal or nearly equal logits in the last bin, 2^26 bins and more) are worked on by that one workgroup alone, a pass over the row for every eight bits of the key.
+// Rows that this does not suit (more than a list of equal logits in the last bin, or of what top_k leaves to top_p; 2^26 bins and more; more than 2^20 logits and a list) are worked on by that one workgroup alone, a pass over the row for every eight bits of the key.
 #include "sample.hpp"
 
 #include "ffn.hpp"
@@ -529,9 +529,15 @@ __device__ __forceinline__ float least_of(double at, double per) {
     return settled(of_key(k));
 }
 
-// the row's histogram, a bin a thread, and the bin in which the run ends
+// the row's histogram, a bin a thread, and the bin in which the run ends.  A bin of more than a list holds (flat rows of large vocabularies) is cut into PARTS of its own first, for which the workgroup
+// reads the row: 8 x 262144 fp32 of N(0, 1), top_p 0.9, 157 us in place of the 632 of one workgroup and the whole key.
+template <typename TL>
 __global__ __launch_bounds__(BINS) void sample_cut_kernel(const SampleArgs a) {
-    constexpr int WAVES = BINS / 64, AHEAD = 8;
+    constexpr int WAVES = BINS / 64, AHEAD = 8, PARTS = 2 * BINS;
+    __shared__ State shared;
+    __shared__ bool narrow;
+    __shared__ uint32_t counts[PARTS], cpart[WAVES], first_part, last_part;
+    __shared__ unsigned long long masses_of[PARTS], mpart[WAVES];
     __shared__ double part[2][WAVES];
     __shared__ int slice_ahead[MOST_SLICES];
     __shared__ float fpart[WAVES];
@@ -543,7 +549,7 @@ __global__ __launch_bounds__(BINS) void sample_cut_kernel(const SampleArgs a) {
     if (!r.filtered()) return;
     Slice own = {0.0, 0, 0};
     if (b < sc.n_slices) own = sc.slices[b];
-    if (b == 0) found = BINS, last_bin = 0, all_count = 0;
+    if (b == 0) found = BINS, last_bin = 0, all_count = 0, first_part = PARTS, last_part = 0;
     const float top = row_top<WAVES>(sc, first_top, fpart);
     if (top == NEVER) {
         if (b == 0) sc.state->path = ALONE;
@@ -590,15 +596,94 @@ __global__ __launch_bounds__(BINS) void sample_cut_kernel(const SampleArgs a) {
     last_of(count > 0, &last_bin);
     __syncthreads();
     const int cut = found < BINS ? (int)found : (int)last_bin;  // (none: fewer tokens than top_k, or sums that were rounded)
-    if (b != cut) return;
-    State s;
-    s.entries = 0, s.before_count = run_count - count, s.top = top, s.before_mass = run_mass - mass, s.mass = all_mass;
-    s.path = odd ? ALONE : run_count <= LIST ? BY_LIST : (r.top_k && r.top_p) || count > LIST || sc.segs > MOST_SUMS ? ALONE : BY_SUMS;
-    s.from = s.to = __builtin_huge_valf();
-    if (s.path != ALONE) {
-        s.from = cut == BINS - 1 ? of_key(key_of(NEVER) + 1) : least_of(bin - cut, per);
-        if (s.path == BY_SUMS && cut > 0) s.to = least_of(bin - cut + 1, per);
+    if (b == cut) {
+        State s;
+        s.entries = 0, s.before_count = run_count - count, s.top = top, s.before_mass = run_mass - mass, s.mass = all_mass;
+        s.path = odd ? ALONE : run_count <= LIST ? BY_LIST : (r.top_k && r.top_p) || sc.segs > MOST_SUMS || (count > LIST && cut == BINS - 1) ? ALONE : BY_SUMS;
+        s.from = s.to = __builtin_huge_valf();
+        if (s.path != ALONE) {
+            s.from = cut == BINS - 1 ? of_key(key_of(NEVER) + 1) : least_of(bin - cut, per);
+            if (s.path == BY_SUMS && cut > 0) s.to = least_of(bin - cut + 1, per);
+        }
+        narrow = s.path == BY_SUMS && count > LIST;
+        if (narrow) shared = s;
+        else *sc.state = s;
     }
+    for (int i = b; i < PARTS; i += BINS) counts[i] = 0, masses_of[i] = 0;
+    __syncthreads();
+    if (!narrow) return;
+    State s = shared;
+    const TL* const row = reinterpret_cast<const TL*>(a.logits + (int64_t)row_at * a.ld);
+    const float low = s.from, high = cut > 0 ? s.to : top, each = (float)PARTS / (high - low);
+    const double scale = (double)(1ull << a.shift);
+    auto part_of = [&](float l) __attribute__((always_inline)) {  // (rises with l; a bin of one value: 0)
+        const float x = (l - low) * each;
+        return x >= PARTS - 1 ? PARTS - 1 : x > 0.0f ? (int)x : 0;
+    };
+    constexpr int TOGETHER = 4;  // segments of a wavefront
+    for (int g0 = wave; g0 < sc.segs; g0 += WAVES * TOGETHER) {
+        Lane16<TL> x[TOGETHER];
+        bool some[TOGETHER];
+#pragma unroll
+        for (int t = 0; t < TOGETHER; t++) {
+            const int g = g0 + t * WAVES;
+            some[t] = g < sc.segs && sc.seg_top[g] >= low;
+            if (some[t]) x[t].ask(row, a.V, g);
+        }
+#pragma unroll
+        for (int t = 0; t < TOGETHER; t++) {
+            if (!some[t]) continue;
+            x[t].get(row, a.V, g0 + t * WAVES);
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const float l = x[t].v[e];
+                if (l < low || l >= s.to) continue;
+                const int at = part_of(l);
+                atomicAdd(&counts[at], 1u);
+                if (!r.top_k) atomicAdd(&masses_of[at], whole(weight_of(l, top, r.per), scale));
+            }
+        }
+    }
+    __syncthreads();
+    // two parts a thread, in descending order
+    const uint32_t n[2] = {counts[PARTS - 1 - 2 * b], counts[PARTS - 2 - 2 * b]};
+    const unsigned long long m[2] = {masses_of[PARTS - 1 - 2 * b], masses_of[PARTS - 2 - 2 * b]};
+    uint32_t c_run = wave_scan(n[0] + n[1]), c_all;
+    unsigned long long m_run = wave_scan(m[0] + m[1]), m_all;
+    if (lane == 63) cpart[wave] = c_run, mpart[wave] = m_run;
+    __syncthreads();
+    c_run += of_waves<WAVES>(cpart, &c_all) - n[0] - n[1];  // (what lies above the first of the two)
+    m_run += of_waves<WAVES>(mpart, &m_all) - m[0] - m[1];
+    auto reaches = [&](uint32_t c, unsigned long long w) __attribute__((always_inline)) { return r.top_k ? s.before_count + c >= (uint32_t)r.k : s.before_mass + (double)w / scale >= r.p * s.mass; };
+    const int here = n[0] && reaches(c_run + n[0], m_run + m[0]) ? 2 * b : n[1] && reaches(c_run + n[0] + n[1], m_run + m[0] + m[1]) ? 2 * b + 1 : -1, held_here = n[1] ? 2 * b + 1 : n[0] ? 2 * b : -1;
+    {
+        const uint64_t hits = __ballot(here >= 0), any = __ballot(held_here >= 0);
+        const int first = of_lane(here, hits ? __builtin_ctzll(hits) : 0), end = of_lane(held_here, any ? 63 - __builtin_clzll(any) : 0);
+        if (lane == 0) {
+            if (hits) atomicMin(&first_part, (uint32_t)first);
+            if (any) atomicMax(&last_part, (uint32_t)end);
+        }
+    }
+    __syncthreads();
+    const int at = first_part < PARTS ? (int)first_part : (int)last_part;
+    if (b != at >> 1) return;
+    const bool second = at & 1;
+    const uint32_t entries = second ? n[1] : n[0];
+    s.before_count += c_run + (second ? n[0] : 0u);
+    s.before_mass += (double)(m_run + (second ? m[0] : 0ull)) / scale;
+    if (entries > LIST) s.path = ALONE;
+    auto least_in = [&](int q) __attribute__((always_inline)) {  // the least logit of part q or a higher one
+        uint32_t from = key_of(low), to = key_of(high);
+        while (from < to) {
+            const uint32_t mid = from + (to - from) / 2;
+            if (part_of(of_key(mid)) >= q) to = mid;
+            else from = mid + 1;
+        }
+        return of_key(from);
+    };
+    const int q = PARTS - 1 - at;
+    if (q < part_of(high)) s.to = least_in(q + 1);
+    s.from = least_in(q);
     *sc.state = s;
 }
 
@@ -1020,7 +1105,7 @@ static int launch(const SampleArgs& a, int B, hipStream_t st) {
         hipLaunchKernelGGL((sample_slices_kernel<TL, 4>), dim3((unsigned)((segs + 3) / 4), (unsigned)B), dim3(256), 0, st, a);
     else
         hipLaunchKernelGGL((sample_slices_kernel<TL, SLICE>), dim3((unsigned)slices, (unsigned)B), dim3(SLICE * 64), 0, st, a);
-    if (!greedy && filters) hipLaunchKernelGGL(sample_cut_kernel, dim3((unsigned)B), dim3(BINS), 0, st, a);
+    if (!greedy && filters) hipLaunchKernelGGL(sample_cut_kernel<TL>, dim3((unsigned)B), dim3(BINS), 0, st, a);
     if (!greedy && !open) hipLaunchKernelGGL(sample_filter_kernel<TL>, dim3((unsigned)((segs + 3) / 4), (unsigned)B), dim3(256), 0, st, a);
     hipLaunchKernelGGL(sample_draw_kernel<TL>, dim3((unsigned)B), dim3(THREADS), 0, st, a);
     return check_hip(hipGetLastError(), "sample_draw_kernel launch");

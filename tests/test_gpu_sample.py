@@ -256,6 +256,17 @@ def test_temperatures_at_the_ends(T):
         check(l, u, T, *f)
 
 
+@pytest.mark.parametrize("V", [200001, 262144])
+@pytest.mark.parametrize("std", [0.005, 0.2, 1.0])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_more_in_the_last_bin_than_a_list_holds(V, std, dtype):
+    """Flat rows: the filters end among thousands of neighbours, in the row's highest bin and in others."""
+    l, u = logits(3, V, V, std=std, dtype=dtype, peaks=0)
+    l[2, 5000:60000] = l[2, 4999]  # (and among equal ones)
+    for f in ((1.0, 0, 0.9, 0.0), (1.0, 50000, 1.0, 0.0), (2.0, 0, 0.5, 0.0), (0.5, 0, 0.999, 0.0), (1.0, V - 1, 1.0, 0.0), (1.0, 0, 0.0001, 0.0), (1.5, 0, 0.8, 0.6), (1.0, 20000, 0.7, 0.0)):
+        check(l, u, *f)
+
+
 def test_the_same_every_time():
     """Nothing depends on the order in which workgroups come: lists, sums and tokens of many replays."""
     l, u = logits(40, 50001, 9, dtype=torch.bfloat16)

@@ -8,7 +8,7 @@
 // What stays is a run of the order whatever the filters are, so it is held as its last element: a key (the bits of l, made to order like l) and, among equal keys, an index.
 // A row is cut into segments of 1024 neighbours, one wavefront's 16 values a lane, whose maxima and sums are what the draw goes by: it finds its segment, then its token in it.
 //
-// Four kernels.  A workgroup for each slice of a row reads the logits: segments' maxima; without filters their sums too; with top_k or top_p a histogram of the slice, counts and weights by
+// Four kernels, or one for a short row (sample_row_kernel).  A workgroup for each slice of a row reads the logits: segments' maxima; without filters their sums too; with top_k or top_p a histogram of the slice, counts and weights by
 // l / T in steps of 1 / 16, on one grid for the row.  With filters a workgroup a row adds the histograms up, which shows the bin in which the run ends.  Workgroups of four segments collect what lies in it
 // and above; or, where that is more than a list holds, what lies in it, and the segments' sums of what lies above.  A workgroup a row sorts out from the list where the run ends, and draws.
 // Bound: the launches and the steps that wait for each other in them (barriers, LDS, a dependent read), each kernel 5 us at the least; HBM only for many rows without filters, where the one pass over
@@ -20,6 +20,8 @@
 #include "ffn.hpp"
 
 namespace mmx {
+
+int num_cus();
 
 constexpr int SEG = 1024;                 // logits of a segment
 constexpr int BINS = 512;                 // the last one: everything below, e^-31.9 of the largest weight or less, which top_p's run takes for nothing
@@ -531,22 +533,21 @@ __device__ __forceinline__ float least_of(double at, double per) {
 
 // the row's histogram, a bin a thread, and the bin in which the run ends.  A bin of more than a list holds (flat rows of large vocabularies) is cut into PARTS of its own first, for which the workgroup
 // reads the row: 8 x 262144 fp32 of N(0, 1), top_p 0.9, 157 us in place of the 632 of one workgroup and the whole key.
-template <typename TL>
-__global__ __launch_bounds__(BINS) void sample_cut_kernel(const SampleArgs a) {
-    constexpr int WAVES = BINS / 64, AHEAD = 8, PARTS = 2 * BINS;
+// (A function of T threads, BINS or more, that all call; counts and masses_of: PARTS each.)
+constexpr int PARTS = 2 * BINS;
+template <typename TL, int T>
+__device__ __forceinline__ void find_cut(const SampleArgs& a, const Scratch& sc, const RowAsks& r, int row_at, uint32_t* counts, unsigned long long* masses_of) {
+    constexpr int WAVES = T / 64, AHEAD = 8;
     __shared__ State shared;
     __shared__ bool narrow;
-    __shared__ uint32_t counts[PARTS], cpart[WAVES], first_part, last_part;
-    __shared__ unsigned long long masses_of[PARTS], mpart[WAVES];
+    __shared__ uint32_t cpart[WAVES], first_part, last_part;
+    __shared__ unsigned long long mpart[WAVES];
     __shared__ double part[2][WAVES];
     __shared__ int slice_ahead[MOST_SLICES];
     __shared__ float fpart[WAVES];
     __shared__ uint32_t found, last_bin, all_count;
-    const int row_at = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, b = threadIdx.x;
-    const Scratch sc = scratch_of(a, row_at);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, b = threadIdx.x;
     const float first_top = b < sc.segs ? sc.seg_top[b] : NEVER;
-    const RowAsks r = asks_of(a, row_at);
-    if (!r.filtered()) return;
     Slice own = {0.0, 0, 0};
     if (b < sc.n_slices) own = sc.slices[b];
     if (b == 0) found = BINS, last_bin = 0, all_count = 0, first_part = PARTS, last_part = 0;
@@ -609,7 +610,7 @@ __global__ __launch_bounds__(BINS) void sample_cut_kernel(const SampleArgs a) {
         if (narrow) shared = s;
         else *sc.state = s;
     }
-    for (int i = b; i < PARTS; i += BINS) counts[i] = 0, masses_of[i] = 0;
+    for (int i = b; i < PARTS; i += T) counts[i] = 0, masses_of[i] = 0;
     __syncthreads();
     if (!narrow) return;
     State s = shared;
@@ -620,7 +621,7 @@ __global__ __launch_bounds__(BINS) void sample_cut_kernel(const SampleArgs a) {
         const float x = (l - low) * each;
         return x >= PARTS - 1 ? PARTS - 1 : x > 0.0f ? (int)x : 0;
     };
-    constexpr int TOGETHER = 4;  // segments of a wavefront
+    constexpr int TOGETHER = T == BINS ? 4 : 1;  // segments of a wavefront (as far as the registers go)
     for (int g0 = wave; g0 < sc.segs; g0 += WAVES * TOGETHER) {
         Lane16<TL> x[TOGETHER];
         bool some[TOGETHER];
@@ -646,8 +647,12 @@ __global__ __launch_bounds__(BINS) void sample_cut_kernel(const SampleArgs a) {
     }
     __syncthreads();
     // two parts a thread, in descending order
-    const uint32_t n[2] = {counts[PARTS - 1 - 2 * b], counts[PARTS - 2 - 2 * b]};
-    const unsigned long long m[2] = {masses_of[PARTS - 1 - 2 * b], masses_of[PARTS - 2 - 2 * b]};
+    uint32_t n[2] = {0, 0};
+    unsigned long long m[2] = {0, 0};
+    if (b < BINS) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) n[i] = counts[PARTS - 1 - i - 2 * b], m[i] = masses_of[PARTS - 1 - i - 2 * b];
+    }
     uint32_t c_run = wave_scan(n[0] + n[1]), c_all;
     unsigned long long m_run = wave_scan(m[0] + m[1]), m_all;
     if (lane == 63) cpart[wave] = c_run, mpart[wave] = m_run;
@@ -685,6 +690,13 @@ __global__ __launch_bounds__(BINS) void sample_cut_kernel(const SampleArgs a) {
     if (q < part_of(high)) s.to = least_in(q + 1);
     s.from = least_in(q);
     *sc.state = s;
+}
+template <typename TL>
+__global__ __launch_bounds__(BINS) void sample_cut_kernel(const SampleArgs a) {
+    __shared__ uint32_t counts[PARTS];
+    __shared__ unsigned long long masses_of[PARTS];
+    const RowAsks r = asks_of(a, blockIdx.x);
+    if (r.filtered()) find_cut<TL, BINS>(a, scratch_of(a, blockIdx.x), r, blockIdx.x, counts, masses_of);
 }
 
 template <typename TL>
@@ -777,6 +789,7 @@ struct Room {
     unsigned long long low, high, best, part[NW], before_mass;
     uint32_t cpart[NW], first, last;
 };
+static_assert(BUCKETS == PARTS, "a short row's cut borrows the buckets");
 static_assert(BUCKETS == THREADS && FEW * 8 == THREADS, "a bucket a thread; eight threads for each that is left");
 
 // Of the entries (a thread's c, no two alike; 0: none) in descending order: the first up to which there are `want` of them, or whose masses m come to `want` (STRICT: to more); the last if none does.
@@ -889,17 +902,14 @@ __device__ unsigned long long sum_of(unsigned long long v, Room& o) {
     return all;
 }
 
-template <typename TL>
-__global__ __launch_bounds__(THREADS) void sample_draw_kernel(const SampleArgs a) {
-    __shared__ Shared s;
-    __shared__ Room o;
-    __shared__ unsigned long long more[MOST_SUMS];
-    const int row_at = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// A workgroup of THREADS for a row.  OWN: without filters, segments' sums are relative to their own maxima.
+template <typename TL, bool OWN, int SUMS>
+__device__ __forceinline__ void draw(const SampleArgs& a, const Scratch& sc, const RowAsks& r, int row_at, Shared& s, Room& o) {
+    __shared__ unsigned long long more[SUMS];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int V = a.V;
     const TL* const row = reinterpret_cast<const TL*>(a.logits + (int64_t)row_at * a.ld);
-    const Scratch sc = scratch_of(a, row_at);
     const int segs = sc.segs;
-    const RowAsks r = asks_of(a, row_at);
     // (what the next steps want, asked for with the first)
     const State state = *sc.state;
     const double first_sum = (int)threadIdx.x < segs ? sc.sums[threadIdx.x] : 0.0;
@@ -1035,7 +1045,7 @@ __global__ __launch_bounds__(THREADS) void sample_draw_kernel(const SampleArgs a
     }
     // A segment's sum: without filters it is relative to its own maximum, with a list there may be more to it.  A thread has up to four neighbouring segments (of 2^22 logits).
     constexpr int MOST = 4;
-    const bool own = !r.filtered() && !r.min, added = r.filtered() && path == BY_SUMS;
+    const bool own = OWN && !r.filtered() && !r.min, added = r.filtered() && path == BY_SUMS;
     const int each = (segs + THREADS - 1) / THREADS, g0 = threadIdx.x * each;
     double sums[MOST], mine = 0, total;
 #pragma unroll
@@ -1087,6 +1097,150 @@ __global__ __launch_bounds__(THREADS) void sample_draw_kernel(const SampleArgs a
     if (threadIdx.x == 0) a.ids[row_at] = seg * SEG + (int)(s.found != 0xffffffffu ? s.found : s.bin);
 }
 
+template <typename TL>
+__global__ __launch_bounds__(THREADS) void sample_draw_kernel(const SampleArgs a) {
+    __shared__ Shared s;
+    __shared__ Room o;
+    draw<TL, true, MOST_SUMS>(a, scratch_of(a, blockIdx.x), asks_of(a, blockIdx.x), blockIdx.x, s, o);
+}
+
+// ---- a short row in one workgroup ---------------------------------------------------------------------------------------------------
+// The same steps with what they hand on in LDS, two segments a wavefront, read once: three launches less, and one CU's exponentials and LDS atomics in place of several's (the rule below).
+constexpr int ROW_SEGS = 2 * NW;
+template <typename TL>
+__global__ __launch_bounds__(THREADS) void sample_row_kernel(const SampleArgs a) {
+    __shared__ Shared s;
+    __shared__ Room o;
+    __shared__ unsigned long long list[LIST], bins[2][BINS];  // (a histogram for eight wavefronts each: up to 2^14 logits)
+    __shared__ State state;
+    __shared__ Slice slices[2];
+    __shared__ double sums[ROW_SEGS];
+    __shared__ float seg_top[ROW_SEGS];
+    const int row_at = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, part = wave / (NW / 2);
+    const TL* const row = reinterpret_cast<const TL*>(a.logits + (int64_t)row_at * a.ld);
+    Scratch sc;
+    sc.segs = (a.V + SEG - 1) / SEG, sc.slice = NW, sc.n_slices = 2;
+    sc.seg_top = seg_top, sc.sums = sums, sc.slices = slices, sc.state = &state, sc.list = list, sc.bins = bins[0];
+    const RowAsks r = asks_of(a, row_at);
+    Lane16<TL> x[2];
+#pragma unroll
+    for (int t = 0; t < 2; t++)
+        if (wave * 2 + t < sc.segs) x[t].ask(row, a.V, wave * 2 + t);
+    bins[threadIdx.x / BINS][threadIdx.x % BINS] = 0;
+    if (threadIdx.x < 2) slices[threadIdx.x].count = 0;
+    if (threadIdx.x == 0) s.found = 0;
+#pragma unroll
+    for (int t = 0; t < 2; t++) {
+        const int g = wave * 2 + t;
+        if (g >= sc.segs) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) x[t].v[e] = NEVER;
+            continue;
+        }
+        x[t].get(row, a.V, g);
+        float mine = NEVER;
+#pragma unroll
+        for (int e = 0; e < 16; e++) mine = fmaxf(mine, x[t].v[e]);
+        mine = wave_max(mine);
+        if (lane == 0) seg_top[g] = mine;
+    }
+    __syncthreads();
+    const float top = wave_max((lane & (ROW_SEGS - 1)) < sc.segs ? seg_top[lane & (ROW_SEGS - 1)] : NEVER);
+    auto weight = [&](float l) __attribute__((always_inline)) {
+        const double v = weight_of(l, top, r.per);
+        return v < r.min_p && l != top ? 0.0 : v;
+    };
+    if (top != NEVER && !r.greedy) {
+        if (!r.filtered()) {
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                double w = 0;
+#pragma unroll
+                for (int e = 0; e < 16; e++) w += weight(x[t].v[e]);
+                w = wave_sum(w);
+                if (lane == 0 && wave * 2 + t < sc.segs) sums[wave * 2 + t] = w;
+            }
+        } else {
+            const double per = PER_UNIT * r.per, bin = floor((double)top * per);
+            double least = -__builtin_huge_val();  // what is smaller is of no interest
+            if (r.top_k && r.k <= THREADS) {
+                // the threads' largest alone: below the bin that the k-th of them lies in nothing can be among the first k (one bin more, for what is rounded here)
+                float mine = NEVER;
+#pragma unroll
+                for (int e = 0; e < 16; e++) mine = fmaxf(mine, fmaxf(x[0].v[e], x[1].v[e]));
+                const double d = bin - floor((double)mine * per);
+                if (mine != NEVER && d < BINS - 1) atomicAdd(&bins[0][(int)d], 1ull);
+                if (threadIdx.x == 0) s.bin = BINS;
+                __syncthreads();
+                const uint32_t held = threadIdx.x < BINS ? (uint32_t)bins[0][threadIdx.x] : 0u;
+                const uint32_t run = wave_scan(held);
+                if (lane == 63) o.cpart[wave] = run;
+                __syncthreads();
+                uint32_t all;
+                first_of(of_waves<NW>(o.cpart, &all) + run >= (uint32_t)r.k, &s.bin);
+                if (threadIdx.x < BINS) bins[0][threadIdx.x] = 0;
+                __syncthreads();
+                if (s.bin < BINS) least = (bin - (double)s.bin - 1.0) / per;
+            }
+            uint32_t n = 0;
+#pragma unroll
+            for (int t = 0; t < 2; t++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    if (x[t].v[e] == NEVER) continue;
+                    n++;
+                    if ((double)x[t].v[e] < least) continue;
+                    const double l = (double)x[t].v[e] * per, low = floor(l), d = bin - low;
+                    unsigned long long w = 1ull << MASS_BITS;
+                    if (!r.top_k) w += (1ull << 34) + (uint32_t)(factor_less_1(l - low) * FACTOR_SCALE + 0.5);
+                    if (d < BINS - 1) atomicAdd(&bins[part][(int)d], w);  // (what lies in the last is counted only)
+                }
+            n = wave_sum(n);
+            if (lane == 0) {
+                if (n) atomicAdd(&slices[part].count, n);
+                slices[part].bin = bin;
+            }
+            __syncthreads();
+            find_cut<TL, THREADS>(a, sc, r, row_at, o.count, o.mass);
+            __syncthreads();
+            const State at = state;
+            if (at.path != ALONE) {
+#pragma unroll
+                for (int t = 0; t < 2; t++) {
+                    if (at.path == BY_SUMS) {
+                        double w = 0;
+#pragma unroll
+                        for (int e = 0; e < 16; e++)
+                            if (__any(x[t].v[e] >= at.to)) w += x[t].v[e] >= at.to ? weight(x[t].v[e]) : 0.0;
+                        w = wave_sum(w);
+                        if (lane == 0 && wave * 2 + t < sc.segs) sums[wave * 2 + t] = w;
+                    }
+                    uint32_t takes = 0;
+#pragma unroll
+                    for (int e = 0; e < 16; e++) takes |= x[t].v[e] >= at.from && x[t].v[e] < at.to ? 1u << e : 0;
+                    if (!__any(takes != 0)) continue;
+                    const uint32_t mine = __popc(takes), upto = wave_scan(mine);
+                    uint32_t to = 0;
+                    if (lane == 63) to = atomicAdd(&s.found, upto);
+                    to = of_lane(to, 63) + upto - mine;
+#pragma unroll
+                    for (int e = 0; e < 16; e++)
+                        if (takes >> e & 1) {
+                            if (to < LIST) list[to] = entry_of<TL>(x[t].v[e], (wave * 2 + t) * SEG + Lane16<TL>::at(e), a.V);
+                            to++;
+                        }
+                }
+                __syncthreads();
+                if (threadIdx.x == 0) state.entries = s.found;
+            }
+        }
+    } else if (threadIdx.x == 0) {
+        state.path = ALONE;  // (no largest logit in it)
+    }
+    __syncthreads();
+    draw<TL, false, ROW_SEGS>(a, sc, r, row_at, s, o);
+}
+
 // Segments of a slice: 4 where 16 would leave most of the chip idle (1 x 32000: 8 workgroups in place of 2); 16 elsewhere, since every slice's histogram is written and read
 int sample_slice(int B, int V) {
     const int64_t segs = ((int64_t)V + SEG - 1) / SEG;
@@ -1101,6 +1255,14 @@ static int launch(const SampleArgs& a, int B, hipStream_t st) {
     const bool greedy = (!a.temperature && !(a.temperature_all > 0.0)) || (!a.top_k && a.top_k_all == 1) || (!a.top_p && a.top_p_all <= 0.0);
     const bool open = !a.top_k && (a.top_k_all <= 0 || a.top_k_all >= a.V) && !a.top_p && a.top_p_all >= 1.0 && !a.min_p && a.min_p_all <= 0.0;
     const bool filters = a.top_k || (a.top_k_all > 0 && a.top_k_all < a.V) || a.top_p || a.top_p_all < 1.0;
+    // (short rows: us in one workgroup / in four kernels, fp32, rows 1, 64, 256: 32000 top_k 50 and top_p 0.9 19 / 22, 21 / 26, 24 / 35; 8000 top_p 0.9 26 / 30, 28 / 33, 28 / 38.  Where every logit has a factor of
+    // a weight to be computed, a row takes longer in one workgroup from some 12 segments on: 32000 top_p 0.9 36 / 27, 37 / 33, 41 / 49; and without filters two kernels are faster: 8000 14 / 10, 16 / 11, 16 / 13.
+    // 1024 rows of 5000, top_p: 104 / 100.)
+    const bool by_count = !a.top_k && a.top_k_all > 0 && a.top_k_all < a.V;
+    if (!greedy && filters && (by_count ? segs <= ROW_SEGS : segs <= 12 && B <= 2 * num_cus())) {
+        hipLaunchKernelGGL(sample_row_kernel<TL>, dim3((unsigned)B), dim3(THREADS), 0, st, a);
+        return check_hip(hipGetLastError(), "sample_row_kernel launch");
+    }
     if (greedy || !filters)  // (no histograms: small workgroups, of which more overlap)
         hipLaunchKernelGGL((sample_slices_kernel<TL, 4>), dim3((unsigned)((segs + 3) / 4), (unsigned)B), dim3(256), 0, st, a);
     else

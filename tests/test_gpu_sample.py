@@ -42,7 +42,7 @@ def test_filters(V, dtype):
         check(l, u, T, k, p, m)
 
 
-@pytest.mark.parametrize("B,V", [(1, 131072), (33, 100003), (64, 20000), (300, 999)])
+@pytest.mark.parametrize("B,V", [(1, 131072), (33, 100003), (64, 20000), (300, 999), (600, 2500)])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_each_row_asks_for_its_own(B, V, dtype):
     l, u = logits(B, V, B, dtype=dtype)
@@ -256,7 +256,7 @@ def test_temperatures_at_the_ends(T):
         check(l, u, T, *f)
 
 
-@pytest.mark.parametrize("V", [200001, 262144])
+@pytest.mark.parametrize("V", [12000, 32000, 200001, 262144])
 @pytest.mark.parametrize("std", [0.005, 0.2, 1.0])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_more_in_the_last_bin_than_a_list_holds(V, std, dtype):

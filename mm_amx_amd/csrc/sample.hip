@@ -12,8 +12,8 @@
 // l / T in steps of 1 / 16, on one grid for the row.  With filters a workgroup a row adds the histograms up, which shows the bin in which the run ends.  Workgroups of four segments collect what lies in it
 // and above; or, where that is more than a list holds, what lies in it, and the segments' sums of what lies above.  A workgroup a row sorts out from the list where the run ends, and draws.
 // Bound: the launches and the steps that wait for each other in them (barriers, LDS, a dependent read), each kernel 5 us at the least; HBM only for many rows without filters, where the one pass over
-// 256 x 131072 fp32 takes 35 us, 3.8 TB/s, of 41.  us, slices / cut / filter / draw: 1 x 32000 fp32, top_k and top_p 5.6 / 4.0 / 4.5 / 8.2; 33 x 100003 fp32, top_p 8.6 / 4.6 / 13 / 12;
-// 64 x 131072 bf16, a mixture 13.0 / 4.8 / 11 / 15.8.  (One kernel, a workgroup a row that passes over it again and again: 130, 349 and 589 us for these three.)
+// 256 x 131072 fp32 takes 35 us, 3.8 TB/s, of 41.  us, slices / cut / filter / draw: 33 x 100003 fp32, top_p 9 / 4.8 / 12 / 12.5;
+// 64 x 131072 bf16, a mixture 13.0 / 5 / 11 / 15.8.  (One kernel, a workgroup a row that passes over it again and again: 349 and 589 us for these two.)
 // Rows that this does not suit (more than a list of equal logits in the last bin, or of what top_k leaves to top_p; 2^26 bins and more; more than 2^20 logits and a list) are worked on by that one workgroup alone, a pass over the row for every eight bits of the key.
 #include "sample.hpp"
 

@@ -47,6 +47,7 @@ __device__ __forceinline__ RowAsks asks_of(const SampleArgs& a, int row) {
     r.k = a.top_k ? a.top_k[row] : a.top_k_all;
     r.p = a.top_p ? (double)a.top_p[row] : a.top_p_all;
     r.min_p = a.min_p ? (double)a.min_p[row] : a.min_p_all;
+    if (r.min_p > 1.0) r.min_p = 1.0;  // (not fmin, which would lose a NaN; with more than 1, tokens whose weight comes out as 1 at a high temperature would fall)
     r.top_k = r.k > 0 && r.k < a.V;
     r.top_p = r.p < 1.0;
     r.min = r.min_p > 0.0;

@@ -117,6 +117,17 @@ def test_out_of_range_in_tensors_is_taken_as_the_nearest():
     assert base(temperature=inf, top_k=3) == [su.token(l[b].double().numpy(), float(u[b]), inf, 3) for b in range(4)]
 
 
+@pytest.mark.parametrize("T", [float("inf"), 1e30])
+@pytest.mark.parametrize("V", [2000, 40000])
+def test_min_p_above_one_in_tensors_keeps_what_one_keeps(T, V):
+    """Where the temperature makes every weight 1, a min_p of 1 drops none, and more than 1 is taken as 1."""
+    l, u = logits(4, V, 5)
+    m = [1.5, float("inf"), 1.0, 2.0]
+    for k, p in ((0, 1.0), (40, 1.0), (40, 0.9), (0, 0.9)):
+        got = check(l, u, T, k, p, m)
+        assert torch.equal(got, mx.sample(l.cuda(), u.cuda(), T, k, p, 1.0))
+
+
 @pytest.mark.parametrize("f", [(1.0, 0, 1.0, 0.0), (0.9, 30, 0.9, 0.0), (1.0, 0, 0.9, 0.0)])
 def test_rows_of_any_stride_and_alignment(f):
     base, u = logits(20, 3333, 4, dtype=torch.bfloat16)

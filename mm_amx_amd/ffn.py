@@ -360,7 +360,7 @@ def block_norm(f, residual=None, *, post=False, post_weight=None, gate=None, sca
     elif isinstance(quantize, str) and not mx4:
         raise MmxError("quantize is False, True ('fp8') or 'mxfp4'")
     if L._native is not None and L._initialised and z is None:
-        made = L._made(L._native.block_norm, f, residual, post, post_weight, gate, scale, pre, pre_weight, eps, weight_offset, 2 if mx4 else quantize, r)
+        made = L._made(L._native.block_norm, f, residual, post, post_weight, gate, scale, pre, pre_weight, eps, weight_offset, 2 if mx4 else bool(quantize), r)
         if made is not None:
             return (made[0], Mxfp4Rows(made[1], *f.shape)) if mx4 else (made[0], Fp8Rows(made[1], made[2], f.shape[1])) if quantize else made
     _gpu(f, "f", (torch.bfloat16,), 2)

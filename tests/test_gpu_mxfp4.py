@@ -551,3 +551,14 @@ def test_the_stack_over_4_bit_weights_with_a_head_and_tokens():
     assert out["tokens"].shape == (5,) and bool(((out["tokens"] >= 0) & (out["tokens"] < 1000)).all())
     # three quantisations to 3 significant bits, 2^-2 of a value at most, against none
     assert out["rel_err_mxfp4_one_layer"] < 3 * 2.0 ** -2
+
+
+def test_any_true_value_of_quantize_is_e4m3(monkeypatch):
+    from mm_amx_amd import _lib as L
+    x = normal((20, 300), 1)
+    r, want = mx.block_norm(x, x, quantize=True)
+    for native in (L._native, None):
+        monkeypatch.setattr(L, "_native", native)
+        for quantize in (1, 2, 3):
+            r1, z = mx.block_norm(x, x, quantize=quantize)
+            assert type(z) is mx.Fp8Rows and torch.equal(r1, r) and torch.equal(z.q.view(torch.uint8), want.q.view(torch.uint8)) and torch.equal(z.scales, want.scales)

@@ -122,3 +122,23 @@ def test_the_definitions():
     assert list(m4.scale_of(np.array([0.0, 6.0, 6.99, 7.0, 13.9, 14.0, 1.75, np.inf, 2.0 ** -140, 3.0e38]))) == [1, 127, 127, 128, 128, 129, 126, 255, 1, 253]
     codes = np.arange(12, dtype=np.uint8).reshape(2, 6)
     assert np.array_equal(m4.single(m4.pairs(codes), 6), codes) and np.array_equal(m4.single(m4.pairs(codes[:, :5]), 5), codes[:, :5])
+
+
+def test_any_true_value_of_quantize_means_e4m3(monkeypatch):
+    """Only "mxfp4" asks for packed rows: the native call's own code for them comes from no caller."""
+    seen = []
+
+    class Native:
+        @staticmethod
+        def block_norm(*a):
+            seen.append(a[10])  # (returns None: not taken, nothing done)
+
+    monkeypatch.setattr(L, "_native", Native)
+    monkeypatch.setattr(L, "_initialised", {0})
+    monkeypatch.setattr(L, "_current_device", lambda: 0)
+    monkeypatch.setattr(L, "_raw_stream", lambda device: 0)
+    x = torch.zeros((4, 128), dtype=torch.bfloat16)
+    for quantize, code in ((False, False), (0, False), (None, False), (True, True), ("fp8", True), (1, True), (2, True), (np.bool_(True), True), ("mxfp4", 2)):
+        with pytest.raises(mx.MmxError, match="on the GPU"):
+            mx.block_norm(x, quantize=quantize)
+        assert seen[-1] == code and type(seen[-1]) is type(code), quantize

@@ -351,18 +351,15 @@ class MLP:
             raise L.MmxError("setup: compress is 'fp8' or 'mxfp4', for weights that come without scales")
         if mx4:
             gate_up = mxfp4.pack_gate_up_mxfp4(w_gate, w_up, None if scales is None else scales[:2])
-            self.down = mxfp4.pack_mxfp4(w_down, None if scales is None else scales[2])
-            self.gate_up, self.m_N, self.m_K, self.mx4 = gate_up, N, K, True
-            return
-        self.mx4 = False
-        if scales is not None or compress:
+            down = mxfp4.pack_mxfp4(w_down, None if scales is None else scales[2])
+        elif scales is not None or compress:
             gate_up = ffn.pack_gate_up_fp8(w_gate, w_up, None if scales is None else scales[:2])
-            self.down = ffn.pack_fp8(w_down, None if scales is None else scales[2])
-            self.gate_up, self.m_N, self.m_K = gate_up, N, K
-            return
-        self.m_N, self.m_K = N, K
-        self.gate_up = L.repack_gate_up(w_gate, w_up)
-        self.down = L.repack_b(w_down, transpose=True)
+            down = ffn.pack_fp8(w_down, None if scales is None else scales[2])
+        else:
+            gate_up = L.repack_gate_up(w_gate, w_up)
+            down = L.repack_b(w_down, transpose=True)
+        # (all at once, behind everything that may refuse: what was set up before stays in use till then)
+        self.gate_up, self.down, self.m_N, self.m_K, self.mx4 = gate_up, down, N, K, mx4
 
     def run(self, x, y=None):
         if self.gate_up is None:

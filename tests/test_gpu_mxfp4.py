@@ -562,3 +562,20 @@ def test_any_true_value_of_quantize_is_e4m3(monkeypatch):
         for quantize in (1, 2, 3):
             r1, z = mx.block_norm(x, x, quantize=quantize)
             assert type(z) is mx.Fp8Rows and torch.equal(r1, r) and torch.equal(z.q.view(torch.uint8), want.q.view(torch.uint8)) and torch.equal(z.scales, want.scales)
+
+
+def test_a_refused_setup_leaves_the_mlp_running():
+    N, K = 96, 256
+    w, d = normal((N, K), 1, 0.05), normal((K, N), 2, 0.05)
+    x = normal((5, K), 3)
+    mlp = mx.MLP()
+    mlp.setup(w, w, d, compress="mxfp4")
+    want = mlp.run(x)
+    for bad in (dict(w_up=w[:32], compress="fp8"), dict(w_up=w[:32]), dict(w_gate=w.cpu()), dict(w_down=d.float(), compress="fp8"), dict(w_down=d.float()), dict(w_down=d.half(), compress="mxfp4")):
+        with pytest.raises(mx.MmxError):
+            mlp.setup(**{**dict(w_gate=w, w_up=w, w_down=d), **bad})
+        assert torch.equal(mlp.run(x), want)
+    mlp.setup(w, w, d)
+    plain = mx.MLP()
+    plain.setup(w, w, d)
+    assert torch.equal(mlp.run(x), plain.run(x))

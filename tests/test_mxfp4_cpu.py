@@ -142,3 +142,13 @@ def test_any_true_value_of_quantize_means_e4m3(monkeypatch):
         with pytest.raises(mx.MmxError, match="on the GPU"):
             mx.block_norm(x, quantize=quantize)
         assert seen[-1] == code and type(seen[-1]) is type(code), quantize
+
+
+@pytest.mark.parametrize("compress", [None, "fp8", "mxfp4"])
+def test_a_refused_setup_leaves_the_mlp_as_it_was(compress):
+    mlp = mx.MLP()
+    mlp.gate_up, mlp.down, mlp.m_N, mlp.m_K, mlp.mx4 = held = ("gate_up", "down", 96, 256, True)
+    w = torch.zeros((64, 128), dtype=torch.bfloat16)
+    with pytest.raises(mx.MmxError, match="on the GPU"):
+        mlp.setup(w, w, torch.zeros((128, 64), dtype=torch.bfloat16), compress=compress)
+    assert (mlp.gate_up, mlp.down, mlp.m_N, mlp.m_K, mlp.mx4) == held

@@ -360,6 +360,7 @@ class MLP:
             down = L.repack_b(w_down, transpose=True)
         # (all at once, behind everything that may refuse: what was set up before stays in use till then)
         self.gate_up, self.down, self.m_N, self.m_K, self.mx4 = gate_up, down, N, K, mx4
+        self.actUp = None  # (of the old N)
 
     def run(self, x, y=None):
         if self.gate_up is None:

@@ -579,3 +579,16 @@ def test_a_refused_setup_leaves_the_mlp_running():
     plain = mx.MLP()
     plain.setup(w, w, d)
     assert torch.equal(mlp.run(x), plain.run(x))
+
+
+def test_a_second_setup_may_have_other_sizes():
+    """Whatever the weights are and were: the intermediate of an earlier run does not stay."""
+    x = {K: normal((5, K), K) for K in (128, 256)}
+    mlp = mx.MLP()
+    for compress in (None, "mxfp4", "fp8", None):
+        for N, K in ((64, 128), (192, 256), (96, 256), (160, 128)):
+            w, d = normal((N, K), N, 0.05), normal((K, N), N + 1, 0.05)
+            mlp.setup(w, w, d, compress=compress)
+            fresh = mx.MLP()
+            fresh.setup(w, w, d, compress=compress)
+            assert torch.equal(mlp.run(x[K]), fresh.run(x[K]))

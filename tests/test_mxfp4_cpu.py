@@ -152,3 +152,14 @@ def test_a_refused_setup_leaves_the_mlp_as_it_was(compress):
     with pytest.raises(mx.MmxError, match="on the GPU"):
         mlp.setup(w, w, torch.zeros((128, 64), dtype=torch.bfloat16), compress=compress)
     assert (mlp.gate_up, mlp.down, mlp.m_N, mlp.m_K, mlp.mx4) == held
+
+
+def test_a_setup_lets_the_old_intermediate_go(monkeypatch):
+    """run makes one of the new width: the old one, kept, was refused as too narrow."""
+    mlp = mx.MLP()
+    mlp.actUp = torch.zeros((4, 32))
+    monkeypatch.setattr(L, "repack_gate_up", lambda gate, up: "gate_up")
+    monkeypatch.setattr(L, "repack_b", lambda w, transpose: "down")
+    w = torch.zeros((64, 128), dtype=torch.bfloat16)
+    mlp.setup(w, w, torch.zeros((128, 64), dtype=torch.bfloat16))
+    assert mlp.actUp is None and (mlp.gate_up, mlp.down, mlp.m_N, mlp.m_K, mlp.mx4) == ("gate_up", "down", 64, 128, False)

@@ -792,8 +792,15 @@ PyObject* sample(PyObject*, PyObject* const* a, Py_ssize_t count) {
         s.dtype = float_code(*l.t);
         s.u = floats(a[1], device, {l.rows});
         const auto asked = [&](PyObject* o, const float*& of, double& all) {
-            if (PyFloat_CheckExact(o)) all = PyFloat_AS_DOUBLE(o);
-            else of = floats(o, device, {l.rows});
+            if (PyFloat_CheckExact(o)) {
+                all = PyFloat_AS_DOUBLE(o);
+            } else if (PyLong_CheckExact(o)) {  // (0 and 1 are written so; not a truth value, which is a number of its own type)
+                int n;
+                if (!whole_number(o, 0, INT32_MAX, n)) throw Leave();
+                all = n;
+            } else {
+                of = floats(o, device, {l.rows});
+            }
         };
         asked(a[2], s.temperature_of, s.temperature);
         asked(a[4], s.top_p_of, s.top_p);

@@ -299,3 +299,28 @@ def test_native_and_python_calls_agree(monkeypatch):
     assert L._native is not None
     monkeypatch.setattr(L, "_native", None)
     assert all(torch.equal(a, b) for a, b in zip(native, calls()))
+
+
+def test_whole_numbers_take_the_native_call(monkeypatch):
+    """temperature=0, top_p=1 and their like are what programs write; the native call takes them as it takes floats."""
+    from mm_amx_amd import _lib as L
+    native, made = L._native, []
+    assert native is not None
+
+    class Spy:
+        @staticmethod
+        def sample(*a):
+            made.append(native.sample(*a))
+            return made[-1]
+
+    l, u = logits(5, 3000, 10)
+    l, u = l.cuda(), u.cuda()
+    asked = (dict(temperature=0), dict(temperature=2, top_k=40), dict(top_p=1, min_p=0), dict(top_p=0), dict(min_p=1, temperature=1), dict(temperature=2 ** 31 - 1, top_k=3))
+    want = [mx.sample(l, u, **{n: v if n == "top_k" else float(v) for n, v in a.items()}) for a in asked]
+    monkeypatch.setattr(L, "_native", Spy)
+    got = [mx.sample(l, u, **a) for a in asked]
+    assert len(made) == len(asked) and all(m is not None for m in made)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for bad in (dict(temperature=-1), dict(top_p=-1), dict(min_p=2), dict(temperature=True)):
+        with pytest.raises(mx.MmxError):
+            mx.sample(l, u, **bad)

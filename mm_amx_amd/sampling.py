@@ -18,7 +18,12 @@ def _asked(v, what, B, dtype, lo, hi):
         return v.data_ptr(), 0
     if isinstance(v, bool) or not isinstance(v, int if dtype == torch.int32 else (int, float)) or not lo <= v <= hi:
         raise MmxError(f"{what} = {v} is out of range")
-    return None, v
+    if dtype == torch.int32:
+        return None, v
+    try:
+        return None, float(v)
+    except OverflowError:  # (a whole number that is below infinity, but no double)
+        raise MmxError(f"{what} is out of range") from None
 
 
 def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None):

@@ -45,3 +45,15 @@ def test_the_definition():
     assert draw(0.9, T=0.0) == 1 and su.token([1.0, 1.0], 0.9, T=0.0) == 0
     assert su.token([-np.inf, np.nan], 0.5) == -1 and su.token([0.0, np.inf, 1.0], 0.99) == 1
     assert list(su.kept(np.zeros(4), k=2)[0]) == [0, 1] and list(su.kept(np.zeros(4), p=0.6)[0]) == [0, 1, 2]
+
+
+def test_whole_numbers_past_64_bits_are_refused():
+    """What no double can hold is an argument out of range like any other."""
+    from mm_amx_amd import sampling
+    inf = float("inf")
+    for v in (10 ** 400, -10 ** 400):
+        with pytest.raises(mx.MmxError, match="out of range"):
+            sampling._asked(v, "temperature", 4, torch.float32, 0, inf)
+    assert sampling._asked(2 ** 70, "temperature", 4, torch.float32, 0, inf) == (None, 2.0 ** 70)
+    assert sampling._asked(inf, "top_p", 4, torch.float32, 0, inf) == (None, inf)
+    assert sampling._asked(40, "top_k", 4, torch.int32, 0, 2 ** 31 - 1) == (None, 40)

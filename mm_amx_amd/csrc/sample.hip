@@ -1012,7 +1012,8 @@ __device__ __forceinline__ void draw(const SampleArgs& a, const Scratch& sc, con
 #pragma unroll
         for (int i = 0; i < MINE; i++)
             if (c[i]) atomicAdd(&more[index_of(c[i], V) / SEG], m[i]);
-        cut = Cut{key_in<TL>(last, V), index_of(last, V)};
+        // (nothing was cut off the list where top_k ends with it: what lies below the list does not stay)
+        cut = last > 1 ? Cut{key_in<TL>(last, V), index_of(last, V)} : Cut{key_of(state.from), V};
         __syncthreads();
     } else if (path == ALONE) {
         if (r.top_k) cut = select(row, V, top, r.per, scale, cut, false, (uint32_t)r.k, 0ull, s);

@@ -324,3 +324,24 @@ def test_whole_numbers_take_the_native_call(monkeypatch):
     for bad in (dict(temperature=-1), dict(top_p=-1), dict(min_p=2), dict(temperature=True)):
         with pytest.raises(mx.MmxError):
             mx.sample(l, u, **bad)
+
+
+@pytest.mark.parametrize("V", [12000, 32000, 40000, 262144])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_top_k_ends_with_a_bin(V, dtype):
+    """k as many as the bins above a border hold, one less and one more; and few of a flat row, where the parts that its bin is cut into hold one or two each."""
+    g = torch.Generator().manual_seed(V)
+    l = -1.0 - 2.0 * torch.rand((4, V), generator=g)
+    for b in range(4):
+        at = torch.randperm(V, generator=g)
+        l[b, at[:3000]] = 0.001 + 0.06 * torch.rand(3000, generator=g)      # the row's first sixteenth
+        l[b, at[3000:5000]] = -0.061 + 0.06 * torch.rand(2000, generator=g)  # and its second
+    l, u = l.to(dtype), torch.rand(4, generator=g)
+    for k in (2999, 3000, 3001, 4096, 4999, 5000, 5001):
+        for m in (0.0, 0.9):
+            check(l, u, 1.0, k, 1.0, m)
+    for std in (0.005, 0.2, 2.0):
+        l, u = logits(4, V, V + 1, std=std, dtype=dtype, peaks=0)
+        for k in (2, 3, 5, 10, 20, 40, 50, 64, 100, 300, 1000):
+            for T in (1.0, 30.0):
+                check(l, u, T, k)

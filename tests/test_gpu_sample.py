@@ -326,7 +326,6 @@ def test_whole_numbers_take_the_native_call(monkeypatch):
             mx.sample(l, u, **bad)
 
 
-<<<<<<< Updated upstream
 @pytest.mark.parametrize("V", [12000, 32000, 40000, 262144])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_top_k_ends_with_a_bin(V, dtype):
@@ -346,7 +345,8 @@ def test_top_k_ends_with_a_bin(V, dtype):
         for k in (2, 3, 5, 10, 20, 40, 50, 64, 100, 300, 1000):
             for T in (1.0, 30.0):
                 check(l, u, T, k)
-=======
+
+
 @pytest.mark.parametrize("V", [4096, 32000, 131072])
 @pytest.mark.parametrize("T", [0.02, 0.1, 0.2])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
@@ -355,4 +355,3 @@ def test_top_k_ends_far_below_the_largest(V, T, dtype):
     l, u = logits(4, V, V, dtype=dtype)
     for k, p, m in ((50, 1.0, 0.0), (50, 0.9, 0.0), (2000, 1.0, 0.0), (2000, 0.95, 0.0), (50, 1.0, 1e-6)):
         check(l, u, T, k, p, m)
->>>>>>> Stashed changes

@@ -963,7 +963,7 @@ __device__ __forceinline__ void draw(const SampleArgs& a, const Scratch& sc, con
             const float l = of_key(key_in<TL>(c[i], V));
             if (!__any(c[i] != 0)) continue;
             const double w = c[i] ? weight_of(l, top, r.per) : 0.0;
-            m[i] = whole(w, scale);
+            m[i] = w > 0.0 ? larger(whole(w, scale), 1ull) : 0ull;  // (what stays can be drawn, by a u of 0 or 1, however small its weight)
             low_weight |= w < r.min_p && l != top ? 1u << i : 0;
         }
         const uint32_t above = path == BY_SUMS ? state.before_count : 0;

@@ -355,3 +355,27 @@ def test_top_k_ends_far_below_the_largest(V, T, dtype):
     l, u = logits(4, V, V, dtype=dtype)
     for k, p, m in ((50, 1.0, 0.0), (50, 0.9, 0.0), (2000, 1.0, 0.0), (2000, 0.95, 0.0), (50, 1.0, 1e-6)):
         check(l, u, T, k, p, m)
+
+
+@pytest.mark.parametrize("V", [20, 3000, 40000])
+def test_what_stays_can_be_drawn_however_small_its_weight(V):
+    """Kept by top_k with weights from 1e-13 down to the smallest that 64 bits hold, in front of the others and behind them; what 64 bits hold as 0 is not drawn."""
+    for d in (30.0, 36.0, 40.0, 100.0, 700.0, 740.0, 800.0):
+        l = torch.full((4, V), -2000.0)
+        l[:, 7], l[:, 2], l[:, V - 2] = 0.0, -d, -d - 1
+        u = torch.tensor([0.0, 1.0, 0.5, 1.0 - 2.0 ** -24])
+        for T, k in ((1.0, 3), (1.0, 10), (0.5, 3)):
+            got = mx.sample(l.cuda(), u.cuda(), T, k).tolist()
+            at, w = su.kept(l[0].double().numpy(), T, k)
+            live = at[w > 0]
+            assert got == [live[0], live[-1], 7, 7], (d, T, k)
+
+
+def test_what_stays_beside_thousands_can_be_drawn_however_small_its_weight():
+    """The same where more than a list holds lies above: a segment of such tokens alone is the first."""
+    V = 262144
+    l, u = torch.full((3, V), -40.0), torch.tensor([0.0, 1.0, 0.25])
+    l[:, 100000:105000] = torch.rand((3, 5000), generator=torch.Generator().manual_seed(1))
+    l[:, :50] = l[:, V - 50:] = -30.9
+    check(l, u, 1.0, 5100)
+    assert mx.sample(l.cuda(), u.cuda(), 1.0, 5100).tolist()[:2] == [0, V - 1]

@@ -254,7 +254,7 @@ enum { BY_LIST, BY_SUMS, ALONE };
 struct State {
     uint32_t entries, path, before_count;
     float top, from, to;       // logits from `from` on go into the list, those from `to` on into the sums
-    double before_mass, mass;  // of what lies above the last bin, and of everything
+    double before_mass, mass;  // of what lies above the last bin, and of everything (0: it is not known, or all in the list)
 };
 // A row's scratch
 struct Scratch {
@@ -607,6 +607,8 @@ __device__ __forceinline__ void find_cut(const SampleArgs& a, const Scratch& sc,
             s.from = cut == BINS - 1 ? of_key(key_of(NEVER) + 1) : least_of(bin - cut, per);
             if (s.path == BY_SUMS && cut > 0) s.to = least_of(bin - cut + 1, per);
         }
+        // (0: all there is lies in the list, whose own sum tells whether a share of it is reached; the histogram's, rounded otherwise, would have two equal logits and top_p 0.5 keep both)
+        if (s.path == BY_LIST && (double)run_count >= counted) s.mass = 0.0;
         narrow = s.path == BY_SUMS && count > LIST;
         if (narrow) shared = s;
         else *sc.state = s;
@@ -978,8 +980,9 @@ __device__ __forceinline__ void draw(const SampleArgs& a, const Scratch& sc, con
                 unsigned long long of = 0;
 #pragma unroll
                 for (int i = 0; i < MINE; i++) of += c[i] ? m[i] : 0ull;
-                if (r.top_k) of = sum_of(of, o);
-                const double goal = ceil(r.p * (r.top_k ? (double)of : state.mass * scale)) - (path == BY_SUMS ? state.before_mass * scale : 0.0);
+                const bool own_sum = state.mass == 0.0;  // (always with top_k)
+                if (own_sum) of = sum_of(of, o);
+                const double goal = ceil(r.p * (own_sum ? (double)of : state.mass * scale)) - (path == BY_SUMS ? state.before_mass * scale : 0.0);
                 mode = BY_MASS, want = goal > 1.0 ? (unsigned long long)goal : 1ull;
             } else {
                 unsigned long long all = 0;

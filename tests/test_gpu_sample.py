@@ -379,3 +379,23 @@ def test_what_stays_beside_thousands_can_be_drawn_however_small_its_weight():
     l[:, :50] = l[:, V - 50:] = -30.9
     check(l, u, 1.0, 5100)
     assert mx.sample(l.cuda(), u.cuda(), 1.0, 5100).tolist()[:2] == [0, V - 1]
+
+
+@pytest.mark.parametrize("n", [2, 3, 4, 10, 20, 50, 96, 512, 3000, 4096, 5000])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_top_p_that_equal_logits_hold_exactly(n, dtype):
+    """n equal logits, alone and beside masked ones: where top_p is a whole number of them, it keeps as many and no more."""
+    g = torch.Generator().manual_seed(n)
+    u = torch.tensor([0.0, 1.0, 0.9, 0.5, 0.999])
+    for at in (0.0, 0.37, -2.6, 1000.0):
+        for V, mask in ((n, 0.0), (n + 1000, -float("inf")), (n + 1000, torch.finfo(torch.float32).min), (n + 40000, -float("inf")), (n + 3000, at - 50.0)):
+            l = torch.full((5, V), mask)
+            for b in range(5):
+                l[b, torch.randperm(V, generator=g)[:n]] = at
+            l = l.to(dtype)
+            for p in (0.5, 0.25, 0.75, 0.9):
+                for T in (1.0, 0.7):
+                    check(l, u, T, 0, p)
+        l = torch.full((5, n), at, dtype=dtype)
+        check(l, u, 1.0, n, 0.5)
+        check(l, u, 1.0, max(n - 1, 1), 0.5)

@@ -951,7 +951,7 @@ __device__ __forceinline__ void draw(const SampleArgs& a, const Scratch& sc, con
     if (r.filtered() && path != ALONE) {
         const int n = (int)state.entries < LIST ? (int)state.entries : LIST;
         unsigned long long last = 1;
-        uint32_t low_weight = 0;
+        uint32_t low_weight = 0, live = 0;
 #pragma unroll
         for (int i = 0; i < MINE; i++) {
             const int at = threadIdx.x + i * THREADS;
@@ -965,7 +965,8 @@ __device__ __forceinline__ void draw(const SampleArgs& a, const Scratch& sc, con
             const float l = of_key(key_in<TL>(c[i], V));
             if (!__any(c[i] != 0)) continue;
             const double w = c[i] ? weight_of(l, top, r.per) : 0.0;
-            m[i] = w > 0.0 ? larger(whole(w, scale), 1ull) : 0ull;  // (what stays can be drawn, by a u of 0 or 1, however small its weight)
+            m[i] = whole(w, scale);
+            live |= w > 0.0 ? 1u << i : 0;
             low_weight |= w < r.min_p && l != top ? 1u << i : 0;
         }
         const uint32_t above = path == BY_SUMS ? state.before_count : 0;
@@ -989,7 +990,8 @@ __device__ __forceinline__ void draw(const SampleArgs& a, const Scratch& sc, con
 #pragma unroll
                 for (int i = 0; i < MINE; i++) {
                     if (low_weight >> i & 1) c[i] = 0;
-                    m[i] = c[i] ? m[i] : 0ull;
+                    // (what stays can be drawn, by a u of 0 or 1, however small its weight; to top_p's share such weights add nothing, as in 64 bits)
+                    m[i] = c[i] ? live >> i & 1 ? larger(m[i], 1ull) : m[i] : 0ull;
                     all += m[i];
                     c[i] = order_of(c[i], V);  // (the order of the vocabulary)
                 }

@@ -399,3 +399,19 @@ def test_top_p_that_equal_logits_hold_exactly(n, dtype):
         l = torch.full((5, n), at, dtype=dtype)
         check(l, u, 1.0, n, 0.5)
         check(l, u, 1.0, max(n - 1, 1), 0.5)
+
+
+@pytest.mark.parametrize("n", [2, 4, 20, 512])
+@pytest.mark.parametrize("V", [600, 5000, 40000])
+def test_hardly_any_weight_adds_nothing_to_top_ps_share(n, V):
+    """Beside n equal logits top_k keeps some of 1e-26 of their weight, which 64 bits add to n without a trace."""
+    g = torch.Generator().manual_seed(n)
+    u = torch.tensor([0.0, 1.0, 0.9, 0.5, 0.999])
+    l = torch.full((5, V), -100.0)
+    for b in range(5):
+        at = torch.randperm(V, generator=g)
+        l[b, at[:n + 40]] = -60.0 - torch.rand(n + 40, generator=g)
+        l[b, at[:n]] = 0.0
+    for k in (n, n + 1, n + 40):
+        for p in (0.5, 0.25, 0.75):
+            check(l, u, 1.0, k, p)

@@ -1067,7 +1067,7 @@ __device__ __forceinline__ void draw(const SampleArgs& a, const Scratch& sc, con
     }
     if (threadIdx.x == 0) s.pick = segs, s.bin = 0;
     double run = scan_before(mine, s.part, &total);
-    const double want = u > 0.0 ? u * total : 0.0;
+    const double want = u >= 1.0 ? __builtin_huge_val() : u > 0.0 ? u * total : 0.0;  // (1: nothing comes to more; sums of another order may)
     int here = -1, last = -1;
     double rest = 0;
 #pragma unroll

@@ -415,3 +415,20 @@ def test_hardly_any_weight_adds_nothing_to_top_ps_share(n, V):
     for k in (n, n + 1, n + 40):
         for p in (0.5, 0.25, 0.75):
             check(l, u, 1.0, k, p)
+
+
+@pytest.mark.parametrize("B,V", [(600, 1500), (300, 31478), (200, 100003)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_u_of_1_takes_the_last_that_stays_in_every_row(B, V, dtype):
+    """Whatever the sums of a row and of its segments were rounded to; the last tokens' weights lie below the sums' last bits."""
+    l, _ = logits(B, V, B, std=0.8, dtype=dtype)
+    l = l.cuda()
+    u = torch.ones(B, device="cuda")
+    u[::2] = 7.0
+    assert mx.sample(l, u, 0.2).tolist() == [V - 1] * B
+    assert mx.sample(l, u, 0.2, min_p=1e-300).tolist() == [V - 1] * B  # (every weight is more)
+    for k in (3, 700, 6000):
+        got = mx.sample(l, u, 0.2, top_k=k).tolist()
+        for b in range(4):
+            at, w = su.kept(l[b].double().cpu().numpy(), 0.2, k)
+            assert got[b] == at[w > 0][-1]

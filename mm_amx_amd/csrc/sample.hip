@@ -46,8 +46,8 @@ __device__ __forceinline__ RowAsks asks_of(const SampleArgs& a, int row) {
     r.per = 1.0 / fmax(r.T, 1e-300);  // (that and less: any two logits that differ are too far apart for a weight; 1 / T must stay a number)
     r.k = a.top_k ? a.top_k[row] : a.top_k_all;
     r.p = a.top_p ? (double)a.top_p[row] : a.top_p_all;
-    r.min_p = a.min_p ? (double)a.min_p[row] : a.min_p_all;
-    if (r.min_p > 1.0) r.min_p = 1.0;  // (not fmin, which would lose a NaN; with more than 1, tokens whose weight comes out as 1 at a high temperature would fall)
+    r.min_p = a.min_p_all;
+    if (a.min_p) r.min_p = a.min_p[row] > 1.0f ? 1.0 : (double)a.min_p[row];  // (not fmin, which would lose a NaN; with more than 1, tokens whose weight comes out as 1 at a high temperature would fall)
     r.top_k = r.k > 0 && r.k < a.V;
     r.top_p = r.p < 1.0;
     r.min = r.min_p > 0.0;
@@ -917,7 +917,8 @@ __device__ __forceinline__ void draw(const SampleArgs& a, const Scratch& sc, con
     const State state = *sc.state;
     const double first_sum = (int)threadIdx.x < segs ? sc.sums[threadIdx.x] : 0.0;
     const float first_top = (int)threadIdx.x < segs ? sc.seg_top[threadIdx.x] : NEVER;
-    const double u = (double)a.u[row_at];
+    const float asked = a.u[row_at];
+    const double u = asked >= 1.0f ? __builtin_huge_val() : (double)asked;  // (nothing comes to 1 of the sum and more, but sums of another order may)
     unsigned long long c[MINE], m[MINE];
 #pragma unroll
     for (int i = 0; i < MINE; i++) {  // (asked for before anything is known of it; sorted out below)
@@ -951,7 +952,8 @@ __device__ __forceinline__ void draw(const SampleArgs& a, const Scratch& sc, con
     if (r.filtered() && path != ALONE) {
         const int n = (int)state.entries < LIST ? (int)state.entries : LIST;
         unsigned long long last = 1;
-        uint32_t low_weight = 0, live = 0;
+        uint32_t low_weight = 0;
+        const double least_p = fmax(r.min_p, 5e-324);  // (what 64 bits hold as 0 isn't drawn)
 #pragma unroll
         for (int i = 0; i < MINE; i++) {
             const int at = threadIdx.x + i * THREADS;
@@ -966,8 +968,7 @@ __device__ __forceinline__ void draw(const SampleArgs& a, const Scratch& sc, con
             if (!__any(c[i] != 0)) continue;
             const double w = c[i] ? weight_of(l, top, r.per) : 0.0;
             m[i] = whole(w, scale);
-            live |= w > 0.0 ? 1u << i : 0;
-            low_weight |= w < r.min_p && l != top ? 1u << i : 0;
+            low_weight |= w < least_p && l != top ? 1u << i : 0;
         }
         const uint32_t above = path == BY_SUMS ? state.before_count : 0;
         for (int step = 0; step < 3; step++) {  // top_k, top_p, the token
@@ -991,7 +992,7 @@ __device__ __forceinline__ void draw(const SampleArgs& a, const Scratch& sc, con
                 for (int i = 0; i < MINE; i++) {
                     if (low_weight >> i & 1) c[i] = 0;
                     // (what stays can be drawn, by a u of 0 or 1, however small its weight; to top_p's share such weights add nothing, as in 64 bits)
-                    m[i] = c[i] ? live >> i & 1 ? larger(m[i], 1ull) : m[i] : 0ull;
+                    m[i] = c[i] ? larger(m[i], 1ull) : 0ull;
                     all += m[i];
                     c[i] = order_of(c[i], V);  // (the order of the vocabulary)
                 }
@@ -1067,7 +1068,7 @@ __device__ __forceinline__ void draw(const SampleArgs& a, const Scratch& sc, con
     }
     if (threadIdx.x == 0) s.pick = segs, s.bin = 0;
     double run = scan_before(mine, s.part, &total);
-    const double want = u >= 1.0 ? __builtin_huge_val() : u > 0.0 ? u * total : 0.0;  // (1: nothing comes to more; sums of another order may)
+    const double want = u > 0.0 ? u * total : 0.0;
     int here = -1, last = -1;
     double rest = 0;
 #pragma unroll

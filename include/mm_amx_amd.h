@@ -361,7 +361,8 @@ int mmx_block_norm(const mmx_block_norm_args* args, int M, int H, void* stream);
 size_t mmx_mxfp4_bytes(int64_t rows, int K);
 
 /* x [M, K] (MMX_BF16 or MMX_F32) -> packed: b is that of the least power of two, 2^-126 at least, with which the block's largest magnitude is less than 7, so that it
- * rounds to 6 at most; values are x / scale to nearest even.  (x / scale is exact, so the result does not depend on how it is computed.)  A block that holds an
+ * rounds to 6 at most; values are x / scale to nearest even.  (x / scale is exact, so the result does not depend on how it is computed.  Quantisers that take 2^(floor(log2 amax) - 2) and clip give the
+ * same scale but for blocks whose largest magnitude is 1.75 to 2 times a power of two, where theirs is half of this one and clips 7 to 8 of it to 6; mmx_repack_mxfp4 takes the codes of any.)  A block that holds an
  * infinity or a NaN gets the scale NaN; a magnitude from 3.5 * 2^126 on rounds to 2^128, which 32 bits cannot hold.  pair: 0; or 1 / 2: x is the gate / up half of a pair of M rows each (M % 32 == 0) and packed the whole pair's,
  * mmx_mxfp4_bytes(2 M, K) bytes, in which gate's panels and up's alternate. */
 int mmx_quantize_mxfp4(int x_dtype, const void* x, int64_t ldx_bytes, int M, int K, int pair, void* packed, void* stream);
@@ -394,7 +395,10 @@ int mmx_mlp_mxfp4(int x_dtype, const void* x, int64_t ldx_bytes, const void* w_g
  *     those what has w >= min_p (the largest always)
  *     ids[b] = the first index, in the order of the vocabulary, up to which the weights that were kept come to more than u times their sum.
  * A temperature of 0 takes the largest (the lowest index of equal ones).  -inf (a masked token) and NaN are never drawn; a row of nothing else gives -1.  Beside +inf nothing else has
- * weight.  Weights and sums are in 64 bits, or whole numbers of 2^-34 of the largest where the end of a run is sought, so the same inputs give the same token every time.
+ * weight.  Weights are good to 2e-13 and summed in 64 bits in an order that does not change, or as whole numbers, so the same inputs give the same token every time:
+ *   - where top_k or top_p ends a run, weights count in steps of 2^-s of the largest, s = 61 less the bits of V - 1 (46 at V = 32000, 39 at 2^22); one that is kept can be drawn however small it is;
+ *   - where top_p alone ends a run, shares of the row's sum are good to some 5e-11 (5e-10 where |l / temperature| nears 2^22), and what lies below e^-31.9 of the largest is not counted, 1.4e-14 each, 6e-8
+ *     of the largest at V = 2^22 together: a top_p nearer to 1, or to a share that tokens hold exactly, than that may end the run a token early or late.  (Equal logits hold their shares exactly.)
  * temperature, top_k, top_p and min_p are the same for all rows, or come as fp32 / int32 [B] (the pointers _of, on the device; what is out of range there is taken as the
  * nearest that is not, NaN as off, a temperature that is NaN as 0).  u of 1 or more takes the last token that is kept, NaN or below 0 the first.
  * B <= 65535, V <= 2^22.  scratch: 256-byte aligned device memory, mmx_sample_scratch_bytes() bytes, free to reuse once the call's work on `stream` has finished. */

@@ -208,8 +208,9 @@ __global__ __launch_bounds__(512) void mxfp4_rows_kernel(const Mxfp4Gemm g) {
 // then their 256 bytes of scales, straight from memory into one of R slots of LDS; with the operands in the instruction's own order every LDS read is a KiB in a row.  A stage has four steps of 64 k;
 // the operands of a step are read during the one before.  The one barrier per stage stands in front of its last step: all of it has been read into registers then, so its slot is free for
 // stage t + R, whose loads are spread over the last step and the next stage's first two, and stage t + 1 has landed.
-// Bound: what a CU gets from L2 into LDS (48 to 65 bytes a nanosecond) and the LDS itself, whose reads and writes a step of the 256 x 192 tile take as long as its MFMAs; 2048 x 4096 x 11008
-// comes to 3250 TFLOP/s, 4096 x 4096 x 4096 to 3500, where the MFMAs alone reach 6670 on random values.  Refilling slots by halves, with loads R - 1 stages ahead, was no faster (57 -> 60 us),
+// Bound: what a CU gets from L2 into LDS (40 bytes a nanosecond in 256 x 192 tiles, two slots holding no more on its way) and the LDS itself, whose reads and writes a step of that tile take as long as
+// its MFMAs; 2048 x 4096 x 11008 takes 61 to 65 us in a trace, by card, 2.8 to 3.0 PFLOP/s (57 with operands that stay in the caches, 3250 TFLOP/s, and 4096 x 4096 x 4096 3500), where the MFMAs alone reach
+// 6670 on random values.  Refilling slots by halves, with loads R - 1 stages ahead, was no faster (57 -> 60 us),
 // nor were 4 x 3 panels a wavefront with a third fewer LDS reads and one wavefront a SIMD (59).
 // KG groups of wavefronts, each with a ring of its own, take the chunks in turn where there are fewer tiles than CUs; their sums are added in LDS, in order.
 template <int PM, int PN, int WGM, int WGN, int R, int KG>
@@ -611,8 +612,8 @@ static int launch_rows(const Mxfp4Gemm& g, hipStream_t st, const char* name) {
 bool mx_takes_bf16(int M, int K, int N, bool pair) { return M <= 8 && (int64_t)M * K * (N / (pair ? 64 : 16) + 460) <= 16400000; }
 
 // Which tile: the least of rounds * (fixed + chunks of 256 k * stage), a round being as many tiles as fit on the chip; one that is not full leaves each of its tiles more of the chip, down to `least` of
-// the time.  The constants are fitted to 86 products of 33 to 4096 rows, 256 to 11008 k and 256 to 32000 columns in every tile, each by how near it comes to the fastest; the tile chosen was 0.5 % behind
-// that on average, 10 % at most.  us at 2048 x 4096 x 11008 / 4096 x 4096 x 4096 / 1024 x 11008 x 4096 / 256 x 4096 x 4096 / 64 x 11008 x 4096:
+// the time.  The constants are fitted to 86 products of 33 to 4096 rows, 256 to 11008 k and 256 to 32000 columns in every tile, each by how near it comes to the fastest; among those same products the tile
+// chosen was 0.5 % behind that on average, 10 % at most (times of all: profiles/mxfp4_tiles_by_size.txt).  us at 2048 x 4096 x 11008 / 4096 x 4096 x 4096 / 1024 x 11008 x 4096 / 256 x 4096 x 4096 / 64 x 11008 x 4096:
 //     256 x 256            64 / 39 / 57 / 25 / 52
 //     256 x 192            57 / 55 / 46 / 21 / 42
 //     128 x 256            61 / 45 / 36 / 16 / 30

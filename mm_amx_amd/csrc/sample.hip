@@ -11,10 +11,15 @@
 // Four kernels, or one for a short row (sample_row_kernel).  A workgroup for each slice of a row reads the logits: segments' maxima; without filters their sums too; with top_k or top_p a histogram of the slice, counts and weights by
 // l / T in steps of 1 / 16, on one grid for the row.  With filters a workgroup a row adds the histograms up, which shows the bin in which the run ends.  Workgroups of four segments collect what lies in it
 // and above; or, where that is more than a list holds, what lies in it, and the segments' sums of what lies above.  A workgroup a row sorts out from the list where the run ends, and draws.
-// Bound: the launches and the steps that wait for each other in them (barriers, LDS, a dependent read), each kernel 5 us at the least; HBM only for many rows without filters, where the one pass over
-// 256 x 131072 fp32 takes 35 us, 3.8 TB/s, of 41.  us, slices / cut / filter / draw: 33 x 100003 fp32, top_p 9 / 4.8 / 12 / 12.5;
-// 64 x 131072 bf16, a mixture 13.0 / 5 / 11 / 15.8.  (One kernel, a workgroup a row that passes over it again and again: 349 and 589 us for these two.)
-// Rows that this does not suit (more than a list of equal logits in the last bin, or of what top_k leaves to top_p; 2^26 bins and more; more than 2^20 logits and a list) are worked on by that one workgroup alone, a pass over the row for every eight bits of the key.
+// Bound: the launches and the steps that wait for each other in them (barriers, LDS, a dependent read), each kernel 5 us at the least.  For many rows without filters the weights beside memory: the one pass
+// over 256 x 131072 fp32 takes 35 us of 42, 3.8 TB/s, and its vector instructions, 30 a logit, 17 of them in 64 bits, 0.69 of that; without weights, temperature 0, the whole draw takes 28.  min_p alone
+// passes twice: 65.  us, slices / cut / filter / draw: 33 x 100003 fp32, top_p 9 / 5 / 13 / 13;
+// 64 x 131072 bf16, a mixture 13 / 5 / 11 / 16.  (One kernel, a workgroup a row that passes over it again and again: 349 and 589 us for these two.)
+// Rows that this does not suit are worked on by that one workgroup alone, a pass over the row for every eight bits of the key.  They are those with more than a list
+//   below the grid, 31.9 T under the largest, where the run ends there (top_k at a low temperature: 64 x 131072 bf16 with a dozen peaks, top_k 50: T 0.8 29 us, 0.2 332; 1 x 32000 fp32 T 0.2 17, 0.1 82);
+//   in the bin in which top_k ends and above it, if there is a top_p too, or more than 2^20 logits;
+//   of equal logits where the run ends;
+// and those of 2^26 bins and more (|l / T| from 2^22 on, +inf) or temperatures past 1e-299 and 1e31.
 #include "sample.hpp"
 
 #include "ffn.hpp"
